@@ -16,6 +16,7 @@ import scipy.sparse
 import torch
 
 from . import tuning
+from .module import block_attention as _block
 from .module import common
 from .module import (EdgeSoftmaxhip, GraphAttentionhip, GSDDMMhip, GSpMMhip, MultiHeadSDDMMhip, VanillaSDDMMhip,
                      placeholder)
@@ -713,3 +714,27 @@ class _Aggregate(torch.autograd.Function):
             return None, dx.index_add(0, flat[valid], dy[valid]).view(ctx.x_shape), None
         (dx,) = _selected_grads(g, g._aggregate_mod(dy.shape[1], reduce)._bop, arg, None, [ctx.x_shape], dy, (True,))
         return None, dx, None
+
+
+def block_attention(q, k, v, bias, blocks, spec, lengths, q_lengths, bounds):
+    """ops.block_attention on checked arguments; spec = (block_size, scale, causal)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+        return _BlockAttention.apply(q, k, v, bias, blocks, spec, lengths, q_lengths, bounds)
+    return _block.block_attention_forward(q, k, v, blocks, *spec, lengths, q_lengths, bias, bounds, False)[0]
+
+
+class _BlockAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, blocks, spec, lengths, q_lengths, bounds):
+        out, lse, rest = _block.block_attention_forward(q, k, v, blocks, *spec, lengths, q_lengths, bias, bounds, True)
+        ctx.spec, ctx.bounds = spec, bounds
+        ctx.save_for_backward(q, k, v, bias, blocks, lengths, q_lengths, out, lse, rest)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, bias, blocks, lengths, q_lengths, out, lse, rest = ctx.saved_tensors
+        keys_too = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        grads = _block.block_attention_backward(q, k, v, blocks, *ctx.spec, lengths, q_lengths, bias, ctx.bounds, out, lse, rest, dout, keys_too)
+        return grads + (None,) * 5

@@ -1,0 +1,195 @@
+"""Attention over blocks of keys that every query selects, on the matrix cores: the calls of the C interface on torch tensors.
+
+The graph of this attention -- which blocks of keys a query attends to -- is made on the GPU by every call's data, so there is nothing
+to lay out ahead of a call and no module to build: the operators are functions of their tensors (`featgraph_amd.ops`).  Outputs and
+workspaces come from torch's allocator on the current stream, so calls on several streams, and captured ones, share nothing.
+The reference has no such operator.
+"""
+import ctypes
+
+import torch
+
+from .. import _lib
+from . import common
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+HEAD_LENGTHS, BLOCK_SIZES, MAX_GROUP, MAX_BUCKETS, MAX_SPAN = (32, 64, 128), (32, 64, 128, 256), 16, 64, 4094
+
+
+def _check(name, t, dims, like=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor on the GPU, got %s" % (name, type(t)))
+    if not t.is_cuda:
+        raise ValueError("%s is on %s: there is no CPU path" % (name, t.device))
+    if t.dtype not in _TYPES:
+        raise ValueError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if t.dim() != dims:
+        raise ValueError("%s must have %d axes, got shape %s" % (name, dims, tuple(t.shape)))
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError("%s is %s on %s, the queries are %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
+
+
+def _check_counts(name, t, batch, device):
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor, got %s" % (name, type(t)))
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != (batch,) or not t.is_contiguous():
+        raise ValueError("%s must be %d int32 values on %s, got %s of %s on %s" % (name, batch, device, tuple(t.shape), t.dtype, t.device))
+
+
+def _check_sizes(head_len, block_size, heads=None, kv_heads=None):
+    if head_len not in HEAD_LENGTHS:
+        raise ValueError("heads of 32, 64 or 128 elements, got %d" % head_len)
+    if block_size not in BLOCK_SIZES:
+        raise ValueError("blocks of 32, 64, 128 or 256 keys, got %s" % (block_size,))
+    if heads is not None and (kv_heads < 1 or heads % kv_heads or not 1 <= heads // kv_heads <= MAX_GROUP):
+        raise ValueError("%d query heads over %d key heads: 1 to %d of the former to each of the latter" % (heads, kv_heads, MAX_GROUP))
+
+
+def _rows(t):
+    """The tensor itself where the kernels can address it -- dense heads at 16-byte addresses -- or else a dense copy."""
+    per = 16 // t.element_size()
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) % per == 0 for i in range(3))
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strides(t):
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def block_pool(k, block_size, lengths):
+    _check("k", k, 4)
+    batch, keys, kv_heads, head_len = k.shape
+    _check_sizes(head_len, block_size)
+    _check_counts("lengths", lengths, batch, k.device)
+    if kv_heads < 1:
+        raise ValueError("k has no heads: shape %s" % (tuple(k.shape),))
+    k = _rows(k)
+    pooled = torch.empty((batch, kv_heads, -(-keys // block_size), head_len), dtype=k.dtype, device=k.device)
+    with torch.cuda.device(k.device):
+        _lib.check(_lib.lib().fg_block_pool(_TYPES[k.dtype], _lib.dev_ptr(k), _strides(k), _lib.dev_ptr(lengths), _lib.dev_ptr(pooled), batch,
+                                            keys, kv_heads, head_len, block_size, common.stream_ptr()))
+    return pooled
+
+
+def block_select(q, pooled, num_keys, block_size, topk, causal, lengths, q_lengths, keep_first, keep_last):
+    _check("q", q, 4)
+    _check("pooled", pooled, 4, q)
+    batch, queries, heads, head_len = q.shape
+    kv_heads = pooled.shape[1]
+    _check_sizes(head_len, block_size, heads, kv_heads)
+    if num_keys < 0 or tuple(pooled.shape) != (batch, kv_heads, -(-num_keys // block_size), head_len):
+        raise ValueError("pooled keys of %s keys in blocks of %d must be (%d, kv_heads, blocks, %d), got %s"
+                         % (num_keys, block_size, batch, head_len, tuple(pooled.shape)))
+    if topk < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > topk:
+        raise ValueError("topk must be at least 1 and hold the first %s and the last %s blocks, got %s" % (keep_first, keep_last, topk))
+    _check_counts("lengths", lengths, batch, q.device)
+    _check_counts("q_lengths", q_lengths, batch, q.device)
+    q, pooled = _rows(q), pooled.contiguous()
+    if pooled.data_ptr() % 16:
+        pooled = pooled.clone()
+    blocks = torch.empty((batch, queries, kv_heads, topk), dtype=torch.int32, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().fg_block_select(_TYPES[q.dtype], _lib.dev_ptr(q), _strides(q), _lib.dev_ptr(pooled), _lib.dev_ptr(lengths),
+                                              _lib.dev_ptr(q_lengths), _lib.dev_ptr(blocks), batch, queries, num_keys, heads, kv_heads, head_len,
+                                              block_size, topk, int(causal), keep_first, keep_last, common.stream_ptr()))
+    return blocks
+
+
+def check_attention(q, k, v, blocks, block_size, lengths, q_lengths, bias, bounds):
+    """The bounds as a tuple, after everything that can be seen of the arguments without looking at their values on the GPU."""
+    _check("q", q, 4)
+    _check("k", k, 4, q)
+    _check("v", v, 4, q)
+    batch, queries, heads, head_len = q.shape
+    keys, kv_heads = k.shape[1], k.shape[2]
+    if tuple(k.shape) != (batch, keys, kv_heads, head_len) or k.shape != v.shape:
+        raise ValueError("k and v must be (%d, keys, kv_heads, %d), got %s and %s" % (batch, head_len, tuple(k.shape), tuple(v.shape)))
+    _check_sizes(head_len, block_size, heads, kv_heads)
+    if not isinstance(blocks, torch.Tensor):
+        raise TypeError("blocks must be a torch tensor, got %s" % type(blocks))
+    if blocks.dtype != torch.int32 or blocks.device != q.device or blocks.dim() != 4 or tuple(blocks.shape[:3]) != (batch, queries, kv_heads) \
+            or blocks.shape[3] < 1:
+        raise ValueError("blocks must be int32 (%d, %d, %d, topk) on %s, got %s of %s on %s"
+                         % (batch, queries, kv_heads, q.device, tuple(blocks.shape), blocks.dtype, blocks.device))
+    _check_counts("lengths", lengths, batch, q.device)
+    _check_counts("q_lengths", q_lengths, batch, q.device)
+    if (bias is None) != (bounds is None):
+        raise ValueError("bias and bounds come together")
+    if bias is None:
+        return ()
+    _check("bias", bias, 2, q)
+    bounds = tuple(int(x) for x in bounds)
+    if not 1 <= bias.shape[0] <= MAX_BUCKETS or bias.shape[1] != heads or len(bounds) != bias.shape[0] - 1:
+        raise ValueError("bias must be (buckets, %d) with 1 to %d buckets and one bound less, got %s and %d bounds"
+                         % (heads, MAX_BUCKETS, tuple(bias.shape), len(bounds)))
+    if any(x >= y for x, y in zip(bounds, bounds[1:])):
+        raise ValueError("the bounds must ascend, got %s" % (bounds,))
+    if bounds and (bounds[-1] - bounds[0] > MAX_SPAN or max(-bounds[0], bounds[-1]) > 2 ** 30):
+        raise ValueError("the last bound must be within %d of the first, got %s" % (MAX_SPAN, bounds))
+    return bounds
+
+
+def _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest):
+    a = _lib.FgBlockAttentionArgs()
+    a.type = _TYPES[q.dtype]
+    a.batch, a.queries, a.heads, a.head_len = q.shape
+    a.keys, a.kv_heads = k.shape[1:3]
+    a.block, a.topk, a.causal, a.scale = block_size, blocks.shape[3], int(causal), scale
+    a.n_buckets = 0 if bias is None else bias.shape[0]
+    for i, x in enumerate(bounds):
+        a.bounds[i] = x
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_strides, a.k_strides, a.v_strides = _strides(q), _strides(k), _strides(v)
+    a.blocks = blocks.data_ptr()
+    a.lengths = 0 if lengths is None else lengths.data_ptr()
+    a.q_lengths = 0 if q_lengths is None else q_lengths.data_ptr()
+    a.bias = 0 if bias is None else bias.data_ptr()
+    a.out = out.data_ptr()
+    a.lse = 0 if lse is None else lse.data_ptr()
+    a.rest = 0 if rest is None else rest.data_ptr()
+    return a
+
+
+def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, train):
+    """(out, lse, rest) of checked arguments; with `train` the latter are what the gradients start from: the logarithm of every row's sum
+    and, in 16 bits, what rounding took from `out`."""
+    q, k, v, blocks = _rows(q), _rows(k), _rows(v), blocks.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if train else None
+    rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+    a = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        need = _lib.check(L.fg_block_attention_workspace(ctypes.byref(a)))
+        work = _bytes(need, q.device)
+        _lib.check(L.fg_block_attention(ctypes.byref(a), _lib.dev_ptr(work), need, common.stream_ptr()))
+    return out, lse, rest
+
+
+def block_attention_backward(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest, dout, keys_too=True):
+    """(dq, dk, dv, dbias) for dL/d(out) = dout; dk and dv None unless `keys_too`, dbias None without a bias."""
+    q, k, v, blocks, dout = _rows(q), _rows(k), _rows(v), blocks.contiguous(), _rows(dout)
+    bias = None if bias is None else bias.contiguous()
+    new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    dq = new(q)
+    dk, dv = (new(k), new(v)) if keys_too else (None, None)
+    dbias = None if bias is None else new(bias)
+    a = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    grads = _lib.FgBlockAttentionGrads(dout=dout.data_ptr(), dout_strides=_strides(dout), dq=dq.data_ptr(), dk=dk.data_ptr() if keys_too else 0,
+                                       dv=dv.data_ptr() if keys_too else 0, dbias=0 if dbias is None else dbias.data_ptr())
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        need = _lib.check(L.fg_block_attention_backward_workspace(ctypes.byref(a)))
+        work = _bytes(need, q.device)
+        _lib.check(L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), _lib.dev_ptr(work), need, common.stream_ptr()))
+    return dq, dk, dv, dbias

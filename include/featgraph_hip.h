@@ -597,6 +597,81 @@ int fg_synth_community_csr(int64_t n, const int32_t *in_degree_host, const doubl
                            const int32_t *comm_member_host, const double *comm_cdf_host, double p_in, uint64_t seed,
                            int num_threads, int32_t *indptr_host, int32_t *indices_host);
 
+/* ---- attention over blocks of keys that every query selects ----------------------------- */
+
+/* Element types of these entry points. */
+typedef enum { FG_TYPE_F32 = 0, FG_TYPE_F16 = 1, FG_TYPE_BF16 = 2 } fg_type;
+
+/*
+ * Q is (batch, queries, heads, head_len), K and V are (batch, keys, kv_heads, head_len); heads / kv_heads (1 to 16) query heads share a
+ * key head.  Strides are in elements, of the axes batch, row and head; a head's elements are dense, and every head starts
+ * at a 16-byte address.  lengths_dev / q_lengths_dev (int32 per sequence, or null: all) count a sequence's keys and queries; what
+ * lies behind them is not read, and counts outside 0 .. keys (queries) are taken as the nearest of the two.
+ * Query i of a sequence stands at position  lengths - q_lengths + i.  Null `stream` is the default stream.
+ * (No counterpart in the reference.)
+ */
+
+/*
+ * pooled[b, g, n, :] = mean over the keys of block n (keys n * block .. of one sequence, key head g), (batch, kv_heads, ceil(keys / block),
+ * head_len) dense; 0 for a block without keys.  Summed in 64 bits and rounded to the type.
+ */
+int fg_block_pool(int type, const void *k_dev, const int64_t *k_strides, const int32_t *lengths_dev, void *pooled_dev,
+                  int batch, int keys, int kv_heads, int head_len, int block, void *stream);
+
+/*
+ * blocks_dev (batch, queries, kv_heads, topk): for every query and key head the ids of the topk blocks with the highest
+ * <sum of the group's queries, rounded to the type; pooled[b, g, n]>, in ascending order, -1 behind the last.  Compared as exact numbers
+ * (products of the stored values, summed without rounding that could change an order by more than 64-bit sums do); equal ones, and NaN, which
+ * counts as -inf, go to the lower id.  Candidates are blocks that hold a key and, with `causal`, start at or before the query's
+ * position; the first keep_first and the last keep_last of them are taken before any other (keep_first + keep_last <= topk).
+ * Rows behind q_lengths are all -1.  At most 2048 blocks.
+ */
+int fg_block_select(int type, const void *q_dev, const int64_t *q_strides, const void *pooled_dev, const int32_t *lengths_dev,
+                    const int32_t *q_lengths_dev, int32_t *blocks_dev, int batch, int queries, int keys, int heads, int kv_heads,
+                    int head_len, int block, int topk, int causal, int keep_first, int keep_last, void *stream);
+
+typedef struct {
+    int32_t type;                      /* fg_type of Q, K, V, bias and results */
+    int32_t batch, queries, keys, heads, kv_heads;
+    int32_t head_len;                  /* 32, 64 or 128 */
+    int32_t block;                     /* keys of a block: 32, 64, 128 or 256 */
+    int32_t topk;                      /* block ids per query and key head */
+    int32_t causal;                    /* non-zero: a query sees no key behind its position */
+    float scale;
+    int32_t n_buckets;                 /* 0: no bias; at most 64 */
+    int32_t bounds[63];                /* n_buckets - 1 ascending distances, the last at most 4094 from the first */
+    const void *q, *k, *v;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    const int32_t *blocks;             /* (batch, queries, kv_heads, topk) dense; ids outside 0 .. ceil(keys / block) - 1 name nothing,
+                                          an id that stands twice counts once */
+    const int32_t *lengths, *q_lengths;
+    const void *bias;                  /* (n_buckets, heads) dense: added to the scaled score of query position i and key j in
+                                          bucket  (number of bounds <= i - j) */
+    void *out;                         /* (batch, queries, heads, head_len) dense; 0 where a query sees no key */
+    float *lse;                        /* (batch, queries, heads) or null: what the gradients start from -- the base-2 logarithm of
+                                          the sum of exponentials, +inf where there is none */
+    void *rest;                        /* as out, or null: what rounding took from out, itself rounded to the type; with it the gradients
+                                          know <dout, out> to twice the type's bits */
+} fg_block_attention_args;
+
+/* Softmax attention over the selected blocks.  workspace: device memory of at least fg_block_attention_workspace(args) bytes (which only
+ * looks at sizes; negative: an error), 256-byte aligned, of this call alone while it runs; null if that is 0. */
+int64_t fg_block_attention_workspace(const fg_block_attention_args *args);
+int fg_block_attention(const fg_block_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+typedef struct {
+    const void *dout;                  /* dL / d(out) */
+    int64_t dout_strides[3];
+    void *dq;                          /* dense, as q; rows behind q_lengths 0 */
+    void *dk, *dv;                     /* dense, as k; rows behind lengths 0 */
+    void *dbias;                       /* (n_buckets, heads) dense, or null */
+} fg_block_attention_grads;
+
+/* Gradients, from the inputs, `out`, `lse` and (if it was given) `rest` as fg_block_attention left them.  The same sums in the same order on every call. */
+int64_t fg_block_attention_backward_workspace(const fg_block_attention_args *args);
+int fg_block_attention_backward(const fg_block_attention_args *args, const fg_block_attention_grads *grads, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

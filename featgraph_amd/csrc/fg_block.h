@@ -34,7 +34,6 @@ template <typename T> using V8 = typename Vec<T>::type;
 constexpr int kUnit = 32;              // keys (or query rows) of one step
 constexpr int kWaves = 4;              // wavefronts of a workgroup
 constexpr int kThreads = 64 * kWaves;
-constexpr int kWindow = 2048;          // blocks that a tile's list covers at a time
 constexpr int kPad = 16;               // elements between staged rows: 16 rows' 32-byte pieces, and 128-bit writes, spread over the banks
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -110,9 +109,14 @@ __device__ __forceinline__ bool not_finite(f32x4 v) {
     return t != t;
 }
 
-// A value that is the same in every lane, in scalar registers.
-__device__ __forceinline__ unsigned long long uniform64(unsigned long long w) {
-    return (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)w) | (unsigned long long)__builtin_amdgcn_readfirstlane((unsigned)(w >> 32)) << 32;
+// Four consecutive elements of a result, rounded to its type, and what the rounding took where that is wanted.
+template <typename T> __device__ __forceinline__ void store_row(T *out, T *rest, int64_t at, f32x4 v) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 x, y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = (T)v[i]; y[i] = (T)(v[i] - (float)x[i]); }
+    *reinterpret_cast<T4 *>(out + at) = x;
+    if (rest) *reinterpret_cast<T4 *>(rest + at) = y;
 }
 
 struct Strides { int64_t batch, row, head; };    // in elements
@@ -138,40 +142,47 @@ __device__ __forceinline__ int query_count(const Problem &p, int b) {
 // Tokens of one tile of 16 rows (all the heads that share a key head), so that a lane's column has the same head in every tile.
 __host__ __device__ __forceinline__ int tile_tokens(int group) { return 16 / group; }
 
-// The blocks that a tile of queries attends to, window by window: block ids (within the window) in ascending order and, for each, the tokens
-// that selected it as bits.  An index that is negative, behind the keys, behind the query or named twice counts for nothing more.
+// The blocks that some tiles of queries attend to, window by window: block ids (within the window) in ascending order and, for each, the tokens
+// that selected it: 16 bits for every tile, bit t for its token t.  An index that is negative, behind the keys, behind the query or named
+// twice counts for nothing more.
+template <int TILES, int WINDOW>
 struct List {
-    unsigned long long bits[kWindow];
-    uint16_t id[kWindow];
+    static constexpr int kWords = (TILES + 3) / 4, kWidth = WINDOW;
+    unsigned long long bits[WINDOW][kWords];
+    uint16_t id[WINDOW];
     int sums[kWaves];
 };
 
-// Builds the list for blocks [first, first + width) and tokens [t0, t0 + nt) of sequence b, key head h; returns its length.  For all threads
-// of the workgroup.
-__device__ __forceinline__ int build_list(List &l, const Problem &p, int b, int h, int t0, int nt, int q_len, int k_len, int first, int width) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Builds the list for blocks [first, first + width) and the tokens of `tiles` tiles from t0 on, of sequence b, key head h; returns its length.  For
+// all threads of the workgroup.
+template <int TILES, int WINDOW>
+__device__ __forceinline__ int build_list(List<TILES, WINDOW> &l, const Problem &p, int b, int h, int t0, int q_len, int k_len, int first, int width) {
+    constexpr int WORDS = List<TILES, WINDOW>::kWords;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tpt = tile_tokens(p.group);
     __syncthreads();                                   // of the last window
-    for (int i = tid; i < width; i += kThreads) l.bits[i] = 0;
+    for (int i = tid; i < width * WORDS; i += kThreads) l.bits[0][i] = 0;
     __syncthreads();
-    const int there = min(nt, q_len - t0), offset = k_len - q_len;
+    const int there = min(TILES * tpt, q_len - t0), offset = k_len - q_len;
     const int64_t row = (int64_t)p.kv_heads * p.topk;
     const int32_t *src = p.list + ((int64_t)b * p.queries + t0) * row + (int64_t)h * p.topk;
     for (int e = tid; e < there * p.topk; e += kThreads) {
         const int t = e / p.topk, blk = src[t * row + (e - t * p.topk)], at = blk - first;
         if (at < 0 || at >= width) continue;           // blk < p.blocks, as first + width is
-        const int key = blk << p.block_shift;
-        if (key < k_len && (!p.causal || key <= offset + t0 + t)) atomicOr(&l.bits[at], 1ull << t);
+        const int key = blk << p.block_shift, tile = t / tpt;
+        if (key < k_len && (!p.causal || key <= offset + t0 + t)) atomicOr(&l.bits[at][tile >> 2], 1ull << ((tile & 3) * 16 + t - tile * tpt));
     }
     __syncthreads();
-    constexpr int C = kWindow / kThreads;
+    constexpr int C = (WINDOW + kThreads - 1) / kThreads;
     const int per = (width + kThreads - 1) / kThreads; // consecutive blocks of a thread, C at most
-    unsigned long long mine[C];
+    unsigned long long mine[C][WORDS];
     int count = 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const int at = tid * per + i;
-        mine[i] = i < per && at < width ? l.bits[at] : 0;
-        count += mine[i] != 0;
+        unsigned long long any = 0;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) any |= mine[i][w] = i < per && at < width ? l.bits[at][w] : 0;
+        count += any != 0;
     }
     int upto = count;
 #pragma unroll
@@ -189,11 +200,16 @@ __device__ __forceinline__ int build_list(List &l, const Problem &p, int b, int 
     }
     int at = before + upto - count;
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-        if (mine[i]) {
-            l.bits[at] = mine[i];
+    for (int i = 0; i < C; ++i) {
+        unsigned long long any = 0;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) any |= mine[i][w];
+        if (any) {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) l.bits[at][w] = mine[i][w];
             l.id[at++] = (uint16_t)(tid * per + i);
         }
+    }
     __syncthreads();
     return total;
 }

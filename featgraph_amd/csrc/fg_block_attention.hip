@@ -3,14 +3,14 @@
 // with g = h / group, pos_i = k_len - q_len + i, and j visible to i where floor(j / block) is in i's list for g, j < k_len and (causal) j <= pos_i.
 // No visible key: 0.
 //
-// One workgroup takes the tokens of RT tiles of 16 rows (16 / group tokens each, all heads of the group) and walks the blocks that any of
-// them selected; neighbouring tokens share most of theirs, so a block's keys are fetched once for all of them.  Its four wavefronts
-// take 32 keys each in turn and keep a softmax (maximum, sum) and an output of their own, joined at the end: no barrier inside the
-// walk.  Keys go from memory into registers as the left operand of (keys x queries); values through a wavefront's own LDS, from which they
-// are read with keys along the registers.  A tile none of whose tokens selected a block skips it.
-// Where there are few queries, the list is dealt out over several workgroups too, and a second kernel joins their sums.
-// Values that are not finite reach the rows that see them and no others: a result that is not finite is computed again
-// with such places apart (mma_masked).
+// Rows of one token's heads and of neighbouring tokens make tiles of 16, and the blocks that any token of a tile selected are walked for all of
+// them: neighbours share most of their blocks, and a token that did not select one has weight 0 there.  Two kernels.
+// many_kernel, where there are queries to fill the card: four wavefronts with tiles of their own walk the union of their lists through
+// LDS, 64 keys at a time, fetched into registers while the 64 before are worked on; each keeps its softmax and its output.
+// few_kernel, for single tokens and short sequences: one tile per workgroup, whose list is dealt out to the four wavefronts and, where
+// that leaves the card idle, to several workgroups; each takes its keys from memory straight into operands.
+// Values that are not finite reach the rows that see them and no others: a result that is not finite is computed again with such places
+// apart (mma_masked).
 #include <algorithm>
 #include <type_traits>
 
@@ -23,63 +23,55 @@ namespace {
 
 constexpr int kMergeStride = 36;       // floats between rows of the joining buffer (32 and 4 of padding)
 
-template <typename T, int D, int RT> constexpr size_t stage_bytes() {
-    const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * RT * 16 * kMergeStride * sizeof(float);
+// ---- few queries ------------------------------------------------------------------------------------------
+
+template <typename T, int D> constexpr size_t few_stage_bytes() {
+    const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
     return values > merge ? values : merge;
 }
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kThreads) void block_attention_kernel(const Problem p, T *out, T *remainder, float *lse, float *part, float2 *part_stats,
-                                                                   int n_tiles, int splits) {
+struct Results { void *out, *rest; float *lse, *part; float2 *part_stats; };
+
+struct FewShared {
+    List<1, 1024> list;
+    float2 stats[kWaves][16], joined[16];
+};
+
+// One tile of 16 rows, or one of `splits` shares of its list.  CAREFUL: with values that are not finite kept apart from the start.
+template <typename T, int D, bool CAREFUL>
+__device__ __forceinline__ void few_rows(const Problem &p, const Results &r, FewShared &shared, unsigned char *dynamic, const Buckets &buckets, int b, int h,
+                                         int tile, int split, int splits) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad;
     constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = 64 / CPR, NV = kUnit / RPL;
-    __shared__ List list;
-    __shared__ float2 stats[kWaves][RT * 16];
-    __shared__ float2 joined[RT * 16];
-    extern __shared__ __align__(16) unsigned char dynamic[];
-
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const int unit = xcd_contiguous_block();
-    const int pair = unit / (n_tiles * splits), rest = unit - pair * n_tiles * splits;
-    const int tile = rest / splits, split = rest - tile * splits;
-    const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
-    const int tpt = tile_tokens(p.group), t0 = tile * RT * tpt, nt = RT * tpt;
-    const int tc = c / p.group, head = h * p.group + (c - tc * p.group);        // this lane's token within a tile, and its head
+    const int tpt = tile_tokens(p.group), t0 = tile * tpt;
+    const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;        // this lane's token within the tile, and its head
     const bool used = tc < tpt;
 
     T *stage = reinterpret_cast<T *>(dynamic) + wave * kUnit * S;
-    Buckets buckets;
-    if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + stage_bytes<T, D, RT>());
-
-    V8<T> qf[RT][DC];
-    int limit[RT];                     // last key that the lane's row may see
+    const bool there = used && t0 + tc < q_len;
+    // last key that the lane's row may see (columns without a row see everything, so that they do not keep the tile from skipping its
+    // masks; nothing is written of them)
+    const int limit = there ? (p.causal ? min(offset + t0 + tc, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
+    V8<T> qf[DC];
+    const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)(t0 + tc) * p.qs.row + head * p.qs.head + 8 * g;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int t = t0 + rt * tpt + tc;
-        const bool there = used && t < q_len;
-        // (columns without a row see everything, so that they do not keep a tile from skipping its masks; nothing is written of them)
-        limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
-        const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
-#pragma unroll
-        for (int dc = 0; dc < DC; ++dc) qf[rt][dc] = there ? load8(src + dc * 32) : zero8<T>();
-    }
-    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + nt, q_len) - 1) : k_len - 1;
+    for (int dc = 0; dc < DC; ++dc) qf[dc] = there ? load8(src + dc * 32) : zero8<T>();
+    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + 8 * g;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + (lane % CPR) * EPC;
     const int sub_shift = p.block_shift - 5;
+    auto &list = shared.list;
 
-    f32x4 o[RT][DT];
-    float m[RT], l[RT];
+    f32x4 o[DT];
+    float m, l;
     auto sweep = [&](auto careful) {
+        m = -__builtin_inff(); l = 0.f;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -__builtin_inff(); l[rt] = 0.f;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        for (int first = 0; first < p.blocks; first += kWindow) {
-            const int units = build_list(list, p, b, h, t0, nt, q_len, k_len, first, min(kWindow, p.blocks - first)) << sub_shift;
+        for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int first = 0; first < p.blocks; first += list.kWidth) {
+            const int units = build_list(list, p, b, h, t0, q_len, k_len, first, min(list.kWidth, p.blocks - first)) << sub_shift;
             auto first_key = [&](int u) {
                 return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
             };
@@ -91,10 +83,10 @@ __global__ __launch_bounds__(kThreads) void block_attention_kernel(const Problem
             V8<T> kf[2][DC];
             u32x4 vr[NV];
             int key0 = 0;
-            unsigned long long bits = 0;
+            unsigned who = 0;
             auto fetch = [&](int u) {
                 key0 = first_key(u);
-                bits = uniform64(list.bits[u >> sub_shift]);
+                who = (unsigned)list.bits[u >> sub_shift][0];
                 // rows behind the last key read it again: what a padded cache holds there is never touched
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -108,172 +100,384 @@ __global__ __launch_bounds__(kThreads) void block_attention_kernel(const Problem
             if (u < units) fetch(u);
             while (u < units) {
                 const int now = key0;
-                const unsigned long long who = bits;
+                const int last = !used || (who >> tc) & 1 ? limit : -1;      // keys that the lane's row sees: now + 16 kt + 4 g + i <= last
                 wave_lds_sync();
 #pragma unroll
                 for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4 *>(stage + (i * RPL + lane / CPR) * S + (lane % CPR) * EPC) = vr[i];
                 wave_lds_sync();
-                f32x4 s[RT][2];
-                unsigned active = 0;
+                f32x4 s[2];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!((who >> (rt * tpt)) & ((1ull << tpt) - 1))) continue;
-                    active |= 1u << rt;
+                for (int kt = 0; kt < 2; ++kt) {
+                    s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int dc = 0; dc < DC; ++dc) s[rt][kt] = mma(kf[kt][dc], qf[rt][dc], s[rt][kt]);
-                    }
+                    for (int dc = 0; dc < DC; ++dc) s[kt] = mma(kf[kt][dc], qf[dc], s[kt]);
                 }
                 u = find(u + kWaves * splits);
                 if (u < units) fetch(u);
 
-                V8<T> pf[RT];
-                unsigned seen[RT];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!(active & (1u << rt))) continue;
-                    // keys that the lane's row sees: now + 16 kt + 4 g + i <= last
-                    const int last = !used || (who >> (rt * tpt + tc)) & 1 ? limit[rt] : -1;
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[kt][i] *= p.scale2;
+                if (p.n_buckets) {
+                    const int pos = offset + t0, near = buckets.at(pos - now - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - now);
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[rt][kt][i] *= p.scale2;
-                    if (p.n_buckets) {
-                        const int pos = offset + t0 + rt * tpt, near = buckets.at(pos - now - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - now);
-                        const int mine = c - tc * p.group;
-                        if (near == far) {
-                            const float x = buckets.value(near, mine);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) { s[rt][0][i] += x; s[rt][1][i] += x; }
-                        } else {
-#pragma unroll
-                            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) s[rt][kt][i] += buckets.value(buckets.at(pos + tc - (now + 16 * kt + 4 * g + i)), mine);
-                        }
-                    }
-                    unsigned mask = 0xff;
-                    if (!__all(now + kUnit - 1 <= last)) {
-                        mask = 0;
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const bool ok = now + 16 * kt + 4 * g + i <= last;
-                                s[rt][kt][i] = ok ? s[rt][kt][i] : -__builtin_inff();
-                                mask |= (unsigned)ok << (4 * kt + i);
-                            }
-                    }
-                    seen[rt] = mask;
-                    const f32x4 a = s[rt][0], e = s[rt][1];
-                    float top = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
-                    top = fmaxf(m[rt], rows_max(top));
-                    const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
-                    if (__any(top != m[rt])) {
-                        const float shrink = __builtin_amdgcn_exp2f(m[rt] - ref);
-                        l[rt] *= shrink;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
-                        m[rt] = top;
-                    }
-                    f32x4 x, y;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { x[i] = __builtin_amdgcn_exp2f(a[i] - ref); y[i] = __builtin_amdgcn_exp2f(e[i] - ref); }
-                    l[rt] += ((x[0] + x[1]) + (x[2] + x[3])) + ((y[0] + y[1]) + (y[2] + y[3]));
-                    // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not
-                    pf[rt] = pack<T>(x, y);
+                        for (int i = 0; i < 4; ++i)
+                            s[kt][i] += buckets.value(near == far ? near : buckets.at(pos + tc - (now + 16 * kt + 4 * g + i)), mine);
                 }
-                if (!careful && active == (1u << RT) - 1) {
+                unsigned seen = 0xff;
+                if (!__all(now + kUnit - 1 <= last)) {
+                    seen = 0;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
+                    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mma(vf, pf[rt], o[rt][dt]);
-                    }
-                } else {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if (!(active & (1u << rt))) continue;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
-                            if constexpr (decltype(careful)::value) o[rt][dt] = mma_masked<T>(vf, pf[rt], seen[rt], o[rt][dt]);
-                            else o[rt][dt] = mma(vf, pf[rt], o[rt][dt]);
+                        for (int i = 0; i < 4; ++i) {
+                            const bool ok = now + 16 * kt + 4 * g + i <= last;
+                            s[kt][i] = ok ? s[kt][i] : -__builtin_inff();
+                            seen |= (unsigned)ok << (4 * kt + i);
                         }
-                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                top = fmaxf(m, rows_max(top));
+                const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
+                if (__any(top != m)) {
+                    const float shrink = __builtin_amdgcn_exp2f(m - ref);
+                    l *= shrink;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[dt] *= shrink;
+                    m = top;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { s[0][i] = __builtin_amdgcn_exp2f(s[0][i] - ref); s[1][i] = __builtin_amdgcn_exp2f(s[1][i] - ref); }
+                l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+                // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not
+                const V8<T> pf = pack<T>(s[0], s[1]);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
+                    if constexpr (decltype(careful)::value) o[dt] = mma_masked<T>(vf, pf, seen, o[dt]);
+                    else o[dt] = mma(vf, pf, o[dt]);
                 }
             }
         }
     };
-    sweep(std::false_type{});
-    bool odd = false;
+    if constexpr (CAREFUL) {
+        sweep(std::true_type{});
+    } else {
+        sweep(std::false_type{});
+        bool odd = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(o[rt][dt]);
-    if (__syncthreads_or(odd)) sweep(std::true_type{});
+        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(o[dt]);
+        if (__syncthreads_or(odd)) sweep(std::true_type{});
+    }
 
     // the four wavefronts' sums, joined a strip of 32 columns at a time
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] = rows_sum(l[rt]);
-        if (g == 0) stats[wave][rt * 16 + c] = make_float2(m[rt], l[rt]);
-    }
+    l = rows_sum(l);
+    __syncthreads();                   // the joining buffer of the tile before has been read
+    if (g == 0) shared.stats[wave][c] = make_float2(m, l);
     __syncthreads();
+    float top = -__builtin_inff(), total = 0.f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        float top = -__builtin_inff(), total = 0.f;
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, shared.stats[w][c].x);
+    const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][rt * 16 + c].x);
-        const float ref = top == -__builtin_inff() ? 0.f : top;
+    for (int w = 0; w < kWaves; ++w) total += shared.stats[w][c].y * __builtin_amdgcn_exp2f(shared.stats[w][c].x - ref);
+    const float share = __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) total += stats[w][rt * 16 + c].y * __builtin_amdgcn_exp2f(stats[w][rt * 16 + c].x - ref);
-        const float share = __builtin_amdgcn_exp2f(m[rt] - ref);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= share;
-        if (wave == 0 && g == 0) joined[rt * 16 + c] = make_float2(top, total);
-    }
+    for (int dt = 0; dt < DT; ++dt) o[dt] *= share;
+    if (wave == 0 && g == 0) shared.joined[c] = make_float2(top, total);
     float *merge = reinterpret_cast<float *>(dynamic);
     const int64_t all_rows = (int64_t)p.batch * p.queries * p.heads;
 #pragma unroll
     for (int strip = 0; strip < DC; ++strip) {
         __syncthreads();               // the values' staging, or the strip before, has been read
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                *reinterpret_cast<f32x4 *>(merge + ((wave * RT + rt) * 16 + c) * kMergeStride + 16 * j + 4 * g) = o[rt][2 * strip + j];
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(merge + (wave * 16 + c) * kMergeStride + 16 * j + 4 * g) = o[2 * strip + j];
         __syncthreads();
-        for (int e = tid; e < RT * 16 * 8; e += kThreads) {
-            const int row = e >> 3, col = (e & 7) * 4, rc = row & 15, rtc = rc / p.group, t = t0 + (row >> 4) * tpt + rtc;
-            if (rtc >= tpt || t >= p.queries) continue;
+        const int row = tid >> 3, col = (tid & 7) * 4, rt = row / p.group, t = t0 + rt;
+        if (tid < 16 * 8 && rt < tpt && t < p.queries) {
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4 *>(merge + (w * RT * 16 + row) * kMergeStride + col);
-            const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (rc - rtc * p.group);
-            const float2 st = joined[row];
+            for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4 *>(merge + (w * 16 + row) * kMergeStride + col);
+            const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (row - rt * p.group);
+            const float2 st = shared.joined[row];
             if (splits == 1) {
                 const float inv = st.y == 0.f ? 0.f : 1.f / st.y;
-                T *dst = out + at * D + strip * 32 + col;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dst[i] = (T)(sum[i] * inv);
-                if (remainder)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) remainder[at * D + strip * 32 + col + i] = (T)(sum[i] * inv - (float)(T)(sum[i] * inv));
-                if (strip == 0 && col == 0 && lse) lse[at] = st.y == 0.f ? __builtin_inff() : st.x + __builtin_amdgcn_logf(st.y);
+                store_row<T>(static_cast<T *>(r.out), static_cast<T *>(r.rest), at * D + strip * 32 + col, sum * inv);
+                if (strip == 0 && col == 0 && r.lse) r.lse[at] = st.y == 0.f ? __builtin_inff() : st.x + __builtin_amdgcn_logf(st.y);
             } else {
-                *reinterpret_cast<f32x4 *>(part + (split * all_rows + at) * D + strip * 32 + col) = sum;
-                if (strip == 0 && col == 0) part_stats[split * all_rows + at] = st;
+                *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + strip * 32 + col) = sum;
+                if (strip == 0 && col == 0) r.part_stats[split * all_rows + at] = st;
             }
         }
     }
 }
 
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void few_kernel(const Problem p, const Results r, int n_tiles, int splits) {
+    __shared__ FewShared shared;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int unit = xcd_contiguous_block(), pair = unit / (n_tiles * splits), rest = unit - pair * n_tiles * splits, tile = rest / splits;
+    const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    Buckets buckets;
+    if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + few_stage_bytes<T, D>());
+    few_rows<T, D, false>(p, r, shared, dynamic, buckets, b, h, tile, rest - tile * splits, splits);
+}
+
+// ---- many queries -----------------------------------------------------------------------------------------
+
+constexpr int kStep = 64;              // keys in LDS
+constexpr int kListed = 512;           // blocks listed at a time
+
+template <typename T, int D> struct Steps {
+    static constexpr int kKeyStride = D + 16 / sizeof(T), kValueStride = D + kPad;
+    static constexpr size_t kBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+};
+
+// RT tiles of 16 rows per wavefront.  flags[workgroup]: whether a result was not finite (see redo_kernel).
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, const Results r, int32_t *flags, int n_groups) {
+    constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;
+    constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = kThreads / CPR, NL = kStep / RPL;
+    constexpr int KS = Steps<T, D>::kKeyStride, VS = Steps<T, D>::kValueStride;
+    __shared__ List<TILES, kListed> list;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int unit = xcd_contiguous_block(), pair = unit / n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
+    const int tpt = tile_tokens(p.group), t0 = (unit - pair * n_groups) * TILES * tpt;
+    const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
+    const bool used = tc < tpt;
+
+    T *keys = reinterpret_cast<T *>(dynamic), *values = keys + kStep * KS;
+    Buckets buckets;
+    if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + Steps<T, D>::kBytes);
+
+    // scores are compared before they are scaled: a negative scale turns the queries' signs instead
+    const float factor = p.n_buckets ? 1.f : fabsf(p.scale2);
+    V8<T> qf[RT][DC];
+    int limit[RT];                     // last key that the lane's row may see; columns without a row see everything, nothing is written of them
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int t = t0 + (wave * RT + rt) * tpt + tc;
+        const bool there = used && t < q_len;
+        limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
+        const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+            qf[rt][dc] = there ? load8(src + dc * 32) : zero8<T>();
+            if (!p.n_buckets && p.scale2 < 0.f) qf[rt][dc] = -qf[rt][dc];
+        }
+    }
+    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
+    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + (tid % CPR) * EPC;
+    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + (tid % CPR) * EPC;
+    const int sub_shift = p.block_shift - 5;
+
+    // The sum that divides the output is that of the rounded powers, which are the weights of the product (a product with ones makes it):
+    // a row that one key dominates keeps that key's value to the last bit.  lse is the logarithm of the powers' own sum.
+    f32x4 o[RT][DT], total[RT];
+    float m[RT], l[RT];
+    V8<T> ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -__builtin_inff(); l[rt] = 0.f;
+        total[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int first = 0; first < p.blocks; first += kListed) {
+        const int units = build_list(list, p, b, h, t0, q_len, k_len, first, min(kListed, p.blocks - first)) << sub_shift;
+        // a step is two units of 32 keys, of one block or (blocks of 32) of two
+        auto first_key = [&](int u) {
+            return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
+        };
+        u32x4 kr[NL], vr[NL];
+        auto fetch = [&](int u) {
+            const int k0 = first_key(u), k1 = u + 1 < units ? first_key(u + 1) : k0;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = i * RPL + tid / CPR;
+                // rows behind the last key read it again: what a padded cache holds there is never touched
+                const int64_t key = min((row < kUnit ? k0 : k1 - kUnit) + row, k_len - 1);
+                kr[i] = *reinterpret_cast<const u32x4 *>(kbase + key * p.ks.row);
+                vr[i] = *reinterpret_cast<const u32x4 *>(vbase + key * p.vs.row);
+            }
+        };
+        if (units) fetch(0);
+        for (int u = 0; u < units; u += 2) {
+            __syncthreads();           // the step before has been read
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = i * RPL + tid / CPR;
+                *reinterpret_cast<u32x4 *>(keys + row * KS + (tid % CPR) * EPC) = kr[i];
+                *reinterpret_cast<u32x4 *>(values + row * VS + (tid % CPR) * EPC) = vr[i];
+            }
+            __syncthreads();
+            int key0[2];
+            unsigned who[2][RT], active = 0;         // tokens of the wavefront's tiles that selected the unit's block
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const bool there = u + x < units;
+                key0[x] = there ? first_key(u + x) : 0;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int tile = wave * RT + rt;
+                    const unsigned bits = there && key0[x] <= last_key ? (unsigned)(list.bits[(u + x) >> sub_shift][tile >> 2] >> ((tile & 3) * 16)) & 0xffffu : 0u;
+                    who[x][rt] = __builtin_amdgcn_readfirstlane(bits);
+                    active |= who[x][rt] ? 1u << rt : 0u;
+                }
+            }
+            if (u + 2 < units) fetch(u + 2);
+            // the wavefront's tiles in SET, those with a token that selected one of the step's blocks
+            auto work = [&](auto set) {
+                constexpr unsigned SET = decltype(set)::value;
+                f32x4 s[RT][4];
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) {
+                        const V8<T> kf = load8(keys + (kt * 16 + c) * KS + dc * 32 + 8 * g);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            if (SET >> rt & 1) s[rt][kt] = mma(kf, qf[rt][dc], s[rt][kt]);
+                    }
+                }
+                V8<T> pf[RT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (!(SET >> rt & 1)) continue;
+                    bool sel[2];
+                    int last[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        sel[x] = !used || (who[x][rt] >> tc) & 1;
+                        last[x] = sel[x] ? limit[rt] : -1;
+                    }
+                    if (p.n_buckets) {
+                        const int pos = offset + t0 + (wave * RT + rt) * tpt;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int near = buckets.at(pos - key0[x] - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - key0[x]);
+                            if (near == far) {
+                                const float y = buckets.value(near, mine);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) { s[rt][2 * x][i] = s[rt][2 * x][i] * p.scale2 + y; s[rt][2 * x + 1][i] = s[rt][2 * x + 1][i] * p.scale2 + y; }
+                            } else {
+#pragma unroll
+                                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        s[rt][2 * x + kt][i] = s[rt][2 * x + kt][i] * p.scale2 + buckets.value(buckets.at(pos + tc - (key0[x] + 16 * kt + 4 * g + i)), mine);
+                            }
+                        }
+                    }
+                    // a row that did not select a block has its powers taken from +inf: 0, whatever finite scores it has there.  Only keys
+                    // behind a row that did are masked one by one.
+                    const bool edge = (sel[0] && key0[0] + kUnit - 1 > limit[rt]) || (sel[1] && key0[1] + kUnit - 1 > limit[rt]);
+                    if (__any(edge)) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    s[rt][2 * x + kt][i] = key0[x] + 16 * kt + 4 * g + i <= last[x] ? s[rt][2 * x + kt][i] : -__builtin_inff();
+                    }
+                    float top[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const f32x4 a = s[rt][2 * x], e = s[rt][2 * x + 1];
+                        top[x] = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
+                        top[x] = sel[x] ? top[x] : -__builtin_inff();
+                    }
+                    const float high = rows_max(fmaxf(top[0], top[1])) * factor;
+                    // sums are kept relative to a reference that follows the maximum when it has moved by more than 2^8
+                    if (__any(high > m[rt] + 8.f)) {
+                        const float up = fmaxf(m[rt], high), from = up == -__builtin_inff() ? 0.f : up;
+                        const float shrink = __builtin_amdgcn_exp2f(m[rt] - from);
+                        l[rt] *= shrink;
+                        total[rt] *= shrink;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
+                        m[rt] = up;
+                    }
+                    const float ref = m[rt] == -__builtin_inff() ? 0.f : m[rt];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float from = sel[x] ? ref : __builtin_inff();
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[rt][2 * x + kt][i] = __builtin_amdgcn_exp2f(s[rt][2 * x + kt][i] * factor - from);
+                        if (r.lse) {
+                            const f32x4 a = s[rt][2 * x] + s[rt][2 * x + 1];
+                            l[rt] += (a[0] + a[1]) + (a[2] + a[3]);
+                        }
+                        // rounded to the operands' type for the product with V, half a step each
+                        pf[rt][x] = pack<T>(s[rt][2 * x], s[rt][2 * x + 1]);
+                        total[rt] = mma(ones, pf[rt][x], total[rt]);
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const V8<T> vf = transposed<T, D>(values + x * kUnit * VS, dt * 16, lane);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            if (SET >> rt & 1) o[rt][dt] = mma(vf, pf[rt][x], o[rt][dt]);
+                    }
+            };
+            if (RT == 1) {
+                if (active) work(std::integral_constant<unsigned, 1>{});
+            } else {
+                if (active == 3) work(std::integral_constant<unsigned, 3>{});
+                else if (active == 1) work(std::integral_constant<unsigned, 1>{});
+                else if (active == 2) work(std::integral_constant<unsigned, 2>{});
+            }
+        }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float inv = total[rt][0] == 0.f ? 0.f : 1.f / total[rt][0], sum = rows_sum(l[rt]);
+        const int t = t0 + (wave * RT + rt) * tpt + tc;
+        const int64_t at = ((int64_t)b * p.queries + t) * p.heads + head;
+        const bool write = used && t < p.queries;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            odd |= not_finite(o[rt][dt]);
+            if (write) store_row<T>(static_cast<T *>(r.out), static_cast<T *>(r.rest), at * D + dt * 16 + 4 * g, o[rt][dt] * inv);
+        }
+        if (write && g == 0 && r.lse) r.lse[at] = sum == 0.f ? __builtin_inff() : m[rt] + __builtin_amdgcn_logf(sum);
+    }
+    odd = __syncthreads_or(odd);
+    if (tid == 0) flags[unit] = odd;
+}
+
+// The tiles of many_kernel's workgroups with a result that was not finite, again.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void redo_kernel(const Problem p, const Results r, const int32_t *flags, int n_groups, int tiles) {
+    __shared__ FewShared shared;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int unit = xcd_contiguous_block();
+    if (!flags[unit]) return;
+    const int pair = unit / n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads, first = (unit - pair * n_groups) * tiles;
+    Buckets buckets;
+    if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + few_stage_bytes<T, D>());
+    for (int i = 0; i < tiles; ++i) few_rows<T, D, true>(p, r, shared, dynamic, buckets, b, h, first + i, 0, 1);
+}
+
 // Joins the sums of several workgroups per row: four columns a thread.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void block_attention_join_kernel(const float *part, const float2 *part_stats, T *out, T *remainder, float *lse, int64_t rows, int splits) {
+__global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const float2 *part_stats, T *out, T *remainder, float *lse, int64_t rows, int splits) {
     const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = e / (D / 4);
     const int col = (int)(e - row * (D / 4)) * 4;
     if (row >= rows) return;
@@ -288,66 +492,58 @@ __global__ __launch_bounds__(kThreads) void block_attention_join_kernel(const fl
         sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * D + col) * share;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[row * D + col + i] = (T)(sum[i] * inv);
-    if (remainder)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) remainder[row * D + col + i] = (T)(sum[i] * inv - (float)(T)(sum[i] * inv));
+    store_row<T>(out, remainder, row * D + col, sum * inv);
     if (col == 0 && lse) lse[row] = total == 0.f ? __builtin_inff() : top + __builtin_amdgcn_logf(total);
 }
 
-// How many tiles of 16 rows a workgroup takes, and over how many workgroups a tile's list is dealt out.
-struct Shape { int rt, n_tiles, splits; };
-Shape shape_of(const Problem &p, int max_rt) {
+// Which kernel takes a call, and how its work is cut.
+struct Shape { bool many; int n_tiles, splits; };
+template <int RT> Shape shape_of(const Problem &p) {
     const int tpt = tile_tokens(p.group);
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
-    Shape s{max_rt, 0, 1};
-    auto tiles = [&](int rt) { return (p.queries + rt * tpt - 1) / (rt * tpt); };
-    while (s.rt > 1 && pairs * tiles(s.rt) < 512) s.rt /= 2;
-    s.n_tiles = tiles(s.rt);
-    const int64_t groups = pairs * s.n_tiles;
+    auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
+    Shape s{true, tiles(kWaves * RT), 1};
+    if (pairs * s.n_tiles >= 256) return s;
+    s = Shape{false, tiles(1), 1};
+    const int64_t groups = std::max<int64_t>(pairs * s.n_tiles, 1);
     // units of a list at most; every wavefront keeps two of them
-    const int64_t named = std::min<int64_t>((int64_t)p.topk * std::min(s.rt * tpt, p.queries), p.blocks);
+    const int64_t named = std::min<int64_t>((int64_t)p.topk * std::min(tpt, p.queries), p.blocks);
     const int64_t units = named << (p.block_shift - 5);
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / std::max<int64_t>(groups, 1), units / (2 * kWaves)));
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / groups, units / (2 * kWaves)));
     return s;
 }
 
 size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-template <typename T, int D, int RT>
-int launch_rt(const Problem &p, const Shape &s, T *out, T *rest, float *lse, float *part, float2 *part_stats, hipStream_t stream) {
-    const size_t lds = stage_bytes<T, D, RT>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);
-    const int64_t grid = (int64_t)p.batch * p.kv_heads * s.n_tiles * s.splits;
-    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "block attention: %lld workgroups do not fit a launch", (long long)grid);
-    block_attention_kernel<T, D, RT><<<dim3((unsigned)grid), dim3(kThreads), lds, stream>>>(p, out, rest, lse, part, part_stats, s.n_tiles, s.splits);
-    FG_HIP_TRY(hipGetLastError());
-    return FG_OK;
-}
-
-template <typename T, int D> constexpr int max_row_tiles() { return sizeof(T) == 4 ? 2 : 4; }
-
 template <typename T, int D>
 int launch(const Problem &p, const fg_block_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
-    const Shape s = shape_of(p, max_row_tiles<T, D>());
+    constexpr int RT = sizeof(T) == 4 ? 1 : 2;
+    const Shape s = shape_of<RT>(p);
     const size_t rows = (size_t)p.batch * p.queries * p.heads;
+    const int64_t grid = (int64_t)p.batch * p.kv_heads * s.n_tiles * s.splits;
+    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "block attention: %lld workgroups do not fit a launch", (long long)grid);
+    const size_t flags = s.many ? round_up((size_t)grid * sizeof(int32_t)) : 0;
     const size_t sums = s.splits > 1 ? round_up(rows * s.splits * D * sizeof(float)) : 0, stats = s.splits > 1 ? round_up(rows * s.splits * sizeof(float2)) : 0;
-    if (need) { *need = sums + stats; return FG_OK; }
-    if (bytes < sums + stats || (sums && !workspace)) return fail(FG_ERR_ARG, "block attention: a workspace of %zu bytes, %zu needed (fg_block_attention_workspace)", bytes, sums + stats);
-    float *part = static_cast<float *>(workspace);
-    float2 *part_stats = reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + sums);
-    T *out = static_cast<T *>(a->out), *rest = static_cast<T *>(a->rest);
-    int rc;
-    if constexpr (max_row_tiles<T, D>() == 4) {
-        rc = s.rt == 4 ? launch_rt<T, D, 4>(p, s, out, rest, a->lse, part, part_stats, stream)
-           : s.rt == 2 ? launch_rt<T, D, 2>(p, s, out, rest, a->lse, part, part_stats, stream)
-                       : launch_rt<T, D, 1>(p, s, out, rest, a->lse, part, part_stats, stream);
+    if (need) { *need = flags + sums + stats; return FG_OK; }
+    if (bytes < flags + sums + stats || (flags + sums && !workspace))
+        return fail(FG_ERR_ARG, "block attention: a workspace of %zu bytes, %zu needed (fg_block_attention_workspace)", bytes, flags + sums + stats);
+    unsigned char *w = static_cast<unsigned char *>(workspace);
+    const Results r{a->out, a->rest, a->lse, reinterpret_cast<float *>(w), reinterpret_cast<float2 *>(w + sums)};
+    const size_t bias = buckets_bytes(p.n_buckets, p.low, p.high, p.group);
+    const dim3 blocks((unsigned)grid), threads(kThreads);
+    if (s.many) {
+        int32_t *marks = reinterpret_cast<int32_t *>(w);
+        many_kernel<T, D, RT><<<blocks, threads, Steps<T, D>::kBytes + bias, stream>>>(p, r, marks, s.n_tiles);
+        FG_HIP_TRY(hipGetLastError());
+        redo_kernel<T, D><<<blocks, threads, few_stage_bytes<T, D>() + bias, stream>>>(p, r, marks, s.n_tiles, kWaves * RT);
     } else {
-        rc = s.rt == 2 ? launch_rt<T, D, 2>(p, s, out, rest, a->lse, part, part_stats, stream) : launch_rt<T, D, 1>(p, s, out, rest, a->lse, part, part_stats, stream);
+        few_kernel<T, D><<<blocks, threads, few_stage_bytes<T, D>() + bias, stream>>>(p, r, s.n_tiles, s.splits);
     }
-    if (rc != FG_OK || s.splits == 1) return rc;
-    const int64_t threads = (int64_t)rows * (D / 4);
-    block_attention_join_kernel<T, D><<<dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream>>>(part, part_stats, out, rest, a->lse, (int64_t)rows, s.splits);
+    FG_HIP_TRY(hipGetLastError());
+    if (s.splits == 1) return FG_OK;
+    const int64_t each = (int64_t)rows * (D / 4);
+    join_kernel<T, D><<<dim3((unsigned)((each + kThreads - 1) / kThreads)), threads, 0, stream>>>(
+        r.part, r.part_stats, static_cast<T *>(r.out), static_cast<T *>(r.rest), r.lse, (int64_t)rows, s.splits);
     FG_HIP_TRY(hipGetLastError());
     return FG_OK;
 }

@@ -17,6 +17,7 @@ namespace block {
 namespace {
 
 constexpr int kMergeStride = 36;       // floats between rows of the joining buffer (32 and 4 of padding)
+constexpr int kWindow = 1024;          // blocks looked at together
 constexpr int kPieceRows = 2048;       // rows (tokens times heads of the group) of one piece of a block's list
 
 struct Piece { int32_t block, start, len, slot; };     // block: of all sequences and key heads; slot: where its sums go, -1: they are all
@@ -126,78 +127,122 @@ __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long
 
 // ---- by query: dQ, dbias and delta ------------------------------------------------------------------------
 
-template <typename T, int D, int RT> constexpr size_t queries_stage_bytes() {
-    const size_t keys = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * RT * 16 * kMergeStride * sizeof(float);
+struct Step { const void *dout, *out, *rest; Strides ds; const float *lse; float *delta; void *dq; float *bias_sums; };
+
+// A lane's row of a tile: dO and Q as operands, and delta.
+template <typename T, int D> struct Row16 {
+    V8<T> q[D / 32], d[D / 32];
+    float lse, delta;
+    int limit;                         // last key that it may see; columns without a row see everything, nothing is written of them
+    __device__ __forceinline__ void load(const Problem &p, const Step &w, int b, int t, int head, bool used, int q_len, int k_len, int offset, int g, bool write) {
+        const bool there = used && t < q_len;
+        limit = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
+        const int64_t at = ((int64_t)b * p.queries + t) * p.heads + head;
+        const T *qs = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
+        const T *dos = static_cast<const T *>(w.dout) + b * w.ds.batch + (int64_t)t * w.ds.row + head * w.ds.head + 8 * g;
+        const T *os = static_cast<const T *>(w.out) + at * D + 8 * g, *rs = static_cast<const T *>(w.rest) + at * D + 8 * g;
+        float sum = 0.f;
+#pragma unroll
+        for (int dc = 0; dc < D / 32; ++dc) {
+            q[dc] = there ? load8(qs + dc * 32) : zero8<T>();
+            d[dc] = there ? load8(dos + dc * 32) : zero8<T>();
+            const V8<T> o = there ? load8(os + dc * 32) : zero8<T>();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)o[i];
+            if (w.rest) {
+                const V8<T> r = there ? load8(rs + dc * 32) : zero8<T>();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)r[i];
+            }
+        }
+        delta = rows_sum(sum);
+        lse = there ? w.lse[at] : __builtin_inff();
+        if (there && write && g == 0) w.delta[at] = delta;
+    }
+};
+
+// The bias's gradient is summed in LDS, [wavefront][bucket][lane]: all rows of a lane have one head, and no two lanes a place.
+__device__ __forceinline__ float *bias_place(const Problem &p, unsigned char *lds) {
+    return reinterpret_cast<float *>(lds + ((buckets_bytes(p.n_buckets, p.low, p.high, p.group) + 15) & ~(size_t)15));
+}
+size_t bias_bytes(const Problem &p) {
+    return p.n_buckets ? ((buckets_bytes(p.n_buckets, p.low, p.high, p.group) + 15) & ~(size_t)15) + (size_t)kWaves * p.n_buckets * 64 * sizeof(float) : 0;
+}
+// A workgroup's share of it, [workgroup of all sequences][head][bucket].
+__device__ __forceinline__ void write_bias(const Problem &p, const float *sums, float *out, int64_t workgroup, int h) {
+    const int tpt = tile_tokens(p.group);
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.n_buckets * p.group; e += kThreads) {
+        const int x = e / p.n_buckets, n = e - x * p.n_buckets;
+        float total = 0.f;
+        for (int w = 0; w < kWaves; ++w)
+            for (int t = 0; t < tpt; ++t)
+                for (int q = 0; q < 4; ++q) total += sums[(w * p.n_buckets + n) * 64 + q * 16 + t * p.group + x];
+        out[(workgroup * p.heads + h * p.group + x) * p.n_buckets + n] = total;
+    }
+}
+
+// Powers p = 2^(z - lse), and from them dS = p (dP - delta), of one tile and 32 keys, into s[]: where `edge`, keys behind `last` have none.
+// The bias's gradient goes to `sums`.
+template <bool MASK>
+__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float delta, int pos, int tpt,
+                                                    int tc, int mine, int key0, int last, int g, int lane) {
+    const int near = p.n_buckets ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = p.n_buckets ? buckets.at(pos + tpt - 1 - key0) : 0;
+    const float common = p.n_buckets && near == far ? buckets.value(near, mine) : 0.f;
+    unsigned seen = MASK ? 0 : 0xff;
+    float total = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 16 * kt + 4 * g + i;
+            float z = s[kt][i] * p.scale2 + (common - lse);
+            int bucket = 0;
+            if (near != far) {
+                bucket = buckets.at(pos + tc - key);
+                z += buckets.value(bucket, mine);
+            }
+            float x = __builtin_amdgcn_exp2f(z) * (dp[kt][i] - delta);
+            if (MASK) {
+                x = key <= last ? x : 0.f;
+                seen |= (unsigned)(key <= last) << (4 * kt + i);
+            }
+            s[kt][i] = x;
+            if (near != far) sums[bucket * 64 + lane] += x;
+            else total += x;
+        }
+    if (p.n_buckets && near == far) sums[near * 64 + lane] += total;
+    return seen;
+}
+
+template <typename T, int D> constexpr size_t few_stage_bytes() {
+    const size_t keys = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
     return keys > merge ? keys : merge;
 }
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kThreads) void queries_kernel(const Problem p, const T *dout, Strides ds, const T *out, const T *remainder, const float *lse, float *delta,
-                                                           T *dq, float *bias_sums, int n_tiles) {
+// One tile of 16 rows, its list dealt out to the four wavefronts, as few_kernel does forward.
+template <typename T, int D, bool CAREFUL>
+__device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1, kWindow> &list, unsigned char *dynamic, const Buckets &buckets, float *sums, int b, int h, int tile) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad;
-    __shared__ List list;
-    extern __shared__ __align__(16) unsigned char dynamic[];
-
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const int unit = xcd_contiguous_block(), pair = unit / n_tiles, tile = unit - pair * n_tiles;
-    const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
-    const int tpt = tile_tokens(p.group), t0 = tile * RT * tpt, nt = RT * tpt;
+    const int tpt = tile_tokens(p.group), t0 = tile * tpt;
     const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
     const bool used = tc < tpt;
-
     T *stage = reinterpret_cast<T *>(dynamic) + wave * kUnit * S;
-    Buckets buckets;
-    float *sums = nullptr;             // [bucket][lane] of this wavefront: a lane's rows all have one head
-    if (p.n_buckets) {
-        unsigned char *at = dynamic + queries_stage_bytes<T, D, RT>();
-        buckets = load_buckets<T>(p, h, at);
-        sums = reinterpret_cast<float *>(at + ((buckets_bytes(p.n_buckets, p.low, p.high, p.group) + 15) & ~(size_t)15)) + wave * p.n_buckets * 64;
-    }
-
-    V8<T> qf[RT][DC], df[RT][DC];
-    int limit[RT];
-    float row_lse[RT], row_delta[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int t = t0 + rt * tpt + tc;
-        const bool there = used && t < q_len;
-        limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
-        const int64_t at = ((int64_t)b * p.queries + t) * p.heads + head;
-        const T *qs = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
-        const T *dos = dout + b * ds.batch + (int64_t)t * ds.row + head * ds.head + 8 * g, *os = out + at * D + 8 * g;
-        float sum = 0.f;
-#pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-            qf[rt][dc] = there ? load8(qs + dc * 32) : zero8<T>();
-            df[rt][dc] = there ? load8(dos + dc * 32) : zero8<T>();
-            const V8<T> o = there ? load8(os + dc * 32) : zero8<T>();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += (float)df[rt][dc][i] * (float)o[i];
-            if (remainder) {
-                const V8<T> r = there ? load8(remainder + at * D + 8 * g + dc * 32) : zero8<T>();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += (float)df[rt][dc][i] * (float)r[i];
-            }
-        }
-        row_delta[rt] = rows_sum(sum);
-        row_lse[rt] = there ? lse[at] : __builtin_inff();
-        if (there && wave == 0 && g == 0) delta[at] = row_delta[rt];
-    }
-    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + nt, q_len) - 1) : k_len - 1;
+    Row16<T, D> row;
+    row.load(p, w, b, t0 + tc, head, used, q_len, k_len, offset, g, wave == 0);
+    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + 8 * g;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + 8 * g;
     const int sub_shift = p.block_shift - 5;
 
-    f32x4 acc[RT][DT];
+    f32x4 acc[DT];
     auto sweep = [&](auto careful) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
+        for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int first = 0; first < p.blocks; first += kWindow) {
-            const int units = build_list(list, p, b, h, t0, nt, q_len, k_len, first, min(kWindow, p.blocks - first)) << sub_shift;
+            const int units = build_list(list, p, b, h, t0, q_len, k_len, first, min(kWindow, p.blocks - first)) << sub_shift;
             auto first_key = [&](int u) {
                 return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
             };
@@ -207,10 +252,10 @@ __global__ __launch_bounds__(kThreads) void queries_kernel(const Problem p, cons
             };
             V8<T> kf[2][DC], vf[2][DC];
             int key0 = 0;
-            unsigned long long bits = 0;
+            unsigned who = 0;
             auto fetch = [&](int u) {
                 key0 = first_key(u);
-                bits = uniform64(list.bits[u >> sub_shift]);
+                who = (unsigned)list.bits[u >> sub_shift][0];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
                     const int64_t key = min(key0 + kt * 16 + c, k_len - 1);
@@ -224,129 +269,254 @@ __global__ __launch_bounds__(kThreads) void queries_kernel(const Problem p, cons
             int u = find(wave);
             if (u < units) fetch(u);
             while (u < units) {
-                const int now = key0;
-                const unsigned long long who = bits;
+                const int now = key0, last = !used || (who >> tc) & 1 ? row.limit : -1;
                 wave_lds_sync();
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int dc = 0; dc < DC; ++dc) *reinterpret_cast<V8<T> *>(stage + (kt * 16 + c) * S + dc * 32 + 8 * g) = kf[kt][dc];
                 wave_lds_sync();
-                f32x4 s[RT][2], dp[RT][2];
-                unsigned active = 0;
+                f32x4 s[2], dp[2];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!((who >> (rt * tpt)) & ((1ull << tpt) - 1))) continue;
-                    active |= 1u << rt;
+                for (int kt = 0; kt < 2; ++kt) {
+                    s[kt] = dp[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int dc = 0; dc < DC; ++dc) {
-                            s[rt][kt] = mma(kf[kt][dc], qf[rt][dc], s[rt][kt]);
-                            dp[rt][kt] = mma(vf[kt][dc], df[rt][dc], dp[rt][kt]);
-                        }
+                    for (int dc = 0; dc < DC; ++dc) {
+                        s[kt] = mma(kf[kt][dc], row.q[dc], s[kt]);
+                        dp[kt] = mma(vf[kt][dc], row.d[dc], dp[kt]);
                     }
                 }
                 u = find(u + kWaves);
                 if (u < units) fetch(u);
-
-                V8<T> pf[RT];
-                unsigned seen[RT];
+                const unsigned seen = score_gradients<true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
+                // rounded to the operands' type for the product with K, half a step each
+                const V8<T> sf = pack<T>(s[0], s[1]);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!(active & (1u << rt))) continue;
-                    const int last = !used || (who >> (rt * tpt + tc)) & 1 ? limit[rt] : -1;
-                    const int pos = offset + t0 + rt * tpt;
-                    const int near = p.n_buckets ? buckets.at(pos - now - (kUnit - 1)) : 0, far = p.n_buckets ? buckets.at(pos + tpt - 1 - now) : 0;
-                    unsigned mask = 0;
-                    float total = 0.f;
-                    const float common = p.n_buckets && near == far ? buckets.value(near, mine) : 0.f;
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = now + 16 * kt + 4 * g + i;
-                            const bool ok = key <= last;
-                            float z = s[rt][kt][i] * p.scale2 + common;
-                            int bucket = 0;
-                            if (near != far) {
-                                bucket = buckets.at(pos + tc - key);
-                                z += buckets.value(bucket, mine);
-                            }
-                            const float x = __builtin_amdgcn_exp2f(z - row_lse[rt]) * (dp[rt][kt][i] - row_delta[rt]);
-                            s[rt][kt][i] = ok ? x : 0.f;
-                            mask |= (unsigned)ok << (4 * kt + i);
-                            if (near != far) sums[bucket * 64 + lane] += s[rt][kt][i];
-                            else total += s[rt][kt][i];
-                        }
-                    if (p.n_buckets && near == far) sums[near * 64 + lane] += total;
-                    seen[rt] = mask;
-                    // rounded to the operands' type for the product with K, half a step each
-                    pf[rt] = pack<T>(s[rt][0], s[rt][1]);
-                }
-                if (!careful && active == (1u << RT) - 1) {
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const V8<T> x = transposed<T, D>(stage, dt * 16, lane);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = mma(x, pf[rt], acc[rt][dt]);
-                    }
-                } else {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if (!(active & (1u << rt))) continue;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const V8<T> x = transposed<T, D>(stage, dt * 16, lane);
-                            if constexpr (decltype(careful)::value) acc[rt][dt] = mma_masked<T>(x, pf[rt], seen[rt], acc[rt][dt]);
-                            else acc[rt][dt] = mma(x, pf[rt], acc[rt][dt]);
-                        }
-                    }
+                for (int dt = 0; dt < DT; ++dt) {
+                    const V8<T> x = transposed<T, D>(stage, dt * 16, lane);
+                    if constexpr (decltype(careful)::value) acc[dt] = mma_masked<T>(x, sf, seen, acc[dt]);
+                    else acc[dt] = mma(x, sf, acc[dt]);
                 }
             }
         }
     };
-    sweep(std::false_type{});
-    bool odd = false;
+    if constexpr (CAREFUL) {
+        sweep(std::true_type{});
+    } else {
+        sweep(std::false_type{});
+        bool odd = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(acc[rt][dt]);
-    if (__syncthreads_or(odd)) sweep(std::true_type{});
-
+        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(acc[dt]);
+        if (__syncthreads_or(odd)) {
+            for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
+            sweep(std::true_type{});
+        }
+    }
     float *merge = reinterpret_cast<float *>(dynamic);
 #pragma unroll
     for (int strip = 0; strip < DC; ++strip) {
         __syncthreads();               // the keys' staging, or the strip before, has been read
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                *reinterpret_cast<f32x4 *>(merge + ((wave * RT + rt) * 16 + c) * kMergeStride + 16 * j + 4 * g) = acc[rt][2 * strip + j];
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(merge + (wave * 16 + c) * kMergeStride + 16 * j + 4 * g) = acc[2 * strip + j];
         __syncthreads();
-        for (int e = tid; e < RT * 16 * 8; e += kThreads) {
-            const int row = e >> 3, col = (e & 7) * 4, rc = row & 15, rtc = rc / p.group, t = t0 + (row >> 4) * tpt + rtc;
-            if (rtc >= tpt || t >= p.queries) continue;
+        const int r = tid >> 3, col = (tid & 7) * 4, rt = r / p.group, t = t0 + rt;
+        if (tid < 16 * 8 && rt < tpt && t < p.queries) {
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4 *>(merge + (w * RT * 16 + row) * kMergeStride + col);
-            T *dst = dq + (((int64_t)b * p.queries + t) * p.heads + h * p.group + (rc - rtc * p.group)) * D + strip * 32 + col;
+            for (int x = 0; x < kWaves; ++x) sum += *reinterpret_cast<const f32x4 *>(merge + (x * 16 + r) * kMergeStride + col);
+            store_row<T>(static_cast<T *>(w.dq), nullptr, (((int64_t)b * p.queries + t) * p.heads + h * p.group + (r - rt * p.group)) * D + strip * 32 + col, sum * p.scale);
+        }
+    }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void queries_few_kernel(const Problem p, const Step w, int n_tiles) {
+    __shared__ List<1, kWindow> list;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int unit = xcd_contiguous_block(), pair = unit / n_tiles, tile = unit - pair * n_tiles, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    Buckets buckets;
+    float *sums = nullptr;
+    if (p.n_buckets) {
+        unsigned char *at = dynamic + few_stage_bytes<T, D>();
+        buckets = load_buckets<T>(p, h, at);
+        sums = bias_place(p, at);
+        for (int i = threadIdx.x; i < kWaves * p.n_buckets * 64; i += kThreads) sums[i] = 0.f;
+    }
+    few_rows<T, D, false>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, tile);
+    if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_tiles + tile, h);
+}
+
+constexpr int kStep = 64;              // keys in LDS
+constexpr int kListed = 512;           // blocks listed at a time
+
+template <typename T, int D> struct Steps {
+    static constexpr int kKeyStride = D + kPad, kValueStride = D + 16 / sizeof(T);
+    static constexpr size_t kBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+};
+
+// RT tiles of 16 rows per wavefront, the list walked by all four together, as many_kernel does forward.
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem p, const Step w, int32_t *flags, int n_groups) {
+    constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;
+    constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = kThreads / CPR, NL = kStep / RPL;
+    constexpr int KS = Steps<T, D>::kKeyStride, VS = Steps<T, D>::kValueStride;
+    __shared__ List<TILES, kListed> list;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int unit = xcd_contiguous_block(), pair = unit / n_groups, group = unit - pair * n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
+    const int tpt = tile_tokens(p.group), t0 = group * TILES * tpt;
+    const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
+    const bool used = tc < tpt;
+    T *keys = reinterpret_cast<T *>(dynamic), *values = keys + kStep * KS;
+    Buckets buckets;
+    float *sums = nullptr;
+    if (p.n_buckets) {
+        unsigned char *at = dynamic + Steps<T, D>::kBytes;
+        buckets = load_buckets<T>(p, h, at);
+        sums = bias_place(p, at) + wave * p.n_buckets * 64;
+        for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
+    }
+    Row16<T, D> row[RT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = (T)(sum[i] * p.scale);
+    for (int rt = 0; rt < RT; ++rt) row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
+    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
+    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + (tid % CPR) * EPC;
+    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + (tid % CPR) * EPC;
+    const int sub_shift = p.block_shift - 5;
+
+    f32x4 acc[RT][DT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < p.blocks; first += kListed) {
+        const int units = build_list(list, p, b, h, t0, q_len, k_len, first, min(kListed, p.blocks - first)) << sub_shift;
+        auto first_key = [&](int u) {
+            return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
+        };
+        u32x4 kr[NL], vr[NL];
+        auto fetch = [&](int u) {
+            const int k0 = first_key(u), k1 = u + 1 < units ? first_key(u + 1) : k0;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int r = i * RPL + tid / CPR;
+                const int64_t key = min((r < kUnit ? k0 : k1 - kUnit) + r, k_len - 1);
+                kr[i] = *reinterpret_cast<const u32x4 *>(kbase + key * p.ks.row);
+                vr[i] = *reinterpret_cast<const u32x4 *>(vbase + key * p.vs.row);
+            }
+        };
+        if (units) fetch(0);
+        for (int u0 = 0; u0 < units; u0 += 2) {
+            __syncthreads();           // the step before has been read
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int r = i * RPL + tid / CPR;
+                *reinterpret_cast<u32x4 *>(keys + r * KS + (tid % CPR) * EPC) = kr[i];
+                *reinterpret_cast<u32x4 *>(values + r * VS + (tid % CPR) * EPC) = vr[i];
+            }
+            __syncthreads();
+            if (u0 + 2 < units) fetch(u0 + 2);
+#pragma unroll 1
+            for (int u = u0; u < min(u0 + 2, units); ++u) {
+                const int key0 = first_key(u);
+                if (key0 > last_key) continue;
+                unsigned who[RT], active = 0;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int tile = wave * RT + rt;
+                    who[rt] = __builtin_amdgcn_readfirstlane((unsigned)(list.bits[u >> sub_shift][tile >> 2] >> ((tile & 3) * 16)) & 0xffffu);
+                    active |= who[rt] ? 1u << rt : 0u;
+                }
+                const T *ktile = keys + (u - u0) * kUnit * KS, *vtile = values + (u - u0) * kUnit * VS;
+                auto work = [&](auto set) {
+                    constexpr unsigned SET = decltype(set)::value;
+                    f32x4 s[RT][2], dp[RT][2];
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int dc = 0; dc < DC; ++dc) {
+                            const V8<T> kf = load8(ktile + (kt * 16 + c) * KS + dc * 32 + 8 * g), vf = load8(vtile + (kt * 16 + c) * VS + dc * 32 + 8 * g);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                if (SET >> rt & 1) {
+                                    s[rt][kt] = mma(kf, row[rt].q[dc], s[rt][kt]);
+                                    dp[rt][kt] = mma(vf, row[rt].d[dc], dp[rt][kt]);
+                                }
+                        }
+                    }
+                    V8<T> sf[RT];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if (!(SET >> rt & 1)) continue;
+                        // a row that did not select the block has its powers relative to +inf: 0
+                        const bool sel = !used || (who[rt] >> tc) & 1;
+                        const float lse = sel ? row[rt].lse : __builtin_inff();
+                        const int pos = offset + t0 + (wave * RT + rt) * tpt;
+                        if (__any(sel && key0 + kUnit - 1 > row[rt].limit))
+                            score_gradients<true>(p, buckets, sums, s[rt], dp[rt], lse, row[rt].delta, pos, tpt, tc, mine, key0, sel ? row[rt].limit : -1, g, lane);
+                        else
+                            score_gradients<false>(p, buckets, sums, s[rt], dp[rt], lse, row[rt].delta, pos, tpt, tc, mine, key0, 0, g, lane);
+                        // rounded to the operands' type for the product with K, half a step each
+                        sf[rt] = pack<T>(s[rt][0], s[rt][1]);
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const V8<T> x = transposed<T, D>(ktile, dt * 16, lane);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            if (SET >> rt & 1) acc[rt][dt] = mma(x, sf[rt], acc[rt][dt]);
+                    }
+                };
+                if (RT == 1) {
+                    if (active) work(std::integral_constant<unsigned, 1>{});
+                } else {
+                    if (active == 3) work(std::integral_constant<unsigned, 3>{});
+                    else if (active == 1) work(std::integral_constant<unsigned, 1>{});
+                    else if (active == 2) work(std::integral_constant<unsigned, 2>{});
+                }
+            }
         }
     }
-    if (p.n_buckets) {                 // the tile's share of the bias's gradient, [sequence and tile][head][bucket]
-        sums -= wave * p.n_buckets * 64;
-        for (int e = tid; e < p.n_buckets * p.group; e += kThreads) {
-            const int x = e / p.n_buckets, n = e - x * p.n_buckets;
-            float total = 0.f;
-            for (int w = 0; w < kWaves; ++w)
-                for (int t = 0; t < tpt; ++t)
-                    for (int q = 0; q < 4; ++q) total += sums[(w * p.n_buckets + n) * 64 + q * 16 + t * p.group + x];
-            bias_sums[(((int64_t)b * n_tiles + tile) * p.heads + h * p.group + x) * p.n_buckets + n] = total;
+    bool odd = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int t = t0 + (wave * RT + rt) * tpt + tc;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            odd |= not_finite(acc[rt][dt]);
+            if (used && t < p.queries)
+                store_row<T>(static_cast<T *>(w.dq), nullptr, (((int64_t)b * p.queries + t) * p.heads + head) * D + dt * 16 + 4 * g, acc[rt][dt] * p.scale);
         }
     }
+    if (p.n_buckets) write_bias(p, sums - wave * p.n_buckets * 64, w.bias_sums, (int64_t)b * n_groups + group, h);
+    odd = __syncthreads_or(odd);
+    if (tid == 0) flags[unit] = odd;
+}
+
+// The tiles of queries_many_kernel's workgroups with a result that was not finite, again.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void queries_redo_kernel(const Problem p, const Step w, const int32_t *flags, int n_groups, int tiles) {
+    __shared__ List<1, kWindow> list;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int unit = xcd_contiguous_block();
+    if (!flags[unit]) return;
+    const int pair = unit / n_groups, group = unit - pair * n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    Buckets buckets;
+    float *sums = nullptr;
+    if (p.n_buckets) {
+        unsigned char *at = dynamic + few_stage_bytes<T, D>();
+        buckets = load_buckets<T>(p, h, at);
+        sums = bias_place(p, at);
+        for (int i = threadIdx.x; i < kWaves * p.n_buckets * 64; i += kThreads) sums[i] = 0.f;
+    }
+    for (int i = 0; i < tiles; ++i) {
+        __syncthreads();               // the joining buffer of the tile before has been read
+        few_rows<T, D, true>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, group * tiles + i);
+    }
+    if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_groups + group, h);
 }
 
 // dbias[n, head]: the tiles' sums in order, a share of them for each group of threads, then the shares in order.
@@ -370,9 +540,10 @@ __global__ __launch_bounds__(1024) void bias_kernel(const float *sums, T *dbias,
 template <typename T, int D> constexpr size_t keys_stage_bytes() { return (size_t)kWaves * 2 * kUnit * (D + kPad) * sizeof(T); }
 
 // A wavefront has 32 keys; where a block has fewer than 4 x 32, several wavefronts share them and take the list's rows in turn.
-template <typename T, int D>
+// flags[workgroup]: whether a sum was not finite; CAREFUL: those again, with such places apart.
+template <typename T, int D, bool CAREFUL>
 __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
-                                                        const int32_t *totals, const int32_t *list, float *partial, T *dk, T *dv) {
+                                                        const int32_t *totals, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad;
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
@@ -380,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int block = 1 << p.block_shift, kw_n = min(kWaves, block / kUnit), rw_n = kWaves / kw_n, parts = block / (kw_n * kUnit);
     const int kw = wave % kw_n, rw = wave / kw_n, work = blockIdx.x / parts, part = blockIdx.x - work * parts;
-    if (work >= totals[0]) return;
+    if (work >= totals[0] || (CAREFUL && !flags[blockIdx.x])) return;
     const Piece piece = pieces[work];
     const int pair = piece.block / p.blocks, blk = piece.block - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
@@ -411,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     Row *own = rows[wave];
 
     f32x4 ak[2][DT], av[2][DT];
-    auto sweep = [&](auto careful) {
+    {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -499,7 +670,7 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
                 const V8<T> d = transposed<T, D>(stage_d, dt * 16, lane), q = transposed<T, D>(stage_q, dt * 16, lane);
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
-                    if constexpr (decltype(careful)::value) {
+                    if constexpr (CAREFUL) {
                         av[kt][dt] = mma_masked<T>(d, pf[kt], seen[kt], av[kt][dt]);
                         ak[kt][dt] = mma_masked<T>(q, sf[kt], seen[kt], ak[kt][dt]);
                     } else {
@@ -509,14 +680,16 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
                 }
             }
         }
-    };
-    sweep(std::false_type{});
+    }
     bool odd = false;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) odd |= not_finite(ak[kt][dt]) || not_finite(av[kt][dt]);
-    if (__any(odd)) sweep(std::true_type{});
+    if (!CAREFUL) {
+        odd = __syncthreads_or(odd);
+        if (tid == 0) flags[blockIdx.x] = odd;
+    }
 
     // wavefronts that share keys: the upper half hands its sums to the lower one, until one has them all
     f32x4 *merge = reinterpret_cast<f32x4 *>(dynamic);
@@ -558,40 +731,37 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     }
 }
 
-// Blocks whose lists were cut: the pieces' sums, in order.
+// Blocks whose lists were cut: the pieces' sums, in order, four columns of a key a thread.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void pieces_kernel(const Problem p, const int32_t *count, const int32_t *slot0, const float *partial, T *dk, T *dv, int piece) {
-    const int m = blockIdx.x, k = (count[m] + piece - 1) / piece;
+    const int block = 1 << p.block_shift, each = 2 * block * (D / 4) / kThreads;       // a multiple of kThreads: blocks of 32 and more, heads of 32 and more
+    const int m = blockIdx.x / each, k = (count[m] + piece - 1) / piece;
     if (k <= 1) return;
-    const int pair = m / p.blocks, blk = m - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads, block = 1 << p.block_shift;
-    const float *src = partial + (int64_t)slot0[m] * 2 * block * D;
-    for (int e = threadIdx.x; e < 2 * block * (D / 4); e += kThreads) {
-        const int row = e / (D / 4), col = (e - row * (D / 4)) * 4, key = (blk << p.block_shift) + (row & (block - 1));
-        if (key >= p.keys) continue;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < k; ++i) sum += *reinterpret_cast<const f32x4 *>(src + ((int64_t)i * 2 * block + row) * D + col);
-        T *dst = (row < block ? dk : dv) + (((int64_t)b * p.keys + key) * p.kv_heads + h) * D + col;
-        const float scale = row < block ? p.scale : 1.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = (T)(sum[i] * scale);
-    }
+    const int pair = m / p.blocks, blk = m - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int e = (blockIdx.x - m * each) * kThreads + threadIdx.x, row = e / (D / 4), col = (e - row * (D / 4)) * 4, key = (blk << p.block_shift) + (row & (block - 1));
+    if (key >= p.keys) return;
+    const float *src = partial + ((int64_t)slot0[m] * 2 * block + row) * D + col;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    each_piece(0, k, [&](int i) { return *reinterpret_cast<const f32x4 *>(src + (int64_t)i * 2 * block * D); }, [&](int, f32x4 v) { sum += v; });
+    store_row<T>(row < block ? dk : dv, nullptr, (((int64_t)b * p.keys + key) * p.kv_heads + h) * D + col, sum * (row < block ? p.scale : 1.f));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
 
 struct Layout {
-    int rt, n_tiles, chunks, piece;
+    bool many;
+    int n_groups, chunks, piece;               // n_groups: workgroups per sequence and key head of the sweep by query
     int64_t all, pieces, slots, entries;       // blocks of all sequences and key heads; bounds on the others
-    size_t delta, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
+    size_t delta, flags, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
 };
 
-int layout_of(const Problem &p, int head_len, int max_rt, Layout *l) {
-    const int tpt = tile_tokens(p.group);
+int layout_of(const Problem &p, int head_len, int row_tiles, Layout *l) {
+    const int tpt = tile_tokens(p.group), block = 1 << p.block_shift, parts = std::max(1, block / (kWaves * kUnit));
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
-    auto tiles = [&](int rt) { return (p.queries + rt * tpt - 1) / (rt * tpt); };
-    l->rt = max_rt;
-    while (l->rt > 1 && pairs * tiles(l->rt) < 512) l->rt /= 2;
-    l->n_tiles = tiles(l->rt);
+    auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
+    l->n_groups = tiles(kWaves * row_tiles);
+    l->many = pairs * l->n_groups >= 256;
+    if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
     l->piece = std::max(1, kPieceRows / p.group);
     l->all = pairs * p.blocks;
@@ -599,11 +769,12 @@ int layout_of(const Problem &p, int head_len, int max_rt, Layout *l) {
     l->pieces = l->all + l->entries / l->piece;
     l->slots = 2 * (l->entries / l->piece);
     const int64_t limit = INT32_MAX;
-    if (l->entries > limit || l->pieces * 2 > limit || pairs * std::max(l->n_tiles, l->chunks) > limit)
-        return fail(FG_ERR_SHAPE, "block attention gradients: %lld selections do not fit the 32-bit lists", (long long)l->entries);
+    if (l->entries > limit || l->pieces * parts > limit || l->all * (2 * block * head_len / 4 / kThreads) > limit || pairs * std::max(l->n_groups, l->chunks) > limit)
+        return fail(FG_ERR_SHAPE, "block attention gradients: %lld selections of %lld blocks do not fit the 32-bit lists", (long long)l->entries, (long long)l->all);
     size_t at = 0;
     auto place = [&](size_t n) { const size_t here = at; at += (n + 255) & ~(size_t)255; return here; };
     l->delta = place((size_t)p.batch * p.queries * p.heads * sizeof(float));
+    l->flags = place((size_t)std::max(pairs * l->n_groups, l->pieces * parts) * sizeof(int32_t));
     l->bits = place((size_t)l->all * l->chunks * 8);
     l->count = place((size_t)l->all * 4);
     l->offset = place((size_t)l->all * 4);
@@ -612,60 +783,61 @@ int layout_of(const Problem &p, int head_len, int max_rt, Layout *l) {
     l->totals = place(4);
     l->list = place((size_t)l->entries * 4);
     l->table = place((size_t)l->pieces * sizeof(Piece));
-    l->partial = place((size_t)l->slots * 2 * ((size_t)1 << p.block_shift) * head_len * sizeof(float));
-    l->bias = place((size_t)p.batch * l->n_tiles * p.heads * p.n_buckets * sizeof(float));
+    l->partial = place((size_t)l->slots * 2 * block * head_len * sizeof(float));
+    l->bias = place((size_t)p.batch * l->n_groups * p.heads * p.n_buckets * sizeof(float));
     l->bytes = at;
-    return FG_OK;
-}
-
-template <typename T, int D, int RT>
-int launch_queries(const Problem &p, const Layout &l, const fg_block_attention_args *a, const fg_block_attention_grads *grads, Strides ds, unsigned char *w, hipStream_t stream) {
-    size_t lds = queries_stage_bytes<T, D, RT>();
-    if (p.n_buckets) lds += ((buckets_bytes(p.n_buckets, p.low, p.high, p.group) + 15) & ~(size_t)15) + (size_t)kWaves * p.n_buckets * 64 * sizeof(float);
-    queries_kernel<T, D, RT><<<dim3((unsigned)(p.batch * p.kv_heads * l.n_tiles)), dim3(kThreads), lds, stream>>>(
-        p, static_cast<const T *>(grads->dout), ds, static_cast<const T *>(a->out), static_cast<const T *>(a->rest), a->lse, reinterpret_cast<float *>(w + l.delta),
-        static_cast<T *>(grads->dq), reinterpret_cast<float *>(w + l.bias), l.n_tiles);
-    FG_HIP_TRY(hipGetLastError());
     return FG_OK;
 }
 
 template <typename T, int D>
 int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_attention_grads *grads, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
+    constexpr int RT = sizeof(T) == 4 ? 1 : 2;
     Layout l;
-    if (int rc = layout_of(p, D, sizeof(T) == 4 || D == 128 ? 2 : 4, &l)) return rc;
+    if (int rc = layout_of(p, D, RT, &l)) return rc;
     if (need) { *need = l.bytes; return FG_OK; }
     if (bytes < l.bytes || (l.bytes && !workspace)) return fail(FG_ERR_ARG, "block attention gradients: a workspace of %zu bytes, %zu needed (fg_block_attention_backward_workspace)", bytes, l.bytes);
     Strides ds;
     if (int rc = strides_of("dout", grads->dout, grads->dout_strides, sizeof(T), &ds)) return rc;
     unsigned char *w = static_cast<unsigned char *>(workspace);
-    int rc = FG_OK;
-    if (p.queries == 0) {
-    } else if constexpr (sizeof(T) == 4 || D == 128)
-        rc = l.rt == 2 ? launch_queries<T, D, 2>(p, l, a, grads, ds, w, stream) : launch_queries<T, D, 1>(p, l, a, grads, ds, w, stream);
-    else
-        rc = l.rt == 4 ? launch_queries<T, D, 4>(p, l, a, grads, ds, w, stream)
-           : l.rt == 2 ? launch_queries<T, D, 2>(p, l, a, grads, ds, w, stream) : launch_queries<T, D, 1>(p, l, a, grads, ds, w, stream);
-    if (rc != FG_OK) return rc;
+    auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w + at); };
+    auto floats = [&](size_t at) { return reinterpret_cast<float *>(w + at); };
+    const Step step{grads->dout, a->out, a->rest, ds, a->lse, floats(l.delta), grads->dq, floats(l.bias)};
+    const dim3 threads(kThreads);
+    if (p.queries) {
+        const dim3 blocks((unsigned)(p.batch * p.kv_heads * l.n_groups));
+        const size_t few = few_stage_bytes<T, D>() + bias_bytes(p);
+        if (l.many) {
+            queries_many_kernel<T, D, RT><<<blocks, threads, Steps<T, D>::kBytes + bias_bytes(p), stream>>>(p, step, ints(l.flags), l.n_groups);
+            FG_HIP_TRY(hipGetLastError());
+            queries_redo_kernel<T, D><<<blocks, threads, few, stream>>>(p, step, ints(l.flags), l.n_groups, kWaves * RT);
+        } else {
+            queries_few_kernel<T, D><<<blocks, threads, few, stream>>>(p, step, l.n_groups);
+        }
+        FG_HIP_TRY(hipGetLastError());
+    }
     if (p.n_buckets && grads->dbias) {
-        bias_kernel<T><<<dim3(p.heads), dim3(1024), 0, stream>>>(reinterpret_cast<const float *>(w + l.bias), static_cast<T *>(grads->dbias), p.batch * l.n_tiles, p.heads, p.n_buckets);
+        bias_kernel<T><<<dim3(p.heads), dim3(1024), 0, stream>>>(floats(l.bias), static_cast<T *>(grads->dbias), p.batch * l.n_groups, p.heads, p.n_buckets);
         FG_HIP_TRY(hipGetLastError());
     }
     if (!grads->dk || l.all == 0) return FG_OK;
     auto bits = reinterpret_cast<unsigned long long *>(w + l.bits);
-    auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w + at); };
     auto pieces = reinterpret_cast<Piece *>(w + l.table);
     const int all = (int)l.all, per_wave = (all + kWaves - 1) / kWaves, block = 1 << p.block_shift, parts = std::max(1, block / (kWaves * kUnit));
-    mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), dim3(kThreads), 0, stream>>>(p, bits, l.chunks);
-    count_kernel<<<dim3(per_wave), dim3(kThreads), 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
+    mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), threads, 0, stream>>>(p, bits, l.chunks);
+    count_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
     scan_kernel<<<dim3(1), dim3(kScan), 0, stream>>>(ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), all, l.piece);
-    fill_kernel<<<dim3(per_wave), dim3(kThreads), 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
+    fill_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
     const size_t lds = keys_stage_bytes<T, D>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);
-    keys_kernel<T, D><<<dim3((unsigned)(l.pieces * parts)), dim3(kThreads), lds, stream>>>(
-        p, static_cast<const T *>(grads->dout), ds, a->lse, reinterpret_cast<const float *>(w + l.delta), pieces, ints(l.totals), ints(l.list),
-        reinterpret_cast<float *>(w + l.partial), static_cast<T *>(grads->dk), static_cast<T *>(grads->dv));
+    auto keys = [&](auto kernel) {
+        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, a->lse, floats(l.delta), pieces, ints(l.totals), ints(l.list),
+                                                                             floats(l.partial), static_cast<T *>(grads->dk), static_cast<T *>(grads->dv), ints(l.flags));
+    };
+    keys(keys_kernel<T, D, false>);
+    FG_HIP_TRY(hipGetLastError());
+    keys(keys_kernel<T, D, true>);
     if (l.slots)
-        pieces_kernel<T, D><<<dim3(all), dim3(kThreads), 0, stream>>>(p, ints(l.count), ints(l.slot0), reinterpret_cast<const float *>(w + l.partial),
-                                                                      static_cast<T *>(grads->dk), static_cast<T *>(grads->dv), l.piece);
+        pieces_kernel<T, D><<<dim3((unsigned)(all * (2 * block * (D / 4) / kThreads))), threads, 0, stream>>>(p, ints(l.count), ints(l.slot0), floats(l.partial), static_cast<T *>(grads->dk),
+                                                                                                            static_cast<T *>(grads->dv), l.piece);
     FG_HIP_TRY(hipGetLastError());
     return FG_OK;
 }

@@ -68,6 +68,16 @@ def test_lengths_and_blocks(dtype, queries, keys, block, topk, causal):
     ref.check(step(s, dout), want(s, dout))
 
 
+@pytest.mark.parametrize("dtype,head_len,block,buckets", [(F32, 32, 32, 8), (F16, 64, 128, 0), (BF16, 128, 64, 32), (BF16, 32, 32, 16), (F32, 128, 64, 0)])
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,causal", [(4, 1030, 8, 8, True), (2, 1030, 16, 4, False), (1, 2060, 16, 1, True), (2, 2610, 6, 2, True)])
+def test_many_queries(dtype, head_len, block, buckets, batch, queries, heads, kv_heads, causal):
+    """Enough of them for the kernels that take several tiles at a time (256 workgroups)."""
+    s, dout = make(dtype, batch, queries, queries, heads, kv_heads, head_len, block, 3, buckets, causal, seed=4)
+    s["blocks"][:, 700:705] = -1
+    ref.check(step(s, dout), want(s, dout))
+    ref.check({"out": call(s)}, want(s))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("buckets,heads,kv_heads,queries,keys", [(32, 4, 2, 200, 200), (16, 3, 1, 90, 90), (64, 2, 2, 33, 150), (4, 16, 1, 70, 70), (7, 4, 4, 1, 300)])
@@ -146,14 +156,28 @@ def test_ids_twice_in_any_order_and_out_of_range():
     assert all(torch.equal(some[x], again[x]) for x in some)
 
 
-def test_masked_infinities_and_nan_reach_nobody():
-    """Keys and values that are not finite in blocks that a neighbouring query selects and this one does not, and behind a causal query."""
+@pytest.mark.parametrize("batch", [1, 120])
+def test_masked_infinities_and_nan_reach_nobody(batch):
+    """Keys and values that are not finite in blocks that a neighbouring query selects and this one does not, and behind a causal query; in the
+    first sequence of a batch that is small, or large enough for the kernels that take many queries (looked at in that sequence)."""
+    def step(s, dout):
+        got = globals()["step"](s, dout)
+        if batch > 1:
+            assert all(torch.isfinite(t[1:]).all() for t in got.values())
+            assert all(torch.equal(got[x][1], clean_step[x][1]) for x in got) if clean_step else True
+        return {x: t[:1] for x, t in got.items()}
+
+    def want(s, dout):
+        return globals()["want"](dict(s, **{x: s[x][:1] for x in ("q", "k", "v", "blocks")}), dout[:1])
+
     for dtype in (F32, BF16):
-        s, dout = make(dtype, 1, 96, 96, 2, 1, 64, 32, 1, seed=12)
+        s, dout = make(dtype, batch, 96, 96, 2, 1, 64, 32, 1, seed=12)
+        clean_step = None
         s["blocks"][:] = 0
         s["blocks"][:, 70:80] = 1                        # these rows alone see block 1
         clean = dict(s, k=s["k"].clone(), v=s["v"].clone())
         value = want(clean, dout)
+        clean_step = globals()["step"](clean, dout)
         for rubbish in (float("nan"), float("inf"), float("-inf")):
             for name in ("k", "v"):
                 t = clean[name].clone()

@@ -119,6 +119,23 @@ template <typename T> __device__ __forceinline__ void store_row(T *out, T *rest,
     if (rest) *reinterpret_cast<T4 *>(rest + at) = y;
 }
 
+// The largest of eight numbers (NaN only if all are).  Written out: of products of the matrix cores the compiler takes every operand's
+// maximum with itself first, which doubles the instructions.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm volatile("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));        // volatile: not moved behind a branch
+    return d;
+}
+__device__ __forceinline__ float largest(f32x4 a, f32x4 b) { return max3(max3(max3(a[0], a[1], a[2]), a[3], b[0]), max3(b[1], b[2], b[3]), b[3]); }
+// The largest of lanes l, l ^ 16, l ^ 32, l ^ 48; every lane gets it.
+__device__ __forceinline__ float largest_of_rows(float v) {
+    float w = v;
+    swap_halves(v, w);
+    float x = max3(v, w, w), y = x;
+    swap_rows(x, y);
+    return max3(x, y, y);
+}
+
 struct Strides { int64_t batch, row, head; };    // in elements
 
 // What every kernel of the operator takes.
@@ -213,6 +230,37 @@ __device__ __forceinline__ int build_list(List<TILES, WINDOW> &l, const Problem 
     __syncthreads();
     return total;
 }
+
+// 64 keys of one operand on their way into LDS: 128-bit words of a workgroup's threads, rows `stride` elements apart there.  The two halves are
+// units of 32 keys, k0 .. and k1 ..; rows behind the last key read it again, so that what a padded cache holds there is never touched.
+template <typename T, int D> struct Stage {
+    static constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = kThreads / CPR, N = 2 * kUnit / RPL;
+    u32x4 word[N];
+    __device__ __forceinline__ void fetch(const T *base, int64_t row_stride, int k0, int k1, int k_len) {
+        const int r0 = threadIdx.x / CPR, col = threadIdx.x % CPR * EPC;
+        if (max(k0, k1) + kUnit <= k_len) {            // the rows' distances are the same in every step
+            const T *own = base + r0 * row_stride + col;
+            if constexpr (RPL <= kUnit) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    word[i] = *reinterpret_cast<const u32x4 *>(own + ((i * RPL < kUnit ? k0 : k1 - kUnit) + i * RPL) * row_stride);
+            } else {
+                word[0] = *reinterpret_cast<const u32x4 *>(own + (r0 < kUnit ? k0 : k1 - kUnit) * row_stride);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = i * RPL + r0;
+                word[i] = *reinterpret_cast<const u32x4 *>(base + min((r < kUnit ? k0 : k1 - kUnit) + r, k_len - 1) * row_stride + col);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *tile, int stride) const {
+        const int r0 = threadIdx.x / CPR, col = threadIdx.x % CPR * EPC;
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4 *>(tile + (i * RPL + r0) * stride + col) = word[i];
+    }
+};
 
 // The bias by relative position, in LDS: the bucket of every distance from `low` to `high`, and every bucket's bias for the heads of one
 // group, times log2(e).

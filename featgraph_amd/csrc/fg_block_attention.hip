@@ -229,18 +229,19 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Problem p, const Re
 // ---- many queries -----------------------------------------------------------------------------------------
 
 constexpr int kStep = 64;              // keys in LDS
-constexpr int kListed = 512;           // blocks listed at a time
+constexpr int kListed = 256;           // blocks listed at a time
 
 template <typename T, int D> struct Steps {
     static constexpr int kKeyStride = D + 16 / sizeof(T), kValueStride = D + kPad;
-    static constexpr size_t kBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+    static constexpr size_t kStepBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+    static constexpr int kBuffers = kStepBytes <= 40 * 1024 ? 2 : 1;      // two workgroups' worth fits a CU's LDS
+    static constexpr size_t kBytes = kBuffers * kStepBytes;
 };
 
 // RT tiles of 16 rows per wavefront.  flags[workgroup]: whether a result was not finite (see redo_kernel).
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool BIAS>
 __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, const Results r, int32_t *flags, int n_groups) {
     constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;
-    constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = kThreads / CPR, NL = kStep / RPL;
     constexpr int KS = Steps<T, D>::kKeyStride, VS = Steps<T, D>::kValueStride;
     __shared__ List<TILES, kListed> list;
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -251,12 +252,13 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
     const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
     const bool used = tc < tpt;
 
-    T *keys = reinterpret_cast<T *>(dynamic), *values = keys + kStep * KS;
+    T *tiles = reinterpret_cast<T *>(dynamic);
+    constexpr int BUFFERS = Steps<T, D>::kBuffers;
     Buckets buckets;
-    if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + Steps<T, D>::kBytes);
+    if (BIAS) buckets = load_buckets<T>(p, h, dynamic + Steps<T, D>::kBytes);
 
     // scores are compared before they are scaled: a negative scale turns the queries' signs instead
-    const float factor = p.n_buckets ? 1.f : fabsf(p.scale2);
+    const float factor = BIAS ? 1.f : fabsf(p.scale2);
     V8<T> qf[RT][DC];
     int limit[RT];                     // last key that the lane's row may see; columns without a row see everything, nothing is written of them
 #pragma unroll
@@ -266,14 +268,14 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
         limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
         const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
 #pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-            qf[rt][dc] = there ? load8(src + dc * 32) : zero8<T>();
-            if (!p.n_buckets && p.scale2 < 0.f) qf[rt][dc] = -qf[rt][dc];
-        }
+        for (int dc = 0; dc < DC; ++dc) qf[rt][dc] = there ? load8(src + dc * 32) : zero8<T>();
+        if (!BIAS && p.scale2 < 0.f)
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) qf[rt][dc] = -qf[rt][dc];
     }
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
-    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + (tid % CPR) * EPC;
-    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + (tid % CPR) * EPC;
+    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head;
+    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head;
     const int sub_shift = p.block_shift - 5;
 
     // The sum that divides the output is that of the rounded powers, which are the weights of the product (a product with ones makes it):
@@ -296,111 +298,109 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
         auto first_key = [&](int u) {
             return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
         };
-        u32x4 kr[NL], vr[NL];
+        Stage<T, D> ks, vs;
+        // ids of the step after the next, and the next step's tokens, are on their way while a step is worked on
+        const int word = wave * RT / 4, shift = wave * RT % 4 * 16;
+        int k0 = 0, k1 = 0;            // first keys of the step in the registers
+        unsigned who = 0, who1 = 0;    // its tokens of the wavefront's tiles, 16 bits a tile, one word a unit
+        auto tokens = [&](int u) { return u < units ? (unsigned)(list.bits[u >> sub_shift][word] >> shift) : 0u; };
         auto fetch = [&](int u) {
-            const int k0 = first_key(u), k1 = u + 1 < units ? first_key(u + 1) : k0;
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int row = i * RPL + tid / CPR;
-                // rows behind the last key read it again: what a padded cache holds there is never touched
-                const int64_t key = min((row < kUnit ? k0 : k1 - kUnit) + row, k_len - 1);
-                kr[i] = *reinterpret_cast<const u32x4 *>(kbase + key * p.ks.row);
-                vr[i] = *reinterpret_cast<const u32x4 *>(vbase + key * p.vs.row);
-            }
+            k0 = first_key(u);
+            k1 = u + 1 < units ? first_key(u + 1) : k0;
+            ks.fetch(kbase, p.ks.row, k0, k1, k_len);
+            vs.fetch(vbase, p.vs.row, k0, k1, k_len);
+            who = k0 <= last_key ? tokens(u) : 0u;
+            who1 = k1 <= last_key ? tokens(u + 1) : 0u;
         };
         if (units) fetch(0);
         for (int u = 0; u < units; u += 2) {
-            __syncthreads();           // the step before has been read
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int row = i * RPL + tid / CPR;
-                *reinterpret_cast<u32x4 *>(keys + row * KS + (tid % CPR) * EPC) = kr[i];
-                *reinterpret_cast<u32x4 *>(values + row * VS + (tid % CPR) * EPC) = vr[i];
-            }
+            if (BUFFERS == 1) __syncthreads();       // the step before has been read
+            T *keys = BUFFERS == 2 && (u & 2) ? tiles + kStep * (KS + VS) : tiles, *values = keys + kStep * KS;
+            ks.store(keys, KS);
+            vs.store(values, VS);
+            const int key0[2] = {k0, k1};
+            constexpr unsigned ALL = RT == 2 ? ~0u : 0xffffu;
+            const unsigned sel[2] = {__builtin_amdgcn_readfirstlane(who) & ALL, __builtin_amdgcn_readfirstlane(who1) & ALL};
             __syncthreads();
-            int key0[2];
-            unsigned who[2][RT], active = 0;         // tokens of the wavefront's tiles that selected the unit's block
+            if (u + 2 < units) fetch(u + 2);
+            if (!(sel[0] | sel[1])) continue;        // none of the wavefront's tokens selected these blocks
+            V8<T> kf[2][DC];
+            auto read_keys = [&](int x) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) kf[kt][dc] = load8(keys + (x * kUnit + kt * 16 + c) * KS + dc * 32 + 8 * g);
+            };
+            read_keys(sel[0] ? 0 : 1);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const bool there = u + x < units;
-                key0[x] = there ? first_key(u + x) : 0;
+                if (!sel[x]) continue;
+                f32x4 s[RT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = mma(kf[kt][dc], qf[rt][dc], s[rt][kt]);
+                // the next keys and the first half of the values are read while the powers are taken
+                if (x == 0 && sel[1]) read_keys(1);
+                V8<T> vf[DT / 2];
+                auto read_values = [&](int half) {
+#pragma unroll
+                    for (int i = 0; i < DT / 2; ++i) vf[i] = transposed<T, D>(values + x * kUnit * VS, (half * (DT / 2) + i) * 16, lane);
+                };
+                read_values(0);
+                __builtin_amdgcn_sched_barrier(0);
+                bool mine_too[RT], edge = false;     // whether the lane's row selected the block
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const int tile = wave * RT + rt;
-                    const unsigned bits = there && key0[x] <= last_key ? (unsigned)(list.bits[(u + x) >> sub_shift][tile >> 2] >> ((tile & 3) * 16)) & 0xffffu : 0u;
-                    who[x][rt] = __builtin_amdgcn_readfirstlane(bits);
-                    active |= who[x][rt] ? 1u << rt : 0u;
+                    mine_too[rt] = !used || (sel[x] >> (16 * rt + tc)) & 1;
+                    edge |= mine_too[rt] && key0[x] + kUnit - 1 > limit[rt];
                 }
-            }
-            if (u + 2 < units) fetch(u + 2);
-            // the wavefront's tiles in SET, those with a token that selected one of the step's blocks
-            auto work = [&](auto set) {
-                constexpr unsigned SET = decltype(set)::value;
-                f32x4 s[RT][4];
+                if (BIAS) {
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int dc = 0; dc < DC; ++dc) {
-                        const V8<T> kf = load8(keys + (kt * 16 + c) * KS + dc * 32 + 8 * g);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            if (SET >> rt & 1) s[rt][kt] = mma(kf, qf[rt][dc], s[rt][kt]);
-                    }
-                }
-                V8<T> pf[RT][2];
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (!(SET >> rt & 1)) continue;
-                    bool sel[2];
-                    int last[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        sel[x] = !used || (who[x][rt] >> tc) & 1;
-                        last[x] = sel[x] ? limit[rt] : -1;
-                    }
-                    if (p.n_buckets) {
+                    for (int rt = 0; rt < RT; ++rt) {
                         const int pos = offset + t0 + (wave * RT + rt) * tpt;
+                        const int near = buckets.at(pos - key0[x] - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - key0[x]);
+                        const float y = buckets.value(near, mine);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int near = buckets.at(pos - key0[x] - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - key0[x]);
-                            if (near == far) {
-                                const float y = buckets.value(near, mine);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) { s[rt][2 * x][i] = s[rt][2 * x][i] * p.scale2 + y; s[rt][2 * x + 1][i] = s[rt][2 * x + 1][i] * p.scale2 + y; }
-                            } else {
-#pragma unroll
-                                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        s[rt][2 * x + kt][i] = s[rt][2 * x + kt][i] * p.scale2 + buckets.value(buckets.at(pos + tc - (key0[x] + 16 * kt + 4 * g + i)), mine);
-                            }
-                        }
-                    }
-                    // a row that did not select a block has its powers taken from +inf: 0, whatever finite scores it has there.  Only keys
-                    // behind a row that did are masked one by one.
-                    const bool edge = (sel[0] && key0[0] + kUnit - 1 > limit[rt]) || (sel[1] && key0[1] + kUnit - 1 > limit[rt]);
-                    if (__any(edge)) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
+                        for (int i = 0; i < 4; ++i) { s[rt][0][i] = s[rt][0][i] * p.scale2 + y; s[rt][1][i] = s[rt][1][i] * p.scale2 + y; }
+                        if (near != far)
 #pragma unroll
                             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    s[rt][2 * x + kt][i] = key0[x] + 16 * kt + 4 * g + i <= last[x] ? s[rt][2 * x + kt][i] : -__builtin_inff();
+                                for (int i = 0; i < 4; ++i) s[rt][kt][i] += buckets.value(buckets.at(pos + tc - (key0[x] + 16 * kt + 4 * g + i)), mine) - y;
                     }
-                    float top[2];
+                }
+                // a row that did not select the block has its powers taken from +inf: 0, whatever finite scores it has there.  Only keys
+                // behind a row that did are masked one by one.
+                if (__any(edge)) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const f32x4 a = s[rt][2 * x], e = s[rt][2 * x + 1];
-                        top[x] = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])));
-                        top[x] = sel[x] ? top[x] : -__builtin_inff();
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const int last = (mine_too[rt] ? limit[rt] : -1) - key0[x] - 4 * g;
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[rt][kt][i] = 16 * kt + i <= last ? s[rt][kt][i] : -__builtin_inff();
                     }
-                    const float high = rows_max(fmaxf(top[0], top[1])) * factor;
-                    // sums are kept relative to a reference that follows the maximum when it has moved by more than 2^8
-                    if (__any(high > m[rt] + 8.f)) {
-                        const float up = fmaxf(m[rt], high), from = up == -__builtin_inff() ? 0.f : up;
+                }
+                float high[RT];
+                bool moved = false;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float most = largest(s[rt][0], s[rt][1]);
+                    high[rt] = largest_of_rows(mine_too[rt] ? most : -__builtin_inff()) * factor;
+                    moved |= high[rt] > m[rt] + 8.f;
+                }
+                // sums are kept relative to a reference that follows the maximum when it has moved by more than 2^8
+                if (__any(moved)) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const float up = fmaxf(m[rt], high[rt]), from = up == -__builtin_inff() ? 0.f : up;
                         const float shrink = __builtin_amdgcn_exp2f(m[rt] - from);
                         l[rt] *= shrink;
                         total[rt] *= shrink;
@@ -408,39 +408,35 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
                         for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
                         m[rt] = up;
                     }
-                    const float ref = m[rt] == -__builtin_inff() ? 0.f : m[rt];
+                }
+                V8<T> pf[RT];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float from = sel[x] ? ref : __builtin_inff();
+                for (int rt = 0; rt < RT; ++rt) {
+                    float from = m[rt] == -__builtin_inff() ? 0.f : m[rt];
+                    from = mine_too[rt] ? from : __builtin_inff();
 #pragma unroll
-                        for (int kt = 0; kt < 2; ++kt)
+                    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[rt][2 * x + kt][i] = __builtin_amdgcn_exp2f(s[rt][2 * x + kt][i] * factor - from);
-                        if (r.lse) {
-                            const f32x4 a = s[rt][2 * x] + s[rt][2 * x + 1];
-                            l[rt] += (a[0] + a[1]) + (a[2] + a[3]);
-                        }
-                        // rounded to the operands' type for the product with V, half a step each
-                        pf[rt][x] = pack<T>(s[rt][2 * x], s[rt][2 * x + 1]);
-                        total[rt] = mma(ones, pf[rt][x], total[rt]);
+                        for (int i = 0; i < 4; ++i) s[rt][kt][i] = __builtin_amdgcn_exp2f(s[rt][kt][i] * factor - from);
+                    // rounded to the operands' type for the product with V, half a step each
+                    pf[rt] = pack<T>(s[rt][0], s[rt][1]);
+                }
+                if (r.lse)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const f32x4 a = s[rt][0] + s[rt][1];
+                        l[rt] += (a[0] + a[1]) + (a[2] + a[3]);
                     }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < DT / 2; ++i)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) o[rt][half * (DT / 2) + i] = mma(vf[i], pf[rt], o[rt][half * (DT / 2) + i]);
+                    if (half == 0) read_values(1);
                 }
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const V8<T> vf = transposed<T, D>(values + x * kUnit * VS, dt * 16, lane);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            if (SET >> rt & 1) o[rt][dt] = mma(vf, pf[rt][x], o[rt][dt]);
-                    }
-            };
-            if (RT == 1) {
-                if (active) work(std::integral_constant<unsigned, 1>{});
-            } else {
-                if (active == 3) work(std::integral_constant<unsigned, 3>{});
-                else if (active == 1) work(std::integral_constant<unsigned, 1>{});
-                else if (active == 2) work(std::integral_constant<unsigned, 2>{});
+                for (int rt = 0; rt < RT; ++rt) total[rt] = mma(ones, pf[rt], total[rt]);
             }
         }
     }
@@ -533,7 +529,8 @@ int launch(const Problem &p, const fg_block_attention_args *a, void *workspace, 
     const dim3 blocks((unsigned)grid), threads(kThreads);
     if (s.many) {
         int32_t *marks = reinterpret_cast<int32_t *>(w);
-        many_kernel<T, D, RT><<<blocks, threads, Steps<T, D>::kBytes + bias, stream>>>(p, r, marks, s.n_tiles);
+        if (p.n_buckets) many_kernel<T, D, RT, true><<<blocks, threads, Steps<T, D>::kBytes + bias, stream>>>(p, r, marks, s.n_tiles);
+        else many_kernel<T, D, RT, false><<<blocks, threads, Steps<T, D>::kBytes, stream>>>(p, r, marks, s.n_tiles);
         FG_HIP_TRY(hipGetLastError());
         redo_kernel<T, D><<<blocks, threads, few_stage_bytes<T, D>() + bias, stream>>>(p, r, marks, s.n_tiles, kWaves * RT);
     } else {

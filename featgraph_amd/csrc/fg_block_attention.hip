@@ -492,20 +492,21 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const
     if (col == 0 && lse) lse[row] = total == 0.f ? __builtin_inff() : top + __builtin_amdgcn_logf(total);
 }
 
-// Which kernel takes a call, and how its work is cut.
+// Which kernel takes a call, and how its work is cut.  many_kernel wants its workgroups' tiles at least half full and 256 workgroups (a CU each).
+// few_kernel's workgroups take about 8 us and 0.35 us for each unit of a wavefront, and joining several costs 6 us with its launch: a list
+// is dealt out to several workgroups where a wavefront would have more than eight units of it, then down to four.
 struct Shape { bool many; int n_tiles, splits; };
 template <int RT> Shape shape_of(const Problem &p) {
     const int tpt = tile_tokens(p.group);
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
     auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
     Shape s{true, tiles(kWaves * RT), 1};
-    if (pairs * s.n_tiles >= 256) return s;
+    if (pairs * s.n_tiles >= 256 && 2 * p.queries >= kWaves * RT * tpt) return s;
     s = Shape{false, tiles(1), 1};
     const int64_t groups = std::max<int64_t>(pairs * s.n_tiles, 1);
-    // units of a list at most; every wavefront keeps two of them
     const int64_t named = std::min<int64_t>((int64_t)p.topk * std::min(tpt, p.queries), p.blocks);
-    const int64_t units = named << (p.block_shift - 5);
-    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / groups, units / (2 * kWaves)));
+    const int64_t units = named << (p.block_shift - 5);            // of a list at most
+    if (units > 8 * kWaves) s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + groups - 1) / groups, units / (4 * kWaves)));
     return s;
 }
 

@@ -760,7 +760,7 @@ int layout_of(const Problem &p, int head_len, int row_tiles, Layout *l) {
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
     auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
     l->n_groups = tiles(kWaves * row_tiles);
-    l->many = pairs * l->n_groups >= 256;
+    l->many = pairs * l->n_groups >= 256 && 2 * p.queries >= kWaves * row_tiles * tpt;
     if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
     l->piece = std::max(1, kPieceRows / p.group);

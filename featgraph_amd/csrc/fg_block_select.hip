@@ -63,17 +63,26 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The count-th largest of the wavefront's keys (R of them in each lane): the largest value that at least `count` of them reach.
+// Where the `count` largest of the wavefront's keys (R in each lane) begin: a value that exactly `count` of them reach, or, where equal keys
+// leave none, the largest value that at least as many reach.  From the top bit down, four bits between looks at whether it is
+// found (a look at every bit costs more than it saves: 256 blocks per query, 16,384 queries 117 us, 512 blocks, one query 20.7; four 108
+// and 15).
 template <int R, typename K>
-__device__ __forceinline__ K nth_largest(const K (&key)[R], int count) {
+__device__ __forceinline__ K cut_off(const K (&key)[R], int count, bool *exactly) {
     K at = 0;
-    for (int bit = 8 * sizeof(K) - 1; bit >= 0; --bit) {
-        const K trial = at | ((K)1 << bit);
-        int n = 0;
+    int reached = -1;
+    for (int bit = 8 * sizeof(K) - 1; bit >= 0 && reached != count; bit -= 4) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) n += __popcll(__ballot(key[r] >= trial));
-        at = n >= count ? trial : at;
+        for (int b = 0; b < 4; ++b) {
+            const K trial = at | ((K)1 << (bit - b));
+            int n = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) n += __popcll(__ballot(key[r] >= trial));
+            at = n >= count ? trial : at;
+            reached = n >= count ? n : reached;
+        }
     }
+    *exactly = reached == count;
     return at;
 }
 
@@ -87,6 +96,7 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const T *q, Strides qs
     constexpr int DC = D / 32;
     __shared__ __align__(16) T summed[kTokens][D + 8];
     __shared__ float mass[kWaves][kTokens];
+    __shared__ int close_ids[kWaves][16];
     extern __shared__ __align__(16) float scores[];        // [kTokens][stride]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int unit = xcd_contiguous_block(), pair = unit / n_tiles, t0 = (unit - pair * n_tiles) * kTokens, b = pair / kv_heads, h = pair - b * kv_heads;
@@ -158,37 +168,70 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const T *q, Strides qs
             const int j = r * 64 + lane;
             key[r] = j >= n ? 0u : j < keep_first || j >= n - keep_last ? ~0u : ordered(scores[tt * stride + j]);
         }
-        const uint32_t nth = nth_largest<R, uint32_t>(key, topk);
+        bool exactly;
+        const uint32_t cut = cut_off<R, uint32_t>(key, topk, &exactly);
         // |32-bit sum of D products - exact| <= D u sum |products|, u = 2^-23 should the matrix cores cut instead of round; twice
-        // that, for the bound is a sum of the same kind.  The topk-th exact score is within one error of the topk-th computed
-        // one: a block two errors above it is in, two below is out.
+        // that, for the bound is a sum of the same kind.  A block two errors above the cut beats every block below it, exactly, and one
+        // two errors below is beaten by the topk above it.
         const float err = (D + 8) * 2.4e-7f * fmaxf(fmaxf(mass[0][tt], mass[1][tt]), fmaxf(mass[2][tt], mass[3][tt])) + 1e-34f;
-        const float at = of_ordered(nth), high = at + 2 * err, low = at - 2 * err;
+        const float at = of_ordered(cut), high = at + 2 * err, low = at - 2 * err;
         unsigned in = 0, maybe = 0;
         int n_in = 0, n_maybe = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float s = of_ordered(key[r]);
-            const bool sure = key[r] == ~0u || (key[r] && nth != ~0u && s > high), close = key[r] && !sure && nth != ~0u && !(s < low);
+            const bool sure = key[r] == ~0u || (key[r] && s > high), close = key[r] && !sure && !(s < low);
             in |= (unsigned)sure << r;
             maybe |= (unsigned)close << r;
             n_in += __popcll(__ballot(sure));
             n_maybe += __popcll(__ballot(close));
         }
         const int need = topk - n_in;
-        if (n_maybe == need) {
+        if (need == n_maybe) {
             in |= maybe;
-        } else {
+        } else if (need > 0 && n_maybe <= 16) {
+            // mostly two or three of them: a quarter of a product to a lane
+            int base = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const unsigned long long all = __ballot((maybe >> r) & 1);
+                if ((maybe >> r) & 1) close_ids[wave][base + __popcll(all & ((1ull << lane) - 1))] = r * 64 + lane;
+                base += __popcll(all);
+            }
+            wave_lds_sync();
+            const int id = c < n_maybe ? close_ids[wave][c] : 0;
+            const T *src = means + (int64_t)id * D + g * (D / 4);
+            double dot = 0;
+#pragma unroll
+            for (int d = 0; d < D / 4; d += 8) {
+                const V8<T> x = load8(src + d), y = load8(&summed[tt][g * (D / 4) + d]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dot += (double)(float)x[e] * (double)(float)y[e];
+            }
+            dot += __shfl_xor(dot, 16);
+            dot += __shfl_xor(dot, 32);
+            const unsigned long long fine[1] = {g == 0 && c < n_maybe ? ordered(dot) : 0};
+            unsigned long long edge = cut_off<1, unsigned long long>(fine, need, &exactly);
+            edge -= exactly;                       // `need` of them are above it, or those above and some that are equal
+            const unsigned long long above = __ballot(fine[0] > edge);
+            unsigned long long same = exactly ? 0 : __ballot(fine[0] && fine[0] == edge), taken = above;
+            for (int left = need - __popcll(above); left > 0; --left, same &= same - 1) taken |= same & -same;     // the lowest ids
+            for (; taken; taken &= taken - 1) {
+                const int one = __shfl(id, __builtin_ctzll(taken));
+                in |= lane == (one & 63) ? 1u << (one >> 6) : 0u;
+            }
+            wave_lds_sync();
+        } else if (need > 0) {
             unsigned long long fine[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) fine[r] = 0;
 #pragma unroll 1
-            for (int r = 0; r * 64 < n; ++r) {             // mostly one or two of them hold a block to look at
+            for (int r = 0; r * 64 < n; ++r) {
                 const bool look = (maybe >> r) & 1;
                 if (!__ballot(look)) continue;
                 const T *src = means + (int64_t)(look ? r * 64 + lane : 0) * D;
                 double dot = 0;
-#pragma unroll 2
+#pragma unroll 4
                 for (int d = 0; d < D; d += 8) {
                     const V8<T> x = load8(src + d), y = load8(&summed[tt][d]);
 #pragma unroll
@@ -198,7 +241,8 @@ __global__ __launch_bounds__(kThreads) void select_kernel(const T *q, Strides qs
 #pragma unroll
                 for (int x = 0; x < R; ++x) fine[x] = x == r ? v : fine[x];
             }
-            const unsigned long long edge = nth_largest<R, unsigned long long>(fine, need);
+            unsigned long long edge = cut_off<R, unsigned long long>(fine, need, &exactly);
+            edge -= exactly;                       // `need` of them are above it, or those above and some that are equal
             int above = 0;
 #pragma unroll
             for (int r = 0; r < R; ++r) above += __popcll(__ballot(fine[r] > edge));
@@ -256,7 +300,7 @@ template <typename T, int D>
 int launch_select(const Choice &c, hipStream_t stream) {
     const int blocks = (c.keys + c.block - 1) / c.block;
     // registers for a query's scores, one per 64 blocks
-    return blocks <= 128 ? launch_select_r<T, D, 2>(c, blocks, stream) : blocks <= 512 ? launch_select_r<T, D, 8>(c, blocks, stream)
+    return blocks <= 128 ? launch_select_r<T, D, 2>(c, blocks, stream) : blocks <= 256 ? launch_select_r<T, D, 4>(c, blocks, stream) : blocks <= 512 ? launch_select_r<T, D, 8>(c, blocks, stream)
                                                                                       : launch_select_r<T, D, 32>(c, blocks, stream);
 }
 

@@ -6,6 +6,8 @@ workspaces come from torch's allocator on the current stream, so calls on severa
 The reference has no such operator.
 """
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -49,20 +51,43 @@ def _check_sizes(head_len, block_size, heads=None, kv_heads=None):
 
 def _rows(t):
     """The tensor itself where the kernels can address it -- dense heads at 16-byte addresses -- or else a dense copy."""
-    per = 16 // t.element_size()
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) % per == 0 for i in range(3))
-    if ok:
+    a, b, c, d = t.stride()
+    if d == 1 and not (a | b | c) * t.element_size() % 16 and not t.data_ptr() % 16:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _on(device):
+    """A guard that makes `device` current, or None where it is already: the common case, without the guard's 2 us."""
+    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+class _Call(object):
+    """The library, and the current stream of the tensors' device, for the calls inside."""
+
+    def __init__(self, device):
+        self._guard = _on(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return _lib.lib(), common.stream_ptr()
+
+    def __exit__(self, *error):
+        if self._guard is not None:
+            self._guard.__exit__(*error)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _strides(t):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+    return _Strides(*t.stride()[:3])
 
 
-def _bytes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+_Strides = ctypes.c_int64 * 3
 
 
 def block_pool(k, block_size, lengths):
@@ -74,9 +99,9 @@ def block_pool(k, block_size, lengths):
         raise ValueError("k has no heads: shape %s" % (tuple(k.shape),))
     k = _rows(k)
     pooled = torch.empty((batch, kv_heads, -(-keys // block_size), head_len), dtype=k.dtype, device=k.device)
-    with torch.cuda.device(k.device):
-        _lib.check(_lib.lib().fg_block_pool(_TYPES[k.dtype], _lib.dev_ptr(k), _strides(k), _lib.dev_ptr(lengths), _lib.dev_ptr(pooled), batch,
-                                            keys, kv_heads, head_len, block_size, common.stream_ptr()))
+    with _Call(k.device) as (L, stream):
+        _lib.check(L.fg_block_pool(_TYPES[k.dtype], k.data_ptr(), _strides(k), _ptr(lengths), pooled.data_ptr(), batch, keys, kv_heads, head_len,
+                                   block_size, stream))
     return pooled
 
 
@@ -97,10 +122,9 @@ def block_select(q, pooled, num_keys, block_size, topk, causal, lengths, q_lengt
     if pooled.data_ptr() % 16:
         pooled = pooled.clone()
     blocks = torch.empty((batch, queries, kv_heads, topk), dtype=torch.int32, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().fg_block_select(_TYPES[q.dtype], _lib.dev_ptr(q), _strides(q), _lib.dev_ptr(pooled), _lib.dev_ptr(lengths),
-                                              _lib.dev_ptr(q_lengths), _lib.dev_ptr(blocks), batch, queries, num_keys, heads, kv_heads, head_len,
-                                              block_size, topk, int(causal), keep_first, keep_last, common.stream_ptr()))
+    with _Call(q.device) as (L, stream):
+        _lib.check(L.fg_block_select(_TYPES[q.dtype], q.data_ptr(), _strides(q), pooled.data_ptr(), _ptr(lengths), _ptr(q_lengths), blocks.data_ptr(),
+                                     batch, queries, num_keys, heads, kv_heads, head_len, block_size, topk, int(causal), keep_first, keep_last, stream))
     return blocks
 
 
@@ -138,25 +162,31 @@ def check_attention(q, k, v, blocks, block_size, lengths, q_lengths, bias, bound
     return bounds
 
 
+# fg_block_attention_args as bytes: 10 whole numbers, scale, buckets, bounds; pointers and strides
+_PLAIN = struct.Struct("=10ifi63i")
+_REST = struct.Struct("=3Q9q7Q")
+assert ctypes.sizeof(_lib.FgBlockAttentionArgs) == (_PLAIN.size + 7) // 8 * 8 + _REST.size
+
+
 def _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest):
+    """(fg_block_attention_args, the part of it that the workspace's size goes by)."""
+    batch, queries, heads, head_len = q.shape
+    sizes = (_TYPES[q.dtype], batch, queries, k.shape[1], heads, k.shape[2], head_len, block_size, blocks.shape[3], causal,
+             scale, 0 if bias is None else len(bounds) + 1) + bounds + (0,) * (63 - len(bounds))
     a = _lib.FgBlockAttentionArgs()
-    a.type = _TYPES[q.dtype]
-    a.batch, a.queries, a.heads, a.head_len = q.shape
-    a.keys, a.kv_heads = k.shape[1:3]
-    a.block, a.topk, a.causal, a.scale = block_size, blocks.shape[3], int(causal), scale
-    a.n_buckets = 0 if bias is None else bias.shape[0]
-    for i, x in enumerate(bounds):
-        a.bounds[i] = x
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_strides, a.k_strides, a.v_strides = _strides(q), _strides(k), _strides(v)
-    a.blocks = blocks.data_ptr()
-    a.lengths = 0 if lengths is None else lengths.data_ptr()
-    a.q_lengths = 0 if q_lengths is None else q_lengths.data_ptr()
-    a.bias = 0 if bias is None else bias.data_ptr()
-    a.out = out.data_ptr()
-    a.lse = 0 if lse is None else lse.data_ptr()
-    a.rest = 0 if rest is None else rest.data_ptr()
-    return a
+    _PLAIN.pack_into(a, 0, *sizes)
+    _REST.pack_into(a, (_PLAIN.size + 7) // 8 * 8, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                    blocks.data_ptr(), _ptr(lengths), _ptr(q_lengths), _ptr(bias), out.data_ptr(), _ptr(lse), _ptr(rest))
+    return a, sizes
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(sizes, backward):
+    """Bytes of device memory that a call of these sizes needs."""
+    a = _lib.FgBlockAttentionArgs()
+    _PLAIN.pack_into(a, 0, *sizes)
+    L = _lib.lib()
+    return _lib.check((L.fg_block_attention_backward_workspace if backward else L.fg_block_attention_workspace)(ctypes.byref(a)))
 
 
 def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, train):
@@ -167,12 +197,11 @@ def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths,
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
-    a = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
-        need = _lib.check(L.fg_block_attention_workspace(ctypes.byref(a)))
-        work = _bytes(need, q.device)
-        _lib.check(L.fg_block_attention(ctypes.byref(a), _lib.dev_ptr(work), need, common.stream_ptr()))
+    a, sizes = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    need = _workspace(sizes, False)
+    with _Call(q.device) as (L, stream):
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.check(L.fg_block_attention(ctypes.byref(a), _ptr(work), need, stream))
     return out, lse, rest
 
 
@@ -184,12 +213,10 @@ def block_attention_backward(q, k, v, blocks, block_size, scale, causal, lengths
     dq = new(q)
     dk, dv = (new(k), new(v)) if keys_too else (None, None)
     dbias = None if bias is None else new(bias)
-    a = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
-    grads = _lib.FgBlockAttentionGrads(dout=dout.data_ptr(), dout_strides=_strides(dout), dq=dq.data_ptr(), dk=dk.data_ptr() if keys_too else 0,
-                                       dv=dv.data_ptr() if keys_too else 0, dbias=0 if dbias is None else dbias.data_ptr())
-    L = _lib.lib()
-    with torch.cuda.device(q.device):
-        need = _lib.check(L.fg_block_attention_backward_workspace(ctypes.byref(a)))
-        work = _bytes(need, q.device)
-        _lib.check(L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), _lib.dev_ptr(work), need, common.stream_ptr()))
+    a, sizes = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    grads = _lib.FgBlockAttentionGrads(dout.data_ptr(), _strides(dout), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dbias))
+    need = _workspace(sizes, True)
+    with _Call(q.device) as (L, stream):
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _lib.check(L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), _ptr(work), need, stream))
     return dq, dk, dv, dbias

@@ -56,6 +56,15 @@ template <typename T> __device__ __forceinline__ V8<T> pack(f32x4 a, f32x4 b) {
     return v;
 }
 
+// The same, and what the rounding took, rounded itself (nothing in 32 bits).
+template <typename T> __device__ __forceinline__ void split(f32x4 a, f32x4 b, V8<T> *high, V8<T> *low) {
+    V8<T> v = pack<T>(a, b), w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { w[i] = (T)(a[i] - (float)v[i]); w[4 + i] = (T)(b[i] - (float)v[4 + i]); }
+    *high = v;
+    *low = w;
+}
+
 // Elements (row, d0 + c) of a staged [32][D + kPad] tile for the rows 4 g + i and 16 + 4 g + i: columns of the tile as a left operand.
 __device__ __forceinline__ s16x4 read_tr(const short *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p));

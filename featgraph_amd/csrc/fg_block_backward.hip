@@ -182,13 +182,13 @@ __device__ __forceinline__ void write_bias(const Problem &p, const float *sums, 
     }
 }
 
-// Powers p = 2^(z - lse), and from them dS = p (dP - delta), of one tile and 32 keys, into s[]: where `edge`, keys behind `last` have none.
+// Powers p = 2^(z - lse), and from them dS = p (dP - delta), of one tile and 32 keys, into s[]: with MASK, keys behind `last` have none.
 // The bias's gradient goes to `sums`.
-template <bool MASK>
+template <bool BIAS, bool MASK>
 __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float delta, int pos, int tpt,
                                                     int tc, int mine, int key0, int last, int g, int lane) {
-    const int near = p.n_buckets ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = p.n_buckets ? buckets.at(pos + tpt - 1 - key0) : 0;
-    const float common = p.n_buckets && near == far ? buckets.value(near, mine) : 0.f;
+    const int near = BIAS ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = BIAS ? buckets.at(pos + tpt - 1 - key0) : 0;
+    const float from = (BIAS && near == far ? buckets.value(near, mine) : 0.f) - lse;
     unsigned seen = MASK ? 0 : 0xff;
     float total = 0.f;
 #pragma unroll
@@ -196,9 +196,9 @@ __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buck
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int key = key0 + 16 * kt + 4 * g + i;
-            float z = s[kt][i] * p.scale2 + (common - lse);
+            float z = s[kt][i] * p.scale2 + from;
             int bucket = 0;
-            if (near != far) {
+            if (BIAS && near != far) {
                 bucket = buckets.at(pos + tc - key);
                 z += buckets.value(bucket, mine);
             }
@@ -208,10 +208,12 @@ __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buck
                 seen |= (unsigned)(key <= last) << (4 * kt + i);
             }
             s[kt][i] = x;
-            if (near != far) sums[bucket * 64 + lane] += x;
-            else total += x;
+            if (BIAS) {
+                if (near != far) sums[bucket * 64 + lane] += x;
+                else total += x;
+            }
         }
-    if (p.n_buckets && near == far) sums[near * 64 + lane] += total;
+    if (BIAS && near == far) sums[near * 64 + lane] += total;
     return seen;
 }
 
@@ -288,14 +290,20 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
                 }
                 u = find(u + kWaves);
                 if (u < units) fetch(u);
-                const unsigned seen = score_gradients<true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
-                // rounded to the operands' type for the product with K, half a step each
-                const V8<T> sf = pack<T>(s[0], s[1]);
+                const unsigned seen = p.n_buckets
+                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane)
+                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
+                V8<T> sf, rf;          // as in queries_many_kernel
+                split<T>(s[0], s[1], &sf, &rf);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const V8<T> x = transposed<T, D>(stage, dt * 16, lane);
-                    if constexpr (decltype(careful)::value) acc[dt] = mma_masked<T>(x, sf, seen, acc[dt]);
-                    else acc[dt] = mma(x, sf, acc[dt]);
+                    if constexpr (decltype(careful)::value) {
+                        acc[dt] = mma_masked<T>(x, sf, seen, acc[dt]);
+                    } else {
+                        acc[dt] = mma(x, sf, acc[dt]);
+                        if (sizeof(T) == 2) acc[dt] = mma(x, rf, acc[dt]);
+                    }
                 }
             }
         }
@@ -347,19 +355,20 @@ __global__ __launch_bounds__(kThreads) void queries_few_kernel(const Problem p, 
 }
 
 constexpr int kStep = 64;              // keys in LDS
-constexpr int kListed = 512;           // blocks listed at a time
+constexpr int kListed = 256;           // blocks listed at a time
 
-template <typename T, int D> struct Steps {
+template <typename T, int D, bool BIAS> struct Steps {
     static constexpr int kKeyStride = D + kPad, kValueStride = D + 16 / sizeof(T);
-    static constexpr size_t kBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+    static constexpr size_t kStepBytes = (size_t)kStep * (kKeyStride + kValueStride) * sizeof(T);
+    static constexpr int kBuffers = !BIAS && kStepBytes <= 40 * 1024 ? 2 : 1;     // two workgroups' worth, with the bias's sums, fits a CU's LDS
+    static constexpr size_t kBytes = kBuffers * kStepBytes;
 };
 
 // RT tiles of 16 rows per wavefront, the list walked by all four together, as many_kernel does forward.
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool BIAS>
 __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem p, const Step w, int32_t *flags, int n_groups) {
-    constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;
-    constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = kThreads / CPR, NL = kStep / RPL;
-    constexpr int KS = Steps<T, D>::kKeyStride, VS = Steps<T, D>::kValueStride;
+    constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT, BUFFERS = Steps<T, D, BIAS>::kBuffers;
+    constexpr int KS = Steps<T, D, BIAS>::kKeyStride, VS = Steps<T, D, BIAS>::kValueStride;
     __shared__ List<TILES, kListed> list;
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
@@ -368,11 +377,11 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     const int tpt = tile_tokens(p.group), t0 = group * TILES * tpt;
     const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
     const bool used = tc < tpt;
-    T *keys = reinterpret_cast<T *>(dynamic), *values = keys + kStep * KS;
+    T *tiles = reinterpret_cast<T *>(dynamic);
     Buckets buckets;
     float *sums = nullptr;
-    if (p.n_buckets) {
-        unsigned char *at = dynamic + Steps<T, D>::kBytes;
+    if (BIAS) {
+        unsigned char *at = dynamic + Steps<T, D, BIAS>::kBytes;
         buckets = load_buckets<T>(p, h, at);
         sums = bias_place(p, at) + wave * p.n_buckets * 64;
         for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
@@ -381,8 +390,8 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
-    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + (tid % CPR) * EPC;
-    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + (tid % CPR) * EPC;
+    const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head;
+    const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head;
     const int sub_shift = p.block_shift - 5;
 
     f32x4 acc[RT][DT];
@@ -395,87 +404,106 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
         auto first_key = [&](int u) {
             return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
         };
-        u32x4 kr[NL], vr[NL];
+        Stage<T, D> ks, vs;
+        const int word = wave * RT / 4, shift = wave * RT % 4 * 16;
+        int k0 = 0, k1 = 0;            // first keys of the step in the registers
+        unsigned who = 0, who1 = 0;    // its tokens of the wavefront's tiles, 16 bits a tile, one word a unit
+        auto tokens = [&](int u) { return u < units ? (unsigned)(list.bits[u >> sub_shift][word] >> shift) : 0u; };
         auto fetch = [&](int u) {
-            const int k0 = first_key(u), k1 = u + 1 < units ? first_key(u + 1) : k0;
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int r = i * RPL + tid / CPR;
-                const int64_t key = min((r < kUnit ? k0 : k1 - kUnit) + r, k_len - 1);
-                kr[i] = *reinterpret_cast<const u32x4 *>(kbase + key * p.ks.row);
-                vr[i] = *reinterpret_cast<const u32x4 *>(vbase + key * p.vs.row);
-            }
+            k0 = first_key(u);
+            k1 = u + 1 < units ? first_key(u + 1) : k0;
+            ks.fetch(kbase, p.ks.row, k0, k1, k_len);
+            vs.fetch(vbase, p.vs.row, k0, k1, k_len);
+            who = k0 <= last_key ? tokens(u) : 0u;
+            who1 = k1 <= last_key ? tokens(u + 1) : 0u;
         };
         if (units) fetch(0);
-        for (int u0 = 0; u0 < units; u0 += 2) {
-            __syncthreads();           // the step before has been read
-#pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int r = i * RPL + tid / CPR;
-                *reinterpret_cast<u32x4 *>(keys + r * KS + (tid % CPR) * EPC) = kr[i];
-                *reinterpret_cast<u32x4 *>(values + r * VS + (tid % CPR) * EPC) = vr[i];
-            }
+        for (int u = 0; u < units; u += 2) {
+            if (BUFFERS == 1) __syncthreads();       // the step before has been read
+            T *keys = BUFFERS == 2 && (u & 2) ? tiles + kStep * (KS + VS) : tiles, *values = keys + kStep * KS;
+            ks.store(keys, KS);
+            vs.store(values, VS);
+            const int key0[2] = {k0, k1};
+            constexpr unsigned ALL = RT == 2 ? ~0u : 0xffffu;
+            const unsigned sel[2] = {__builtin_amdgcn_readfirstlane(who) & ALL, __builtin_amdgcn_readfirstlane(who1) & ALL};
             __syncthreads();
-            if (u0 + 2 < units) fetch(u0 + 2);
+            if (u + 2 < units) fetch(u + 2);
 #pragma unroll 1
-            for (int u = u0; u < min(u0 + 2, units); ++u) {
-                const int key0 = first_key(u);
-                if (key0 > last_key) continue;
-                unsigned who[RT], active = 0;
+            for (int x = 0; x < 2; ++x) {
+                const unsigned bits = x ? sel[1] : sel[0];
+                if (!bits) continue;                 // none of the wavefront's tokens selected the block
+                const int now = x ? key0[1] : key0[0];
+                const T *ktile = keys + x * kUnit * KS, *vtile = values + x * kUnit * VS;
+                f32x4 s[RT][2], dp[RT][2];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    // two strips of 32 columns at a time: with all of them in registers a head of 128 spills
+                    constexpr int STRIPS = DC < 2 ? DC : 2;
+#pragma unroll
+                    for (int d0 = 0; d0 < DC; d0 += STRIPS) {
+                        V8<T> kf[STRIPS], vf[STRIPS];
+#pragma unroll
+                        for (int i = 0; i < STRIPS; ++i) {
+                            kf[i] = load8(ktile + (kt * 16 + c) * KS + (d0 + i) * 32 + 8 * g);
+                            vf[i] = load8(vtile + (kt * 16 + c) * VS + (d0 + i) * 32 + 8 * g);
+                        }
+#pragma unroll
+                        for (int i = 0; i < STRIPS; ++i)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) {
+                                s[rt][kt] = mma(kf[i], row[rt].q[d0 + i], s[rt][kt]);
+                                dp[rt][kt] = mma(vf[i], row[rt].d[d0 + i], dp[rt][kt]);
+                            }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                // the first columns of the keys are read while the powers are taken
+                constexpr int XB = DT < 4 ? DT / 2 : DT / 4;
+                V8<T> xf[XB];
+                auto read_keys = [&](int part) {
+#pragma unroll
+                    for (int i = 0; i < XB; ++i) xf[i] = transposed<T, D>(ktile, (part * XB + i) * 16, lane);
+                };
+                read_keys(0);
+                __builtin_amdgcn_sched_barrier(0);
+                bool edge = false;
+                float lse[RT];
+                int last[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const int tile = wave * RT + rt;
-                    who[rt] = __builtin_amdgcn_readfirstlane((unsigned)(list.bits[u >> sub_shift][tile >> 2] >> ((tile & 3) * 16)) & 0xffffu);
-                    active |= who[rt] ? 1u << rt : 0u;
+                    // a row that did not select the block has its powers relative to +inf: 0
+                    const bool one = !used || (bits >> (16 * rt + tc)) & 1;
+                    lse[rt] = one ? row[rt].lse : __builtin_inff();
+                    last[rt] = one ? row[rt].limit : -1;
+                    edge |= one && now + kUnit - 1 > row[rt].limit;
                 }
-                const T *ktile = keys + (u - u0) * kUnit * KS, *vtile = values + (u - u0) * kUnit * VS;
-                auto work = [&](auto set) {
-                    constexpr unsigned SET = decltype(set)::value;
-                    f32x4 s[RT][2], dp[RT][2];
+                const int pos = offset + t0 + wave * RT * tpt;
+                if (__any(edge)) {
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int dc = 0; dc < DC; ++dc) {
-                            const V8<T> kf = load8(ktile + (kt * 16 + c) * KS + dc * 32 + 8 * g), vf = load8(vtile + (kt * 16 + c) * VS + dc * 32 + 8 * g);
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
-                                if (SET >> rt & 1) {
-                                    s[rt][kt] = mma(kf, row[rt].q[dc], s[rt][kt]);
-                                    dp[rt][kt] = mma(vf, row[rt].d[dc], dp[rt][kt]);
-                                }
-                        }
-                    }
-                    V8<T> sf[RT];
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if (!(SET >> rt & 1)) continue;
-                        // a row that did not select the block has its powers relative to +inf: 0
-                        const bool sel = !used || (who[rt] >> tc) & 1;
-                        const float lse = sel ? row[rt].lse : __builtin_inff();
-                        const int pos = offset + t0 + (wave * RT + rt) * tpt;
-                        if (__any(sel && key0 + kUnit - 1 > row[rt].limit))
-                            score_gradients<true>(p, buckets, sums, s[rt], dp[rt], lse, row[rt].delta, pos, tpt, tc, mine, key0, sel ? row[rt].limit : -1, g, lane);
-                        else
-                            score_gradients<false>(p, buckets, sums, s[rt], dp[rt], lse, row[rt].delta, pos, tpt, tc, mine, key0, 0, g, lane);
-                        // rounded to the operands' type for the product with K, half a step each
-                        sf[rt] = pack<T>(s[rt][0], s[rt][1]);
-                    }
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const V8<T> x = transposed<T, D>(ktile, dt * 16, lane);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            if (SET >> rt & 1) acc[rt][dt] = mma(x, sf[rt], acc[rt][dt]);
-                    }
-                };
-                if (RT == 1) {
-                    if (active) work(std::integral_constant<unsigned, 1>{});
+                    for (int rt = 0; rt < RT; ++rt)
+                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
                 } else {
-                    if (active == 3) work(std::integral_constant<unsigned, 3>{});
-                    else if (active == 1) work(std::integral_constant<unsigned, 1>{});
-                    else if (active == 2) work(std::integral_constant<unsigned, 2>{});
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
+                }
+                // dS goes into the product with K rounded, and what that took (in 16 bits) in a second one: a row's dS add up to 0, and its keys
+                // have much in common, so that the rounding alone would be larger than dQ's own
+                V8<T> sf[RT], rf[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) split<T>(s[rt][0], s[rt][1], &sf[rt], &rf[rt]);
+#pragma unroll
+                for (int part = 0; part < DT / XB; ++part) {
+#pragma unroll
+                    for (int i = 0; i < XB; ++i)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            acc[rt][part * XB + i] = mma(xf[i], sf[rt], acc[rt][part * XB + i]);
+                            if (sizeof(T) == 2) acc[rt][part * XB + i] = mma(xf[i], rf[rt], acc[rt][part * XB + i]);
+                        }
+                    if (part + 1 < DT / XB) read_keys(part + 1);
                 }
             }
         }
@@ -491,7 +519,7 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
                 store_row<T>(static_cast<T *>(w.dq), nullptr, (((int64_t)b * p.queries + t) * p.heads + head) * D + dt * 16 + 4 * g, acc[rt][dt] * p.scale);
         }
     }
-    if (p.n_buckets) write_bias(p, sums - wave * p.n_buckets * 64, w.bias_sums, (int64_t)b * n_groups + group, h);
+    if (BIAS) write_bias(p, sums - wave * p.n_buckets * 64, w.bias_sums, (int64_t)b * n_groups + group, h);
     odd = __syncthreads_or(odd);
     if (tid == 0) flags[unit] = odd;
 }
@@ -539,23 +567,33 @@ __global__ __launch_bounds__(1024) void bias_kernel(const float *sums, T *dbias,
 
 template <typename T, int D> constexpr size_t keys_stage_bytes() { return (size_t)kWaves * 2 * kUnit * (D + kPad) * sizeof(T); }
 
-// A wavefront has 32 keys; where a block has fewer than 4 x 32, several wavefronts share them and take the list's rows in turn.
+// A wavefront has KT tiles of 16 keys; where a block has fewer than four wavefronts' keys, several share them and take the list's rows in turn.
 // flags[workgroup]: whether a sum was not finite; CAREFUL: those again, with such places apart.
+template <typename T, int D> struct Keys {
+    // heads of 128: two tiles' operands and sums leave room for one wavefront per SIMD alone, and still take less than one tile each of two
+    // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us)
+    static constexpr int kTiles = sizeof(T) == 4 ? 1 : 2;
+    static constexpr int kResident = D == 128 ? 1 : 2;
+    static int parts(int block) { return std::max(1, block / (kWaves * 16 * kTiles)); }       // workgroups of a block
+};
+
 template <typename T, int D, bool CAREFUL>
-__global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
+__global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
                                                         const int32_t *totals, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
-    constexpr int DC = D / 32, DT = D / 16, S = D + kPad;
+    constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const int block = 1 << p.block_shift, kw_n = min(kWaves, block / kUnit), rw_n = kWaves / kw_n, parts = block / (kw_n * kUnit);
-    const int kw = wave % kw_n, rw = wave / kw_n, work = blockIdx.x / parts, part = blockIdx.x - work * parts;
-    if (work >= totals[0] || (CAREFUL && !flags[blockIdx.x])) return;
+    const int block = 1 << p.block_shift, kw_n = min(kWaves, block / (16 * KT)), rw_n = kWaves / kw_n, parts = block / (kw_n * 16 * KT);
+    const int kw = wave % kw_n, rw = wave / kw_n;
+    // (dealt to the XCDs in turn: contiguous shares, for the L2s' sake, are uneven and take 4 to 15 % more)
+    const int unit = blockIdx.x, work = unit / parts, part = unit - work * parts;
+    if (work >= totals[0] || (CAREFUL && !flags[unit])) return;
     const Piece piece = pieces[work];
     const int pair = piece.block / p.blocks, blk = piece.block - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
-    const int in_block = (part * kw_n + kw) * kUnit, key0 = (blk << p.block_shift) + in_block, n_rows = piece.len * p.group;
+    const int in_block = (part * kw_n + kw) * 16 * KT, key0 = (blk << p.block_shift) + in_block, n_rows = piece.len * p.group;
 
     T *stage_q = reinterpret_cast<T *>(dynamic) + wave * 2 * kUnit * S, *stage_d = stage_q + kUnit * S;
     Buckets buckets;
@@ -564,9 +602,9 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
         __syncthreads();
     }
 
-    V8<T> kf[2][DC], vf[2][DC];
+    V8<T> kf[KT][DC], vf[KT][DC];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < KT; ++kt) {
         const int key = key0 + kt * 16 + c;
         const bool there = key < k_len;
         const T *ks = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + (int64_t)key * p.ks.row + 8 * g;
@@ -581,40 +619,50 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     const T *dbase = dout + b * ds.batch + (int64_t)h * p.group * ds.head + 8 * g;
     Row *own = rows[wave];
 
-    f32x4 ak[2][DT], av[2][DT];
+    f32x4 ak[KT][DT], av[KT][DT];
     {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) ak[kt][dt] = av[kt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         V8<T> qf[2][DC], df[2][DC];
         Row next;                      // lane 16 rt + c: row 16 rt + c of the step
+        // the token of the lane's row of the step that is fetched next: its load has a step's time before the rows' own depend on it
+        int token = 0, x = 0;
+        auto look = [&](int r0) {
+            const int r = min(r0 + (lane & 31), n_rows - 1), at = r / p.group;
+            x = r - at * p.group;
+            token = list[piece.start + at];
+        };
         auto fetch = [&](int r0) {
-            const int r = r0 + (lane & 31);
-            const bool there = r < n_rows;
-            int token = 0, x = 0;
-            next = Row{__builtin_inff(), 0.f, -1, 0};
-            if (there) {
-                const int at = r / p.group;
-                x = r - at * p.group;
-                token = list[piece.start + at];
-                const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
-                next = Row{lse[row], delta[row], offset + token, x};
-            }
+            const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
+            next = Row{lse[row], delta[row], offset + token, x};
+            if (r0 + (lane & 31) >= n_rows) next = Row{__builtin_inff(), 0.f, -1, 0};     // a row behind the last has no weight
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
                 const int t = __shfl(token, rt * 16 + c), y = __shfl(x, rt * 16 + c);
-                const bool ok = r0 + rt * 16 + c < n_rows;
                 const T *q = qbase + (int64_t)t * p.qs.row + y * p.qs.head, *d = dbase + (int64_t)t * ds.row + y * ds.head;
+                const bool ok = r0 + rt * 16 + c < n_rows;
 #pragma unroll
                 for (int dc = 0; dc < DC; ++dc) {
-                    qf[rt][dc] = ok ? load8(q + dc * 32) : zero8<T>();
-                    df[rt][dc] = ok ? load8(d + dc * 32) : zero8<T>();
+                    qf[rt][dc] = load8(q + dc * 32);
+                    df[rt][dc] = load8(d + dc * 32);
                 }
+                if (r0 + kUnit > n_rows)
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) {
+                        qf[rt][dc] = ok ? qf[rt][dc] : zero8<T>();
+                        df[rt][dc] = ok ? df[rt][dc] : zero8<T>();
+                    }
             }
         };
         int r0 = rw * kUnit;
-        if (r0 < n_rows) fetch(r0);
+        const int stride = rw_n * kUnit;
+        if (r0 < n_rows) {
+            look(r0);
+            fetch(r0);
+            look(r0 + stride);
+        }
         while (r0 < n_rows) {
             wave_lds_sync();
 #pragma unroll
@@ -626,11 +674,11 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
                 }
             if (lane < kUnit) own[lane] = next;
             wave_lds_sync();
-            f32x4 s[2][2], dp[2][2];   // [rows][keys]
+            f32x4 s[2][KT], dp[2][KT];  // [rows][keys]
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
+                for (int kt = 0; kt < KT; ++kt) {
                     s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int dc = 0; dc < DC; ++dc) {
@@ -638,19 +686,22 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
                         dp[rt][kt] = mma(df[rt][dc], vf[kt][dc], dp[rt][kt]);
                     }
                 }
-            r0 += rw_n * kUnit;
-            if (r0 < n_rows) fetch(r0);
+            r0 += stride;
+            if (r0 < n_rows) {
+                fetch(r0);
+                look(r0 + stride);
+            }
 
-            unsigned seen[2] = {0, 0};
+            unsigned seen[KT] = {};
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const Row row = own[rt * 16 + 4 * g + i];
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
+                    for (int kt = 0; kt < KT; ++kt) {
                         const int key = key0 + kt * 16 + c;
-                        const bool ok = key <= (p.causal ? row.pos : k_len - 1);     // a row behind the last has no weight: lse is inf
+                        const bool ok = key <= (p.causal ? row.pos : k_len - 1);     
                         float z = s[rt][kt][i] * p.scale2;
                         if (p.n_buckets) z += buckets.value(buckets.at(row.pos - key), row.head);
                         const float x = ok ? __builtin_amdgcn_exp2f(z - row.lse) : 0.f;
@@ -659,9 +710,9 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
                         seen[kt] |= (unsigned)ok << (4 * rt + i);
                     }
                 }
-            V8<T> pf[2], sf[2];
+            V8<T> pf[KT], sf[KT];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
+            for (int kt = 0; kt < KT; ++kt) {
                 pf[kt] = pack<T>(s[0][kt], s[1][kt]);
                 sf[kt] = pack<T>(dp[0][kt], dp[1][kt]);
             }
@@ -669,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
             for (int dt = 0; dt < DT; ++dt) {
                 const V8<T> d = transposed<T, D>(stage_d, dt * 16, lane), q = transposed<T, D>(stage_q, dt * 16, lane);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
+                for (int kt = 0; kt < KT; ++kt) {
                     if constexpr (CAREFUL) {
                         av[kt][dt] = mma_masked<T>(d, pf[kt], seen[kt], av[kt][dt]);
                         ak[kt][dt] = mma_masked<T>(q, sf[kt], seen[kt], ak[kt][dt]);
@@ -683,12 +734,12 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     }
     bool odd = false;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) odd |= not_finite(ak[kt][dt]) || not_finite(av[kt][dt]);
     if (!CAREFUL) {
         odd = __syncthreads_or(odd);
-        if (tid == 0) flags[blockIdx.x] = odd;
+        if (tid == 0) flags[unit] = odd;
     }
 
     // wavefronts that share keys: the upper half hands its sums to the lower one, until one has them all
@@ -696,24 +747,24 @@ __global__ __launch_bounds__(kThreads) void keys_kernel(const Problem p, const T
     for (int half = rw_n >> 1; half; half >>= 1) {
         __syncthreads();
         if (rw >= half && rw < 2 * half) {
-            f32x4 *to = merge + ((rw - half) * kw_n + kw) * (4 * DT * 64) + lane;
+            f32x4 *to = merge + ((rw - half) * kw_n + kw) * (2 * KT * DT * 64) + lane;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) { to[(kt * DT + dt) * 128] = ak[kt][dt]; to[(kt * DT + dt) * 128 + 64] = av[kt][dt]; }
         }
         __syncthreads();
         if (rw < half) {
-            const f32x4 *from = merge + (rw * kw_n + kw) * (4 * DT * 64) + lane;
+            const f32x4 *from = merge + (rw * kw_n + kw) * (2 * KT * DT * 64) + lane;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) { ak[kt][dt] += from[(kt * DT + dt) * 128]; av[kt][dt] += from[(kt * DT + dt) * 128 + 64]; }
         }
     }
     if (rw) return;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < KT; ++kt) {
         const int key = key0 + kt * 16 + c;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -755,8 +806,8 @@ struct Layout {
     size_t delta, flags, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
 };
 
-int layout_of(const Problem &p, int head_len, int row_tiles, Layout *l) {
-    const int tpt = tile_tokens(p.group), block = 1 << p.block_shift, parts = std::max(1, block / (kWaves * kUnit));
+int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *l) {
+    const int tpt = tile_tokens(p.group), block = 1 << p.block_shift;
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
     auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
     l->n_groups = tiles(kWaves * row_tiles);
@@ -793,7 +844,8 @@ template <typename T, int D>
 int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_attention_grads *grads, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
     constexpr int RT = sizeof(T) == 4 ? 1 : 2;
     Layout l;
-    if (int rc = layout_of(p, D, RT, &l)) return rc;
+    const int block = 1 << p.block_shift, parts = Keys<T, D>::parts(block);
+    if (int rc = layout_of(p, D, RT, parts, &l)) return rc;
     if (need) { *need = l.bytes; return FG_OK; }
     if (bytes < l.bytes || (l.bytes && !workspace)) return fail(FG_ERR_ARG, "block attention gradients: a workspace of %zu bytes, %zu needed (fg_block_attention_backward_workspace)", bytes, l.bytes);
     Strides ds;
@@ -807,7 +859,8 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
         const dim3 blocks((unsigned)(p.batch * p.kv_heads * l.n_groups));
         const size_t few = few_stage_bytes<T, D>() + bias_bytes(p);
         if (l.many) {
-            queries_many_kernel<T, D, RT><<<blocks, threads, Steps<T, D>::kBytes + bias_bytes(p), stream>>>(p, step, ints(l.flags), l.n_groups);
+            if (p.n_buckets) queries_many_kernel<T, D, RT, true><<<blocks, threads, Steps<T, D, true>::kBytes + bias_bytes(p), stream>>>(p, step, ints(l.flags), l.n_groups);
+            else queries_many_kernel<T, D, RT, false><<<blocks, threads, Steps<T, D, false>::kBytes, stream>>>(p, step, ints(l.flags), l.n_groups);
             FG_HIP_TRY(hipGetLastError());
             queries_redo_kernel<T, D><<<blocks, threads, few, stream>>>(p, step, ints(l.flags), l.n_groups, kWaves * RT);
         } else {
@@ -822,7 +875,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     if (!grads->dk || l.all == 0) return FG_OK;
     auto bits = reinterpret_cast<unsigned long long *>(w + l.bits);
     auto pieces = reinterpret_cast<Piece *>(w + l.table);
-    const int all = (int)l.all, per_wave = (all + kWaves - 1) / kWaves, block = 1 << p.block_shift, parts = std::max(1, block / (kWaves * kUnit));
+    const int all = (int)l.all, per_wave = (all + kWaves - 1) / kWaves;
     mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), threads, 0, stream>>>(p, bits, l.chunks);
     count_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
     scan_kernel<<<dim3(1), dim3(kScan), 0, stream>>>(ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), all, l.piece);

@@ -26,6 +26,7 @@ class FgPlanOpts(ctypes.Structure):
                 ("pass_buffers", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
 
 
+# fg_block_attention_args: the calls take a pointer to one, or its bytes
 class FgBlockAttentionArgs(ctypes.Structure):
     _fields_ = [("type", ctypes.c_int32), ("batch", ctypes.c_int32), ("queries", ctypes.c_int32), ("keys", ctypes.c_int32),
                 ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_len", ctypes.c_int32), ("block", ctypes.c_int32),
@@ -100,10 +101,10 @@ SIGNATURES = {
     "fg_graph_attention_additive_backward_elv_f32": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, ctypes.c_float, _vp]),
     "fg_block_pool": (_int, [_int, _vp, ctypes.POINTER(_i64), _vp, _vp, _int, _int, _int, _int, _int, _vp]),
     "fg_block_select": (_int, [_int, _vp, ctypes.POINTER(_i64), _vp, _vp, _vp, _vp] + [_int] * 11 + [_vp]),
-    "fg_block_attention_workspace": (_i64, [ctypes.POINTER(FgBlockAttentionArgs)]),
-    "fg_block_attention": (_int, [ctypes.POINTER(FgBlockAttentionArgs), _vp, ctypes.c_size_t, _vp]),
-    "fg_block_attention_backward_workspace": (_i64, [ctypes.POINTER(FgBlockAttentionArgs)]),
-    "fg_block_attention_backward": (_int, [ctypes.POINTER(FgBlockAttentionArgs), ctypes.POINTER(FgBlockAttentionGrads), _vp, ctypes.c_size_t, _vp]),
+    "fg_block_attention_workspace": (_i64, [_vp]),
+    "fg_block_attention": (_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "fg_block_attention_backward_workspace": (_i64, [_vp]),
+    "fg_block_attention_backward": (_int, [_vp, ctypes.POINTER(FgBlockAttentionGrads), _vp, ctypes.c_size_t, _vp]),
     "fg_synth_powerlaw_csr": (_int, [_i64, _vp, _vp, _vp, ctypes.c_uint64, _int, _vp, _vp]),
     "fg_synth_community_csr": (_int, [_i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, ctypes.c_double, ctypes.c_uint64, _int, _vp, _vp]),
 }

@@ -101,6 +101,29 @@ __global__ __launch_bounds__(kScan) void scan_kernel(const int32_t *count, int32
     if (tid == 0) totals[0] = base[1];
 }
 
+// Short sequences, whose lists are never cut: a place for every query in every block's list, which one wavefront per block finds by looking
+// through the selections themselves.
+__global__ __launch_bounds__(kThreads) void short_lists_kernel(const Problem p, int32_t *count, int32_t *list, int all) {
+    const int m = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (m >= all) return;
+    const int pair = m / p.blocks, blk = m - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads, key = blk << p.block_shift;
+    const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
+    const int64_t row = (int64_t)p.kv_heads * p.topk;
+    const int32_t *src = p.list + (int64_t)b * p.queries * row + (int64_t)h * p.topk;
+    int32_t *dst = list + (int64_t)m * p.queries;
+    int n = 0;
+    // causal queries before the block do not see it
+    for (int t0 = p.causal ? max(key - offset, 0) & ~63 : 0; t0 < q_len; t0 += 64) {
+        const int t = t0 + lane;
+        bool named = false;
+        for (int j = 0; j < p.topk; ++j) named |= src[min(t, q_len - 1) * row + j] == blk;
+        const unsigned long long all_named = __ballot(named && t < q_len && key < k_len && (!p.causal || key <= offset + t));
+        if ((all_named >> lane) & 1) dst[n + __popcll(all_named & ((1ull << lane) - 1))] = t;
+        n += __popcll(all_named);
+    }
+    if (lane == 0) count[m] = n;
+}
+
 // The tokens of every block in ascending order, and its pieces: one wavefront per block.
 __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long *bits, const int32_t *count, const int32_t *offset, const int32_t *piece0,
                                                         const int32_t *slot0, int32_t *list, Piece *pieces, int all, int blocks, int chunks, int piece) {
@@ -579,7 +602,7 @@ template <typename T, int D> struct Keys {
 
 template <typename T, int D, bool CAREFUL>
 __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
-                                                        const int32_t *totals, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
+                                                        const int32_t *totals, const int32_t *count, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
@@ -589,8 +612,8 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     const int kw = wave % kw_n, rw = wave / kw_n;
     // (dealt to the XCDs in turn: contiguous shares, for the L2s' sake, are uneven and take 4 to 15 % more)
     const int unit = blockIdx.x, work = unit / parts, part = unit - work * parts;
-    if (work >= totals[0] || (CAREFUL && !flags[unit])) return;
-    const Piece piece = pieces[work];
+    if ((count ? false : work >= totals[0]) || (CAREFUL && !flags[unit])) return;
+    const Piece piece = count ? Piece{work, work * p.queries, count[work], -1} : pieces[work];      // short lists have a place each
     const int pair = piece.block / p.blocks, blk = piece.block - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
     const int in_block = (part * kw_n + kw) * 16 * KT, key0 = (blk << p.block_shift) + in_block, n_rows = piece.len * p.group;
@@ -800,7 +823,7 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(const Problem p, const
 // ---- host -------------------------------------------------------------------------------------------------
 
 struct Layout {
-    bool many;
+    bool many, short_lists;
     int n_groups, chunks, piece;               // n_groups: workgroups per sequence and key head of the sweep by query
     int64_t all, pieces, slots, entries;       // blocks of all sequences and key heads; bounds on the others
     size_t delta, flags, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
@@ -816,9 +839,11 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     l->chunks = std::max(1, (p.queries + 63) / 64);
     l->piece = std::max(1, kPieceRows / p.group);
     l->all = pairs * p.blocks;
-    l->entries = pairs * p.queries * std::min(p.topk, p.blocks);
-    l->pieces = l->all + l->entries / l->piece;
-    l->slots = 2 * (l->entries / l->piece);
+    // short lists: one kernel instead of five, whose looks through the selections stay below their launches' time
+    l->short_lists = p.queries <= l->piece && (int64_t)p.queries * p.topk <= 4096;
+    l->entries = l->short_lists ? l->all * p.queries : pairs * p.queries * std::min(p.topk, p.blocks);
+    l->pieces = l->short_lists ? l->all : l->all + l->entries / l->piece;
+    l->slots = p.queries <= l->piece ? 0 : 2 * (l->entries / l->piece);
     const int64_t limit = INT32_MAX;
     if (l->entries > limit || l->pieces * parts > limit || l->all * (2 * block * head_len / 4 / kThreads) > limit || pairs * std::max(l->n_groups, l->chunks) > limit)
         return fail(FG_ERR_SHAPE, "block attention gradients: %lld selections of %lld blocks do not fit the 32-bit lists", (long long)l->entries, (long long)l->all);
@@ -826,14 +851,14 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     auto place = [&](size_t n) { const size_t here = at; at += (n + 255) & ~(size_t)255; return here; };
     l->delta = place((size_t)p.batch * p.queries * p.heads * sizeof(float));
     l->flags = place((size_t)std::max(pairs * l->n_groups, l->pieces * parts) * sizeof(int32_t));
-    l->bits = place((size_t)l->all * l->chunks * 8);
+    l->bits = place(l->short_lists ? 0 : (size_t)l->all * l->chunks * 8);
     l->count = place((size_t)l->all * 4);
     l->offset = place((size_t)l->all * 4);
     l->piece0 = place((size_t)l->all * 4);
     l->slot0 = place((size_t)l->all * 4);
     l->totals = place(4);
     l->list = place((size_t)l->entries * 4);
-    l->table = place((size_t)l->pieces * sizeof(Piece));
+    l->table = place(l->short_lists ? 0 : (size_t)l->pieces * sizeof(Piece));
     l->partial = place((size_t)l->slots * 2 * block * head_len * sizeof(float));
     l->bias = place((size_t)p.batch * l->n_groups * p.heads * p.n_buckets * sizeof(float));
     l->bytes = at;
@@ -876,13 +901,19 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     auto bits = reinterpret_cast<unsigned long long *>(w + l.bits);
     auto pieces = reinterpret_cast<Piece *>(w + l.table);
     const int all = (int)l.all, per_wave = (all + kWaves - 1) / kWaves;
-    mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), threads, 0, stream>>>(p, bits, l.chunks);
-    count_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
-    scan_kernel<<<dim3(1), dim3(kScan), 0, stream>>>(ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), all, l.piece);
-    fill_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
+    if (l.short_lists) {
+        short_lists_kernel<<<dim3(per_wave), threads, 0, stream>>>(p, ints(l.count), ints(l.list), all);
+    } else {
+        mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), threads, 0, stream>>>(p, bits, l.chunks);
+        count_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
+        scan_kernel<<<dim3(1), dim3(kScan), 0, stream>>>(ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), all, l.piece);
+        fill_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
+    }
+    FG_HIP_TRY(hipGetLastError());
     const size_t lds = keys_stage_bytes<T, D>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);
     auto keys = [&](auto kernel) {
-        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, a->lse, floats(l.delta), pieces, ints(l.totals), ints(l.list),
+        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, a->lse, floats(l.delta), pieces, ints(l.totals),
+                                                                             l.short_lists ? ints(l.count) : nullptr, ints(l.list),
                                                                              floats(l.partial), static_cast<T *>(grads->dk), static_cast<T *>(grads->dv), ints(l.flags));
     };
     keys(keys_kernel<T, D, false>);

@@ -58,25 +58,12 @@ def _rows(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _on(device):
-    """A guard that makes `device` current, or None where it is already: the common case, without the guard's 2 us."""
-    return None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-class _Call(object):
-    """The library, and the current stream of the tensors' device, for the calls inside."""
-
-    def __init__(self, device):
-        self._guard = _on(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return _lib.lib(), common.stream_ptr()
-
-    def __exit__(self, *error):
-        if self._guard is not None:
-            self._guard.__exit__(*error)
+def _call(device, f):
+    """f(library, current stream) with `device` current; the common case, where it is already, without the guard's 2 us."""
+    if torch.cuda.current_device() == device.index:
+        return f(_lib.lib(), common.stream_ptr())
+    with torch.cuda.device(device):
+        return f(_lib.lib(), common.stream_ptr())
 
 
 def _ptr(t):
@@ -99,9 +86,8 @@ def block_pool(k, block_size, lengths):
         raise ValueError("k has no heads: shape %s" % (tuple(k.shape),))
     k = _rows(k)
     pooled = torch.empty((batch, kv_heads, -(-keys // block_size), head_len), dtype=k.dtype, device=k.device)
-    with _Call(k.device) as (L, stream):
-        _lib.check(L.fg_block_pool(_TYPES[k.dtype], k.data_ptr(), _strides(k), _ptr(lengths), pooled.data_ptr(), batch, keys, kv_heads, head_len,
-                                   block_size, stream))
+    _lib.check(_call(k.device, lambda L, stream: L.fg_block_pool(
+        _TYPES[k.dtype], k.data_ptr(), _strides(k), _ptr(lengths), pooled.data_ptr(), batch, keys, kv_heads, head_len, block_size, stream)))
     return pooled
 
 
@@ -122,14 +108,30 @@ def block_select(q, pooled, num_keys, block_size, topk, causal, lengths, q_lengt
     if pooled.data_ptr() % 16:
         pooled = pooled.clone()
     blocks = torch.empty((batch, queries, kv_heads, topk), dtype=torch.int32, device=q.device)
-    with _Call(q.device) as (L, stream):
-        _lib.check(L.fg_block_select(_TYPES[q.dtype], q.data_ptr(), _strides(q), pooled.data_ptr(), _ptr(lengths), _ptr(q_lengths), blocks.data_ptr(),
-                                     batch, queries, num_keys, heads, kv_heads, head_len, block_size, topk, int(causal), keep_first, keep_last, stream))
+    _lib.check(_call(q.device, lambda L, stream: L.fg_block_select(
+        _TYPES[q.dtype], q.data_ptr(), _strides(q), pooled.data_ptr(), _ptr(lengths), _ptr(q_lengths), blocks.data_ptr(), batch, queries, num_keys,
+        heads, kv_heads, head_len, block_size, topk, int(causal), keep_first, keep_last, stream)))
     return blocks
+
+
+def _plain(q, k, v, blocks, block_size):
+    """Whether the arguments are fine as they are, at a glance (1 us); what is not is looked at one by one for the message."""
+    try:
+        batch, queries, heads, head_len = q.shape
+        _, keys, kv_heads, _ = k.shape
+        device, dtype = q.device, q.dtype
+        return (k.shape == (batch, keys, kv_heads, head_len) and v.shape == k.shape and blocks.shape[:3] == (batch, queries, kv_heads)
+                and blocks.dim() == 4 and blocks.shape[3] > 0 and blocks.dtype == torch.int32 and dtype in _TYPES and k.dtype == dtype and v.dtype == dtype
+                and device.type == "cuda" and k.device == device and v.device == device and blocks.device == device and head_len in HEAD_LENGTHS
+                and block_size in BLOCK_SIZES and kv_heads > 0 and heads % kv_heads == 0 and 1 <= heads // kv_heads <= MAX_GROUP)
+    except (AttributeError, ValueError, TypeError, IndexError):
+        return False
 
 
 def check_attention(q, k, v, blocks, block_size, lengths, q_lengths, bias, bounds):
     """The bounds as a tuple, after everything that can be seen of the arguments without looking at their values on the GPU."""
+    if bias is None and bounds is None and lengths is None and q_lengths is None and _plain(q, k, v, blocks, block_size):
+        return ()
     _check("q", q, 4)
     _check("k", k, 4, q)
     _check("v", v, 4, q)
@@ -162,31 +164,39 @@ def check_attention(q, k, v, blocks, block_size, lengths, q_lengths, bias, bound
     return bounds
 
 
-# fg_block_attention_args as bytes: 10 whole numbers, scale, buckets, bounds; pointers and strides
-_PLAIN = struct.Struct("=10ifi63i")
+# fg_block_attention_args as bytes: whole numbers, scale, buckets and bounds; pointers and strides
+_SIZES = struct.Struct("=10ifi63i4x")
 _REST = struct.Struct("=3Q9q7Q")
-assert ctypes.sizeof(_lib.FgBlockAttentionArgs) == (_PLAIN.size + 7) // 8 * 8 + _REST.size
+assert ctypes.sizeof(_lib.FgBlockAttentionArgs) == _SIZES.size + _REST.size and _lib.FgBlockAttentionArgs.q.offset == _SIZES.size
 
 
-def _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest):
-    """(fg_block_attention_args, the part of it that the workspace's size goes by)."""
-    batch, queries, heads, head_len = q.shape
-    sizes = (_TYPES[q.dtype], batch, queries, k.shape[1], heads, k.shape[2], head_len, block_size, blocks.shape[3], causal,
-             scale, 0 if bias is None else len(bounds) + 1) + bounds + (0,) * (63 - len(bounds))
-    a = _lib.FgBlockAttentionArgs()
-    _PLAIN.pack_into(a, 0, *sizes)
-    _REST.pack_into(a, (_PLAIN.size + 7) // 8 * 8, q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                    blocks.data_ptr(), _ptr(lengths), _ptr(q_lengths), _ptr(bias), out.data_ptr(), _ptr(lse), _ptr(rest))
-    return a, sizes
+class _Sizes(object):
+    """The part of a call's arguments that goes by its tensors' sizes, and the device memory that it needs."""
+
+    def __init__(self, sizes, bounds, buckets):
+        self.bytes = _SIZES.pack(*sizes, buckets, *bounds, *(0,) * (63 - len(bounds)))
+        self._need = [None, None]
+
+    def workspace(self, backward):
+        if self._need[backward] is None:
+            L, raw = _lib.lib(), self.bytes + bytes(_REST.size)
+            self._need[backward] = _lib.check((L.fg_block_attention_backward_workspace if backward else L.fg_block_attention_workspace)(raw))
+        return self._need[backward]
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(sizes, backward):
-    """Bytes of device memory that a call of these sizes needs."""
-    a = _lib.FgBlockAttentionArgs()
-    _PLAIN.pack_into(a, 0, *sizes)
-    L = _lib.lib()
-    return _lib.check((L.fg_block_attention_backward_workspace if backward else L.fg_block_attention_workspace)(ctypes.byref(a)))
+def _sizes(*key):
+    return _Sizes(*key)
+
+
+def _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest):
+    """(the part of fg_block_attention_args that goes by sizes, all of it as bytes)."""
+    batch, queries, heads, head_len = q.shape
+    _, keys, kv_heads, _ = k.shape
+    sizes = _sizes((_TYPES[q.dtype], batch, queries, keys, heads, kv_heads, head_len, block_size, blocks.shape[3], causal, scale), bounds,
+                   0 if bias is None else len(bounds) + 1)
+    return sizes, sizes.bytes + _REST.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                                           blocks.data_ptr(), _ptr(lengths), _ptr(q_lengths), _ptr(bias), out.data_ptr(), _ptr(lse), _ptr(rest))
 
 
 def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, train):
@@ -194,14 +204,14 @@ def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths,
     and, in 16 bits, what rounding took from `out`."""
     q, k, v, blocks = _rows(q), _rows(k), _rows(v), blocks.contiguous()
     bias = None if bias is None else bias.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if train else None
+    device = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
-    a, sizes = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
-    need = _workspace(sizes, False)
-    with _Call(q.device) as (L, stream):
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _lib.check(L.fg_block_attention(ctypes.byref(a), _ptr(work), need, stream))
+    sizes, raw = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    need = sizes.workspace(False)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _lib.check(_call(device, lambda L, stream: L.fg_block_attention(raw, _ptr(work), need, stream)))
     return out, lse, rest
 
 
@@ -213,10 +223,9 @@ def block_attention_backward(q, k, v, blocks, block_size, scale, causal, lengths
     dq = new(q)
     dk, dv = (new(k), new(v)) if keys_too else (None, None)
     dbias = None if bias is None else new(bias)
-    a, sizes = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
+    sizes, raw = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
     grads = _lib.FgBlockAttentionGrads(dout.data_ptr(), _strides(dout), dq.data_ptr(), _ptr(dk), _ptr(dv), _ptr(dbias))
-    need = _workspace(sizes, True)
-    with _Call(q.device) as (L, stream):
-        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _lib.check(L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), _ptr(work), need, stream))
+    need = sizes.workspace(True)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(_call(q.device, lambda L, stream: L.fg_block_attention_backward(raw, ctypes.byref(grads), _ptr(work), need, stream)))
     return dq, dk, dv, dbias

@@ -248,7 +248,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int unit = xcd_contiguous_block(), pair = unit / n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
-    const int tpt = tile_tokens(p.group), t0 = (unit - pair * n_groups) * TILES * tpt;
+    const int tpt = tile_tokens(p.group), t0 = group_of(p, unit - pair * n_groups, n_groups) * TILES * tpt;
     const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
     const bool used = tc < tpt;
 
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void redo_kernel(const Problem p, const R
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int unit = xcd_contiguous_block();
     if (!flags[unit]) return;
-    const int pair = unit / n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads, first = (unit - pair * n_groups) * tiles;
+    const int pair = unit / n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads, first = group_of(p, unit - pair * n_groups, n_groups) * tiles;
     Buckets buckets;
     if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + few_stage_bytes<T, D>());
     for (int i = 0; i < tiles; ++i) few_rows<T, D, true>(p, r, shared, dynamic, buckets, b, h, first + i, 0, 1);

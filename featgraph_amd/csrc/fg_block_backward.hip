@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kMergeStride = 36;       // floats between rows of the joining buffer (32 and 4 of padding)
 constexpr int kWindow = 1024;          // blocks looked at together
-constexpr int kPieceRows = 2048;       // rows (tokens times heads of the group) of one piece of a block's list
 
 struct Piece { int32_t block, start, len, slot; };     // block: of all sequences and key heads; slot: where its sums go, -1: they are all
 
@@ -395,7 +394,7 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     __shared__ List<TILES, kListed> list;
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const int unit = xcd_contiguous_block(), pair = unit / n_groups, group = unit - pair * n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int unit = xcd_contiguous_block(), pair = unit / n_groups, group = group_of(p, unit - pair * n_groups, n_groups), b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
     const int tpt = tile_tokens(p.group), t0 = group * TILES * tpt;
     const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;
@@ -554,7 +553,7 @@ __global__ __launch_bounds__(kThreads) void queries_redo_kernel(const Problem p,
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int unit = xcd_contiguous_block();
     if (!flags[unit]) return;
-    const int pair = unit / n_groups, group = unit - pair * n_groups, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int pair = unit / n_groups, group = group_of(p, unit - pair * n_groups, n_groups), b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     Buckets buckets;
     float *sums = nullptr;
     if (p.n_buckets) {
@@ -837,7 +836,12 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     l->many = pairs * l->n_groups >= 256 && 2 * p.queries >= kWaves * row_tiles * tpt;
     if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
-    l->piece = std::max(1, kPieceRows / p.group);
+    // a block's list is cut into pieces of 768 to 2,048 rows (tokens times heads of the group), some 1,024 pieces in all: longer
+    // pieces leave CUs idle at the end, shorter ones write more sums. All of the keys' gradients with pieces of 1,024 / 1,536 /
+    // 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 / 219 us, 8,192 of 16 / 1 heads of 64 216 / 217 / 248,
+    // 2 x 4,096 of 16 / 4 heads of 128 410 / 398 / 396
+    const int64_t rows = pairs * p.queries * std::min(p.topk, p.blocks) * p.group;
+    l->piece = (int)std::max<int64_t>(1, std::min<int64_t>(2048, std::max<int64_t>(768, rows / 1024)) / p.group);
     l->all = pairs * p.blocks;
     // short lists: one kernel instead of five, whose looks through the selections stay below their launches' time
     l->short_lists = p.queries <= l->piece && (int64_t)p.queries * p.topk <= 4096;

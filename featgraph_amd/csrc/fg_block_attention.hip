@@ -152,14 +152,19 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { s[0][i] = __builtin_amdgcn_exp2f(s[0][i] - ref); s[1][i] = __builtin_amdgcn_exp2f(s[1][i] - ref); }
                 l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-                // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not
-                const V8<T> pf = pack<T>(s[0], s[1]);
+                // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not.  For gradients
+                // what the rounding took follows in a second product, as in many_kernel.
+                V8<T> pf, pl;
+                block::split<T>(s[0], s[1], &pf, &pl);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
                     if constexpr (decltype(careful)::value) o[dt] = mma_masked<T>(vf, pf, seen, o[dt]);
                     else o[dt] = mma(vf, pf, o[dt]);
                 }
+                if (sizeof(T) == 2 && !decltype(careful)::value && r.rest)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[dt] = mma(transposed<T, D>(stage, dt * 16, lane), pl, o[dt]);
             }
         }
     };
@@ -239,7 +244,10 @@ template <typename T, int D> struct Steps {
 };
 
 // RT tiles of 16 rows per wavefront.  flags[workgroup]: whether a result was not finite (see redo_kernel).
-template <typename T, int D, int RT, bool BIAS>
+// EXACT: what the powers' rounding took goes into a second product with V.  Gradients start from <dO, O>, which a row's dS takes away from
+// numbers of its own size: with rounded powers it would be further off than the gradients' own rounding (2 x 4,096 tokens, 16 / 4 heads
+// 174 and 210 us).
+template <typename T, int D, int RT, bool BIAS, bool EXACT>
 __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, const Results r, int32_t *flags, int n_groups) {
     constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;
     constexpr int KS = Steps<T, D>::kKeyStride, VS = Steps<T, D>::kValueStride;
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
                         m[rt] = up;
                     }
                 }
-                V8<T> pf[RT];
+                V8<T> pf[RT], pl[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     float from = m[rt] == -__builtin_inff() ? 0.f : m[rt];
@@ -419,7 +427,8 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[rt][kt][i] = __builtin_amdgcn_exp2f(s[rt][kt][i] * factor - from);
                     // rounded to the operands' type for the product with V, half a step each
-                    pf[rt] = pack<T>(s[rt][0], s[rt][1]);
+                    if (EXACT) split<T>(s[rt][0], s[rt][1], &pf[rt], &pl[rt]);
+                    else pf[rt] = pack<T>(s[rt][0], s[rt][1]);
                 }
                 if (r.lse)
 #pragma unroll
@@ -432,11 +441,17 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
 #pragma unroll
                     for (int i = 0; i < DT / 2; ++i)
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) o[rt][half * (DT / 2) + i] = mma(vf[i], pf[rt], o[rt][half * (DT / 2) + i]);
+                        for (int rt = 0; rt < RT; ++rt) {
+                            o[rt][half * (DT / 2) + i] = mma(vf[i], pf[rt], o[rt][half * (DT / 2) + i]);
+                            if (EXACT) o[rt][half * (DT / 2) + i] = mma(vf[i], pl[rt], o[rt][half * (DT / 2) + i]);
+                        }
                     if (half == 0) read_values(1);
                 }
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) total[rt] = mma(ones, pf[rt], total[rt]);
+                for (int rt = 0; rt < RT; ++rt) {
+                    total[rt] = mma(ones, pf[rt], total[rt]);
+                    if (EXACT) total[rt] = mma(ones, pl[rt], total[rt]);
+                }
             }
         }
     }
@@ -530,8 +545,17 @@ int launch(const Problem &p, const fg_block_attention_args *a, void *workspace, 
     const dim3 blocks((unsigned)grid), threads(kThreads);
     if (s.many) {
         int32_t *marks = reinterpret_cast<int32_t *>(w);
-        if (p.n_buckets) many_kernel<T, D, RT, true><<<blocks, threads, Steps<T, D>::kBytes + bias, stream>>>(p, r, marks, s.n_tiles);
-        else many_kernel<T, D, RT, false><<<blocks, threads, Steps<T, D>::kBytes, stream>>>(p, r, marks, s.n_tiles);
+        auto go = [&](auto exact) {
+            constexpr bool EXACT = decltype(exact)::value;
+            if (p.n_buckets) many_kernel<T, D, RT, true, EXACT><<<blocks, threads, Steps<T, D>::kBytes + bias, stream>>>(p, r, marks, s.n_tiles);
+            else many_kernel<T, D, RT, false, EXACT><<<blocks, threads, Steps<T, D>::kBytes, stream>>>(p, r, marks, s.n_tiles);
+        };
+        if constexpr (sizeof(T) == 2) {
+            if (r.rest) go(std::true_type{});
+            else go(std::false_type{});
+        } else {
+            go(std::false_type{});
+        }
         FG_HIP_TRY(hipGetLastError());
         redo_kernel<T, D><<<blocks, threads, few_stage_bytes<T, D>() + bias, stream>>>(p, r, marks, s.n_tiles, kWaves * RT);
     } else {

@@ -596,6 +596,8 @@ template <typename T, int D> struct Keys {
     // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us)
     static constexpr int kTiles = sizeof(T) == 4 ? 1 : 2;
     static constexpr int kResident = D == 128 ? 1 : 2;
+    // powers of rows with many keys are small: in 16-bit floats they are kept 2^10 times as large, away from the smallest numbers
+    static constexpr int kGain = std::is_same<T, _Float16>::value ? 10 : 0;
     static int parts(int block) { return std::max(1, block / (kWaves * 16 * kTiles)); }       // workgroups of a block
 };
 
@@ -603,6 +605,7 @@ template <typename T, int D, bool CAREFUL>
 __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
                                                         const int32_t *totals, const int32_t *count, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
+    constexpr float kLess = 1.f / (1 << Keys<T, D>::kGain);
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -658,7 +661,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         };
         auto fetch = [&](int r0) {
             const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
-            next = Row{lse[row], delta[row], offset + token, x};
+            next = Row{lse[row] - Keys<T, D>::kGain, delta[row] * kLess, offset + token, x};
             if (r0 + (lane & 31) >= n_rows) next = Row{__builtin_inff(), 0.f, -1, 0};     // a row behind the last has no weight
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
@@ -728,14 +731,16 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         if (p.n_buckets) z += buckets.value(buckets.at(row.pos - key), row.head);
                         const float x = ok ? __builtin_amdgcn_exp2f(z - row.lse) : 0.f;
                         s[rt][kt][i] = x;
-                        dp[rt][kt][i] = ok ? x * (dp[rt][kt][i] - row.delta) : 0.f;
+                        dp[rt][kt][i] = ok ? x * (dp[rt][kt][i] * kLess - row.delta) : 0.f;
                         seen[kt] |= (unsigned)ok << (4 * rt + i);
                     }
                 }
-            V8<T> pf[KT], sf[KT];
+            // the powers go into dV's product rounded, and what that took (in 16 bits) in a second one: nearly even ones are all rounded the
+            // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 372 and 399 us)
+            V8<T> pf[KT], pl[KT], sf[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                pf[kt] = pack<T>(s[0][kt], s[1][kt]);
+                split<T>(s[0][kt], s[1][kt], &pf[kt], &pl[kt]);
                 sf[kt] = pack<T>(dp[0][kt], dp[1][kt]);
             }
 #pragma unroll
@@ -748,6 +753,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         ak[kt][dt] = mma_masked<T>(q, sf[kt], seen[kt], ak[kt][dt]);
                     } else {
                         av[kt][dt] = mma(d, pf[kt], av[kt][dt]);
+                        if (sizeof(T) == 2) av[kt][dt] = mma(d, pl[kt], av[kt][dt]);
                         ak[kt][dt] = mma(q, sf[kt], ak[kt][dt]);
                     }
                 }
@@ -763,6 +769,12 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         odd = __syncthreads_or(odd);
         if (tid == 0) flags[unit] = odd;
     }
+
+    if (Keys<T, D>::kGain)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) av[kt][dt] *= kLess;
 
     // wavefronts that share keys: the upper half hands its sums to the lower one, until one has them all
     f32x4 *merge = reinterpret_cast<f32x4 *>(dynamic);

@@ -12,6 +12,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
+
 #include "fg_common.h"
 #include "fg_device.h"
 
@@ -300,7 +302,9 @@ __device__ __forceinline__ Buckets load_buckets(const Problem &p, int h, unsigne
     const T *src = static_cast<const T *>(p.bias);
     for (int i = threadIdx.x; i < p.n_buckets * p.group; i += kThreads) {
         const int n = i / p.group;
-        bias[i] = (float)src[(int64_t)n * p.heads + h * p.group + (i - n * p.group)] * kLog2e;
+        // the type's lowest value, used as a mask, stays finite: rows that see nothing else have a softmax
+        const float x = (float)src[(int64_t)n * p.heads + h * p.group + (i - n * p.group)], y = x * kLog2e;
+        bias[i] = fabsf(x) < __builtin_inff() ? fminf(fmaxf(y, -FLT_MAX), FLT_MAX) : y;
     }
     return Buckets{lds, bias, p.low, p.high, p.group};
 }

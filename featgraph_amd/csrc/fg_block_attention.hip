@@ -25,12 +25,18 @@ constexpr int kMergeStride = 36;       // floats between rows of the joining buf
 
 // ---- few queries ------------------------------------------------------------------------------------------
 
+// What gradients start from: a row's scores are relative to the first number, their powers' sum is 2 to the second.  In one number a reference
+// beyond 2^24, of a row that sees only masked keys, would take the sum away.
+__device__ __forceinline__ float2 log_sum(float reference, float sum) {
+    return sum == 0.f ? make_float2(__builtin_inff(), 0.f) : make_float2(reference, __builtin_amdgcn_logf(sum));
+}
+
 template <typename T, int D> constexpr size_t few_stage_bytes() {
     const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
     return values > merge ? values : merge;
 }
 
-struct Results { void *out, *rest; float *lse, *part; float2 *part_stats; };
+struct Results { void *out, *rest; float2 *lse; float *part; float2 *part_stats; };
 
 struct FewShared {
     List<1, 1024> list;
@@ -211,7 +217,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
             if (splits == 1) {
                 const float inv = st.y == 0.f ? 0.f : 1.f / st.y;
                 store_row<T>(static_cast<T *>(r.out), static_cast<T *>(r.rest), at * D + strip * 32 + col, sum * inv);
-                if (strip == 0 && col == 0 && r.lse) r.lse[at] = st.y == 0.f ? __builtin_inff() : st.x + __builtin_amdgcn_logf(st.y);
+                if (strip == 0 && col == 0 && r.lse) r.lse[at] = log_sum(st.x, st.y);
             } else {
                 *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + strip * 32 + col) = sum;
                 if (strip == 0 && col == 0) r.part_stats[split * all_rows + at] = st;
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
     const int sub_shift = p.block_shift - 5;
 
     // The sum that divides the output is that of the rounded powers, which are the weights of the product (a product with ones makes it):
-    // a row that one key dominates keeps that key's value to the last bit.  lse is the logarithm of the powers' own sum.
+    // a row that one key dominates keeps that key's value to the last bit.
     f32x4 o[RT][DT], total[RT];
     float m[RT], l[RT];
     V8<T> ones;
@@ -374,14 +380,14 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
                     for (int rt = 0; rt < RT; ++rt) {
                         const int pos = offset + t0 + (wave * RT + rt) * tpt;
                         const int near = buckets.at(pos - key0[x] - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - key0[x]);
-                        const float y = buckets.value(near, mine);
+                        const float y = near == far ? buckets.value(near, mine) : 0.f;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) { s[rt][0][i] = s[rt][0][i] * p.scale2 + y; s[rt][1][i] = s[rt][1][i] * p.scale2 + y; }
                         if (near != far)
 #pragma unroll
                             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) s[rt][kt][i] += buckets.value(buckets.at(pos + tc - (key0[x] + 16 * kt + 4 * g + i)), mine) - y;
+                                for (int i = 0; i < 4; ++i) s[rt][kt][i] += buckets.value(buckets.at(pos + tc - (key0[x] + 16 * kt + 4 * g + i)), mine);
                     }
                 }
                 // a row that did not select the block has its powers taken from +inf: 0, whatever finite scores it has there.  Only keys
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
             odd |= not_finite(o[rt][dt]);
             if (write) store_row<T>(static_cast<T *>(r.out), static_cast<T *>(r.rest), at * D + dt * 16 + 4 * g, o[rt][dt] * inv);
         }
-        if (write && g == 0 && r.lse) r.lse[at] = sum == 0.f ? __builtin_inff() : m[rt] + __builtin_amdgcn_logf(sum);
+        if (write && g == 0 && r.lse) r.lse[at] = log_sum(m[rt], sum);
     }
     odd = __syncthreads_or(odd);
     if (tid == 0) flags[unit] = odd;
@@ -488,7 +494,7 @@ __global__ __launch_bounds__(kThreads) void redo_kernel(const Problem p, const R
 
 // Joins the sums of several workgroups per row: four columns a thread.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const float2 *part_stats, T *out, T *remainder, float *lse, int64_t rows, int splits) {
+__global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const float2 *part_stats, T *out, T *remainder, float2 *lse, int64_t rows, int splits) {
     const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = e / (D / 4);
     const int col = (int)(e - row * (D / 4)) * 4;
     if (row >= rows) return;
@@ -504,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     store_row<T>(out, remainder, row * D + col, sum * inv);
-    if (col == 0 && lse) lse[row] = total == 0.f ? __builtin_inff() : top + __builtin_amdgcn_logf(total);
+    if (col == 0 && lse) lse[row] = log_sum(top, total);
 }
 
 // Which kernel takes a call, and how its work is cut.  many_kernel wants its workgroups' tiles at least half full and 256 workgroups (a CU each).
@@ -540,7 +546,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, void *workspace, 
     if (bytes < flags + sums + stats || (flags + sums && !workspace))
         return fail(FG_ERR_ARG, "block attention: a workspace of %zu bytes, %zu needed (fg_block_attention_workspace)", bytes, flags + sums + stats);
     unsigned char *w = static_cast<unsigned char *>(workspace);
-    const Results r{a->out, a->rest, a->lse, reinterpret_cast<float *>(w), reinterpret_cast<float2 *>(w + sums)};
+    const Results r{a->out, a->rest, reinterpret_cast<float2 *>(a->lse), reinterpret_cast<float *>(w), reinterpret_cast<float2 *>(w + sums)};
     const size_t bias = buckets_bytes(p.n_buckets, p.low, p.high, p.group);
     const dim3 blocks((unsigned)grid), threads(kThreads);
     if (s.many) {

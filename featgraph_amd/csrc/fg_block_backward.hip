@@ -1,4 +1,4 @@
-// Gradients of attention over selected blocks of keys.  With p_ij = 2^(z_ij - lse_i) the forward pass's softmax:
+// Gradients of attention over selected blocks of keys.  With p_ij = 2^(z_ij - m_i - log2 l_i) the forward pass's softmax:
 //   dP_ij = <dO_i, V_j>,  dS_ij = p_ij (dP_ij - delta_i),  delta_i = <dO_i, O_i>
 //   dQ_i = scale sum_j dS_ij K_j,  dK_j = scale sum_i dS_ij Q_i,  dV_j = sum_i p_ij dO_i,  dbias[n, h] = sum of dS_ij in bucket n
 //
@@ -149,12 +149,12 @@ __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long
 
 // ---- by query: dQ, dbias and delta ------------------------------------------------------------------------
 
-struct Step { const void *dout, *out, *rest; Strides ds; const float *lse; float *delta; void *dq; float *bias_sums; };
+struct Step { const void *dout, *out, *rest; Strides ds; const float2 *lse; float *delta; void *dq; float *bias_sums; };
 
 // A lane's row of a tile: dO and Q as operands, and delta.
 template <typename T, int D> struct Row16 {
     V8<T> q[D / 32], d[D / 32];
-    float lse, delta;
+    float lse, more, delta;            // powers are 2^(z - lse - more); more is 0 where one number holds both
     int limit;                         // last key that it may see; columns without a row see everything, nothing is written of them
     __device__ __forceinline__ void load(const Problem &p, const Step &w, int b, int t, int head, bool used, int q_len, int k_len, int offset, int g, bool write) {
         const bool there = used && t < q_len;
@@ -178,8 +178,18 @@ template <typename T, int D> struct Row16 {
             }
         }
         delta = rows_sum(sum);
-        lse = there ? w.lse[at] : __builtin_inff();
+        const float2 ls = there ? w.lse[at] : make_float2(__builtin_inff(), 0.f);
+        lse = ls.x;
+        more = ls.y;
         if (there && write && g == 0) w.delta[at] = delta;
+    }
+    // Whether a row of the wavefront is relative to a number, out of the bias, that would take its sum away (2^12 leaves it 11 bits more than
+    // a score of that size has).
+    __device__ __forceinline__ bool join() {
+        if (__any(fabsf(lse) > 4096.f && fabsf(lse) < __builtin_inff())) return true;
+        lse += more;
+        more = 0.f;
+        return false;
     }
 };
 
@@ -205,12 +215,12 @@ __device__ __forceinline__ void write_bias(const Problem &p, const float *sums, 
 }
 
 // Powers p = 2^(z - lse), and from them dS = p (dP - delta), of one tile and 32 keys, into s[]: with MASK, keys behind `last` have none.
-// The bias's gradient goes to `sums`.
+// The bias's gradient goes to `sums`.  far_off: `more` counts, and the scores are formed as the forward pass does.
 template <bool BIAS, bool MASK>
-__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float delta, int pos, int tpt,
-                                                    int tc, int mine, int key0, int last, int g, int lane) {
+__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float more, bool far_off, float delta,
+                                                    int pos, int tpt, int tc, int mine, int key0, int last, int g, int lane) {
     const int near = BIAS ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = BIAS ? buckets.at(pos + tpt - 1 - key0) : 0;
-    const float from = (BIAS && near == far ? buckets.value(near, mine) : 0.f) - lse;
+    const float from = (BIAS && near == far ? buckets.value(near, mine) : 0.f) - (BIAS && far_off ? 0.f : lse);
     unsigned seen = MASK ? 0 : 0xff;
     float total = 0.f;
 #pragma unroll
@@ -224,6 +234,7 @@ __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buck
                 bucket = buckets.at(pos + tc - key);
                 z += buckets.value(bucket, mine);
             }
+            if (BIAS && far_off) z = (z - lse) - more;
             float x = __builtin_amdgcn_exp2f(z) * (dp[kt][i] - delta);
             if (MASK) {
                 x = key <= last ? x : 0.f;
@@ -256,6 +267,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
     T *stage = reinterpret_cast<T *>(dynamic) + wave * kUnit * S;
     Row16<T, D> row;
     row.load(p, w, b, t0 + tc, head, used, q_len, k_len, offset, g, wave == 0);
+    const bool far_off = row.join();
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + 8 * g;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + 8 * g;
@@ -313,8 +325,8 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
                 u = find(u + kWaves);
                 if (u < units) fetch(u);
                 const unsigned seen = p.n_buckets
-                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane)
-                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
+                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.more, far_off, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane)
+                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.more, far_off, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
                 V8<T> sf, rf;          // as in queries_many_kernel
                 split<T>(s[0], s[1], &sf, &rf);
 #pragma unroll
@@ -411,6 +423,9 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     Row16<T, D> row[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
+    bool far_off = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) far_off |= row[rt].join();
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head;
@@ -505,11 +520,11 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
                 if (__any(edge)) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
+                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].more, far_off, row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
                 } else {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
+                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].more, far_off, row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
                 }
                 // dS goes into the product with K rounded, and what that took (in 16 bits) in a second one: a row's dS add up to 0, and its keys
                 // have much in common, so that the rounding alone would be larger than dQ's own
@@ -596,18 +611,16 @@ template <typename T, int D> struct Keys {
     // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us)
     static constexpr int kTiles = sizeof(T) == 4 ? 1 : 2;
     static constexpr int kResident = D == 128 ? 1 : 2;
-    // powers of rows with many keys are small: in 16-bit floats they are kept 2^10 times as large, away from the smallest numbers
-    static constexpr int kGain = std::is_same<T, _Float16>::value ? 10 : 0;
     static int parts(int block) { return std::max(1, block / (kWaves * 16 * kTiles)); }       // workgroups of a block
 };
 
 template <typename T, int D, bool CAREFUL>
-__global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float *lse, const float *delta, const Piece *pieces,
+__global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float2 *lse, const float *delta, const Piece *pieces,
                                                         const int32_t *totals, const int32_t *count, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
-    constexpr float kLess = 1.f / (1 << Keys<T, D>::kGain);
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
+    __shared__ float mores[kWaves][kUnit];
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int block = 1 << p.block_shift, kw_n = min(kWaves, block / (16 * KT)), rw_n = kWaves / kw_n, parts = block / (kw_n * 16 * KT);
@@ -643,6 +656,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     const T *qbase = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)h * p.group * p.qs.head + 8 * g;
     const T *dbase = dout + b * ds.batch + (int64_t)h * p.group * ds.head + 8 * g;
     Row *own = rows[wave];
+    float *more = mores[wave];         // with a bias, as Row16::more
 
     f32x4 ak[KT][DT], av[KT][DT];
     {
@@ -651,6 +665,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) ak[kt][dt] = av[kt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         V8<T> qf[2][DC], df[2][DC];
+        float next_more = 0.f;
         Row next;                      // lane 16 rt + c: row 16 rt + c of the step
         // the token of the lane's row of the step that is fetched next: its load has a step's time before the rows' own depend on it
         int token = 0, x = 0;
@@ -661,7 +676,9 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         };
         auto fetch = [&](int r0) {
             const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
-            next = Row{lse[row] - Keys<T, D>::kGain, delta[row] * kLess, offset + token, x};
+            const float2 ls = lse[row];
+            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + token, x};
+            next_more = ls.y;
             if (r0 + (lane & 31) >= n_rows) next = Row{__builtin_inff(), 0.f, -1, 0};     // a row behind the last has no weight
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
@@ -697,7 +714,10 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                     *reinterpret_cast<V8<T> *>(stage_q + (rt * 16 + c) * S + dc * 32 + 8 * g) = qf[rt][dc];
                     *reinterpret_cast<V8<T> *>(stage_d + (rt * 16 + c) * S + dc * 32 + 8 * g) = df[rt][dc];
                 }
-            if (lane < kUnit) own[lane] = next;
+            if (lane < kUnit) {
+                own[lane] = next;
+                if (p.n_buckets) more[lane] = next_more;
+            }
             wave_lds_sync();
             f32x4 s[2][KT], dp[2][KT];  // [rows][keys]
 #pragma unroll
@@ -729,9 +749,11 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         const bool ok = key <= (p.causal ? row.pos : k_len - 1);     
                         float z = s[rt][kt][i] * p.scale2;
                         if (p.n_buckets) z += buckets.value(buckets.at(row.pos - key), row.head);
-                        const float x = ok ? __builtin_amdgcn_exp2f(z - row.lse) : 0.f;
+                        z -= row.lse;
+                        if (p.n_buckets) z -= more[rt * 16 + 4 * g + i];
+                        const float x = ok ? __builtin_amdgcn_exp2f(z) : 0.f;
                         s[rt][kt][i] = x;
-                        dp[rt][kt][i] = ok ? x * (dp[rt][kt][i] * kLess - row.delta) : 0.f;
+                        dp[rt][kt][i] = ok ? x * (dp[rt][kt][i] - row.delta) : 0.f;
                         seen[kt] |= (unsigned)ok << (4 * rt + i);
                     }
                 }
@@ -769,12 +791,6 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         odd = __syncthreads_or(odd);
         if (tid == 0) flags[unit] = odd;
     }
-
-    if (Keys<T, D>::kGain)
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) av[kt][dt] *= kLess;
 
     // wavefronts that share keys: the upper half hands its sums to the lower one, until one has them all
     f32x4 *merge = reinterpret_cast<f32x4 *>(dynamic);
@@ -849,11 +865,12 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
     // a block's list is cut into pieces of 768 to 2,048 rows (tokens times heads of the group), some 1,024 pieces in all: longer
-    // pieces leave CUs idle at the end, shorter ones write more sums. All of the keys' gradients with pieces of 1,024 / 1,536 /
+    // pieces leave CUs idle at the end, shorter ones write more sums (of the largest calls longer ones, so that the sums need not much
+    // more memory than the gradients). All of the keys' gradients with pieces of 1,024 / 1,536 /
     // 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 / 219 us, 8,192 of 16 / 1 heads of 64 216 / 217 / 248,
     // 2 x 4,096 of 16 / 4 heads of 128 410 / 398 / 396
     const int64_t rows = pairs * p.queries * std::min(p.topk, p.blocks) * p.group;
-    l->piece = (int)std::max<int64_t>(1, std::min<int64_t>(2048, std::max<int64_t>(768, rows / 1024)) / p.group);
+    l->piece = (int)std::max<int64_t>(1, std::min(std::max<int64_t>(2048, rows / 8192), std::max<int64_t>(768, rows / 1024)) / p.group);
     l->all = pairs * p.blocks;
     // short lists: one kernel instead of five, whose looks through the selections stay below their launches' time
     l->short_lists = p.queries <= l->piece && (int64_t)p.queries * p.topk <= 4096;
@@ -894,7 +911,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     unsigned char *w = static_cast<unsigned char *>(workspace);
     auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w + at); };
     auto floats = [&](size_t at) { return reinterpret_cast<float *>(w + at); };
-    const Step step{grads->dout, a->out, a->rest, ds, a->lse, floats(l.delta), grads->dq, floats(l.bias)};
+    const Step step{grads->dout, a->out, a->rest, ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), grads->dq, floats(l.bias)};
     const dim3 threads(kThreads);
     if (p.queries) {
         const dim3 blocks((unsigned)(p.batch * p.kv_heads * l.n_groups));
@@ -928,7 +945,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     FG_HIP_TRY(hipGetLastError());
     const size_t lds = keys_stage_bytes<T, D>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);
     auto keys = [&](auto kernel) {
-        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, a->lse, floats(l.delta), pieces, ints(l.totals),
+        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), pieces, ints(l.totals),
                                                                              l.short_lists ? ints(l.count) : nullptr, ints(l.list),
                                                                              floats(l.partial), static_cast<T *>(grads->dk), static_cast<T *>(grads->dv), ints(l.flags));
     };

@@ -200,13 +200,13 @@ def _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, b
 
 
 def block_attention_forward(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, train):
-    """(out, lse, rest) of checked arguments; with `train` the latter are what the gradients start from: the logarithm of every row's sum
-    and, in 16 bits, what rounding took from `out`."""
+    """(out, lse, rest) of checked arguments; with `train` the latter are what the gradients start from: every row's reference and
+    the logarithm of its sum and, in 16 bits, what rounding took from `out`."""
     q, k, v, blocks = _rows(q), _rows(k), _rows(v), blocks.contiguous()
     bias = None if bias is None else bias.contiguous()
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if train else None
+    lse = torch.empty(q.shape[:3] + (2,), dtype=torch.float32, device=device) if train else None
     rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
     sizes, raw = _arguments(q, k, v, blocks, block_size, scale, causal, lengths, q_lengths, bias, bounds, out, lse, rest)
     need = sizes.workspace(False)

@@ -648,8 +648,9 @@ typedef struct {
     const void *bias;                  /* (n_buckets, heads) dense: added to the scaled score of query position i and key j in
                                           bucket  (number of bounds <= i - j) */
     void *out;                         /* (batch, queries, heads, head_len) dense; 0 where a query sees no key */
-    float *lse;                        /* (batch, queries, heads) or null: what the gradients start from -- the base-2 logarithm of
-                                          the sum of exponentials, +inf where there is none */
+    float *lse;                        /* (batch, queries, heads, 2) or null: what the gradients start from -- a number near the row's
+                                          largest base-2 exponent (+inf where it sees no key), and the base-2 logarithm of the sum of
+                                          the powers relative to it */
     void *rest;                        /* as out, or null: what rounding took from out, itself rounded to the type; with it the gradients
                                           know <dout, out> to twice the type's bits */
 } fg_block_attention_args;

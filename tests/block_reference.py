@@ -2,7 +2,7 @@
 test_gpu_block_*.py.
 
 Bounds.  u is the largest relative error of one rounding to the type (half a step), w = 2^-23 one step of 32 bits.  Scores are sums of D products
-in 32 bits, whose order is not fixed: |dz| <= (D + 4) w sum |q k| scale, plus w |z| for the scaling and the power of two, whose own error is
+in 32 bits, whose order is not fixed: |dz| <= (D + 4) w sum |q k| |scale|, plus w |z| for the scaling and the power of two, whose own error is
 below 4 w.  Probabilities are off by a factor e^dz and, where they are an operand of the second product in 16 bits, by u; a sum of n
 terms adds n w of their absolute sum.  Results are rounded once more, u of their value."""
 import numpy as np
@@ -62,7 +62,7 @@ def attention(q, k, v, blocks, block, scale=None, causal=True, lengths=None, q_l
             p = np.exp(z)
             p /= p.sum(1, keepdims=True)
             n = s.sum(1, keepdims=True)
-            dz = (D + 4) * W * scale * (np.abs(Q) @ np.abs(K).T) + 2 * W * (np.where(s, np.abs(z), 0) + np.abs(add)) + 4 * W
+            dz = (D + 4) * W * abs(scale) * (np.abs(Q) @ np.abs(K).T) + 2 * W * (np.where(s, np.abs(z), 0) + np.abs(add)) + 4 * W
             dz = np.where(s, dz, 0).max(1, keepdims=True)                   # of the row: its sum and maximum carry them too
             o = p @ V
             mass = p @ np.abs(V)
@@ -83,9 +83,9 @@ def attention(q, k, v, blocks, block, scale=None, causal=True, lengths=None, q_l
             edp = D * W * (np.abs(d) @ np.abs(V).T)
             eds = p * (edp + edelta) + np.abs(ds) * (half + 2 * dz + 8 * W)
             val["dq"][b, rows, h] = ds @ K * scale
-            tol["dq"][b, rows, h] = ((eds + n * W * np.abs(ds)) @ np.abs(K)) * scale
+            tol["dq"][b, rows, h] = ((eds + n * W * np.abs(ds)) @ np.abs(K)) * abs(scale)
             val["dk"][b, cols, g] += ds.T @ Q * scale
-            tol["dk"][b, cols, g] += ((eds + len(d) * W * np.abs(ds)).T @ np.abs(Q)) * scale
+            tol["dk"][b, cols, g] += ((eds + len(d) * W * np.abs(ds)).T @ np.abs(Q)) * abs(scale)
             if bn is not None:
                 where = bucket[np.ix_(rows, cols)][s]
                 val["dbias"][:, h] += np.bincount(where, ds[s], len(bn))

@@ -68,6 +68,19 @@ def test_c_interface_refuses_null_pointers_and_small_workspaces():
         assert L.fg_block_attention(ctypes.byref(a), None, 0, None) == 0
 
 
+def test_c_interface_refuses_lists_beyond_32_bits():
+    L = _lib.lib()
+    size = 1 << 20
+    a = _args(batch=64, queries=size, keys=size, topk=16, q_strides=(size * 512, 512, 64), k_strides=(size * 128, 128, 64), v_strides=(size * 128, 128, 64))
+    assert L.fg_block_attention_workspace(ctypes.byref(a)) >= 0
+    assert L.fg_block_attention_backward_workspace(ctypes.byref(a)) == -2
+    with pytest.raises(ValueError, match="32-bit lists"):
+        _lib.check(-2)
+    a.batch = 1
+    # the lists' sums stay within some times the gradients' memory (K's: 256 MiB in 16 bits)
+    assert 0 < L.fg_block_attention_backward_workspace(ctypes.byref(a)) < 2 ** 33
+
+
 def test_pool_and_select_refuse():
     L = _lib.lib()
     strides = (ctypes.c_int64 * 3)(64 * 200 * 2, 64 * 2, 64)

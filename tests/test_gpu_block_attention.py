@@ -220,6 +220,56 @@ def test_scores_of_infinite_size():
     assert call(s).isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,heads,kv_heads", [(2, 2, 1), (64, 8, 8)])
+def test_bias_of_the_lowest_value(dtype, batch, heads, kv_heads):
+    """Distances below 5 have the type's lowest value, as a mask: the first five rows of a block see nothing else."""
+    s, dout = make(dtype, batch, 150, 150, heads, kv_heads, 64, 32, 1, seed=20)
+    masked = torch.arange(150, device="cuda") % 32 < 5
+    # their queries are 0, so that their softmax is the one over equal scores; 2^-140 and 2^-1000000 are both nothing beside the other rows' scores
+    s["q"][:, masked] = 0
+    s["bias"], s["bounds"] = torch.randn(3, heads, generator=torch.Generator().manual_seed(1)).to(dtype).cuda(), (5, 20)
+    low = s["bias"].clone()
+    s["bias"][0], low[0] = -97, torch.finfo(dtype).min
+    value = want(dict(s, **{x: s[x][:1] for x in ("q", "k", "v", "blocks")}), dout[:1]) if batch > 2 else want(s, dout)
+    got = step(dict(s, bias=low), dout)
+    assert all(torch.isfinite(t).all() for t in got.values())
+    if batch > 2:                                        # the first of them alone: the bias's gradient is all sequences'
+        got = {x: t[:1] for x, t in got.items() if x != "dbias"}
+    ref.check(got, value)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch", [1, 64])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+def test_scales(dtype, batch, scale):
+    from featgraph_amd import ops
+    s, dout = make(dtype, batch, 70, 70, 8, 8, 32, 32, 2, seed=21)
+    leaves = [s[x].detach().requires_grad_() for x in ("q", "k", "v")]
+    out = ops.block_attention(*leaves, s["blocks"], 32, scale)
+    got = [out] + list(torch.autograd.grad(out, leaves, dout))
+    value = ref.attention(*(s[x][:1] for x in ("q", "k", "v", "blocks")), 32, scale, dout=dout[:1])
+    ref.check({x: t[:1] for x, t in zip(("out", "dq", "dk", "dv"), got)}, value)
+
+
+def test_more_blocks_than_one_list_of_many_queries():
+    """256 blocks are listed at a time where there are queries to fill the card; a row's blocks lie in several lists."""
+    for dtype in (F32, BF16):
+        s, dout = make(dtype, 256, 8, 17000, 16, 1, 32, 32, 3, seed=22)
+        got = step(s, dout)
+        for b in (0, 255):
+            value = want(dict(s, **{x: s[x][b:b + 1] for x in ("q", "k", "v", "blocks")}), dout[b:b + 1])
+            ref.check({x: t[b:b + 1] for x, t in got.items()}, value)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("queries", [40, 2100])
+def test_the_most_buckets(dtype, queries):
+    s, dout = make(dtype, 1, queries, queries, 16, 1, 128, 32, 2, seed=23)
+    s["bias"], s["bounds"] = torch.randn(64, 16, generator=torch.Generator().manual_seed(1)).to(dtype).cuda(), tuple(range(-31, 31)) + (4063,)
+    ref.check(step(s, dout), want(s, dout))
+
+
 def test_strides_and_alignment():
     for dtype in (F32, BF16):
         s, dout = make(dtype, 2, 70, 70, 4, 4, 64, 32, 3, seed=14)

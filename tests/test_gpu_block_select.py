@@ -100,6 +100,22 @@ def test_scores_next_to_each_other():
         chosen(q, torch.zeros(1, 300 * 32, 1, 128, dtype=dtype, device="cuda"), 32, 9, pooled=pooled.cuda())
 
 
+def test_few_scores_next_to_each_other():
+    """A dozen blocks that 32-bit sums cannot order at the cut, among others that they can."""
+    for dtype, step in ((F32, 2.0 ** -23), (F16, 2.0 ** -10), (BF16, 2.0 ** -7)):
+        gen = torch.Generator().manual_seed(13)
+        q = torch.randn(1, 40, 1, 64, generator=gen).abs().to(dtype).cuda()
+        base = torch.randn(64, generator=gen).abs().to(dtype)
+        pooled = base.repeat(1, 1, 100, 1)
+        q[..., 7] = 1e-3
+        pooled[0, 0, :, 7] = (1 + step * torch.randint(0, 40, (100,), generator=gen)).to(dtype)
+        pooled[0, 0, 30:34] *= 2                         # four above the rest
+        pooled[0, 0, 46:] /= 2                           # most below it
+        pooled[0, 0, :30] /= 4
+        for topk in (3, 9, 16):
+            chosen(q, torch.zeros(1, 100 * 32, 1, 64, dtype=dtype, device="cuda"), 32, topk, causal=False, first=0, last=0, pooled=pooled.cuda())
+
+
 def test_infinite_and_nan_scores():
     q, k = make(BF16, 1, 20, 3200, 2, 1, 64, seed=7)
     from featgraph_amd import ops

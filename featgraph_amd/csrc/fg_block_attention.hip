@@ -612,7 +612,7 @@ int problem_of(const fg_block_attention_args *a, Problem *p) {
     if (a->heads % a->kv_heads || a->heads / a->kv_heads > 16)
         return fail(FG_ERR_SHAPE, "block attention: %d heads over %d key heads: the former have to be 1 to 16 times the latter", a->heads, a->kv_heads);
     // positions, keys and the rows of a list are counted in 32 bits; the arrays behind them are addressed in 64
-    if (a->keys > (1 << 30) || a->queries > (1 << 30) || (int64_t)a->topk * 64 > INT32_MAX / a->kv_heads)
+    if (a->keys > (1 << 30) || a->queries > (1 << 30) || (int64_t)a->topk * 128 > INT32_MAX / a->kv_heads)
         return fail(FG_ERR_SHAPE, "block attention: more than 2^30 keys or queries, or too long a list");
     if (a->n_buckets < 0 || a->n_buckets > 64) return fail(FG_ERR_SHAPE, "block attention: %d buckets: 1 to 64, or 0 for no bias", a->n_buckets);
     *p = Problem{};

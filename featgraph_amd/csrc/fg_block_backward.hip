@@ -913,7 +913,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     auto floats = [&](size_t at) { return reinterpret_cast<float *>(w + at); };
     const Step step{grads->dout, a->out, a->rest, ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), grads->dq, floats(l.bias)};
     const dim3 threads(kThreads);
-    if (p.queries) {
+    if (p.queries && p.batch) {
         const dim3 blocks((unsigned)(p.batch * p.kv_heads * l.n_groups));
         const size_t few = few_stage_bytes<T, D>() + bias_bytes(p);
         if (l.many) {
@@ -991,9 +991,8 @@ extern "C" int fg_block_attention_backward(const fg_block_attention_args *args, 
     fg::block::Problem p;
     if (int rc = fg::block::problem_of(args, &p)) return rc;
     if (!grads) return fg::fail(FG_ERR_ARG, "block attention gradients: null pointer");
-    if (p.batch == 0) return FG_OK;
-    if ((p.queries && (!p.q || !p.list || !args->out || !args->lse || !grads->dout || !grads->dq)) || (p.keys && (!p.k || !p.v)) ||
-        !grads->dk != !grads->dv || (p.n_buckets && !p.bias))
+    if (p.batch && ((p.queries && (!p.q || !p.list || !args->out || !args->lse || !grads->dout || !grads->dq)) || (p.keys && (!p.k || !p.v)) ||
+        !grads->dk != !grads->dv || (p.n_buckets && !p.bias)))
         return fg::fail(FG_ERR_ARG, "block attention gradients: null pointer");
     return fg::block::launch_t(p, args, grads, workspace, workspace_bytes, nullptr, static_cast<hipStream_t>(stream));
 }

@@ -30,7 +30,7 @@ def _args(**change):
 @pytest.mark.parametrize("change,status,words", [
     (dict(type=3), -1, "type"), (dict(batch=-1), -1, "negative"), (dict(topk=0), -1, "no heads or blocks"), (dict(kv_heads=0), -1, "no heads"),
     (dict(head_len=48), -2, "48"), (dict(block=16), -2, "16"), (dict(block=96), -2, "96"), (dict(kv_heads=3), -2, "1 to 16"),
-    (dict(heads=34), -2, "1 to 16"), (dict(keys=(1 << 30) + 1), -2, "2\\^30"), (dict(n_buckets=65), -2, "65"), (dict(n_buckets=-1), -2, "buckets"),
+    (dict(heads=34), -2, "1 to 16"), (dict(topk=1 << 24), -2, "too long a list"), (dict(keys=(1 << 30) + 1), -2, "2\\^30"), (dict(n_buckets=65), -2, "65"), (dict(n_buckets=-1), -2, "buckets"),
     (dict(n_buckets=3, bounds=(5, 5)), -1, "ascend"), (dict(n_buckets=3, bounds=(0, 4095)), -2, "apart"),
     (dict(n_buckets=2, bounds=((1 << 30) + 1,)), -2, "apart"), (dict(q_strides=(1, 512, 64)), -1, "16 bytes"), (dict(k=8), -1, "16 bytes")])
 def test_c_interface_refuses(change, status, words):

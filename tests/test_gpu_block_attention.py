@@ -270,6 +270,15 @@ def test_the_most_buckets(dtype, queries):
     ref.check(step(s, dout), want(s, dout))
 
 
+@pytest.mark.parametrize("batch,queries,keys", [(0, 30, 30), (2, 0, 30), (2, 30, 0), (2, 30, 30)])
+def test_gradients_of_nothing_are_zero(batch, queries, keys):
+    s, dout = make(BF16, 2, 30, 30, buckets=8, seed=24)
+    s.update(q=s["q"][:batch, :queries], k=s["k"][:batch, :keys], v=s["v"][:batch, :keys], blocks=torch.full_like(s["blocks"], -1)[:batch, :queries])
+    torch.full((2 ** 20,), float("nan"), device="cuda")          # memory that the gradients may come to lie in
+    got = step(s, dout[:batch, :queries])
+    assert all(not t.any() for t in got.values()) and got["dbias"].shape == (8, 4) and got["dk"].shape == s["k"].shape
+
+
 def test_strides_and_alignment():
     for dtype in (F32, BF16):
         s, dout = make(dtype, 2, 70, 70, 4, 4, 64, 32, 3, seed=14)

@@ -667,43 +667,53 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         V8<T> qf[2][DC], df[2][DC];
         float next_more = 0.f;
         Row next;                      // lane 16 rt + c: row 16 rt + c of the step
-        // the token of the lane's row of the step that is fetched next: its load has a step's time before the rows' own depend on it
-        int token = 0, x = 0;
-        auto look = [&](int r0) {
-            const int r = min(r0 + (lane & 31), n_rows - 1), at = r / p.group;
-            x = r - at * p.group;
-            token = list[piece.start + at];
+        // the lane's rows c and 16 + c of the step that is fetched next: place in the list, head, and the token, whose load has a step's time
+        // before the rows' own depend on it
+        const int stride = rw_n * kUnit, places = stride / p.group, heads = stride - places * p.group;
+        typedef int Pair __attribute__((ext_vector_type(2)));
+        Pair at, x, token;
+        auto look = [&]() {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) token[rt] = list[piece.start + min(at[rt], piece.len - 1)];
         };
-        auto fetch = [&](int r0) {
-            const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
+        // rows behind the last read it again, and have no weight
+        auto fetch = [&]() {
+            const bool high = lane & 16;
+            const int t = high ? token[1] : token[0], y = high ? x[1] : x[0];
+            const int64_t row = ((int64_t)b * p.queries + t) * p.heads + h * p.group + y;
             const float2 ls = lse[row];
-            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + token, x};
+            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + t, y};
             next_more = ls.y;
-            if (r0 + (lane & 31) >= n_rows) next = Row{__builtin_inff(), 0.f, -1, 0};     // a row behind the last has no weight
+            if ((high ? at[1] : at[0]) >= piece.len) {
+                next.lse = __builtin_inff();
+                next.delta = next_more = 0.f;
+            }
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
-                const int t = __shfl(token, rt * 16 + c), y = __shfl(x, rt * 16 + c);
-                const T *q = qbase + (int64_t)t * p.qs.row + y * p.qs.head, *d = dbase + (int64_t)t * ds.row + y * ds.head;
-                const bool ok = r0 + rt * 16 + c < n_rows;
+                const T *q = qbase + (int64_t)token[rt] * p.qs.row + x[rt] * p.qs.head, *d = dbase + (int64_t)token[rt] * ds.row + x[rt] * ds.head;
 #pragma unroll
                 for (int dc = 0; dc < DC; ++dc) {
                     qf[rt][dc] = load8(q + dc * 32);
                     df[rt][dc] = load8(d + dc * 32);
                 }
-                if (r0 + kUnit > n_rows)
+            }
 #pragma unroll
-                    for (int dc = 0; dc < DC; ++dc) {
-                        qf[rt][dc] = ok ? qf[rt][dc] : zero8<T>();
-                        df[rt][dc] = ok ? df[rt][dc] : zero8<T>();
-                    }
+            for (int rt = 0; rt < 2; ++rt) {
+                at[rt] += places;
+                x[rt] += heads;
+                if (x[rt] >= p.group) { x[rt] -= p.group; ++at[rt]; }
             }
         };
         int r0 = rw * kUnit;
-        const int stride = rw_n * kUnit;
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            at[rt] = (r0 + rt * 16 + c) / p.group;
+            x[rt] = r0 + rt * 16 + c - at[rt] * p.group;
+        }
         if (r0 < n_rows) {
-            look(r0);
-            fetch(r0);
-            look(r0 + stride);
+            look();
+            fetch();
+            look();
         }
         while (r0 < n_rows) {
             wave_lds_sync();
@@ -731,32 +741,54 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         dp[rt][kt] = mma(df[rt][dc], vf[kt][dc], dp[rt][kt]);
                     }
                 }
+            // tokens ascend
+            const int from = __builtin_amdgcn_readfirstlane(next.pos), to = __builtin_amdgcn_readlane(next.pos, kUnit - 1);
             r0 += stride;
-            if (r0 < n_rows) {
-                fetch(r0);
-                look(r0 + stride);
-            }
+            fetch();
+            look();
 
             unsigned seen[KT] = {};
+            auto gradients = [&](auto masked) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+                for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const Row row = own[rt * 16 + 4 * g + i];
+                    for (int i = 0; i < 4; ++i) {
+                        const Row row = own[rt * 16 + 4 * g + i];
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const int key = key0 + kt * 16 + c;
-                        const bool ok = key <= (p.causal ? row.pos : k_len - 1);     
-                        float z = s[rt][kt][i] * p.scale2;
-                        if (p.n_buckets) z += buckets.value(buckets.at(row.pos - key), row.head);
-                        z -= row.lse;
-                        if (p.n_buckets) z -= more[rt * 16 + 4 * g + i];
-                        const float x = ok ? __builtin_amdgcn_exp2f(z) : 0.f;
-                        s[rt][kt][i] = x;
-                        dp[rt][kt][i] = ok ? x * (dp[rt][kt][i] - row.delta) : 0.f;
-                        seen[kt] |= (unsigned)ok << (4 * rt + i);
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const float z = p.n_buckets ? s[rt][kt][i] : s[rt][kt][i] * p.scale2 - row.lse;
+                            float y = __builtin_amdgcn_exp2f(z);
+                            float e = y * (dp[rt][kt][i] - row.delta);
+                            if constexpr (decltype(masked)::value) {
+                                const int key = key0 + kt * 16 + c;
+                                const bool ok = key <= (p.causal ? row.pos : k_len - 1) && (!CAREFUL || row.lse < __builtin_inff());
+                                y = ok ? y : 0.f;
+                                e = ok ? e : 0.f;
+                                seen[kt] |= (unsigned)ok << (4 * rt + i);
+                            }
+                            s[rt][kt][i] = y;
+                            dp[rt][kt][i] = e;
+                        }
                     }
-                }
+            };
+            if (p.n_buckets) {
+                const int near = buckets.at(from - (key0 + 16 * KT - 1)), far = buckets.at(to - key0);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Row row = own[rt * 16 + 4 * g + i];
+                        const float less = more[rt * 16 + 4 * g + i], same = near == far ? buckets.value(near, row.head) : 0.f;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            float z = s[rt][kt][i] * p.scale2 + same;
+                            if (near != far) z += buckets.value(buckets.at(row.pos - (key0 + kt * 16 + c)), row.head);
+                            s[rt][kt][i] = (z - row.lse) - less;
+                        }
+                    }
+            }
+            if (CAREFUL || key0 + 16 * KT > k_len || (p.causal && from < key0 + 16 * KT - 1)) gradients(std::true_type{});
+            else gradients(std::false_type{});
             // the powers go into dV's product rounded, and what that took (in 16 bits) in a second one: nearly even ones are all rounded the
             // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 372 and 399 us)
             V8<T> pf[KT], pl[KT], sf[KT];

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const unsigned long lon
     if (lane == 0) count[m] = n;
 }
 
-// Where each block's tokens, pieces and partial sums begin; totals[0]: all pieces.  One workgroup.
+// Where each block's tokens, whole pieces and partial sums begin; totals[0]: all whole pieces.  One workgroup.
 constexpr int kScan = 1024;
 __global__ __launch_bounds__(kScan) void scan_kernel(const int32_t *count, int32_t *offset, int32_t *piece0, int32_t *slot0, int32_t *totals, int all, int piece) {
     __shared__ int sums[3][kScan / 64];
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kScan) void scan_kernel(const int32_t *count, int32
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int m0 = 0; m0 < all; m0 += kScan) {
         const int m = m0 + tid, n = m < all ? count[m] : 0, k = (n + piece - 1) / piece;
-        const int own[3] = {n, m < all ? max(k, 1) : 0, k > 1 ? k : 0};
+        const int own[3] = {n, n / piece, k > 1 ? k : 0};
         int upto[3] = {own[0], own[1], own[2]};
 #pragma unroll
         for (int x = 0; x < 3; ++x) {
@@ -123,13 +123,15 @@ __global__ __launch_bounds__(kThreads) void short_lists_kernel(const Problem p, 
     if (lane == 0) count[m] = n;
 }
 
-// The tokens of every block in ascending order, and its pieces: one wavefront per block.
+// The tokens of every block in ascending order, and its pieces: one wavefront per block.  Whole pieces of all blocks come first, then what is
+// left of every block's list (len 0: nothing chose the block; -1: nothing is left), so that the short ones fill the card's last round.
 __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long *bits, const int32_t *count, const int32_t *offset, const int32_t *piece0,
-                                                        const int32_t *slot0, int32_t *list, Piece *pieces, int all, int blocks, int chunks, int piece) {
+                                                        const int32_t *slot0, const int32_t *totals, int32_t *list, Piece *pieces, int all, int blocks, int chunks, int piece) {
     const int m = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (m >= all) return;
-    const int pair = m / blocks, n = count[m], k = max((n + piece - 1) / piece, 1), at0 = offset[m];
-    for (int i = lane; i < k; i += 64) pieces[piece0[m] + i] = Piece{m, at0 + i * piece, min(piece, n - i * piece), k > 1 ? slot0[m] + i : -1};
+    const int pair = m / blocks, n = count[m], whole = n / piece, left = n - whole * piece, k = whole + (left > 0), at0 = offset[m];
+    for (int i = lane; i < whole; i += 64) pieces[piece0[m] + i] = Piece{m, at0 + i * piece, piece, k > 1 ? slot0[m] + i : -1};
+    if (lane == 0) pieces[totals[0] + m] = Piece{m, at0 + whole * piece, left || !whole ? left : -1, k > 1 ? slot0[m] + whole : -1};
     const unsigned long long *src = bits + (int64_t)pair * chunks * blocks + (m - pair * blocks);
     int base = at0;
     for (int c0 = 0; c0 < chunks; c0 += 64) {
@@ -611,6 +613,10 @@ template <typename T, int D> struct Keys {
     // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us)
     static constexpr int kTiles = sizeof(T) == 4 ? 1 : 2;
     static constexpr int kResident = D == 128 ? 1 : 2;
+    // neighbouring lanes fetch neighbouring 16 bytes of a row, and the operands are read from LDS: a third of the accesses that lanes with rows of
+    // their own, as the operands lie, make (8,192 tokens, 16 / 1 heads of 64 171 and 191 us).  With heads of 128, where a wavefront is
+    // alone, the way through LDS costs more than that (2 x 4,096 tokens, 16 / 4 heads 406 and 344 us).
+    static constexpr bool kAlong = D != 128;
     static int parts(int block) { return std::max(1, block / (kWaves * 16 * kTiles)); }       // workgroups of a block
 };
 
@@ -618,6 +624,8 @@ template <typename T, int D, bool CAREFUL>
 __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float2 *lse, const float *delta, const Piece *pieces,
                                                         const int32_t *totals, const int32_t *count, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
+    constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = 64 / CPR, N = kUnit / RPL;
+    constexpr bool ALONG = Keys<T, D>::kAlong;
     struct Row { float lse, delta; int pos, head; };
     __shared__ Row rows[kWaves][kUnit];
     __shared__ float mores[kWaves][kUnit];
@@ -627,8 +635,9 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     const int kw = wave % kw_n, rw = wave / kw_n;
     // (dealt to the XCDs in turn: contiguous shares, for the L2s' sake, are uneven and take 4 to 15 % more)
     const int unit = blockIdx.x, work = unit / parts, part = unit - work * parts;
-    if ((count ? false : work >= totals[0]) || (CAREFUL && !flags[unit])) return;
+    if ((!count && work >= totals[0] + p.batch * p.kv_heads * p.blocks) || (CAREFUL && !flags[unit])) return;
     const Piece piece = count ? Piece{work, work * p.queries, count[work], -1} : pieces[work];      // short lists have a place each
+    if (piece.len < 0) return;
     const int pair = piece.block / p.blocks, blk = piece.block - pair * p.blocks, b = pair / p.kv_heads, h = pair - b * p.kv_heads;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
     const int in_block = (part * kw_n + kw) * 16 * KT, key0 = (blk << p.block_shift) + in_block, n_rows = piece.len * p.group;
@@ -653,8 +662,8 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
             vf[kt][dc] = there ? load8(vs + dc * 32) : zero8<T>();
         }
     }
-    const T *qbase = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)h * p.group * p.qs.head + 8 * g;
-    const T *dbase = dout + b * ds.batch + (int64_t)h * p.group * ds.head + 8 * g;
+    const T *qbase = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)h * p.group * p.qs.head + (ALONG ? lane % CPR * EPC : 8 * g);
+    const T *dbase = dout + b * ds.batch + (int64_t)h * p.group * ds.head + (ALONG ? lane % CPR * EPC : 8 * g);
     Row *own = rows[wave];
     float *more = mores[wave];         // with a bias, as Row16::more
 
@@ -664,52 +673,48 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) ak[kt][dt] = av[kt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        V8<T> qf[2][DC], df[2][DC];
+        u32x4 qr[N], dr[N];            // rows as they lie in memory, or
+        V8<T> qf[2][DC], df[2][DC];    // operands
         float next_more = 0.f;
-        Row next;                      // lane 16 rt + c: row 16 rt + c of the step
-        // the lane's rows c and 16 + c of the step that is fetched next: place in the list, head, and the token, whose load has a step's time
+        Row next;                      // lane r, up to 31: row r of the step
+        // the lane's row (lane & 31) of the step that is fetched next: place in the list, head, and the token, whose load has a step's time
         // before the rows' own depend on it
         const int stride = rw_n * kUnit, places = stride / p.group, heads = stride - places * p.group;
-        typedef int Pair __attribute__((ext_vector_type(2)));
-        Pair at, x, token;
-        auto look = [&]() {
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) token[rt] = list[piece.start + min(at[rt], piece.len - 1)];
-        };
+        int r0 = rw * kUnit, at = (r0 + (lane & 31)) / p.group, x = r0 + (lane & 31) - at * p.group, token = 0;
+        auto look = [&]() { token = list[piece.start + min(at, piece.len - 1)]; };
         // rows behind the last read it again, and have no weight
         auto fetch = [&]() {
-            const bool high = lane & 16;
-            const int t = high ? token[1] : token[0], y = high ? x[1] : x[0];
-            const int64_t row = ((int64_t)b * p.queries + t) * p.heads + h * p.group + y;
+            const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
             const float2 ls = lse[row];
-            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + t, y};
+            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + token, x};
             next_more = ls.y;
-            if ((high ? at[1] : at[0]) >= piece.len) {
+            if (at >= piece.len) {
                 next.lse = __builtin_inff();
                 next.delta = next_more = 0.f;
             }
+            if constexpr (ALONG) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                const T *q = qbase + (int64_t)token[rt] * p.qs.row + x[rt] * p.qs.head, *d = dbase + (int64_t)token[rt] * ds.row + x[rt] * ds.head;
+                for (int i = 0; i < N; ++i) {
+                    const int t = __shfl(token, i * RPL + lane / CPR), y = __shfl(x, i * RPL + lane / CPR);
+                    qr[i] = *reinterpret_cast<const u32x4 *>(qbase + (int64_t)t * p.qs.row + y * p.qs.head);
+                    dr[i] = *reinterpret_cast<const u32x4 *>(dbase + (int64_t)t * ds.row + y * ds.head);
+                }
+            } else {
 #pragma unroll
-                for (int dc = 0; dc < DC; ++dc) {
-                    qf[rt][dc] = load8(q + dc * 32);
-                    df[rt][dc] = load8(d + dc * 32);
+                for (int rt = 0; rt < 2; ++rt) {
+                    const int t = __shfl(token, rt * 16 + c), y = __shfl(x, rt * 16 + c);
+                    const T *q = qbase + (int64_t)t * p.qs.row + y * p.qs.head, *d = dbase + (int64_t)t * ds.row + y * ds.head;
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) {
+                        qf[rt][dc] = load8(q + dc * 32);
+                        df[rt][dc] = load8(d + dc * 32);
+                    }
                 }
             }
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                at[rt] += places;
-                x[rt] += heads;
-                if (x[rt] >= p.group) { x[rt] -= p.group; ++at[rt]; }
-            }
+            at += places;
+            x += heads;
+            if (x >= p.group) { x -= p.group; ++at; }
         };
-        int r0 = rw * kUnit;
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            at[rt] = (r0 + rt * 16 + c) / p.group;
-            x[rt] = r0 + rt * 16 + c - at[rt] * p.group;
-        }
         if (r0 < n_rows) {
             look();
             fetch();
@@ -717,35 +722,60 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         }
         while (r0 < n_rows) {
             wave_lds_sync();
+            if constexpr (ALONG) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int dc = 0; dc < DC; ++dc) {
-                    *reinterpret_cast<V8<T> *>(stage_q + (rt * 16 + c) * S + dc * 32 + 8 * g) = qf[rt][dc];
-                    *reinterpret_cast<V8<T> *>(stage_d + (rt * 16 + c) * S + dc * 32 + 8 * g) = df[rt][dc];
+                for (int i = 0; i < N; ++i) {
+                    const int to = (i * RPL + lane / CPR) * S + lane % CPR * EPC;
+                    *reinterpret_cast<u32x4 *>(stage_q + to) = qr[i];
+                    *reinterpret_cast<u32x4 *>(stage_d + to) = dr[i];
                 }
+            } else {
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) {
+                        *reinterpret_cast<V8<T> *>(stage_q + (rt * 16 + c) * S + dc * 32 + 8 * g) = qf[rt][dc];
+                        *reinterpret_cast<V8<T> *>(stage_d + (rt * 16 + c) * S + dc * 32 + 8 * g) = df[rt][dc];
+                    }
+            }
             if (lane < kUnit) {
                 own[lane] = next;
                 if (p.n_buckets) more[lane] = next_more;
             }
             wave_lds_sync();
-            f32x4 s[2][KT], dp[2][KT];  // [rows][keys]
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int dc = 0; dc < DC; ++dc) {
-                        s[rt][kt] = mma(qf[rt][dc], kf[kt][dc], s[rt][kt]);
-                        dp[rt][kt] = mma(df[rt][dc], vf[kt][dc], dp[rt][kt]);
-                    }
-                }
             // tokens ascend
             const int from = __builtin_amdgcn_readfirstlane(next.pos), to = __builtin_amdgcn_readlane(next.pos, kUnit - 1);
             r0 += stride;
-            fetch();
-            look();
+            if (ALONG) {
+                fetch();
+                look();
+            }
+            f32x4 s[2][KT], dp[2][KT];  // [rows][keys]
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) s[rt][kt] = dp[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int dc = 0; dc < DC; ++dc) {
+                    V8<T> q, d;
+                    if constexpr (ALONG) {
+                        q = load8(stage_q + (rt * 16 + c) * S + dc * 32 + 8 * g);
+                        d = load8(stage_d + (rt * 16 + c) * S + dc * 32 + 8 * g);
+                    } else {
+                        q = qf[rt][dc];
+                        d = df[rt][dc];
+                    }
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        s[rt][kt] = mma(q, kf[kt][dc], s[rt][kt]);
+                        dp[rt][kt] = mma(d, vf[kt][dc], dp[rt][kt]);
+                    }
+                }
+            }
+            if (!ALONG) {
+                fetch();
+                look();
+            }
 
             unsigned seen[KT] = {};
             auto gradients = [&](auto masked) {
@@ -972,7 +1002,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
         mark_kernel<<<dim3((unsigned)(p.batch * p.kv_heads * l.chunks)), threads, 0, stream>>>(p, bits, l.chunks);
         count_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), all, p.blocks, l.chunks);
         scan_kernel<<<dim3(1), dim3(kScan), 0, stream>>>(ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), all, l.piece);
-        fill_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
+        fill_kernel<<<dim3(per_wave), threads, 0, stream>>>(bits, ints(l.count), ints(l.offset), ints(l.piece0), ints(l.slot0), ints(l.totals), ints(l.list), pieces, all, p.blocks, l.chunks, l.piece);
     }
     FG_HIP_TRY(hipGetLastError());
     const size_t lds = keys_stage_bytes<T, D>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);

@@ -926,19 +926,19 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     l->many = pairs * l->n_groups >= 256 && 2 * p.queries >= kWaves * row_tiles * tpt;
     if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
-    // a block's list is cut into pieces of 768 to 2,048 rows (tokens times heads of the group), some 1,024 pieces in all: longer
-    // pieces leave CUs idle at the end, shorter ones write more sums (of the largest calls longer ones, so that the sums need not much
-    // more memory than the gradients). All of the keys' gradients with pieces of 1,024 / 1,536 /
-    // 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 / 219 us, 8,192 of 16 / 1 heads of 64 216 / 217 / 248,
-    // 2 x 4,096 of 16 / 4 heads of 128 410 / 398 / 396
+    // a block's list is cut into pieces of 768 to 2,048 rows (tokens times heads of the group), some 1,024 pieces in all, or of 512 where those
+    // would not fill the CUs: longer ones leave CUs idle, shorter ones write more sums (of the largest calls longer ones, so that the sums need not much more memory than the
+    // gradients). All of the keys' gradients with pieces of 1,024 / 1,536 / 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 /
+    // 219 us, 8,192 of 16 / 1 heads of 64 216 / 217 / 248, 2 x 4,096 of 16 / 4 heads of 128 410 / 398 / 396; a whole step of 1,070
+    // tokens x 2 heads of 128 in 32 bits with 256 / 512 / 768: 178 / 164 / 211, the first case's keys with 512 / 768: 194 / 169
     const int64_t rows = pairs * p.queries * std::min(p.topk, p.blocks) * p.group;
-    l->piece = (int)std::max<int64_t>(1, std::min(std::max<int64_t>(2048, rows / 8192), std::max<int64_t>(768, rows / 1024)) / p.group);
+    l->piece = (int)std::max<int64_t>(1, std::min(std::max<int64_t>(2048, rows / 8192), std::max<int64_t>(rows < 256 * 768 ? 512 : 768, rows / 1024)) / p.group);
     l->all = pairs * p.blocks;
     // short lists: one kernel instead of five, whose looks through the selections stay below their launches' time
-    l->short_lists = p.queries <= l->piece && (int64_t)p.queries * p.topk <= 4096;
+    l->short_lists = (int64_t)p.queries * p.group <= 768 && (int64_t)p.queries * p.topk <= 4096;
     l->entries = l->short_lists ? l->all * p.queries : pairs * p.queries * std::min(p.topk, p.blocks);
     l->pieces = l->short_lists ? l->all : l->all + l->entries / l->piece;
-    l->slots = p.queries <= l->piece ? 0 : 2 * (l->entries / l->piece);
+    l->slots = l->short_lists || p.queries <= l->piece ? 0 : 2 * (l->entries / l->piece);
     const int64_t limit = INT32_MAX;
     if (l->entries > limit || l->pieces * parts > limit || l->all * (2 * block * head_len / 4 / kThreads) > limit || pairs * std::max(l->n_groups, l->chunks) > limit)
         return fail(FG_ERR_SHAPE, "block attention gradients: %lld selections of %lld blocks do not fit the 32-bit lists", (long long)l->entries, (long long)l->all);

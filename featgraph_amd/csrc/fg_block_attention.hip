@@ -11,6 +11,12 @@
 // that leaves the card idle, to several workgroups; each takes its keys from memory straight into operands.
 // Values that are not finite reach the rows that see them and no others: a result that is not finite is computed again with such places
 // apart (mma_masked).
+//
+// What bounds them.  many_kernel, 8,192 tokens, 32 / 8 heads of 128 in bfloat16, 16 blocks of 64: 402 us, 320 TFLOP/s of the selected pairs;
+// the matrix cores are busy a fifth of the time, for unions are larger than their tokens' lists, 256 registers allow two wavefronts per
+// SIMD, and these wait for LDS and for one another at each step (walking the lists and staging alone take 184 us).  few_kernel, 32
+// sequences with 16 blocks each of 32 / 8 heads of 128: 28.3 us, 4.8 TB/s of keys and values, the rate of a large copy; with less to read
+// (1 sequence, 8 heads of 64: 10 us) the chain list, keys, softmax, joining.
 #include <algorithm>
 #include <type_traits>
 

@@ -6,6 +6,11 @@
 // the lists are turned round -- for every block the tokens that selected it, in order -- and a workgroup takes a block, or a piece of a long
 // list, with its keys in registers, and gathers the rows of its tokens' heads.  Nothing is added by atomics: sums over pieces,
 // wavefronts and tiles are joined in a fixed order, so that a step gives the same bits every time.
+//
+// What bounds them (2 x 4,096 tokens, 16 / 4 heads of 128 in bfloat16, 16 blocks of 64): queries_many_kernel 275 us, as the forward pass,
+// with two products more; keys_kernel 341 us: one wavefront per SIMD (sums of 32 keys, their operands and the rows under way take 396
+// registers), so that every wait shows, and 70 us of beginnings and ends of 1,100 pieces; the lists 24 us in four launches, the sums of
+// pieces 14 (5 TB/s).  With heads of 64 two wavefronts fit (8,192 tokens, 16 / 1 heads, 8 blocks of 128: 151 and 171 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -610,7 +615,7 @@ template <typename T, int D> constexpr size_t keys_stage_bytes() { return (size_
 // flags[workgroup]: whether a sum was not finite; CAREFUL: those again, with such places apart.
 template <typename T, int D> struct Keys {
     // heads of 128: two tiles' operands and sums leave room for one wavefront per SIMD alone, and still take less than one tile each of two
-    // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us)
+    // wavefronts that fetch and turn every row for half the keys (2 x 4,096 tokens, 16 / 4 heads 371 and 565 us, either with one product less)
     static constexpr int kTiles = sizeof(T) == 4 ? 1 : 2;
     static constexpr int kResident = D == 128 ? 1 : 2;
     // neighbouring lanes fetch neighbouring 16 bytes of a row, and the operands are read from LDS: a third of the accesses that lanes with rows of
@@ -820,7 +825,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
             if (CAREFUL || key0 + 16 * KT > k_len || (p.causal && from < key0 + 16 * KT - 1)) gradients(std::true_type{});
             else gradients(std::false_type{});
             // the powers go into dV's product rounded, and what that took (in 16 bits) in a second one: nearly even ones are all rounded the
-            // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 372 and 399 us)
+            // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 27 us)
             V8<T> pf[KT], pl[KT], sf[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
@@ -927,10 +932,10 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     if (!l->many) l->n_groups = tiles(1);
     l->chunks = std::max(1, (p.queries + 63) / 64);
     // a block's list is cut into pieces of 768 to 2,048 rows (tokens times heads of the group), some 1,024 pieces in all, or of 512 where those
-    // would not fill the CUs: longer ones leave CUs idle, shorter ones write more sums (of the largest calls longer ones, so that the sums need not much more memory than the
-    // gradients). All of the keys' gradients with pieces of 1,024 / 1,536 / 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 /
+    // would not fill the CUs: longer ones leave CUs idle, shorter ones write more sums (of the largest calls longer ones, so that the sums
+    // need not much more memory than the gradients). All of the keys' gradients with pieces of 1,024 / 1,536 / 2,048 rows: 2 x 2,048 tokens of 16 / 4 heads of 128 186 / 190 /
     // 219 us, 8,192 of 16 / 1 heads of 64 216 / 217 / 248, 2 x 4,096 of 16 / 4 heads of 128 410 / 398 / 396; a whole step of 1,070
-    // tokens x 2 heads of 128 in 32 bits with 256 / 512 / 768: 178 / 164 / 211, the first case's keys with 512 / 768: 194 / 169
+    // tokens x 2 heads of 128 in 32 bits with 256 / 512 / 768: 178 / 164 / 211
     const int64_t rows = pairs * p.queries * std::min(p.topk, p.blocks) * p.group;
     l->piece = (int)std::max<int64_t>(1, std::min(std::max<int64_t>(2048, rows / 8192), std::max<int64_t>(rows < 256 * 768 ? 512 : 768, rows / 1024)) / p.group);
     l->all = pairs * p.blocks;

@@ -1,10 +1,12 @@
 // Choosing blocks of keys by a cheap score: the keys' mean over each block, and for every query the blocks with the highest product of
 // that mean and the sum of the queries that share the key head.
 //
-// fg_block_pool reads the keys once (HBM bound).  fg_block_select forms the scores of 16 queries on the matrix cores, keeps them in LDS (they
+// fg_block_pool reads the keys once (HBM bound: 16,384 keys of 8 heads of 128 7.6 us, 4.4 TB/s).  fg_block_select forms the scores of 16 queries on the matrix cores, keeps them in LDS (they
 // are never written to memory) and lets one wavefront at a time find a query's topk.  Two blocks whose scores the 32-bit sums
 // cannot tell apart would come out in an order that depends on the order of the sums, and with them the whole attention of a
-// query; so a second product bounds the error, and blocks within it of the topk-th score are compared again in 64 bits.
+// query; so a second product bounds the error, and blocks within it of the topk-th score are compared again in 64 bits.  Finding the topk is
+// what takes the time (16,384 queries, 32 / 8 heads of 128, up to 256 blocks: 110 us, of which the queries' bytes would take 30 and the
+// products 7): vector and scalar instructions of counting, in one wavefront per query.
 #include <algorithm>
 #include <type_traits>
 

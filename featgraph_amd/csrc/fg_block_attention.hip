@@ -127,18 +127,17 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
                 u = find(u + kWaves * splits);
                 if (u < units) fetch(u);
 
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[kt][i] *= p.scale2;
+                // z = s factor; powers are taken of z - reference in one operation, unrounded between, as many_kernel and the gradients take them
+                const float factor = p.n_buckets ? 1.f : p.scale2;
                 if (p.n_buckets) {
                     const int pos = offset + t0, near = buckets.at(pos - now - (kUnit - 1)), far = buckets.at(pos + tpt - 1 - now);
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            s[kt][i] += buckets.value(near == far ? near : buckets.at(pos + tc - (now + 16 * kt + 4 * g + i)), mine);
+                            s[kt][i] = s[kt][i] * p.scale2 + buckets.value(near == far ? near : buckets.at(pos + tc - (now + 16 * kt + 4 * g + i)), mine);
                 }
+                f32x4 z[2] = {s[0] * factor, s[1] * factor};
                 unsigned seen = 0xff;
                 if (!__all(now + kUnit - 1 <= last)) {
                     seen = 0;
@@ -147,11 +146,11 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const bool ok = now + 16 * kt + 4 * g + i <= last;
-                            s[kt][i] = ok ? s[kt][i] : -__builtin_inff();
+                            z[kt][i] = ok ? z[kt][i] : -__builtin_inff();
                             seen |= (unsigned)ok << (4 * kt + i);
                         }
                 }
-                float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
                 top = fmaxf(m, rows_max(top));
                 const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
                 if (__any(top != m)) {
@@ -162,7 +161,10 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
                     m = top;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { s[0][i] = __builtin_amdgcn_exp2f(s[0][i] - ref); s[1][i] = __builtin_amdgcn_exp2f(s[1][i] - ref); }
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[kt][i] = z[kt][i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], factor, -ref));
                 l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
                 // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not.  For gradients
                 // what the rounding took follows in a second product, as in many_kernel.

@@ -161,7 +161,9 @@ struct Step { const void *dout, *out, *rest; Strides ds; const float2 *lse; floa
 // A lane's row of a tile: dO and Q as operands, and delta.
 template <typename T, int D> struct Row16 {
     V8<T> q[D / 32], d[D / 32];
-    float lse, more, delta;            // powers are 2^(z - lse - more); more is 0 where one number holds both
+    // p is 2^(z - lse) weight, and dS is 2^(z - lse) (dP weight - less): the row's sum is a factor of the second one, in one operation, and never
+    // added to the reference, which from 2^24 on would take it away
+    float lse, weight, less;
     int limit;                         // last key that it may see; columns without a row see everything, nothing is written of them
     __device__ __forceinline__ void load(const Problem &p, const Step &w, int b, int t, int head, bool used, int q_len, int k_len, int offset, int g, bool write) {
         const bool there = used && t < q_len;
@@ -184,20 +186,16 @@ template <typename T, int D> struct Row16 {
                 for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)r[i];
             }
         }
-        delta = rows_sum(sum);
+        const float delta = rows_sum(sum);
         const float2 ls = there ? w.lse[at] : make_float2(__builtin_inff(), 0.f);
         lse = ls.x;
-        more = ls.y;
+        weight = __builtin_amdgcn_exp2f(-ls.y);
+        less = delta * weight;
         if (there && write && g == 0) w.delta[at] = delta;
     }
-    // Whether a row of the wavefront is relative to a number, out of the bias, that would take its sum away (2^12 leaves it 11 bits more than
-    // a score of that size has).
-    __device__ __forceinline__ bool join() {
-        if (__any(fabsf(lse) > 4096.f && fabsf(lse) < __builtin_inff())) return true;
-        lse += more;
-        more = 0.f;
-        return false;
-    }
+    // Whether a row of the wavefront is relative to a number, out of the bias, so large that adding the bias to the reference first would
+    // leave other scores than the forward pass had.
+    __device__ __forceinline__ bool far_off() const { return __any(fabsf(lse) > 4096.f && fabsf(lse) < __builtin_inff()); }
 };
 
 // The bias's gradient is summed in LDS, [wavefront][bucket][lane]: all rows of a lane have one head, and no two lanes a place.
@@ -221,10 +219,10 @@ __device__ __forceinline__ void write_bias(const Problem &p, const float *sums, 
     }
 }
 
-// Powers p = 2^(z - lse), and from them dS = p (dP - delta), of one tile and 32 keys, into s[]: with MASK, keys behind `last` have none.
-// The bias's gradient goes to `sums`.  far_off: `more` counts, and the scores are formed as the forward pass does.
+// dS = 2^(z - lse) (dP weight - less) of one tile and 32 keys, into s[]: with MASK, keys behind `last` have none.  The bias's gradient goes to
+// `sums`.  far_off: the scores are formed as the forward pass does.
 template <bool BIAS, bool MASK>
-__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float more, bool far_off, float delta,
+__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float weight, float less, bool far_off,
                                                     int pos, int tpt, int tc, int mine, int key0, int last, int g, int lane) {
     const int near = BIAS ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = BIAS ? buckets.at(pos + tpt - 1 - key0) : 0;
     const float from = (BIAS && near == far ? buckets.value(near, mine) : 0.f) - (BIAS && far_off ? 0.f : lse);
@@ -241,8 +239,8 @@ __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buck
                 bucket = buckets.at(pos + tc - key);
                 z += buckets.value(bucket, mine);
             }
-            if (BIAS && far_off) z = (z - lse) - more;
-            float x = __builtin_amdgcn_exp2f(z) * (dp[kt][i] - delta);
+            if (BIAS && far_off) z -= lse;
+            float x = __builtin_amdgcn_exp2f(z) * (dp[kt][i] * weight - less);
             if (MASK) {
                 x = key <= last ? x : 0.f;
                 seen |= (unsigned)(key <= last) << (4 * kt + i);
@@ -274,7 +272,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
     T *stage = reinterpret_cast<T *>(dynamic) + wave * kUnit * S;
     Row16<T, D> row;
     row.load(p, w, b, t0 + tc, head, used, q_len, k_len, offset, g, wave == 0);
-    const bool far_off = row.join();
+    const bool far_off = p.n_buckets && row.far_off();
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + 8 * g;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + 8 * g;
@@ -332,8 +330,8 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
                 u = find(u + kWaves);
                 if (u < units) fetch(u);
                 const unsigned seen = p.n_buckets
-                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.more, far_off, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane)
-                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.more, far_off, row.delta, offset + t0, tpt, tc, mine, now, last, g, lane);
+                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, far_off, offset + t0, tpt, tc, mine, now, last, g, lane)
+                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, far_off, offset + t0, tpt, tc, mine, now, last, g, lane);
                 V8<T> sf, rf;          // as in queries_many_kernel
                 split<T>(s[0], s[1], &sf, &rf);
 #pragma unroll
@@ -432,7 +430,7 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     for (int rt = 0; rt < RT; ++rt) row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
     bool far_off = false;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) far_off |= row[rt].join();
+    for (int rt = 0; rt < RT; ++rt) far_off |= BIAS && row[rt].far_off();
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + TILES * tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head;
@@ -527,11 +525,11 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
                 if (__any(edge)) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].more, far_off, row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
+                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, far_off, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
                 } else {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].more, far_off, row[rt].delta, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
+                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, far_off, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
                 }
                 // dS goes into the product with K rounded, and what that took (in 16 bits) in a second one: a row's dS add up to 0, and its keys
                 // have much in common, so that the rounding alone would be larger than dQ's own

@@ -252,6 +252,33 @@ def test_scales(dtype, batch, scale):
     ref.check({x: t[:1] for x, t in zip(("out", "dq", "dk", "dv"), got)}, value)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [-6000, 6000])
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len", [(2, 70, 4, 2, 64), (1, 5, 16, 1, 32), (4, 1030, 8, 8, 32), (2, 1030, 16, 4, 128)])
+def test_rows_of_large_scores_leave_their_neighbours_alone(dtype, size, batch, queries, heads, kv_heads, head_len):
+    """One head of a few tokens has scores of thousands, near enough to one another for a softmax over many keys; the rest are ordinary."""
+    s, dout = make(dtype, batch, queries, queries, heads, kv_heads, head_len, 32, 3, seed=25)
+    s["k"][..., 0] = 64                                  # all of a row's scores move together
+    odd = s["k"][:, 1::2]
+    odd.copy_(s["k"][:, :2 * odd.shape[1]:2])            # keys in pairs of equal ones: no row is one key's alone
+    s["q"][:, 4::37, 0, 0] = size / 64 * head_len ** 0.5
+    ref.check(step(s, dout), want(s, dout))
+
+
+@pytest.mark.parametrize("batch", [2, 64])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 26, -2.0 ** 28])
+def test_queries_gradients_of_scores_that_hold_no_fraction(batch, size):
+    """Keys that are equal where the query is not 0 have equal scores, whatever rounding makes of them: a row's softmax is the one of a query
+    of zeros.  From 2^24 on a score and the logarithm of a row's sum do not fit one 32-bit number."""
+    s, dout = make(F32, batch, 90, 90, 8, 4, 64, 32, 2, seed=26)
+    s["k"][..., 0] = 2.0 ** 10
+    s["q"].zero_()
+    value = ref.attention(*(s[x][:2] for x in ("q", "k", "v", "blocks")), 32, dout=dout[:2])
+    s["q"][:, 3::5, 1, 0] = size / 2 ** 10 * 8
+    got = step(s, dout)
+    ref.check({x: got[x][:2] for x in ("out", "dq")}, value)
+
+
 def test_more_blocks_than_one_list_of_many_queries():
     """256 blocks are listed at a time where there are queries to fill the card; a row's blocks lie in several lists."""
     for dtype in (F32, BF16):

@@ -668,7 +668,9 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     const T *qbase = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)h * p.group * p.qs.head + (ALONG ? lane % CPR * EPC : 8 * g);
     const T *dbase = dout + b * ds.batch + (int64_t)h * p.group * ds.head + (ALONG ? lane % CPR * EPC : 8 * g);
     Row *own = rows[wave];
-    float *more = mores[wave];         // with a bias, as Row16::more
+    // Logarithms of the rows' sums, where they are not added to the references: with a bias, whose scores are formed apart from them as the forward
+    // pass does, and in steps with a reference so large that the sum would lose its last bits (from 2^24 on all of it).
+    float *more = mores[wave];
 
     f32x4 ak[KT][DT], av[KT][DT];
     {
@@ -689,7 +691,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
         auto fetch = [&]() {
             const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
             const float2 ls = lse[row];
-            next = Row{p.n_buckets ? ls.x : ls.x + ls.y, delta[row], offset + token, x};
+            next = Row{ls.x, delta[row], offset + token, x};
             next_more = ls.y;
             if (at >= piece.len) {
                 next.lse = __builtin_inff();
@@ -741,9 +743,11 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         *reinterpret_cast<V8<T> *>(stage_d + (rt * 16 + c) * S + dc * 32 + 8 * g) = df[rt][dc];
                     }
             }
+            const bool apart = p.n_buckets || __any(fabsf(next.lse) > 4096.f && next.lse < __builtin_inff());
+            if (!apart) next.lse += next_more;
             if (lane < kUnit) {
                 own[lane] = next;
-                if (p.n_buckets) more[lane] = next_more;
+                if (apart) more[lane] = next_more;
             }
             wave_lds_sync();
             // tokens ascend
@@ -789,7 +793,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         const Row row = own[rt * 16 + 4 * g + i];
 #pragma unroll
                         for (int kt = 0; kt < KT; ++kt) {
-                            const float z = p.n_buckets ? s[rt][kt][i] : s[rt][kt][i] * p.scale2 - row.lse;
+                            const float z = apart ? s[rt][kt][i] : s[rt][kt][i] * p.scale2 - row.lse;
                             float y = __builtin_amdgcn_exp2f(z);
                             float e = y * (dp[rt][kt][i] - row.delta);
                             if constexpr (decltype(masked)::value) {
@@ -818,6 +822,15 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                             if (near != far) z += buckets.value(buckets.at(row.pos - (key0 + kt * 16 + c)), row.head);
                             s[rt][kt][i] = (z - row.lse) - less;
                         }
+                    }
+            } else if (apart) {
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float lse = own[rt * 16 + 4 * g + i].lse, less = more[rt * 16 + 4 * g + i];
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) s[rt][kt][i] = __builtin_fmaf(s[rt][kt][i], p.scale2, -lse) - less;
                     }
             }
             if (CAREFUL || key0 + 16 * KT > k_len || (p.causal && from < key0 + 16 * KT - 1)) gradients(std::true_type{});

@@ -279,6 +279,23 @@ def test_queries_gradients_of_scores_that_hold_no_fraction(batch, size):
     ref.check({x: got[x][:2] for x in ("out", "dq")}, value)
 
 
+@pytest.mark.parametrize("batch,queries,block", [(2, 90, 32), (64, 90, 128), (1, 1030, 64)])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 26, -2.0 ** 28])
+def test_keys_gradients_of_scores_that_hold_no_fraction(batch, queries, block, size):
+    """As the queries' gradients.  The upper half of a query meets zeros in every key: the keys' gradients there are large and know nothing of the
+    scores but the softmax."""
+    s, dout = make(F32, batch, queries, queries, 8, 4, 64, block, 2, seed=27)
+    s["q"].zero_()
+    s["k"][..., 32:] = 0
+    s["k"][..., 0] = 2.0 ** 10
+    s["q"][..., 32:] = torch.randn(s["q"].shape[:3] + (32,), generator=torch.Generator().manual_seed(1)).cuda()      # meets zeros alone
+    value = ref.attention(*(s[x][:2] for x in ("q", "k", "v", "blocks")), block, dout=dout[:2])
+    s["q"][:, 3::5, 1, 0] = size / 2 ** 10 * 8
+    got = step(s, dout)
+    ref.check({"dv": got["dv"][:2]}, value)
+    ref.check({"dk": got["dk"][:2, :, :, 32:]}, {"dk": tuple(a[..., 32:] for a in value["dk"])})
+
+
 def test_more_blocks_than_one_list_of_many_queries():
     """256 blocks are listed at a time where there are queries to fill the card; a row's blocks lie in several lists."""
     for dtype in (F32, BF16):

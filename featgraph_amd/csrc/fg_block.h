@@ -87,10 +87,10 @@ template <typename T, int D> __device__ __forceinline__ V8<T> transposed(const T
     return v;
 }
 
-// acc + a b, where b's element is a factor only if its bit in `seen` is set, with what infinities and NaN in a give: a masked pair adds
-// nothing whatever a holds.  Their places are marked by further products of ones and zeros.  For tiles in which the plain
-// product left something that is not finite; everything else takes mma() alone.
-template <typename T> __device__ __forceinline__ f32x4 mma_masked(V8<T> a, V8<T> b, unsigned seen, f32x4 acc) {
+// acc + a (b + low), where b's element is a factor only if its bit in `seen` is set, with what infinities and NaN in a give: a masked pair adds
+// nothing whatever a holds.  `low` is what rounding took from b (split), or 0.  Their places are marked by further products of ones and
+// zeros.  For tiles in which the plain product left something that is not finite; everything else takes mma() alone.
+template <typename T> __device__ __forceinline__ f32x4 mma_masked(V8<T> a, V8<T> b, V8<T> low, unsigned seen, f32x4 acc) {
     V8<T> fin, ap, an, ax, bad, bs, bp, bn, bz;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -99,11 +99,13 @@ template <typename T> __device__ __forceinline__ f32x4 mma_masked(V8<T> a, V8<T>
         fin[i] = inf || nan ? (T)0.f : a[i];
         ap[i] = (T)(inf && x > 0 ? 1.f : 0.f); an[i] = (T)(inf && x < 0 ? 1.f : 0.f);
         ax[i] = (T)(nan ? 1.f : 0.f);          bad[i] = (T)(inf || nan ? 1.f : 0.f);
+        low[i] = fabsf(y) < __builtin_inff() ? low[i] : (T)0.f;
         bs[i] = (T)(s ? 1.f : 0.f);            bz[i] = (T)(s && !(y > 0 || y < 0) ? 1.f : 0.f);
         bp[i] = (T)(s && y > 0 ? 1.f : 0.f);   bn[i] = (T)(s && y < 0 ? 1.f : 0.f);
     }
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
     acc = mma(fin, b, acc);
+    if (sizeof(T) == 2) acc = mma(fin, low, acc);
     const f32x4 pos = mma(ap, bp, mma(an, bn, none)), neg = mma(ap, bn, mma(an, bp, none)), no = mma(bad, bz, mma(ax, bs, none));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

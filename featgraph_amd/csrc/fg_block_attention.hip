@@ -170,10 +170,11 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
                 // what the rounding took follows in a second product, as in many_kernel.
                 V8<T> pf, pl;
                 block::split<T>(s[0], s[1], &pf, &pl);
+                if (decltype(careful)::value && !r.rest) pl = zero8<T>();
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
-                    if constexpr (decltype(careful)::value) o[dt] = mma_masked<T>(vf, pf, seen, o[dt]);
+                    if constexpr (decltype(careful)::value) o[dt] = mma_masked<T>(vf, pf, pl, seen, o[dt]);
                     else o[dt] = mma(vf, pf, o[dt]);
                 }
                 if (sizeof(T) == 2 && !decltype(careful)::value && r.rest)

@@ -156,14 +156,25 @@ __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long
 
 // ---- by query: dQ, dbias and delta ------------------------------------------------------------------------
 
-struct Step { const void *dout, *out, *rest; Strides ds; const float2 *lse; float *delta; void *dq; float *bias_sums; };
+struct Step { const void *dout, *out, *rest; Strides ds; const float2 *lse; float *delta; float2 *largest; void *dq; float *bias_sums; };
+
+// float16 holds numbers from 6e-5 (in full) to 65504, and dS has the gradients' range: loss scaling moves it, but between rows and heads it
+// remains wide.  So dS enters its products times a power of two and the sums are taken back in 32 bits.  By query every row has its own:
+// with |dO| 2^up <= 2^room, dS is p (dP - delta) 2^up <= p |V| 2^room.  Room of 2^6 is enough for |V_j| up to 2^9 and leaves p down to
+// 2^-20 in full; longer values make dS infinite, and such tiles are computed again (as those with infinities are) with room 2^-4: all that
+// 128 elements of 65504, |V_j| < 2^19.5, can ask for, since p (dP - delta) <= |dO| max |V| / 2.  By key see keys_kernel.
+template <typename T> constexpr bool kNarrow = std::is_same<T, _Float16>::value;
+constexpr int kRoom = 6, kSafeRoom = -4;
 
 // A lane's row of a tile: dO and Q as operands, and delta.
 template <typename T, int D> struct Row16 {
     V8<T> q[D / 32], d[D / 32];
     // p is 2^(z - lse) weight, and dS is 2^(z - lse) (dP weight - less): the row's sum is a factor of the second one, in one operation, and never
     // added to the reference, which from 2^24 on would take it away
-    float lse, weight, less;
+    float lse, weight, less, down;     // in float16 weight and less are 2^up times that, down is 2^-up
+    float delta, more;
+    float norm;                        // |dO|
+    int size;                          // |dO| <= 2^size
     int limit;                         // last key that it may see; columns without a row see everything, nothing is written of them
     __device__ __forceinline__ void load(const Problem &p, const Step &w, int b, int t, int head, bool used, int q_len, int k_len, int offset, int g, bool write) {
         const bool there = used && t < q_len;
@@ -172,7 +183,7 @@ template <typename T, int D> struct Row16 {
         const T *qs = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
         const T *dos = static_cast<const T *>(w.dout) + b * w.ds.batch + (int64_t)t * w.ds.row + head * w.ds.head + 8 * g;
         const T *os = static_cast<const T *>(w.out) + at * D + 8 * g, *rs = static_cast<const T *>(w.rest) + at * D + 8 * g;
-        float sum = 0.f;
+        float sum = 0.f, squares = 0.f;
 #pragma unroll
         for (int dc = 0; dc < D / 32; ++dc) {
             q[dc] = there ? load8(qs + dc * 32) : zero8<T>();
@@ -180,18 +191,40 @@ template <typename T, int D> struct Row16 {
             const V8<T> o = there ? load8(os + dc * 32) : zero8<T>();
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)o[i];
+            if (kNarrow<T>)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) squares += (float)d[dc][i] * (float)d[dc][i];
             if (w.rest) {
                 const V8<T> r = there ? load8(rs + dc * 32) : zero8<T>();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)r[i];
             }
         }
-        const float delta = rows_sum(sum);
+        delta = rows_sum(sum);
         const float2 ls = there ? w.lse[at] : make_float2(__builtin_inff(), 0.f);
         lse = ls.x;
-        weight = __builtin_amdgcn_exp2f(-ls.y);
-        less = delta * weight;
+        more = ls.y;
         if (there && write && g == 0) w.delta[at] = delta;
+        norm = 0.f;
+        size = 0;
+        if (kNarrow<T>) {
+            squares = rows_sum(squares);
+            size = (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1;
+            norm = __builtin_sqrtf(squares);
+        }
+    }
+    // The largest |dO| and |delta| of the tile that are finite, for the sweep by key (float16).
+    __device__ __forceinline__ float2 largest() const {
+        float2 v = make_float2(norm < __builtin_inff() ? norm : 0.f, fabsf(delta) < __builtin_inff() ? fabsf(delta) : 0.f);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) { v.x = fmaxf(v.x, __shfl_xor(v.x, d)); v.y = fmaxf(v.y, __shfl_xor(v.y, d)); }
+        return v;
+    }
+    __device__ __forceinline__ void weigh(int room) {
+        const float up = kNarrow<T> ? room - size : 0.f;
+        weight = __builtin_amdgcn_exp2f(up - more);
+        less = delta * weight;
+        down = __builtin_amdgcn_exp2f(-up);
     }
     // Whether a row of the wavefront is relative to a number, out of the bias, so large that adding the bias to the reference first would
     // leave other scores than the forward pass had.
@@ -220,9 +253,9 @@ __device__ __forceinline__ void write_bias(const Problem &p, const float *sums, 
 }
 
 // dS = 2^(z - lse) (dP weight - less) of one tile and 32 keys, into s[]: with MASK, keys behind `last` have none.  The bias's gradient goes to
-// `sums`.  far_off: the scores are formed as the forward pass does.
-template <bool BIAS, bool MASK>
-__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float weight, float less, bool far_off,
+// `sums`, times `down`.  far_off: the scores are formed as the forward pass does.
+template <bool BIAS, bool MASK, bool NARROW>
+__device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buckets &buckets, float *sums, f32x4 *s, const f32x4 *dp, float lse, float weight, float less, float down, bool far_off,
                                                     int pos, int tpt, int tc, int mine, int key0, int last, int g, int lane) {
     const int near = BIAS ? buckets.at(pos - key0 - (kUnit - 1)) : 0, far = BIAS ? buckets.at(pos + tpt - 1 - key0) : 0;
     const float from = (BIAS && near == far ? buckets.value(near, mine) : 0.f) - (BIAS && far_off ? 0.f : lse);
@@ -247,11 +280,11 @@ __device__ __forceinline__ unsigned score_gradients(const Problem &p, const Buck
             }
             s[kt][i] = x;
             if (BIAS) {
-                if (near != far) sums[bucket * 64 + lane] += x;
+                if (near != far) sums[bucket * 64 + lane] += NARROW ? x * down : x;
                 else total += x;
             }
         }
-    if (BIAS && near == far) sums[near * 64 + lane] += total;
+    if (BIAS && near == far) sums[near * 64 + lane] += NARROW ? total * down : total;
     return seen;
 }
 
@@ -262,7 +295,7 @@ template <typename T, int D> constexpr size_t few_stage_bytes() {
 
 // One tile of 16 rows, its list dealt out to the four wavefronts, as few_kernel does forward.
 template <typename T, int D, bool CAREFUL>
-__device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1, kWindow> &list, unsigned char *dynamic, const Buckets &buckets, float *sums, int b, int h, int tile) {
+__device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1, kWindow> &list, unsigned char *dynamic, const Buckets &buckets, float *sums, int b, int h, int tile, float2 *largest) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
@@ -273,6 +306,10 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
     Row16<T, D> row;
     row.load(p, w, b, t0 + tc, head, used, q_len, k_len, offset, g, wave == 0);
     const bool far_off = p.n_buckets && row.far_off();
+    if (kNarrow<T> && largest && wave == 0) {
+        const float2 v = row.largest();
+        if (lane == 0) *largest = v;
+    }
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + tpt, q_len) - 1) : k_len - 1;
     const T *kbase = static_cast<const T *>(p.k) + b * p.ks.batch + h * p.ks.head + 8 * g;
     const T *vbase = static_cast<const T *>(p.v) + b * p.vs.batch + h * p.vs.head + 8 * g;
@@ -280,6 +317,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
 
     f32x4 acc[DT];
     auto sweep = [&](auto careful) {
+        row.weigh(decltype(careful)::value ? kSafeRoom : kRoom);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int first = 0; first < p.blocks; first += kWindow) {
@@ -330,15 +368,15 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
                 u = find(u + kWaves);
                 if (u < units) fetch(u);
                 const unsigned seen = p.n_buckets
-                    ? score_gradients<true, true>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, far_off, offset + t0, tpt, tc, mine, now, last, g, lane)
-                    : score_gradients<false, true>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, far_off, offset + t0, tpt, tc, mine, now, last, g, lane);
+                    ? score_gradients<true, true, kNarrow<T>>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, row.down, far_off, offset + t0, tpt, tc, mine, now, last, g, lane)
+                    : score_gradients<false, true, kNarrow<T>>(p, buckets, sums, s, dp, row.lse, row.weight, row.less, row.down, far_off, offset + t0, tpt, tc, mine, now, last, g, lane);
                 V8<T> sf, rf;          // as in queries_many_kernel
                 split<T>(s[0], s[1], &sf, &rf);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const V8<T> x = transposed<T, D>(stage, dt * 16, lane);
                     if constexpr (decltype(careful)::value) {
-                        acc[dt] = mma_masked<T>(x, sf, seen, acc[dt]);
+                        acc[dt] = mma_masked<T>(x, sf, rf, seen, acc[dt]);
                     } else {
                         acc[dt] = mma(x, sf, acc[dt]);
                         if (sizeof(T) == 2) acc[dt] = mma(x, rf, acc[dt]);
@@ -359,6 +397,9 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
             sweep(std::true_type{});
         }
     }
+    if (kNarrow<T>)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= row.down;
     float *merge = reinterpret_cast<float *>(dynamic);
 #pragma unroll
     for (int strip = 0; strip < DC; ++strip) {
@@ -389,7 +430,7 @@ __global__ __launch_bounds__(kThreads) void queries_few_kernel(const Problem p, 
         sums = bias_place(p, at);
         for (int i = threadIdx.x; i < kWaves * p.n_buckets * 64; i += kThreads) sums[i] = 0.f;
     }
-    few_rows<T, D, false>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, tile);
+    few_rows<T, D, false>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, tile, w.largest + unit);
     if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_tiles + tile, h);
 }
 
@@ -409,6 +450,7 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT, BUFFERS = Steps<T, D, BIAS>::kBuffers;
     constexpr int KS = Steps<T, D, BIAS>::kKeyStride, VS = Steps<T, D, BIAS>::kValueStride;
     __shared__ List<TILES, kListed> list;
+    __shared__ float2 tops[kWaves];
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int unit = xcd_contiguous_block(), pair = unit / n_groups, group = group_of(p, unit - pair * n_groups, n_groups), b = pair / p.kv_heads, h = pair - b * p.kv_heads;
@@ -427,7 +469,19 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
     }
     Row16<T, D> row[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
+    for (int rt = 0; rt < RT; ++rt) {
+        row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
+        row[rt].weigh(kRoom);
+    }
+    if (kNarrow<T>) {
+        float2 top = row[0].largest();
+#pragma unroll
+        for (int rt = 1; rt < RT; ++rt) {
+            const float2 v = row[rt].largest();
+            top = make_float2(fmaxf(top.x, v.x), fmaxf(top.y, v.y));
+        }
+        if (lane == 0) tops[wave] = top;
+    }
     bool far_off = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) far_off |= BIAS && row[rt].far_off();
@@ -525,11 +579,11 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
                 if (__any(edge)) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, true>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, far_off, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
+                        score_gradients<BIAS, true, kNarrow<T>>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, row[rt].down, far_off, pos + rt * tpt, tpt, tc, mine, now, last[rt], g, lane);
                 } else {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
-                        score_gradients<BIAS, false>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, far_off, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
+                        score_gradients<BIAS, false, kNarrow<T>>(p, buckets, sums, s[rt], dp[rt], lse[rt], row[rt].weight, row[rt].less, row[rt].down, far_off, pos + rt * tpt, tpt, tc, mine, now, 0, g, lane);
                 }
                 // dS goes into the product with K rounded, and what that took (in 16 bits) in a second one: a row's dS add up to 0, and its keys
                 // have much in common, so that the rounding alone would be larger than dQ's own
@@ -558,12 +612,20 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
         for (int dt = 0; dt < DT; ++dt) {
             odd |= not_finite(acc[rt][dt]);
             if (used && t < p.queries)
-                store_row<T>(static_cast<T *>(w.dq), nullptr, (((int64_t)b * p.queries + t) * p.heads + head) * D + dt * 16 + 4 * g, acc[rt][dt] * p.scale);
+                store_row<T>(static_cast<T *>(w.dq), nullptr, (((int64_t)b * p.queries + t) * p.heads + head) * D + dt * 16 + 4 * g,
+                             acc[rt][dt] * (kNarrow<T> ? p.scale * row[rt].down : p.scale));
         }
     }
     if (BIAS) write_bias(p, sums - wave * p.n_buckets * 64, w.bias_sums, (int64_t)b * n_groups + group, h);
     odd = __syncthreads_or(odd);
-    if (tid == 0) flags[unit] = odd;
+    if (tid == 0) {
+        flags[unit] = odd;
+        if (kNarrow<T>) {
+            float2 top = tops[0];
+            for (int i = 1; i < kWaves; ++i) top = make_float2(fmaxf(top.x, tops[i].x), fmaxf(top.y, tops[i].y));
+            w.largest[unit] = top;
+        }
+    }
 }
 
 // The tiles of queries_many_kernel's workgroups with a result that was not finite, again.
@@ -584,7 +646,7 @@ __global__ __launch_bounds__(kThreads) void queries_redo_kernel(const Problem p,
     }
     for (int i = 0; i < tiles; ++i) {
         __syncthreads();               // the joining buffer of the tile before has been read
-        few_rows<T, D, true>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, group * tiles + i);
+        few_rows<T, D, true>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, group * tiles + i, nullptr);
     }
     if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_groups + group, h);
 }
@@ -624,7 +686,7 @@ template <typename T, int D> struct Keys {
 };
 
 template <typename T, int D, bool CAREFUL>
-__global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float2 *lse, const float *delta, const Piece *pieces,
+__global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel(const Problem p, const T *dout, Strides ds, const float2 *lse, const float *delta, const float2 *tops, int n_tops, const Piece *pieces,
                                                         const int32_t *totals, const int32_t *count, const int32_t *list, float *partial, T *dk, T *dv, int32_t *flags) {
     constexpr int DC = D / 32, DT = D / 16, S = D + kPad, KT = Keys<T, D>::kTiles;
     constexpr int EPC = 16 / sizeof(T), CPR = D / EPC, RPL = 64 / CPR, N = kUnit / RPL;
@@ -672,6 +734,45 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     // pass does, and in steps with a reference so large that the sum would lose its last bits (from 2^24 on all of it).
     float *more = mores[wave];
 
+    // float16: powers are 2^kGain times p, so that shares of one in a million keep their bits, and dS is 2^kGain gain p (dP - delta) with a
+    // power of two that keeps gain (|dO| |V| + |delta|), a bound on gain |dP - delta|, below 2^4.  It goes by the longest of this wavefront's
+    // values and the largest rows of the sequence's heads, of those that are finite.  (A gain that follows the rows of the list,
+    // reducing the sums when a larger one comes, takes 24 us more of 8,192 tokens' 176, this 7.  p may pass 1 by what rounding does to
+    // large scores.)
+    constexpr int kGain = kNarrow<T> ? 10 : 0;
+    float gain = 1.f;
+    if constexpr (kNarrow<T>) {
+        float longest = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            float squares = 0.f;
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) squares += (float)vf[kt][dc][i] * (float)vf[kt][dc][i];
+            squares = rows_sum(squares);
+            longest = fmaxf(longest, squares < __builtin_inff() ? squares : 0.f);
+        }
+        float2 top = make_float2(0.f, 0.f);
+#pragma unroll 4
+        for (int i = tid; i < n_tops; i += kThreads) {
+            const float2 v = tops[(int64_t)pair * n_tops + i];
+            top = make_float2(fmaxf(top.x, v.x), fmaxf(top.y, v.y));
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            longest = fmaxf(longest, __shfl_xor(longest, d));
+            top.x = fmaxf(top.x, __shfl_xor(top.x, d));
+            top.y = fmaxf(top.y, __shfl_xor(top.y, d));
+        }
+        if (lane < 2) mores[wave][lane] = lane ? top.y : top.x;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) top = make_float2(fmaxf(top.x, mores[i][0]), fmaxf(top.y, mores[i][1]));
+        gain = __builtin_amdgcn_ldexpf(16.f, -__builtin_amdgcn_frexp_expf(top.x * __builtin_sqrtf(longest) + top.y));
+        __syncthreads();
+    }
+
     f32x4 ak[KT][DT], av[KT][DT];
     {
 #pragma unroll
@@ -692,7 +793,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
             const int64_t row = ((int64_t)b * p.queries + token) * p.heads + h * p.group + x;
             const float2 ls = lse[row];
             next = Row{ls.x, delta[row], offset + token, x};
-            next_more = ls.y;
+            next_more = ls.y - kGain;
             if (at >= piece.len) {
                 next.lse = __builtin_inff();
                 next.delta = next_more = 0.f;
@@ -745,6 +846,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
             }
             const bool apart = p.n_buckets || __any(fabsf(next.lse) > 4096.f && next.lse < __builtin_inff());
             if (!apart) next.lse += next_more;
+            if (kNarrow<T>) next.delta *= gain;
             if (lane < kUnit) {
                 own[lane] = next;
                 if (apart) more[lane] = next_more;
@@ -795,7 +897,7 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                         for (int kt = 0; kt < KT; ++kt) {
                             const float z = apart ? s[rt][kt][i] : s[rt][kt][i] * p.scale2 - row.lse;
                             float y = __builtin_amdgcn_exp2f(z);
-                            float e = y * (dp[rt][kt][i] - row.delta);
+                            float e = y * (kNarrow<T> ? dp[rt][kt][i] * gain - row.delta : dp[rt][kt][i] - row.delta);
                             if constexpr (decltype(masked)::value) {
                                 const int key = key0 + kt * 16 + c;
                                 const bool ok = key <= (p.causal ? row.pos : k_len - 1) && (!CAREFUL || row.lse < __builtin_inff());
@@ -849,8 +951,8 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     if constexpr (CAREFUL) {
-                        av[kt][dt] = mma_masked<T>(d, pf[kt], seen[kt], av[kt][dt]);
-                        ak[kt][dt] = mma_masked<T>(q, sf[kt], seen[kt], ak[kt][dt]);
+                        av[kt][dt] = mma_masked<T>(d, pf[kt], pl[kt], seen[kt], av[kt][dt]);
+                        ak[kt][dt] = mma_masked<T>(q, sf[kt], zero8<T>(), seen[kt], ak[kt][dt]);
                     } else {
                         av[kt][dt] = mma(d, pf[kt], av[kt][dt]);
                         if (sizeof(T) == 2) av[kt][dt] = mma(d, pl[kt], av[kt][dt]);
@@ -868,6 +970,14 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
     if (!CAREFUL) {
         odd = __syncthreads_or(odd);
         if (tid == 0) flags[unit] = odd;
+    }
+
+    if constexpr (kNarrow<T>) {
+        const float share = 1.f / (1 << kGain);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) { ak[kt][dt] *= share / gain; av[kt][dt] *= share; }
     }
 
     // wavefronts that share keys: the upper half hands its sums to the lower one, until one has them all
@@ -931,10 +1041,10 @@ struct Layout {
     bool many, short_lists;
     int n_groups, chunks, piece;               // n_groups: workgroups per sequence and key head of the sweep by query
     int64_t all, pieces, slots, entries;       // blocks of all sequences and key heads; bounds on the others
-    size_t delta, flags, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
+    size_t delta, largest, flags, bits, count, offset, piece0, slot0, totals, list, table, partial, bias, bytes;
 };
 
-int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *l) {
+int layout_of(const Problem &p, int head_len, int row_tiles, int parts, bool narrow, Layout *l) {
     const int tpt = tile_tokens(p.group), block = 1 << p.block_shift;
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
     auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
@@ -961,6 +1071,7 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, Layout *
     size_t at = 0;
     auto place = [&](size_t n) { const size_t here = at; at += (n + 255) & ~(size_t)255; return here; };
     l->delta = place((size_t)p.batch * p.queries * p.heads * sizeof(float));
+    l->largest = place(narrow ? (size_t)pairs * l->n_groups * sizeof(float2) : 0);
     l->flags = place((size_t)std::max(pairs * l->n_groups, l->pieces * parts) * sizeof(int32_t));
     l->bits = place(l->short_lists ? 0 : (size_t)l->all * l->chunks * 8);
     l->count = place((size_t)l->all * 4);
@@ -981,7 +1092,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     constexpr int RT = sizeof(T) == 4 ? 1 : 2;
     Layout l;
     const int block = 1 << p.block_shift, parts = Keys<T, D>::parts(block);
-    if (int rc = layout_of(p, D, RT, parts, &l)) return rc;
+    if (int rc = layout_of(p, D, RT, parts, kNarrow<T>, &l)) return rc;
     if (need) { *need = l.bytes; return FG_OK; }
     if (bytes < l.bytes || (l.bytes && !workspace)) return fail(FG_ERR_ARG, "block attention gradients: a workspace of %zu bytes, %zu needed (fg_block_attention_backward_workspace)", bytes, l.bytes);
     Strides ds;
@@ -989,7 +1100,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     unsigned char *w = static_cast<unsigned char *>(workspace);
     auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(w + at); };
     auto floats = [&](size_t at) { return reinterpret_cast<float *>(w + at); };
-    const Step step{grads->dout, a->out, a->rest, ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), grads->dq, floats(l.bias)};
+    const Step step{grads->dout, a->out, a->rest, ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), reinterpret_cast<float2 *>(w + l.largest), grads->dq, floats(l.bias)};
     const dim3 threads(kThreads);
     if (p.queries && p.batch) {
         const dim3 blocks((unsigned)(p.batch * p.kv_heads * l.n_groups));
@@ -1023,7 +1134,7 @@ int launch(const Problem &p, const fg_block_attention_args *a, const fg_block_at
     FG_HIP_TRY(hipGetLastError());
     const size_t lds = keys_stage_bytes<T, D>() + buckets_bytes(p.n_buckets, p.low, p.high, p.group);
     auto keys = [&](auto kernel) {
-        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), pieces, ints(l.totals),
+        kernel<<<dim3((unsigned)(l.pieces * parts)), threads, lds, stream>>>(p, static_cast<const T *>(grads->dout), ds, reinterpret_cast<const float2 *>(a->lse), floats(l.delta), step.largest, l.n_groups, pieces, ints(l.totals),
                                                                              l.short_lists ? ints(l.count) : nullptr, ints(l.list),
                                                                              floats(l.partial), static_cast<T *>(grads->dk), static_cast<T *>(grads->dv), ints(l.flags));
     };

@@ -296,6 +296,77 @@ def test_keys_gradients_of_scores_that_hold_no_fraction(batch, queries, block, s
     ref.check({"dk": got["dk"][:2, :, :, 32:]}, {"dk": tuple(a[..., 32:] for a in value["dk"])})
 
 
+# Shapes of the two kernels for queries, and of blocks whose keys one wavefront has and several share
+HALF_SHAPES = [(2, 70, 4, 2, 64, 32, 0), (1, 40, 16, 1, 128, 128, 8), (4, 1030, 8, 8, 32, 64, 0), (2, 1030, 16, 4, 128, 64, 16)]
+
+
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len,block,buckets", HALF_SHAPES)
+@pytest.mark.parametrize("long", ["q", "k"])
+@pytest.mark.parametrize("size", [2.0 ** -16, 2.0 ** -12])
+def test_small_gradients_of_16_bits(batch, queries, heads, kv_heads, head_len, block, buckets, long, size):
+    """Scores' gradients of 1e-6 are below float16's normal numbers, the results that long keys (queries) make of them are not."""
+    s, dout = make(F16, batch, queries, queries, heads, kv_heads, head_len, block, 3, buckets, seed=28)
+    s[long] *= 64
+    s["k" if long == "q" else "q"] /= 64
+    dout = (dout.float() * size).half()
+    ref.check(step(s, dout), want(s, dout))
+
+
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len,block,buckets", HALF_SHAPES)
+@pytest.mark.parametrize("values,gradients", [(64, 512), (4096, 1 / 16), (2 ** -6, 1024), (4096, 64)])
+def test_large_score_gradients_of_16_bits(batch, queries, heads, kv_heads, head_len, block, buckets, values, gradients):
+    """<dout, v> beyond float16's largest number; what comes of it, with short queries and keys, is within."""
+    s, dout = make(F16, batch, queries, queries, heads, kv_heads, head_len, block, 3, 0, seed=29)
+    s["q"] /= 1024
+    s["k"] /= 1024
+    s["v"] *= values
+    dout = (dout.float() * gradients).half()
+    ref.check(step(s, dout), want(s, dout))
+
+
+def test_gradients_of_16_bits_of_unequal_rows():
+    """Rows whose gradients are 2^20 times their neighbours'; keys that only the small ones see, and rows that come before and after them."""
+    s, dout = make(F16, 2, 200, 200, 4, 2, 64, 32, 2, seed=30)
+    s["k"] *= 64
+    s["q"] /= 64
+    s["blocks"][..., 1] = -1                             # each its own block
+    dout = (dout.float() * 2.0 ** -12).half()
+    dout[:, 40::32] *= 2.0 ** 14
+    dout[:, 60::64, 1] *= 2.0 ** 14
+    ref.check(step(s, dout), want(s, dout))
+
+
+@pytest.mark.parametrize("keys,block", [(1000, 64), (600, 32)])
+def test_shares_below_the_normal_numbers_of_16_bits(keys, block):
+    """One key has most of a row and the others 6e-6 each, between two multiples of float16's smallest number."""
+    nb = -(-keys // block)
+    s, dout = make(F16, 1, 1, keys, 1, 1, 32, block, nb, causal=False, seed=31)
+    s["blocks"][:] = torch.arange(nb, dtype=torch.int32, device="cuda")
+    s["q"].zero_(), s["k"].zero_()
+    s["q"][..., 0] = 32 ** 0.5                           # in float16 5.65625
+    top = [x for x in np.arange(11.5, 12.5, 2.0 ** -7) if 0.4 < 2.0 ** 24 / (np.exp(x * 5.65625 / 32 ** 0.5) + keys - 1) % 1 < 0.6][0]
+    s["k"][0, 5, 0, 0] = top
+    dout.fill_(2048)
+    ref.check(step(s, dout), want(s, dout))
+
+
+@pytest.mark.parametrize("batch", [2, 64])
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_small_gradients_of_16_bits_beside_infinities(batch, name):
+    s, dout = make(F16, batch, 96, 96, 4, 4, 64, 32, 1, seed=32)
+    s["q"] /= 64
+    s["k"] *= 64
+    s["blocks"][:] = 0
+    s["blocks"][:, 70:80] = 1                            # these rows alone see block 1
+    dout = (dout.float() * 2.0 ** -14).half()
+    value = ref.attention(*(s[x][:2] for x in ("q", "k", "v", "blocks")), 32, dout=dout[:2])
+    s[name][:, 40, :, 3] = float("inf")
+    got = step(s, dout)
+    keep = [i for i in range(96) if not 70 <= i < 80]
+    ref.check({x: got[x][:2, keep] for x in ("out", "dq")}, {x: tuple(a[:, keep] for a in value[x]) for x in ("out", "dq")})
+    ref.check({x: got[x][:2, :32] for x in ("dk", "dv")}, {x: tuple(a[:, :32] for a in value[x]) for x in ("dk", "dv")})
+
+
 def test_more_blocks_than_one_list_of_many_queries():
     """256 blocks are listed at a time where there are queries to fill the card; a row's blocks lie in several lists."""
     for dtype in (F32, BF16):

@@ -37,6 +37,10 @@ __device__ __forceinline__ float2 log_sum(float reference, float sum) {
     return sum == 0.f ? make_float2(__builtin_inff(), 0.f) : make_float2(reference, __builtin_amdgcn_logf(sum));
 }
 
+// How far below the largest score a row's reference stands, in base 2: float16 holds powers from 2^-14 on in full, and a long row's output may be
+// that of many small ones.  (They stay below 2^15: many_kernel's reference follows the maximum by up to 2^8.)
+template <typename T> constexpr float kBelow = std::is_same<T, _Float16>::value ? 7.f : 0.f;
+
 template <typename T, int D> constexpr size_t few_stage_bytes() {
     const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(T), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
     return values > merge ? values : merge;
@@ -151,7 +155,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
                         }
                 }
                 float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
-                top = fmaxf(m, rows_max(top));
+                top = fmaxf(m, rows_max(top) - kBelow<T>);
                 const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
                 if (__any(top != m)) {
                     const float shrink = __builtin_amdgcn_exp2f(m - ref);
@@ -416,7 +420,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, cons
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     const float most = largest(s[rt][0], s[rt][1]);
-                    high[rt] = largest_of_rows(mine_too[rt] ? most : -__builtin_inff()) * factor;
+                    high[rt] = largest_of_rows(mine_too[rt] ? most : -__builtin_inff()) * factor - kBelow<T>;
                     moved |= high[rt] > m[rt] + 8.f;
                 }
                 // sums are kept relative to a reference that follows the maximum when it has moved by more than 2^8

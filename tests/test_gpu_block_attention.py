@@ -350,6 +350,21 @@ def test_shares_below_the_normal_numbers_of_16_bits(keys, block):
     ref.check(step(s, dout), want(s, dout))
 
 
+@pytest.mark.parametrize("batch,queries", [(1, 1), (2, 40), (64, 32)])
+def test_outputs_of_shares_below_the_normal_numbers_of_16_bits(batch, queries):
+    """One key has most of a row and a value of 0; the others have 6e-7 each, and all of the output."""
+    s, _ = make(F16, batch, queries, 1000, 16, 1, 32, 64, 16, causal=False, seed=33)
+    s["blocks"][:] = torch.arange(16, dtype=torch.int32, device="cuda")
+    s["q"].zero_(), s["k"].zero_()
+    s["q"][..., 0] = 32 ** 0.5                           # in float16 5.65625
+    s["k"][:, 5, 0, 0] = [x for x in np.arange(14, 15, 2.0 ** -7) if 0.4 < 2.0 ** 24 * np.exp(-x * 5.65625 / 32 ** 0.5) % 1 < 0.6][0]
+    s["v"][:] = 1
+    s["v"][:, 5] = 0
+    value = ref.attention(*(s[x][:1] for x in ("q", "k", "v", "blocks")), 64, causal=False)
+    ref.check({"out": call(s)[:1]}, value)
+    ref.check({"out": call(s, q=s["q"].detach().requires_grad_())[:1]}, value)
+
+
 @pytest.mark.parametrize("batch", [2, 64])
 @pytest.mark.parametrize("name", ["k", "v"])
 def test_small_gradients_of_16_bits_beside_infinities(batch, name):

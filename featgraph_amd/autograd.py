@@ -718,7 +718,10 @@ class _Aggregate(torch.autograd.Function):
 
 def block_attention(q, k, v, bias, blocks, spec, lengths, q_lengths, bounds):
     """ops.block_attention on checked arguments; spec = (block_size, scale, causal)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+    # (inside a forward-mode level always: the function refuses inputs with a tangent, which would be dropped without a word.  Everywhere would
+    # cost a call without gradients 6 us)
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 \
+            or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
         return _BlockAttention.apply(q, k, v, bias, blocks, spec, lengths, q_lengths, bounds)
     return _block.block_attention_forward(q, k, v, blocks, *spec, lengths, q_lengths, bias, bounds, False)[0]
 

@@ -525,6 +525,20 @@ def test_rows_beyond_32_bit_offsets():
     assert all(torch.equal(got[x], value[x]) for x in got)
 
 
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as forward
+    s, _ = make(BF16, buckets=8)
+    plain = call(s)
+    with forward.dual_level():
+        torch.testing.assert_close(call(s), plain, rtol=2 ** -7, atol=1e-2)
+        for name in ("q", "k", "v", "bias"):
+            dual = forward.make_dual(s[name], torch.ones_like(s[name]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
+                    call(s, **{name: dual})
+    assert torch.equal(call(s), plain)
+
+
 def test_refusals():
     from featgraph_amd import ops
     s, _ = make(BF16)

@@ -1064,7 +1064,8 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, bool nar
     l->short_lists = (int64_t)p.queries * p.group <= 768 && (int64_t)p.queries * p.topk <= 4096;
     l->entries = l->short_lists ? l->all * p.queries : pairs * p.queries * std::min(p.topk, p.blocks);
     l->pieces = l->short_lists ? l->all : l->all + l->entries / l->piece;
-    l->slots = l->short_lists || p.queries <= l->piece ? 0 : 2 * (l->entries / l->piece);
+    // a list of n tokens that is cut has floor(n / piece) + 1 pieces at most, and no more than 2 floor(n / piece)
+    l->slots = l->short_lists || p.queries <= l->piece ? 0 : std::min(2 * (l->entries / l->piece), l->entries / l->piece + l->all);
     const int64_t limit = INT32_MAX;
     if (l->entries > limit || l->pieces * parts > limit || l->all * (2 * block * head_len / 4 / kThreads) > limit || pairs * std::max(l->n_groups, l->chunks) > limit)
         return fail(FG_ERR_SHAPE, "block attention gradients: %lld selections of %lld blocks do not fit the 32-bit lists", (long long)l->entries, (long long)l->all);

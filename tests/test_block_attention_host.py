@@ -81,6 +81,24 @@ def test_c_interface_refuses_lists_beyond_32_bits():
     assert 0 < L.fg_block_attention_backward_workspace(ctypes.byref(a)) < 2 ** 33
 
 
+@pytest.mark.parametrize("queries,heads,kv_heads,head_len,block,topk", [(8192, 16, 1, 64, 128, 8), (16384, 32, 8, 128, 256, 16), (4096, 16, 4, 128, 64, 16)])
+def test_gradients_reserve_no_more_pieces_than_there_can_be(queries, heads, kv_heads, head_len, block, topk):
+    L = _lib.lib()
+    a = _args(type=1, queries=queries, keys=queries, heads=heads, kv_heads=kv_heads, head_len=head_len, block=block, topk=topk)
+    for x, h in ((a.q_strides, heads), (a.k_strides, kv_heads), (a.v_strides, kv_heads)):
+        x[0], x[1], x[2] = queries * h * head_len, h * head_len, head_len
+    # a list of n tokens has floor(n / piece) + 1 pieces at most, and a piece some 768 rows at least; beside their sums there are rows of delta, marks
+    # (a bit for each token and block) and the lists
+    entries, blocks = queries * kv_heads * topk, kv_heads * queries // block
+    sums = (entries * (heads // kv_heads) // 768 + blocks) * 2 * block * head_len * 4
+    rest = 4 * queries * heads + blocks * queries // 8 + 4 * entries + 2 ** 20
+    need = L.fg_block_attention_backward_workspace(ctypes.byref(a))
+    assert 0 < need <= sums + rest
+    rows = entries * (heads // kv_heads)
+    piece = min(max(2048, rows // 8192), max(768, rows // 1024))
+    assert need <= (entries * (heads // kv_heads) // piece + blocks) * 2 * block * head_len * 4 + rest
+
+
 def test_pool_and_select_refuse():
     L = _lib.lib()
     strides = (ctypes.c_int64 * 3)(64 * 200 * 2, 64 * 2, 64)

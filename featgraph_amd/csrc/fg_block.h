@@ -313,6 +313,8 @@ __device__ __forceinline__ Buckets load_buckets(const Problem &p, int h, unsigne
 
 // Fills a Problem from the C interface's arguments; FG_OK or an error with its message.
 int problem_of(const fg_block_attention_args *a, Problem *p);
+// A dense array that the kernels access `bytes` at a time; null is fine.
+int aligned(const char *name, const void *ptr, int bytes);
 // A strided operand: dense heads, every one of them at a 16-byte address.
 int strides_of(const char *name, const void *ptr, const int64_t *stride, int size, Strides *s);
 }  // namespace block

@@ -607,6 +607,10 @@ int launch_t(const Problem &p, const fg_block_attention_args *a, void *workspace
 
 }  // namespace
 
+int aligned(const char *name, const void *ptr, int bytes) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes ? fail(FG_ERR_ARG, "block attention: %s has to stand at a multiple of %d bytes", name, bytes) : FG_OK;
+}
+
 int strides_of(const char *name, const void *ptr, const int64_t *stride, int size, Strides *s) {
     const int64_t per = 16 / size;
     if (reinterpret_cast<uintptr_t>(ptr) % 16 || stride[0] % per || stride[1] % per || stride[2] % per)
@@ -643,7 +647,9 @@ int problem_of(const fg_block_attention_args *a, Problem *p) {
     const int size = a->type == FG_TYPE_F32 ? 4 : 2;
     int rc;
     if ((rc = strides_of("q", a->q, a->q_strides, size, &p->qs)) || (rc = strides_of("k", a->k, a->k_strides, size, &p->ks)) ||
-        (rc = strides_of("v", a->v, a->v_strides, size, &p->vs))) return rc;
+        (rc = strides_of("v", a->v, a->v_strides, size, &p->vs)) || (rc = aligned("out", a->out, 16)) || (rc = aligned("rest", a->rest, 16)) ||
+        (rc = aligned("lse", a->lse, 8)) || (rc = aligned("blocks", a->blocks, 4)) || (rc = aligned("lengths", a->lengths, 4)) ||
+        (rc = aligned("q_lengths", a->q_lengths, 4)) || (rc = aligned("bias", a->bias, size))) return rc;
     p->batch = a->batch; p->queries = a->queries; p->keys = a->keys; p->heads = a->heads; p->kv_heads = a->kv_heads; p->group = a->heads / a->kv_heads;
     p->block_shift = a->block == 32 ? 5 : a->block == 64 ? 6 : a->block == 128 ? 7 : 8;
     p->blocks = (a->keys + a->block - 1) / a->block;
@@ -668,5 +674,6 @@ extern "C" int fg_block_attention(const fg_block_attention_args *args, void *wor
     if (int rc = fg::block::problem_of(args, &p)) return rc;
     if ((int64_t)p.batch * p.queries == 0) return FG_OK;
     if (!p.q || !p.list || !args->out || (p.keys && (!p.k || !p.v)) || (p.n_buckets && !p.bias)) return fg::fail(FG_ERR_ARG, "block attention: null pointer");
+    if (int rc = fg::block::aligned("the workspace", workspace, 16)) return rc;
     return fg::block::launch_t(p, args, workspace, workspace_bytes, nullptr, static_cast<hipStream_t>(stream));
 }

@@ -1184,5 +1184,9 @@ extern "C" int fg_block_attention_backward(const fg_block_attention_args *args, 
     if (p.batch && ((p.queries && (!p.q || !p.list || !args->out || !args->lse || !grads->dout || !grads->dq)) || (p.keys && (!p.k || !p.v)) ||
         !grads->dk != !grads->dv || (p.n_buckets && !p.bias)))
         return fg::fail(FG_ERR_ARG, "block attention gradients: null pointer");
+    using fg::block::aligned;
+    int rc;
+    if ((rc = aligned("the workspace", workspace, 16)) || (rc = aligned("dq", grads->dq, 16)) || (rc = aligned("dk", grads->dk, 16)) ||
+        (rc = aligned("dv", grads->dv, 16)) || (rc = aligned("dbias", grads->dbias, args->type == FG_TYPE_F32 ? 4 : 2))) return rc;
     return fg::block::launch_t(p, args, grads, workspace, workspace_bytes, nullptr, static_cast<hipStream_t>(stream));
 }

@@ -647,8 +647,8 @@ typedef struct {
     const int32_t *lengths, *q_lengths;
     const void *bias;                  /* (n_buckets, heads) dense: added to the scaled score of query position i and key j in
                                           bucket  (number of bounds <= i - j) */
-    void *out;                         /* (batch, queries, heads, head_len) dense; 0 where a query sees no key */
-    float *lse;                        /* (batch, queries, heads, 2) or null: what the gradients start from -- a number near the row's
+    void *out;                         /* (batch, queries, heads, head_len) dense, at a multiple of 16 bytes; 0 where a query sees no key */
+    float *lse;                        /* (batch, queries, heads, 2) at a multiple of 8 bytes, or null: what the gradients start from -- a number near the row's
                                           largest base-2 exponent (+inf where it sees no key), and the base-2 logarithm of the sum of
                                           the powers relative to it */
     void *rest;                        /* as out, or null: what rounding took from out, itself rounded to the type; with it the gradients
@@ -656,15 +656,15 @@ typedef struct {
 } fg_block_attention_args;
 
 /* Softmax attention over the selected blocks.  workspace: device memory of at least fg_block_attention_workspace(args) bytes (which only
- * looks at sizes; negative: an error), 256-byte aligned, of this call alone while it runs; null if that is 0. */
+ * looks at sizes; negative: an error), 16-byte aligned, of this call alone while it runs; null if that is 0. */
 int64_t fg_block_attention_workspace(const fg_block_attention_args *args);
 int fg_block_attention(const fg_block_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 typedef struct {
     const void *dout;                  /* dL / d(out) */
     int64_t dout_strides[3];
-    void *dq;                          /* dense, as q; rows behind q_lengths 0 */
-    void *dk, *dv;                     /* dense, as k; rows behind lengths 0 */
+    void *dq;                          /* dense, as q, at a multiple of 16 bytes; rows behind q_lengths 0 */
+    void *dk, *dv;                     /* dense, as k, at multiples of 16 bytes; rows behind lengths 0; both or neither (null) */
     void *dbias;                       /* (n_buckets, heads) dense, or null */
 } fg_block_attention_grads;
 

@@ -68,6 +68,30 @@ def test_c_interface_refuses_null_pointers_and_small_workspaces():
         assert L.fg_block_attention(ctypes.byref(a), None, 0, None) == 0
 
 
+def test_c_interface_refuses_what_vector_accesses_cannot_reach():
+    L = _lib.lib()
+    good = dict(queries=1, keys=8192, topk=64, q=64, k=64, v=64, blocks=64, out=64, lse=64, rest=64)
+    work = ctypes.c_void_p(256)
+    for name, value in (("out", 72), ("rest", 80 + 2), ("lse", 68), ("q", 72), ("k", 66), ("v", 68), ("blocks", 66), ("lengths", 66), ("q_lengths", 65), ("bias", 65)):
+        a = _args(**dict(good, **{name: value}))
+        if name == "bias":
+            a.n_buckets = 1
+        assert L.fg_block_attention(ctypes.byref(a), work, 1 << 40, None) == -1, name
+        with pytest.raises(ValueError, match="bytes"):
+            _lib.check(-1)
+    a = _args(**good)
+    assert L.fg_block_attention(ctypes.byref(a), ctypes.c_void_p(264), 1 << 40, None) == -1
+    with pytest.raises(ValueError, match="bytes"):
+        _lib.check(-1)
+    for name, value in (("dout", 72), ("dq", 72), ("dk", 66), ("dv", 68), ("dbias", 65)):
+        grads = _lib.FgBlockAttentionGrads(**dict(dict(dout=64, dout_strides=a.q_strides, dq=64, dk=64, dv=64), **{name: value}))
+        assert L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), work, 1 << 40, None) == -1, name
+        with pytest.raises(ValueError, match="bytes"):
+            _lib.check(-1)
+    grads = _lib.FgBlockAttentionGrads(dout=64, dout_strides=a.q_strides, dq=64, dk=64, dv=64)
+    assert L.fg_block_attention_backward(ctypes.byref(a), ctypes.byref(grads), ctypes.c_void_p(264), 1 << 40, None) == -1
+
+
 def test_c_interface_refuses_lists_beyond_32_bits():
     L = _lib.lib()
     size = 1 << 20

@@ -170,18 +170,17 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Results &r, Few
                     for (int i = 0; i < 4; ++i)
                         s[kt][i] = z[kt][i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], factor, -ref));
                 l += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
-                // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not.  For gradients
-                // what the rounding took follows in a second product, as in many_kernel.
+                // the powers are rounded to the operands' type for the product with V, half a step each; their sum is not.  What the rounding
+                // took follows in a second product, with gradients or without: it takes no time that shows here.
                 V8<T> pf, pl;
                 block::split<T>(s[0], s[1], &pf, &pl);
-                if (decltype(careful)::value && !r.rest) pl = zero8<T>();
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     const V8<T> vf = transposed<T, D>(stage, dt * 16, lane);
                     if constexpr (decltype(careful)::value) o[dt] = mma_masked<T>(vf, pf, pl, seen, o[dt]);
                     else o[dt] = mma(vf, pf, o[dt]);
                 }
-                if (sizeof(T) == 2 && !decltype(careful)::value && r.rest)
+                if (sizeof(T) == 2 && !decltype(careful)::value)
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) o[dt] = mma(transposed<T, D>(stage, dt * 16, lane), pl, o[dt]);
             }
@@ -264,8 +263,8 @@ template <typename T, int D> struct Steps {
 
 // RT tiles of 16 rows per wavefront.  flags[workgroup]: whether a result was not finite (see redo_kernel).
 // EXACT: what the powers' rounding took goes into a second product with V.  Gradients start from <dO, O>, which a row's dS takes away from
-// numbers of its own size: with rounded powers it would be further off than the gradients' own rounding (2 x 4,096 tokens, 16 / 4 heads
-// 174 and 210 us).
+// numbers of its own size: with rounded powers it would be further off than the gradients' own rounding.  Without gradients the powers' rounding
+// is of the size of the output's own, and the second product is left out (8,192 tokens, 32 / 8 heads 372 and 450 us).
 template <typename T, int D, int RT, bool BIAS, bool EXACT>
 __global__ __launch_bounds__(kThreads, 2) void many_kernel(const Problem p, const Results r, int32_t *flags, int n_groups) {
     constexpr int DC = D / 32, DT = D / 16, TILES = kWaves * RT;

@@ -134,7 +134,10 @@ def block_attention(q, k, v, blocks, block_size, scale=None, causal=True, length
     bias (buckets, heads), at most 64 buckets, with `bounds`, buckets - 1 ascending distances (position_bounds): query position less key
     position is in bucket (number of bounds that are not above it).
 
-    Differentiable in q, k, v and bias; the same bits on every call.  head_len 32, 64 or 128, block_size 32, 64, 128 or 256."""
+    Differentiable in q, k, v and bias.  The same bits on every call, whatever else runs; but in float16 and bfloat16 a call over enough
+    queries to fill the card rounds the softmax's powers to the type, half a step each, where no gradient is wanted, and keeps what that takes
+    where one is: with and without gradients its outputs differ by about their own rounding (also under checkpointing that runs the
+    first forward pass without).  head_len 32, 64 or 128, block_size 32, 64, 128 or 256."""
     bounds = _block.check_attention(q, k, v, blocks, block_size, lengths, q_lengths, bias, bounds)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     return autograd.block_attention(q, k, v, bias, blocks, (block_size, scale, bool(causal)), lengths, q_lengths, bounds)

@@ -446,6 +446,15 @@ def test_gradients_of_some_inputs_only():
     torch.testing.assert_close(g, part["dk"] + part["dv"])
 
 
+@pytest.mark.parametrize("dtype,batch,queries,keys,topk", [(F16, 2, 70, 70, 2), (BF16, 2, 70, 70, 2), (BF16, 3, 1, 5000, 60), (F16, 1, 5, 3000, 40), (F32, 64, 70, 70, 2)])
+def test_outputs_with_and_without_gradients_are_the_same(dtype, batch, queries, keys, topk):
+    """Of a few queries in every type, and of any number of them in 32 bits."""
+    s, _ = make(dtype, batch, queries, keys, 8, 4, 64, 32, topk, 8, seed=34)
+    with torch.no_grad():
+        plain = call(s, q=s["q"].detach().requires_grad_())
+    assert torch.equal(plain, call(s)) and torch.equal(plain, call(s, q=s["q"].detach().requires_grad_()))
+
+
 def test_gradients_against_differences():
     s, dout = make(F32, 1, 40, 40, 2, 1, 32, 32, 2, 6, seed=15)
     got = step(s, dout)

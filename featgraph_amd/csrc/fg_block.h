@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
+#include <type_traits>
 
 #include "fg_common.h"
 #include "fg_device.h"
@@ -122,12 +123,16 @@ __device__ __forceinline__ bool not_finite(f32x4 v) {
     return t != t;
 }
 
+// What rounding took from a result is at most half of its last place.  float16 has no numbers for that below 2^-24, and few bits for it below 2^-3: it
+// is stored 2^11 times as large, of the result's own size.
+template <typename T> constexpr float kRestScale = std::is_same<T, _Float16>::value ? 2048.f : 1.f;
+
 // Four consecutive elements of a result, rounded to its type, and what the rounding took where that is wanted.
 template <typename T> __device__ __forceinline__ void store_row(T *out, T *rest, int64_t at, f32x4 v) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     T4 x, y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = (T)v[i]; y[i] = (T)(v[i] - (float)x[i]); }
+    for (int i = 0; i < 4; ++i) { x[i] = (T)v[i]; y[i] = (T)((v[i] - (float)x[i]) * kRestScale<T>); }
     *reinterpret_cast<T4 *>(out + at) = x;
     if (rest) *reinterpret_cast<T4 *>(rest + at) = y;
 }

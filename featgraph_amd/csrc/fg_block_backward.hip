@@ -159,12 +159,12 @@ __global__ __launch_bounds__(kThreads) void fill_kernel(const unsigned long long
 struct Step { const void *dout, *out, *rest; Strides ds; const float2 *lse; float *delta; float2 *largest; void *dq; float *bias_sums; };
 
 // float16 holds numbers from 6e-5 (in full) to 65504, and dS has the gradients' range: loss scaling moves it, but between rows and heads it
-// remains wide.  So dS enters its products times a power of two and the sums are taken back in 32 bits.  By query every row has its own:
-// with |dO| 2^up <= 2^room, dS is p (dP - delta) 2^up <= p |V| 2^room.  Room of 2^6 is enough for |V_j| up to 2^9 and leaves p down to
-// 2^-20 in full; longer values make dS infinite, and such tiles are computed again (as those with infinities are) with room 2^-4: all that
-// 128 elements of 65504, |V_j| < 2^19.5, can ask for, since p (dP - delta) <= |dO| max |V| / 2.  By key see keys_kernel.
+// remains wide.  So dS enters its products times a power of two and the sums are taken back in 32 bits.  By query every row has its own, 2^up:
+// 2^kRoom over |dO_i| |O_i|, where dS = p <dO_i, V_j - O_i> is of the size of p 2^kRoom, or of some times that.  A row whose values nearly cancel
+// one another makes it infinite: it is computed again, as tiles with infinities are, with 2^kSafeRoom over |dO_i|, which nothing
+// finite can exceed: |dS| <= |dO_i| max |V| / 2, and 128 elements of 65504 are |V| < 2^19.5.  By key see keys_kernel.
 template <typename T> constexpr bool kNarrow = std::is_same<T, _Float16>::value;
-constexpr int kRoom = 6, kSafeRoom = -4;
+constexpr int kRoom = 8, kSafeRoom = -4;
 
 // A lane's row of a tile: dO and Q as operands, and delta.
 template <typename T, int D> struct Row16 {
@@ -174,7 +174,7 @@ template <typename T, int D> struct Row16 {
     float lse, weight, less, down;     // in float16 weight and less are 2^up times that, down is 2^-up
     float delta, more;
     float norm;                        // |dO|
-    int size;                          // |dO| <= 2^size
+    int up, safe_up;
     int limit;                         // last key that it may see; columns without a row see everything, nothing is written of them
     __device__ __forceinline__ void load(const Problem &p, const Step &w, int b, int t, int head, bool used, int q_len, int k_len, int offset, int g, bool write) {
         const bool there = used && t < q_len;
@@ -183,7 +183,7 @@ template <typename T, int D> struct Row16 {
         const T *qs = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head + 8 * g;
         const T *dos = static_cast<const T *>(w.dout) + b * w.ds.batch + (int64_t)t * w.ds.row + head * w.ds.head + 8 * g;
         const T *os = static_cast<const T *>(w.out) + at * D + 8 * g, *rs = static_cast<const T *>(w.rest) + at * D + 8 * g;
-        float sum = 0.f, squares = 0.f;
+        float sum = 0.f, squares = 0.f, of_out = 0.f;
 #pragma unroll
         for (int dc = 0; dc < D / 32; ++dc) {
             q[dc] = there ? load8(qs + dc * 32) : zero8<T>();
@@ -193,11 +193,11 @@ template <typename T, int D> struct Row16 {
             for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)o[i];
             if (kNarrow<T>)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) squares += (float)d[dc][i] * (float)d[dc][i];
+                for (int i = 0; i < 8; ++i) { squares += (float)d[dc][i] * (float)d[dc][i]; of_out += (float)o[i] * (float)o[i]; }
             if (w.rest) {
                 const V8<T> r = there ? load8(rs + dc * 32) : zero8<T>();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * (float)r[i];
+                for (int i = 0; i < 8; ++i) sum += (float)d[dc][i] * ((float)r[i] * (1.f / kRestScale<T>));
             }
         }
         delta = rows_sum(sum);
@@ -206,10 +206,13 @@ template <typename T, int D> struct Row16 {
         more = ls.y;
         if (there && write && g == 0) w.delta[at] = delta;
         norm = 0.f;
-        size = 0;
+        up = safe_up = 0;
         if (kNarrow<T>) {
             squares = rows_sum(squares);
-            size = (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1;
+            of_out = rows_sum(of_out);
+            const int size = (__builtin_amdgcn_frexp_expf(squares) + 1) >> 1;          // |dO| <= 2^size
+            safe_up = kSafeRoom - size;
+            up = of_out > 0.f ? kRoom - size - ((__builtin_amdgcn_frexp_expf(of_out) + 1) >> 1) : safe_up;
             norm = __builtin_sqrtf(squares);
         }
     }
@@ -220,11 +223,11 @@ template <typename T, int D> struct Row16 {
         for (int d = 1; d < 16; d <<= 1) { v.x = fmaxf(v.x, __shfl_xor(v.x, d)); v.y = fmaxf(v.y, __shfl_xor(v.y, d)); }
         return v;
     }
-    __device__ __forceinline__ void weigh(int room) {
-        const float up = kNarrow<T> ? room - size : 0.f;
-        weight = __builtin_amdgcn_exp2f(up - more);
+    __device__ __forceinline__ void weigh(bool safe) {
+        const float by = kNarrow<T> ? (float)(safe ? safe_up : up) : 0.f;
+        weight = __builtin_amdgcn_exp2f(by - more);
         less = delta * weight;
-        down = __builtin_amdgcn_exp2f(-up);
+        down = __builtin_amdgcn_exp2f(-by);
     }
     // Whether a row of the wavefront is relative to a number, out of the bias, so large that adding the bias to the reference first would
     // leave other scores than the forward pass had.
@@ -238,8 +241,8 @@ __device__ __forceinline__ float *bias_place(const Problem &p, unsigned char *ld
 size_t bias_bytes(const Problem &p) {
     return p.n_buckets ? ((buckets_bytes(p.n_buckets, p.low, p.high, p.group) + 15) & ~(size_t)15) + (size_t)kWaves * p.n_buckets * 64 * sizeof(float) : 0;
 }
-// A workgroup's share of it, [workgroup of all sequences][head][bucket].
-__device__ __forceinline__ void write_bias(const Problem &p, const float *sums, float *out, int64_t workgroup, int h) {
+// A workgroup's share of it, [workgroup of all sequences][head][bucket]; `more`: added to what it was.
+__device__ __forceinline__ void write_bias(const Problem &p, const float *sums, float *out, int64_t workgroup, int h, bool more = false) {
     const int tpt = tile_tokens(p.group);
     __syncthreads();
     for (int e = threadIdx.x; e < p.n_buckets * p.group; e += kThreads) {
@@ -248,7 +251,8 @@ __device__ __forceinline__ void write_bias(const Problem &p, const float *sums, 
         for (int w = 0; w < kWaves; ++w)
             for (int t = 0; t < tpt; ++t)
                 for (int q = 0; q < 4; ++q) total += sums[(w * p.n_buckets + n) * 64 + q * 16 + t * p.group + x];
-        out[(workgroup * p.heads + h * p.group + x) * p.n_buckets + n] = total;
+        float *to = out + (workgroup * p.heads + h * p.group + x) * p.n_buckets + n;
+        *to = more ? *to + total : total;
     }
 }
 
@@ -317,7 +321,7 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
 
     f32x4 acc[DT];
     auto sweep = [&](auto careful) {
-        row.weigh(decltype(careful)::value ? kSafeRoom : kRoom);
+        for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int first = 0; first < p.blocks; first += kWindow) {
@@ -385,16 +389,28 @@ __device__ __forceinline__ void few_rows(const Problem &p, const Step &w, List<1
             }
         }
     };
-    if constexpr (CAREFUL) {
-        sweep(std::true_type{});
-    } else {
-        sweep(std::false_type{});
-        bool odd = false;
+    auto odd = [&]() {
+        bool any = false;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(acc[dt]);
-        if (__syncthreads_or(odd)) {
-            for (int n = 0; n < p.n_buckets; ++n) sums[n * 64 + lane] = 0.f;
+        for (int dt = 0; dt < DT; ++dt) any |= not_finite(acc[dt]);
+        return any;
+    };
+    bool again = CAREFUL;
+    row.weigh(false);
+    if constexpr (!CAREFUL) {
+        sweep(std::false_type{});
+        again = __syncthreads_or(odd());
+    }
+    if (again) {
+        // a second time where rows are left that are not finite (they may want the smaller power of two)
+        __shared__ unsigned safe;
+        if (tid == 0) safe = 0;
+        for (int i = 0; i < 2; ++i) {
             sweep(std::true_type{});
+            if (!kNarrow<T> || i || !__syncthreads_or(odd())) break;
+            if (odd()) atomicOr(&safe, 1u << c);
+            __syncthreads();
+            row.weigh((safe >> c) & 1);
         }
     }
     if (kNarrow<T>)
@@ -428,7 +444,6 @@ __global__ __launch_bounds__(kThreads) void queries_few_kernel(const Problem p, 
         unsigned char *at = dynamic + few_stage_bytes<T, D>();
         buckets = load_buckets<T>(p, h, at);
         sums = bias_place(p, at);
-        for (int i = threadIdx.x; i < kWaves * p.n_buckets * 64; i += kThreads) sums[i] = 0.f;
     }
     few_rows<T, D, false>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, tile, w.largest + unit);
     if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_tiles + tile, h);
@@ -471,7 +486,7 @@ __global__ __launch_bounds__(kThreads, 2) void queries_many_kernel(const Problem
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         row[rt].load(p, w, b, t0 + (wave * RT + rt) * tpt + tc, head, used, q_len, k_len, offset, g, true);
-        row[rt].weigh(kRoom);
+        row[rt].weigh(false);
     }
     if (kNarrow<T>) {
         float2 top = row[0].largest();
@@ -642,13 +657,12 @@ __global__ __launch_bounds__(kThreads) void queries_redo_kernel(const Problem p,
         unsigned char *at = dynamic + few_stage_bytes<T, D>();
         buckets = load_buckets<T>(p, h, at);
         sums = bias_place(p, at);
-        for (int i = threadIdx.x; i < kWaves * p.n_buckets * 64; i += kThreads) sums[i] = 0.f;
     }
     for (int i = 0; i < tiles; ++i) {
-        __syncthreads();               // the joining buffer of the tile before has been read
+        __syncthreads();               // the joining buffer and the bias's sums of the tile before have been read
         few_rows<T, D, true>(p, w, list, dynamic, buckets, sums + (threadIdx.x >> 6) * p.n_buckets * 64, b, h, group * tiles + i, nullptr);
+        if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_groups + group, h, i > 0);
     }
-    if (p.n_buckets) write_bias(p, sums, w.bias_sums, (int64_t)b * n_groups + group, h);
 }
 
 // dbias[n, head]: the tiles' sums in order, a share of them for each group of threads, then the shares in order.

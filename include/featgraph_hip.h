@@ -651,7 +651,7 @@ typedef struct {
     float *lse;                        /* (batch, queries, heads, 2) at a multiple of 8 bytes, or null: what the gradients start from -- a number near the row's
                                           largest base-2 exponent (+inf where it sees no key), and the base-2 logarithm of the sum of
                                           the powers relative to it */
-    void *rest;                        /* as out, or null: what rounding took from out, itself rounded to the type; with it the gradients
+    void *rest;                        /* as out, or null: what rounding took from out (in float16 2^11 times that), itself rounded to the type; with it the gradients
                                           know <dout, out> to twice the type's bits */
 } fg_block_attention_args;
 

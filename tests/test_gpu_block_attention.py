@@ -324,6 +324,28 @@ def test_large_score_gradients_of_16_bits(batch, queries, heads, kv_heads, head_
     ref.check(step(s, dout), want(s, dout))
 
 
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len,block,buckets", HALF_SHAPES)
+def test_gradients_of_small_values_of_16_bits(batch, queries, heads, kv_heads, head_len, block, buckets):
+    """Outputs of a few times float16's smallest number: <dout, out> has to hold what their rounding took, for keys have much in common."""
+    s, dout = make(F16, batch, queries, queries, heads, kv_heads, head_len, block, 3, buckets, seed=35)
+    s["k"] += 64
+    s["q"] /= 64
+    s["v"] *= 2.0 ** -20
+    dout *= 1024
+    ref.check(step(s, dout), want(s, dout))
+
+
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len,block,buckets", HALF_SHAPES)
+def test_gradients_of_16_bits_of_values_that_cancel(batch, queries, heads, kv_heads, head_len, block, buckets):
+    """Equal keys with opposite values, but for the last bit of one element: outputs far below the values, whose differences are not."""
+    s, dout = make(F16, batch, queries, queries, heads, kv_heads, head_len, block, 3, buckets, causal=False, seed=36)
+    s["k"][:, 1::2], s["v"][:, 1::2] = s["k"][:, ::2], -s["v"][:, ::2]
+    s["v"][:, 1::2, :, 0] *= 1 + 2.0 ** -10
+    if buckets:
+        s["bias"][:] = s["bias"][:1]                     # equal keys in two buckets keep equal scores
+    ref.check(step(s, dout), want(s, dout))
+
+
 def test_gradients_of_16_bits_of_unequal_rows():
     """Rows whose gradients are 2^20 times their neighbours'; keys that only the small ones see, and rows that come before and after them."""
     s, dout = make(F16, 2, 200, 200, 4, 2, 64, 32, 2, seed=30)

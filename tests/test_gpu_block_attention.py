@@ -414,6 +414,17 @@ def test_more_blocks_than_one_list_of_many_queries():
             ref.check({x: t[b:b + 1] for x, t in got.items()}, value)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch,queries,heads,keys,ends", [(1, 20, 2, 70001, (1023, 1024, 2047, 2048)), (256, 8, 16, 17000, (255, 256, 511, 512))])
+def test_blocks_at_the_ends_of_windows(dtype, batch, queries, heads, keys, ends):
+    """Few queries list 1,024 blocks at a time, many 256: the last of a list and the first of the next."""
+    s, dout = make(dtype, batch, queries, keys, heads, 1, 32, 32, 6, seed=37)
+    s["blocks"][..., 1:5] = ints(*ends)
+    got = step(s, dout)
+    value = want(dict(s, **{x: s[x][:1] for x in ("q", "k", "v", "blocks")}), dout[:1])
+    ref.check({x: t[:1] for x, t in got.items()}, value)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("queries", [40, 2100])
 def test_the_most_buckets(dtype, queries):

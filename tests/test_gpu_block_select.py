@@ -66,6 +66,18 @@ def test_ragged_batch():
         assert (got[:, :, :, 0] >= got[:, :, :, 1]).logical_or(got[:, :, :, 1] > got[:, :, :, 0]).all()
 
 
+@pytest.mark.parametrize("topk", [2, 3, 9, 40])
+@pytest.mark.parametrize("causal", [True, False])
+def test_lists_ascend_and_end_in_minus_one(topk, causal):
+    from featgraph_amd import ops
+    q, k = make(BF16, 4, 60, 1000, 4, 2, 64, seed=14)
+    lengths, q_lengths = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([1000, 77, 0, 500], [60, 60, 60, 5]))
+    got = ops.select_blocks(q, ops.pool_blocks(k, 32, lengths), 1000, 32, topk, causal, lengths, q_lengths)
+    before, after = got[..., :-1], got[..., 1:]
+    assert ((after == -1) | ((before >= 0) & (after > before))).all()
+    assert (got >= -1).all() and (got < 32).all()
+
+
 def test_first_and_last_blocks_are_kept():
     q, k = make(F16, 1, 80, 640, 2, 1, 32, seed=3)
     for first, last, topk in ((0, 0, 4), (2, 0, 4), (0, 3, 4), (2, 2, 4), (4, 0, 4), (0, 0, 1)):

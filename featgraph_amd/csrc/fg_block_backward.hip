@@ -7,10 +7,11 @@
 // list, with its keys in registers, and gathers the rows of its tokens' heads.  Nothing is added by atomics: sums over pieces,
 // wavefronts and tiles are joined in a fixed order, so that a step gives the same bits every time.
 //
-// What bounds them (2 x 4,096 tokens, 16 / 4 heads of 128 in bfloat16, 16 blocks of 64): queries_many_kernel 275 us, as the forward pass,
-// with two products more; keys_kernel 341 us: one wavefront per SIMD (sums of 32 keys, their operands and the rows under way take 396
+// What bounds them (2 x 4,096 tokens, 16 / 4 heads of 128 in bfloat16, 16 blocks of 64): queries_many_kernel 278 us, as the forward pass,
+// with two products more; keys_kernel 369 us: one wavefront per SIMD (sums of 32 keys, their operands and the rows under way take 398
 // registers), so that every wait shows, and 70 us of beginnings and ends of 1,100 pieces; the lists 24 us in four launches, the sums of
-// pieces 14 (5 TB/s).  With heads of 64 two wavefronts fit (8,192 tokens, 16 / 1 heads, 8 blocks of 128: 151 and 171 us).
+// pieces 14 (5 TB/s).  With heads of 64 two wavefronts fit (8,192 tokens, 16 / 1 heads, 8 blocks of 128 in float16: 152 and 206 us, 7 of them
+// for the scale of dS).
 #include <algorithm>
 #include <type_traits>
 
@@ -952,12 +953,13 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
             if (CAREFUL || key0 + 16 * KT > k_len || (p.causal && from < key0 + 16 * KT - 1)) gradients(std::true_type{});
             else gradients(std::false_type{});
             // the powers go into dV's product rounded, and what that took (in 16 bits) in a second one: nearly even ones are all rounded the
-            // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 27 us)
-            V8<T> pf[KT], pl[KT], sf[KT];
+            // same way, which no sum evens out (2 x 4,096 tokens, 16 / 4 heads 27 us); so does dS into dK's, whose error would be 1.4 times that
+            // of rounding dK itself (22 us)
+            V8<T> pf[KT], pl[KT], sf[KT], sl[KT];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 split<T>(s[0][kt], s[1][kt], &pf[kt], &pl[kt]);
-                sf[kt] = pack<T>(dp[0][kt], dp[1][kt]);
+                split<T>(dp[0][kt], dp[1][kt], &sf[kt], &sl[kt]);
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
@@ -966,11 +968,12 @@ __global__ __launch_bounds__(kThreads, (Keys<T, D>::kResident)) void keys_kernel
                 for (int kt = 0; kt < KT; ++kt) {
                     if constexpr (CAREFUL) {
                         av[kt][dt] = mma_masked<T>(d, pf[kt], pl[kt], seen[kt], av[kt][dt]);
-                        ak[kt][dt] = mma_masked<T>(q, sf[kt], zero8<T>(), seen[kt], ak[kt][dt]);
+                        ak[kt][dt] = mma_masked<T>(q, sf[kt], sl[kt], seen[kt], ak[kt][dt]);
                     } else {
                         av[kt][dt] = mma(d, pf[kt], av[kt][dt]);
                         if (sizeof(T) == 2) av[kt][dt] = mma(d, pl[kt], av[kt][dt]);
                         ak[kt][dt] = mma(q, sf[kt], ak[kt][dt]);
+                        if (sizeof(T) == 2) ak[kt][dt] = mma(q, sl[kt], ak[kt][dt]);
                     }
                 }
             }
@@ -1062,6 +1065,8 @@ int layout_of(const Problem &p, int head_len, int row_tiles, int parts, bool nar
     const int tpt = tile_tokens(p.group), block = 1 << p.block_shift;
     const int64_t pairs = (int64_t)p.batch * p.kv_heads;
     auto tiles = [&](int n) { return (p.queries + n * tpt - 1) / (n * tpt); };
+    // as the forward pass decides it; a whole step with the kernels for few / many queries: 1,024 tokens of 32 / 8 heads of 128 in bfloat16 (256
+    // workgroups) 326 / 225 us, 2,048 788 / 403; 2 x 1,024 tokens of 8 / 8 heads of 64 in 32 bits 207 / 221, 2 x 2,048 387 / 371
     l->n_groups = tiles(kWaves * row_tiles);
     l->many = pairs * l->n_groups >= 256 && 2 * p.queries >= kWaves * row_tiles * tpt;
     if (!l->many) l->n_groups = tiles(1);

@@ -488,6 +488,21 @@ def test_outputs_with_and_without_gradients_are_the_same(dtype, batch, queries, 
     assert torch.equal(plain, call(s)) and torch.equal(plain, call(s, q=s["q"].detach().requires_grad_()))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("batch,queries,heads,kv_heads,head_len,block,buckets", HALF_SHAPES)
+def test_gradients_of_16_bits_are_off_by_their_own_rounding(dtype, batch, queries, heads, kv_heads, head_len, block, buckets):
+    """The root mean square error is that of rounding the exact results, r.  Operands in two parts are off by 2^-16 (float16: 2^-22) and less,
+    independent of one another from term to term; even with sums 30 times as large as what is left of them that is below r / 4,
+    and the two together below 1.05 r.  One part alone, off by as much as the result, would make 1.4 r."""
+    s, dout = make(dtype, batch, queries, queries, heads, kv_heads, head_len, block, 3, buckets, seed=38)
+    got, value = step(s, dout), want(s, dout)
+    for x in ("out", "dq", "dk", "dv"):
+        exact = value[x][0]
+        own = torch.from_numpy(exact).to(dtype).double().numpy() - exact
+        error = got[x].detach().cpu().double().numpy() - exact
+        assert np.sqrt((error ** 2).mean()) <= 1.05 * np.sqrt((own ** 2).mean()), x
+
+
 def test_gradients_against_differences():
     s, dout = make(F32, 1, 40, 40, 2, 1, 32, 32, 2, 6, seed=15)
     got = step(s, dout)

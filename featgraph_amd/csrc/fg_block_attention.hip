@@ -4,7 +4,9 @@
 // No visible key: 0.
 //
 // Rows of one token's heads and of neighbouring tokens make tiles of 16, and the blocks that any token of a tile selected are walked for all of
-// them: neighbours share most of their blocks, and a token that did not select one has weight 0 there.  Two kernels.
+// them; a token that did not select one has weight 0 there.  That pays as far as neighbours select the same blocks: 8,192 tokens, 32 / 8
+// heads of 128, 16 blocks of 64 take 373 us where they look for what a stretch of 128 tokens looks for, and 661 where every one draws its
+// own.  Two kernels.
 // many_kernel, where there are queries to fill the card: four wavefronts with tiles of their own walk the union of their lists through
 // LDS, 64 keys at a time, fetched into registers while the 64 before are worked on; each keeps its softmax and its output.
 // few_kernel, for single tokens and short sequences: one tile per workgroup, whose list is dealt out to the four wavefronts and, where
@@ -12,10 +14,10 @@
 // Values that are not finite reach the rows that see them and no others: a result that is not finite is computed again with such places
 // apart (mma_masked).
 //
-// What bounds them.  many_kernel, 8,192 tokens, 32 / 8 heads of 128 in bfloat16, 16 blocks of 64: 402 us, 320 TFLOP/s of the selected pairs;
+// What bounds them.  many_kernel, those 8,192 tokens in bfloat16: 406 us, 320 TFLOP/s of the selected pairs;
 // the matrix cores are busy a fifth of the time, for unions are larger than their tokens' lists, 256 registers allow two wavefronts per
 // SIMD, and these wait for LDS and for one another at each step (walking the lists and staging alone take 184 us).  few_kernel, 32
-// sequences with 16 blocks each of 32 / 8 heads of 128: 28.3 us, 4.8 TB/s of keys and values, the rate of a large copy; with less to read
+// sequences with 16 blocks each of 32 / 8 heads of 128: 27.6 us, 4.9 TB/s of keys and values, the rate of a large copy; with less to read
 // (1 sequence, 8 heads of 64: 10 us) the chain list, keys, softmax, joining.
 #include <algorithm>
 #include <type_traits>
@@ -526,6 +528,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const
 }
 
 // Which kernel takes a call, and how its work is cut.  many_kernel wants its workgroups' tiles at least half full and 256 workgroups (a CU each).
+// Both sides, few_kernel / many_kernel, heads of 128 in bfloat16, 16 blocks of 64.  One sequence of 32 / 8 heads: 256 tokens (64 workgroups)
+// 19 / 18 us, 512 40 / 26, 1,024 (256 workgroups) 98 / 42, 2,048 257 / 71.  32 sequences of 8 / 8 heads over 2,048 keys: 16 tokens (an eighth
+// of a workgroup's rows) 49 / 67, 32 61 / 70, 48 86 / 73, 64 112 / 74, 128 213 / 80.  In 32 bits, heads of 64, 8 blocks of 32, two sequences of 8
+// heads: 1,024 tokens (256 workgroups) 41 / 53, 2,048 82 / 89.  So the cut comes late for long lists in 16 bits and early for short ones in 32.
 // few_kernel's workgroups take about 8 us and 0.35 us for each unit of a wavefront, and joining several costs 6 us with its launch: a list
 // is dealt out to several workgroups where a wavefront would have more than eight units of it, then down to four.
 struct Shape { bool many; int n_tiles, splits; };

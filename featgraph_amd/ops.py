@@ -101,8 +101,8 @@ def edge_softmax(g, scores):
 
 
 def pool_blocks(k, block_size, lengths=None):
-    """Mean of the keys of every block, (batch, kv_heads, ceil(keys / block_size), head_len), in the keys' type (summed in 64 bits, rounded
-    once); 0 for a block without keys.  k (batch, keys, kv_heads, head_len); lengths: int32 (batch,), the keys of each
+    """Mean of the keys of every block, (batch, kv_heads, ceil(keys / block_size), head_len), in the keys' type (summed in 64 bits, rounded to
+    32 and then to the type); 0 for a block without keys.  k (batch, keys, kv_heads, head_len); lengths: int32 (batch,), the keys of each
     sequence, the rest is not read.  head_len 32, 64 or 128, block_size 32, 64, 128 or 256.  Not differentiable."""
     return _block.block_pool(k.detach() if isinstance(k, torch.Tensor) else k, block_size, lengths)
 
@@ -111,7 +111,7 @@ def select_blocks(q, pooled, num_keys, block_size, topk, causal=True, lengths=No
     """The topk blocks of keys that every query scores highest, int32 (batch, queries, kv_heads, topk), ascending, -1 behind the last.
 
     q (batch, queries, heads, head_len) against pooled = pool_blocks(k, ...) of `num_keys` keys; a block's score is its pooled key times the
-    sum of the queries of the heads that share the key head (rounded to their type), compared as exact numbers, equal ones
+    sum of the queries of the heads that share the key head (rounded to 32 bits and then to their type), compared as exact numbers, equal ones
     by the lower id.  A sequence's last query stands at its last key; with `causal` a query may choose its own block and those before.
     The first `keep_first` blocks (default 1, or 0 with topk = 1) and the last `keep_last` a query may choose are always among
     them.  Rows behind q_lengths are -1.  At most 2048 blocks.  Not differentiable."""

@@ -613,14 +613,14 @@ typedef enum { FG_TYPE_F32 = 0, FG_TYPE_F16 = 1, FG_TYPE_BF16 = 2 } fg_type;
 
 /*
  * pooled[b, g, n, :] = mean over the keys of block n (keys n * block .. of one sequence, key head g), (batch, kv_heads, ceil(keys / block),
- * head_len) dense; 0 for a block without keys.  Summed in 64 bits and rounded to the type.
+ * head_len) dense; 0 for a block without keys.  Summed in 64 bits, rounded to 32 and then to the type.
  */
 int fg_block_pool(int type, const void *k_dev, const int64_t *k_strides, const int32_t *lengths_dev, void *pooled_dev,
                   int batch, int keys, int kv_heads, int head_len, int block, void *stream);
 
 /*
  * blocks_dev (batch, queries, kv_heads, topk): for every query and key head the ids of the topk blocks with the highest
- * <sum of the group's queries, rounded to the type; pooled[b, g, n]>, in ascending order, -1 behind the last.  Compared as exact numbers
+ * <sum of the group's queries, rounded to 32 bits and then to the type; pooled[b, g, n]>, in ascending order, -1 behind the last.  Compared as exact numbers
  * (products of the stored values, summed without rounding that could change an order by more than 64-bit sums do); equal ones, and NaN, which
  * counts as -inf, go to the lower id.  Candidates are blocks that hold a key and, with `causal`, start at or before the query's
  * position; the first keep_first and the last keep_last of them are taken before any other (keep_first + keep_last <= topk).

@@ -39,6 +39,30 @@ class FgBlockAttentionGrads(ctypes.Structure):
     _fields_ = [("dout", _vp), ("dout_strides", _i64 * 3), ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dbias", _vp)]
 
 
+class FgRotateArgs(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_len", ctypes.c_int32), ("rotary_len", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("turns", ctypes.c_double * 64), ("axis", ctypes.c_uint8 * 64), ("q", _vp), ("k", _vp), ("q_strides", _i64 * 3),
+                ("k_strides", _i64 * 3), ("q_weight", _vp), ("k_weight", _vp), ("positions", _vp), ("lengths", _vp), ("q_lengths", _vp),
+                ("q_out", _vp), ("k_out", _vp)]
+
+
+class FgRotateGrads(ctypes.Structure):
+    _fields_ = [("dq_out", _vp), ("dk_out", _vp), ("dq_out_strides", _i64 * 3), ("dk_out_strides", _i64 * 3), ("dq", _vp), ("dk", _vp),
+                ("dq_weight", _vp), ("dk_weight", _vp)]
+
+
+class FgKvCache(ctypes.Structure):
+    _fields_ = [("bits", ctypes.c_int32), ("batch", ctypes.c_int32), ("keys", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_len", ctypes.c_int32),
+                ("k", _vp), ("k_scales", _vp), ("v", _vp), ("v_scales", _vp)]
+
+
+class FgCacheAttentionArgs(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("queries", ctypes.c_int32), ("heads", ctypes.c_int32), ("causal", ctypes.c_int32), ("block", ctypes.c_int32),
+                ("topk", ctypes.c_int32), ("scale", ctypes.c_float), ("cache", FgKvCache), ("q", _vp), ("q_strides", _i64 * 3), ("blocks", _vp),
+                ("lengths", _vp), ("q_lengths", _vp), ("out", _vp)]
+
+
 # Options every module passes to fg_spmm_plan_create (None: the library's defaults).
 plan_opts = None
 
@@ -105,6 +129,13 @@ SIGNATURES = {
     "fg_block_attention": (_int, [_vp, _vp, ctypes.c_size_t, _vp]),
     "fg_block_attention_backward_workspace": (_i64, [_vp]),
     "fg_block_attention_backward": (_int, [_vp, ctypes.POINTER(FgBlockAttentionGrads), _vp, ctypes.c_size_t, _vp]),
+    "fg_rotate_heads": (_int, [_vp, _vp]),
+    "fg_rotate_heads_backward_workspace": (_i64, [_vp]),
+    "fg_rotate_heads_backward": (_int, [_vp, ctypes.POINTER(FgRotateGrads), _vp, ctypes.c_size_t, _vp]),
+    "fg_cache_write": (_int, [_vp, _int, _vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64), _int, _vp, _vp, _vp]),
+    "fg_cache_read": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp]),
+    "fg_cache_attention_workspace": (_i64, [_vp]),
+    "fg_cache_attention": (_int, [_vp, _vp, ctypes.c_size_t, _vp]),
     "fg_synth_powerlaw_csr": (_int, [_i64, _vp, _vp, _vp, ctypes.c_uint64, _int, _vp, _vp]),
     "fg_synth_community_csr": (_int, [_i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, ctypes.c_double, ctypes.c_uint64, _int, _vp, _vp]),
 }

@@ -18,6 +18,7 @@ import torch
 from . import tuning
 from .module import block_attention as _block
 from .module import common
+from .module import rotate as _rotate
 from .module import (EdgeSoftmaxhip, GraphAttentionhip, GSDDMMhip, GSpMMhip, MultiHeadSDDMMhip, VanillaSDDMMhip,
                      placeholder)
 from .module.general import parse_message
@@ -741,3 +742,26 @@ class _BlockAttention(torch.autograd.Function):
         keys_too = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         grads = _block.block_attention_backward(q, k, v, blocks, *ctx.spec, lengths, q_lengths, bias, ctx.bounds, out, lse, rest, dout, keys_too)
         return grads + (None,) * 5
+
+
+def rotate_heads(q, k, q_weight, k_weight, spec, positions, lengths, q_lengths):
+    """ops.rotate_heads on checked arguments; spec as module.rotate.check gives it."""
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 \
+            or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _RotateHeads.apply(q, k, q_weight, k_weight, spec, positions, lengths, q_lengths)
+    return _rotate.forward(q, k, q_weight, k_weight, spec, positions, lengths, q_lengths)
+
+
+class _RotateHeads(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, spec, positions, lengths, q_lengths):
+        ctx.spec = spec
+        normed = q_weight is not None       # a rotation alone is undone without its inputs
+        ctx.save_for_backward(q if normed else None, k if normed else None, q_weight, k_weight, positions, lengths, q_lengths)
+        return _rotate.forward(q, k, q_weight, k_weight, spec, positions, lengths, q_lengths)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, positions, lengths, q_lengths = ctx.saved_tensors
+        return _rotate.backward(q, k, q_weight, k_weight, ctx.spec, positions, lengths, q_lengths, dq_out, dk_out) + (None,) * 4

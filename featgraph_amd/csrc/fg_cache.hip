@@ -1,0 +1,235 @@
+// Keys and values into a cache of 4 or 8 bits, and back.
+//   write:  for 32 neighbouring elements x of a head  e = the least power with which max |x| 2^-e rounds to at most the largest element (6 of e2m1,
+//           448 of e4m3), -127 <= e; codes = x 2^-e to the nearest element, ties to the even code.  A power of two divides without rounding, so that
+//           codes are the same on every machine that follows the rule.
+//   read:   code 2^e, rounded to the type (and no further than its largest number: an element may be up to 1 / 16 above the value it came from).
+#include <algorithm>
+#include <limits>
+
+#include "fg_cache.h"
+
+namespace fg {
+namespace cache {
+
+namespace {
+
+using block::Strides;
+using block::V8;
+using block::load8;
+
+constexpr int kThreads = 256;
+
+struct Window {                        // tokens of a call and where they stand in the cache
+    int batch, tokens, keys, kv_heads;
+    const int32_t *lengths, *q_lengths, *first;
+};
+
+// A thread takes eight elements; the D / 8 of a row follow one another, then the rows of one head: codes are written, and read, as whole lines.
+struct Place { int64_t row; int b, g, i, col; };       // row: of (batch, kv_heads); col: in elements
+template <int D> __device__ __forceinline__ Place place_of(int64_t at, const Window &w) {
+    constexpr int C = D / 8;
+    const int64_t token = at / C;
+    Place p;
+    p.col = (int)(at - token * C) * 8;
+    p.row = token / w.tokens;
+    p.i = (int)(token - p.row * w.tokens);
+    p.b = (int)(p.row / w.kv_heads);
+    p.g = (int)(p.row - (int64_t)p.b * w.kv_heads);
+    return p;
+}
+
+// The larger of two lanes' numbers, over four neighbouring lanes.
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));      // quad_perm [1,0,3,2]
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));   // quad_perm [2,3,0,1]
+}
+
+struct Source { const void *data; Strides s; void *codes, *scales; };
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(kThreads) void write_kernel(const Window w, const Source ks, const Source vs, int64_t n) {
+    const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (at >= 2 * n) return;           // n is a multiple of four: lanes of one scale stay together
+    const bool second = at >= n;
+    const Source &s = second ? vs : ks;
+    const Place p = place_of<D>(second ? at - n : at, w);
+    const int q_len = w.q_lengths ? min(max(w.q_lengths[p.b], 0), w.tokens) : w.tokens;
+    const int k_len = w.lengths ? min(max(w.lengths[p.b], 0), w.keys) : w.keys;
+    const int key = k_len - q_len + p.i;
+    if (p.i >= q_len || key < 0) return;
+    const V8<T> x = load8(static_cast<const T *>(s.data) + p.b * s.s.batch + (int64_t)p.i * s.s.row + p.g * s.s.head + p.col);
+    float f[8];
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f[i] = (float)x[i];
+        most = max(most, __float_as_uint(f[i]) & 0x7fffffffu);     // as numbers are ordered; infinities and NaN above them
+    }
+    most = quad_max(most);
+    const bool odd = most >= 0x7f800000u;
+    // max |x| = 2^(high - 127) (1 + low / 2^23); 1.75 and more (e2m1) and what is above 1.8125 (e4m3) would round to the next power of two
+    const int high = (int)(most >> 23), low = (int)(most & 0x7fffffu);
+    const int up = BITS == 4 ? low >= 0x600000 : low > 0x680000;
+    const int byte = min(max(high - (BITS == 4 ? 2 : 8) + up, 0), kTopExponent<BITS> + 127);
+    const float scale = scale_of((unsigned)byte);
+    uint32_t word[BITS / 4];
+    if constexpr (BITS == 4) {
+        uint32_t c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], scale, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], scale, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], scale, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], scale, 3);
+        word[0] = c;
+    } else {
+        // the conversion makes NaN of what is beyond the largest element, which the scale's own limit allows: 448 2^119 at most
+        constexpr float TOP = 0x1.cp127f;
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fminf(fmaxf(f[4 * h + i], -TOP), TOP);
+            s16x2 c = {0, 0};
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, y[0], y[1], scale, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, y[2], y[3], scale, true);
+            word[h] = __builtin_bit_cast(uint32_t, c);
+        }
+    }
+    const int64_t row = p.row * w.keys + key;
+    uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(s.codes) + row * (D * BITS / 8) + p.col * BITS / 8);
+    if constexpr (BITS == 4) {
+        out[0] = odd ? 0u : word[0];
+    } else {
+        *reinterpret_cast<uint2 *>(out) = odd ? make_uint2(0u, 0u) : make_uint2(word[0], word[1]);
+    }
+    if (p.col % kGroup == 0) static_cast<uint8_t *>(s.scales)[row * (D / kGroup) + p.col / kGroup] = odd ? (uint8_t)255 : (uint8_t)byte;
+}
+
+struct Target { const void *codes, *scales; void *out; };
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(kThreads) void read_kernel(const Window w, const Target kt, const Target vt, int64_t n) {
+    const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (at >= 2 * n) return;
+    const bool second = at >= n;
+    const Target &t = second ? vt : kt;
+    const Place p = place_of<D>(second ? at - n : at, w);
+    const int k_len = w.lengths ? min(max(w.lengths[p.b], 0), w.keys) : w.keys;
+    const int64_t key = (int64_t)(w.first ? w.first[p.b] : 0) + p.i;
+    V8<T> x = block::zero8<T>();
+    if (key >= 0 && key < k_len) {
+        const int64_t row = p.row * w.keys + key;
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(t.codes) + row * (D * BITS / 8) + p.col * BITS / 8);
+        uint32_t word[BITS / 4];
+#pragma unroll
+        for (int i = 0; i < BITS / 4; ++i) word[i] = src[i];
+        const auto y = values<BITS, typename std::conditional<sizeof(T) == 4, float, __bf16>::type>(
+            word, scale_of(static_cast<const uint8_t *>(t.scales)[row * (D / kGroup) + p.col / kGroup]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = (float)y[i];
+            if constexpr (std::is_same<T, _Float16>::value) x[i] = (T)(f != f ? f : fminf(fmaxf(f, -65504.f), 65504.f));
+            else x[i] = (T)f;
+        }
+    }
+    *reinterpret_cast<V8<T> *>(static_cast<T *>(t.out) + (((int64_t)p.b * w.tokens + p.i) * w.kv_heads + p.g) * D + p.col) = x;
+}
+
+template <typename F> int by_shape(int type, int head_len, int bits, F f) {
+    auto with_bits = [&](auto t, auto d) {
+        return bits == 4 ? f(t, d, std::integral_constant<int, 4>{}) : f(t, d, std::integral_constant<int, 8>{});
+    };
+    auto with_length = [&](auto t) {
+        switch (head_len) {
+        case 32: return with_bits(t, std::integral_constant<int, 32>{});
+        case 64: return with_bits(t, std::integral_constant<int, 64>{});
+        default: return with_bits(t, std::integral_constant<int, 128>{});
+        }
+    };
+    switch (type) {
+    case FG_TYPE_F32: return with_length(float{});
+    case FG_TYPE_F16: return with_length(_Float16{});
+    default: return with_length(__bf16{});
+    }
+}
+
+// Workgroups for 2 n threads.
+int grid_of(int64_t n, unsigned *grid) {
+    const int64_t g = (2 * n + kThreads - 1) / kThreads;
+    if (g >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache: %lld workgroups do not fit a launch", (long long)g);
+    *grid = (unsigned)g;
+    return FG_OK;
+}
+
+int known(int type) {
+    return type == FG_TYPE_F32 || type == FG_TYPE_F16 || type == FG_TYPE_BF16 ? FG_OK : fail(FG_ERR_ARG, "cache: unknown type %d", type);
+}
+
+}  // namespace
+
+int check(const fg_kv_cache *c) {
+    if (!c) return fail(FG_ERR_ARG, "cache: null pointer");
+    if (c->bits != 4 && c->bits != 8) return fail(FG_ERR_ARG, "cache: elements of 4 or 8 bits, got %d", c->bits);
+    if (c->batch < 0 || c->keys < 0 || c->kv_heads < 1) return fail(FG_ERR_ARG, "cache: negative sizes, or no heads");
+    if (c->head_len != 32 && c->head_len != 64 && c->head_len != 128) return fail(FG_ERR_SHAPE, "cache: heads of 32, 64 or 128 elements, got %d", c->head_len);
+    if (c->keys > (1 << 30)) return fail(FG_ERR_SHAPE, "cache: more than 2^30 keys");
+    const bool any = (int64_t)c->batch * c->keys;
+    if (any && (!c->k || !c->v || !c->k_scales || !c->v_scales)) return fail(FG_ERR_ARG, "cache: null pointer");
+    if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16 || reinterpret_cast<uintptr_t>(c->k_scales) % 4 ||
+        reinterpret_cast<uintptr_t>(c->v_scales) % 4)
+        return fail(FG_ERR_ARG, "cache: codes have to stand at multiples of 16 bytes, scales of 4 bytes");
+    return FG_OK;
+}
+
+}  // namespace cache
+}  // namespace fg
+
+extern "C" int fg_cache_write(const fg_kv_cache *cache, int type, const void *k_dev, const int64_t *k_strides, const void *v_dev, const int64_t *v_strides,
+                              int tokens, const int32_t *lengths_dev, const int32_t *q_lengths_dev, void *stream) {
+    using namespace fg;
+    using namespace fg::cache;
+    int rc;
+    if ((rc = cache::check(cache)) || (rc = known(type))) return rc;
+    if (tokens < 0 || tokens > (1 << 30)) return fail(FG_ERR_ARG, "cache: %d new tokens", tokens);
+    if (!k_strides || !v_strides) return fail(FG_ERR_ARG, "cache: null pointer");
+    const int size = type == FG_TYPE_F32 ? 4 : 2;
+    Source ks{k_dev, {}, cache->k, cache->k_scales}, vs{v_dev, {}, cache->v, cache->v_scales};
+    if ((rc = block::strides_of("k", k_dev, k_strides, size, &ks.s, "cache")) || (rc = block::strides_of("v", v_dev, v_strides, size, &vs.s, "cache")) ||
+        (rc = block::aligned("lengths", lengths_dev, 4, "cache")) || (rc = block::aligned("q_lengths", q_lengths_dev, 4, "cache"))) return rc;
+    if ((int64_t)cache->batch * tokens == 0 || cache->keys == 0) return FG_OK;
+    if (!k_dev || !v_dev) return fail(FG_ERR_ARG, "cache: null pointer");
+    const Window w{cache->batch, tokens, cache->keys, cache->kv_heads, lengths_dev, q_lengths_dev, nullptr};
+    const int64_t n = (int64_t)cache->batch * tokens * cache->kv_heads * (cache->head_len / 8);
+    unsigned grid;
+    if ((rc = grid_of(n, &grid))) return rc;
+    by_shape(type, cache->head_len, cache->bits, [&](auto t, auto d, auto bits) {
+        write_kernel<decltype(t), decltype(d)::value, decltype(bits)::value><<<dim3(grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(w, ks, vs, n);
+        return 0;
+    });
+    FG_HIP_TRY(hipGetLastError());
+    return FG_OK;
+}
+
+extern "C" int fg_cache_read(const fg_kv_cache *cache, int type, void *k_dev, void *v_dev, int count, const int32_t *first_dev, const int32_t *lengths_dev,
+                             void *stream) {
+    using namespace fg;
+    using namespace fg::cache;
+    int rc;
+    if ((rc = cache::check(cache)) || (rc = known(type))) return rc;
+    if (count < 0 || count > (1 << 30)) return fail(FG_ERR_ARG, "cache: %d keys to read", count);
+    if ((rc = block::aligned("k", k_dev, 16, "cache")) || (rc = block::aligned("v", v_dev, 16, "cache")) || (rc = block::aligned("first", first_dev, 4, "cache")) ||
+        (rc = block::aligned("lengths", lengths_dev, 4, "cache"))) return rc;
+    if ((int64_t)cache->batch * count == 0) return FG_OK;
+    if (!k_dev || !v_dev) return fail(FG_ERR_ARG, "cache: null pointer");
+    const Window w{cache->batch, count, cache->keys, cache->kv_heads, lengths_dev, nullptr, first_dev};
+    const int64_t n = (int64_t)cache->batch * count * cache->kv_heads * (cache->head_len / 8);
+    unsigned grid;
+    if ((rc = grid_of(n, &grid))) return rc;
+    const Target kt{cache->k, cache->k_scales, k_dev}, vt{cache->v, cache->v_scales, v_dev};
+    by_shape(type, cache->head_len, cache->bits, [&](auto t, auto d, auto bits) {
+        read_kernel<decltype(t), decltype(d)::value, decltype(bits)::value><<<dim3(grid), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(w, kt, vt, n);
+        return 0;
+    });
+    FG_HIP_TRY(hipGetLastError());
+    return FG_OK;
+}

@@ -1,0 +1,461 @@
+// Softmax attention of a few queries over a cache of 4 or 8 bits, whole or the blocks that a list names:
+//   out[i, h] = sum_j p_ij V[j, g],  p_i = softmax over the visible keys j of  scale <Q[i, h], K[j, g]>
+// with g = h / group, pos_i = k_len - q_len + i, and j visible to i where j < k_len, (causal) j <= pos_i and, where there is a list, floor(j / block)
+// is in i's list for g.  No visible key: 0.
+//
+// Every value of the cache is a bfloat16, so that products with it are bfloat16 products of the matrix cores, exact up to the sums in 32
+// bits, whatever type the queries have: a float16 is the sum of two bfloat16, a number of 32 bits of three.  Powers are taken apart the
+// same way, into two parts for 16-bit results (2^-17 of a power is lost) and three for 32-bit ones.
+// Rows of one token's heads and of neighbouring tokens make tiles of 16, RT of them a workgroup.  Its four wavefronts deal the keys out among themselves, 32 at a
+// time, and where there are too few workgroups for the card so do several workgroups, whose sums are joined after.  A
+// lane's keys come from memory as operands lie in registers (the sum over a head's elements takes them in any order), values go
+// through LDS as bfloat16 to be read by columns; the next two steps are under way while one is worked on.
+// A result that is not finite is computed again with infinities and NaN kept from the rows that do not see them (mma_masked).
+#include <algorithm>
+#include <type_traits>
+
+#include "fg_cache.h"
+
+namespace fg {
+namespace cache {
+
+namespace {
+
+using namespace block;
+
+template <typename T> constexpr int kQueryParts = sizeof(T) == 4 ? 3 : std::is_same<T, _Float16>::value ? 2 : 1;
+template <typename T> constexpr int kPowerParts = sizeof(T) == 4 ? 3 : 2;
+
+struct Held { const void *k, *k_scales, *v, *v_scales; };
+struct Results { void *out; float *part; float2 *part_stats; };
+
+// How 32 keys of a cache come to a wavefront's lanes.  Keys: lane (g, c) takes chunks of rows c and 16 + c, the g-th of each four.  Values: chunks of
+// all rows one after the other.
+template <int D, int BITS> struct Layout {
+    static constexpr int kRow = D * BITS / 8;
+    static constexpr int kKeyBytes = kRow / 4, kKeyChunk = kKeyBytes < 16 ? kKeyBytes : 16, kKeyChunks = kKeyBytes / kKeyChunk;
+    static constexpr int kKeyElements = kKeyChunk * 8 / BITS;
+    static constexpr int kValueBytes = kRow / 2, kValueChunk = kValueBytes < 16 ? kValueBytes : 16, kValueChunks = kValueBytes / kValueChunk;
+    static constexpr int kValueElements = kValueChunk * 8 / BITS, kPerRow = kRow / kValueChunk;
+    // first of the elements 8 n .. 8 n + 7 of lane group g
+    static __device__ __forceinline__ int element(int n, int g) { return (8 * n / kKeyElements * 4 + g) * kKeyElements + 8 * n % kKeyElements; }
+};
+
+template <int BYTES> __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
+    if constexpr (BYTES == 16) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
+        w[0] = x[0]; w[1] = x[1]; w[2] = x[2]; w[3] = x[3];
+    } else if constexpr (BYTES == 8) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(p);
+        w[0] = x.x; w[1] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+template <int D, int BITS> struct Step {
+    typedef Layout<D, BITS> Y;
+    int key0;
+    unsigned who[2];                   // tokens of each tile that selected these keys
+    uint32_t kw[2][Y::kKeyBytes / 4], vw[Y::kValueBytes / 4];
+    unsigned ks[2][Y::kKeyChunks], vs[Y::kValueChunks];
+
+    // rows behind the last key read it again: what a padded cache holds there is never touched
+    __device__ __forceinline__ void fetch(const Rows<D, BITS> &k, const Rows<D, BITS> &v, int first, int k_len, int lane) {
+        const int g = lane >> 4, c = lane & 15;
+        key0 = first;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const int64_t row = min(first + 16 * kt + c, k_len - 1);
+#pragma unroll
+            for (int j = 0; j < Y::kKeyChunks; ++j) {
+                load_words<Y::kKeyChunk>(k.codes + row * Y::kRow + (4 * j + g) * Y::kKeyChunk, kw[kt] + j * Y::kKeyChunk / 4);
+                ks[kt][j] = k.scales[row * (D / kGroup) + (4 * j + g) * Y::kKeyElements / kGroup];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < Y::kValueChunks; ++j) {
+            const int at = j * 64 + lane, col = at % Y::kPerRow;
+            const int64_t row = min(first + at / Y::kPerRow, k_len - 1);
+            load_words<Y::kValueChunk>(v.codes + row * Y::kRow + col * Y::kValueChunk, vw + j * Y::kValueChunk / 4);
+            vs[j] = v.scales[row * (D / kGroup) + col * Y::kValueElements / kGroup];
+        }
+    }
+    __device__ __forceinline__ bf16x8 keys(int kt, int n) const {
+        constexpr int W = BITS / 4;
+        return values<BITS>(kw[kt] + n * W, scale_of(ks[kt][8 * n / Y::kKeyElements]));
+    }
+    __device__ __forceinline__ void store_values(__bf16 *stage, int lane) const {
+        constexpr int W = BITS / 4, S = D + kPad;
+#pragma unroll
+        for (int j = 0; j < Y::kValueChunks; ++j) {
+            const int at = j * 64 + lane;
+            __bf16 *to = stage + at / Y::kPerRow * S + at % Y::kPerRow * Y::kValueElements;
+#pragma unroll
+            for (int n = 0; n < Y::kValueElements / 8; ++n)
+                *reinterpret_cast<bf16x8 *>(to + 8 * n) = values<BITS>(vw + j * Y::kValueChunk / 4 + n * W, scale_of(vs[j]));
+        }
+    }
+};
+
+// Eight elements of a query as a sum of bfloat16.  Cut, not rounded: a part never leaves the range.
+template <typename T> __device__ __forceinline__ void parts_of(const T *src, bf16x8 *part, int stride) {
+    const V8<T> x = load8(src);
+    if constexpr (std::is_same<T, __bf16>::value) {
+        part[0] = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float f = (float)x[i];
+#pragma unroll
+            for (int j = 0; j < kQueryParts<T>; ++j) {
+                const float high = __uint_as_float(__float_as_uint(f) & 0xffff0000u);
+                part[j * stride][i] = (__bf16)high;
+                f = fabsf(f) < __builtin_inff() ? f - high : 0.f;
+            }
+        }
+    }
+}
+
+constexpr int kListed = 1024;          // blocks listed at a time
+struct NoList {};
+
+template <int D> constexpr size_t stage_bytes() {
+    const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(__bf16), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
+    return values > merge ? values : merge;
+}
+
+template <typename T, int D, int BITS, int RT, bool LISTED>
+__global__ __launch_bounds__(kThreads) void attention_kernel(const Problem p, const Held held, const Results r, int n_groups, int splits) {
+    constexpr int DC = D / 32, DT = D / 16, NQ = kQueryParts<T>, NP = kPowerParts<T>;
+    typedef List<RT, kListed> Listing;
+    __shared__ typename std::conditional<LISTED, Listing, NoList>::type list;
+    __shared__ float2 stats[kWaves][16], joined[16];
+    __shared__ __align__(16) unsigned char dynamic[stage_bytes<D>()];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int unit = xcd_contiguous_block(), pair = unit / (n_groups * splits), rest = unit - pair * n_groups * splits;
+    const int group = rest / splits, split = rest - group * splits;
+    const int b = pair / p.kv_heads, h = pair - b * p.kv_heads;
+    const int k_len = key_count(p, b), q_len = query_count(p, b), offset = k_len - q_len;
+    const int tpt = tile_tokens(p.group), t0 = group * RT * tpt;
+    const int tc = c / p.group, mine = c - tc * p.group, head = h * p.group + mine;        // this lane's token within a tile, and its head
+    const bool used = tc < tpt;
+
+    __bf16 *stage = reinterpret_cast<__bf16 *>(dynamic) + wave * kUnit * (D + kPad);
+    const Rows<D, BITS> keys(held.k, held.k_scales, pair, p.keys), vals(held.v, held.v_scales, pair, p.keys);
+    bf16x8 qf[RT][NQ][DC];
+    int limit[RT];                     // last key that the lane's row may see; columns without a row see everything, nothing is written of them
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int t = t0 + rt * tpt + tc;
+        const bool there = used && t < q_len;
+        limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
+        const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head;
+#pragma unroll
+        for (int n = 0; n < DC; ++n) {
+            if (there) {
+                parts_of<T>(src + Layout<D, BITS>::element(n, g), &qf[rt][0][n], DC);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) qf[rt][j][n] = zero8<__bf16>();
+            }
+        }
+    }
+    const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + RT * tpt, q_len) - 1) : k_len - 1;
+    const int sub_shift = LISTED ? p.block_shift - 5 : 0, stride = kWaves * splits;
+
+    f32x4 o[RT][DT];
+    float m[RT], l[RT];
+    auto sweep = [&](auto careful) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -__builtin_inff(); l[rt] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        auto window = [&](int first, int units) {
+            auto first_key = [&](int u) {
+                if constexpr (LISTED) return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
+                else return u << 5;
+            };
+            // the next unit, from u on, that holds a key anyone may see
+            auto find = [&](int u) {
+                if constexpr (LISTED)
+                    while (u < units && first_key(u) > last_key) u += stride;
+                return u;
+            };
+            auto fetch = [&](Step<D, BITS> &s, int u) {
+                s.fetch(keys, vals, first_key(u), k_len, lane);
+                if constexpr (LISTED)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s.who[rt] = (unsigned)(list.bits[u >> sub_shift][0] >> (16 * rt)) & 0xffffu;
+            };
+            auto work = [&](const Step<D, BITS> &now) {
+                wave_lds_sync();
+                now.store_values(stage, lane);
+                f32x4 s[RT][2];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int n = 0; n < DC; ++n) {
+                        const bf16x8 kf = now.keys(kt, n);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int j = NQ; j-- > 0;) s[rt][kt] = mma(kf, qf[rt][j][n], s[rt][kt]);
+                    }
+                }
+                wave_lds_sync();
+                bf16x8 pf[RT][NP];
+                unsigned seen[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int last = !LISTED || !used || (now.who[rt] >> tc) & 1 ? limit[rt] : -1;      // keys that the lane's row sees: key0 + 16 kt + 4 g + i <= last
+                    f32x4 z[2] = {s[rt][0] * p.scale2, s[rt][1] * p.scale2};
+                    seen[rt] = 0xff;
+                    if (!__all(now.key0 + kUnit - 1 <= last)) {
+                        seen[rt] = 0;
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const bool ok = now.key0 + 16 * kt + 4 * g + i <= last;
+                                z[kt][i] = ok ? z[kt][i] : -__builtin_inff();
+                                seen[rt] |= (unsigned)ok << (4 * kt + i);
+                            }
+                    }
+                    const float top = fmaxf(m[rt], largest_of_rows(largest(z[0], z[1])));
+                    const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
+                    if (__any(top != m[rt])) {
+                        const float shrink = __builtin_amdgcn_exp2f(m[rt] - ref);
+                        l[rt] *= shrink;
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
+                        m[rt] = top;
+                    }
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            z[kt][i] = z[kt][i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][i], p.scale2, -ref));
+                    l[rt] += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) {
+                        pf[rt][j] = pack<__bf16>(z[0], z[1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { z[0][i] -= (float)pf[rt][j][i]; z[1][i] -= (float)pf[rt][j][4 + i]; }
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const bf16x8 vf = transposed<__bf16, D>(stage, dt * 16, lane);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if constexpr (decltype(careful)::value) {
+                            o[rt][dt] = mma_masked<__bf16>(vf, pf[rt][0], pf[rt][1], seen[rt], o[rt][dt]);
+                            if (NP == 3) o[rt][dt] = mma_masked<__bf16>(vf, pf[rt][NP - 1], zero8<__bf16>(), seen[rt], o[rt][dt]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < NP; ++j) o[rt][dt] = mma(vf, pf[rt][j], o[rt][dt]);     // in the order of mma_masked: the same bits
+                        }
+                    }
+                }
+            };
+            Step<D, BITS> a, z;
+            int u = find(wave + kWaves * split);
+            if (u < units) {
+                fetch(a, u);
+                u = find(u + stride);
+                while (true) {
+                    const bool more = u < units;
+                    if (more) { fetch(z, u); u = find(u + stride); }
+                    work(a);
+                    if (!more) break;
+                    const bool again = u < units;
+                    if (again) { fetch(a, u); u = find(u + stride); }
+                    work(z);
+                    if (!again) break;
+                }
+            }
+        };
+        if constexpr (LISTED) {
+            for (int first = 0; first < p.blocks; first += kListed)
+                window(first, build_list(list, p, b, h, t0, q_len, k_len, first, min(kListed, p.blocks - first)) << sub_shift);
+        } else {
+            window(0, (last_key + kUnit) / kUnit);
+        }
+    };
+    sweep(std::false_type{});
+    bool odd = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(o[rt][dt]);
+    if (__syncthreads_or(odd)) sweep(std::true_type{});
+
+    // the four wavefronts' sums, joined a strip of 32 columns at a time
+    float *merge = reinterpret_cast<float *>(dynamic);
+    const int64_t all_rows = (int64_t)p.batch * p.queries * p.heads;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float sum = rows_sum(l[rt]);
+        __syncthreads();               // the joining buffer of the tile before has been read
+        if (g == 0) stats[wave][c] = make_float2(m[rt], sum);
+        __syncthreads();
+        float top = -__builtin_inff(), total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][c].x);
+        const float ref = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) total += stats[w][c].y * __builtin_amdgcn_exp2f(stats[w][c].x - ref);
+        const float share = __builtin_amdgcn_exp2f(m[rt] - ref);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= share;
+        if (wave == 0 && g == 0) joined[c] = make_float2(top, total);
+#pragma unroll
+        for (int strip = 0; strip < DC; ++strip) {
+            __syncthreads();           // the values' staging, or the strip before, has been read
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(merge + (wave * 16 + c) * kMergeStride + 16 * j + 4 * g) = o[rt][2 * strip + j];
+            __syncthreads();
+            const int row = tid >> 3, col = (tid & 7) * 4, at_token = row / p.group, t = t0 + rt * tpt + at_token;
+            if (tid < 16 * 8 && at_token < tpt && t < p.queries) {
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(merge + (w * 16 + row) * kMergeStride + col);
+                const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (row - at_token * p.group);
+                const float2 st = joined[row];
+                if (splits == 1) {
+                    store_row<T>(static_cast<T *>(r.out), nullptr, at * D + strip * 32 + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
+                } else {
+                    *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + strip * 32 + col) = v;
+                    if (strip == 0 && col == 0) r.part_stats[split * all_rows + at] = st;
+                }
+            }
+        }
+    }
+}
+
+// How a call's work is cut: workgroups that take all keys where they fill the card, else shares of at least four steps a wavefront.
+struct Shape { int n_groups, splits; };
+template <int RT> Shape shape_of(const Problem &p) {
+    const int tokens = RT * tile_tokens(p.group);
+    Shape s{(int)(((int64_t)p.queries + tokens - 1) / tokens), 1};
+    const int64_t groups = std::max<int64_t>((int64_t)p.batch * p.kv_heads * s.n_groups, 1);
+    int64_t units = ((int64_t)p.keys + kUnit - 1) / kUnit;
+    if (p.list) units = std::min<int64_t>(units, ((int64_t)p.topk * std::min(tokens, p.queries)) << (p.block_shift - 5));
+    if (units > 8 * kWaves) s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + groups - 1) / groups, units / (4 * kWaves)));
+    return s;
+}
+
+size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+template <typename T, int D, int BITS>
+int launch(const Problem &p, const fg_cache_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
+    constexpr int RT = 1;
+    const Shape s = shape_of<RT>(p);
+    const size_t rows = (size_t)p.batch * p.queries * p.heads;
+    const int64_t grid = (int64_t)p.batch * p.kv_heads * s.n_groups * s.splits;
+    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)grid);
+    const size_t sums = s.splits > 1 ? round_up(rows * s.splits * D * sizeof(float)) : 0, stats = s.splits > 1 ? round_up(rows * s.splits * sizeof(float2)) : 0;
+    if (need) { *need = sums + stats; return FG_OK; }
+    if (bytes < sums + stats || (sums && !workspace))
+        return fail(FG_ERR_ARG, "cache attention: a workspace of %zu bytes, %zu needed (fg_cache_attention_workspace)", bytes, sums + stats);
+    unsigned char *w = static_cast<unsigned char *>(workspace);
+    const Results r{a->out, reinterpret_cast<float *>(w), reinterpret_cast<float2 *>(w + sums)};
+    const Held held{a->cache.k, a->cache.k_scales, a->cache.v, a->cache.v_scales};
+    const dim3 blocks((unsigned)grid), threads(kThreads);
+    if (p.list) attention_kernel<T, D, BITS, RT, true><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
+    else attention_kernel<T, D, BITS, RT, false><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
+    FG_HIP_TRY(hipGetLastError());
+    if (s.splits == 1) return FG_OK;
+    const int64_t each = (int64_t)rows * (D / 4), groups = (each + kThreads - 1) / kThreads;
+    if (groups >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)groups);
+    join_kernel<T, D><<<dim3((unsigned)groups), threads, 0, stream>>>(r.part, r.part_stats, static_cast<T *>(r.out), nullptr, nullptr, (int64_t)rows, s.splits);
+    FG_HIP_TRY(hipGetLastError());
+    return FG_OK;
+}
+
+template <typename T, int D> int launch_b(const Problem &p, const fg_cache_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
+    return a->cache.bits == 4 ? launch<T, D, 4>(p, a, workspace, bytes, need, stream) : launch<T, D, 8>(p, a, workspace, bytes, need, stream);
+}
+
+template <typename T> int launch_d(const Problem &p, const fg_cache_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
+    switch (a->cache.head_len) {
+    case 32: return launch_b<T, 32>(p, a, workspace, bytes, need, stream);
+    case 64: return launch_b<T, 64>(p, a, workspace, bytes, need, stream);
+    default: return launch_b<T, 128>(p, a, workspace, bytes, need, stream);
+    }
+}
+
+int launch_t(const Problem &p, const fg_cache_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
+    switch (a->type) {
+    case FG_TYPE_F32: return launch_d<float>(p, a, workspace, bytes, need, stream);
+    case FG_TYPE_F16: return launch_d<_Float16>(p, a, workspace, bytes, need, stream);
+    default: return launch_d<__bf16>(p, a, workspace, bytes, need, stream);
+    }
+}
+
+constexpr const char *kWhat = "cache attention";
+
+int problem_of(const fg_cache_attention_args *a, Problem *p, bool sizes_only) {
+    if (!a) return fail(FG_ERR_ARG, "cache attention: arguments are a null pointer");
+    int rc;
+    if (sizes_only) {
+        fg_kv_cache c = a->cache;
+        c.k = c.v = c.k_scales = c.v_scales = reinterpret_cast<void *>(16);
+        rc = check(&c);
+    } else {
+        rc = check(&a->cache);
+    }
+    if (rc) return rc;
+    const fg_kv_cache &c = a->cache;
+    if (a->type != FG_TYPE_F32 && a->type != FG_TYPE_F16 && a->type != FG_TYPE_BF16) return fail(FG_ERR_ARG, "cache attention: unknown type %d", a->type);
+    if (a->queries < 0 || a->heads < 1) return fail(FG_ERR_ARG, "cache attention: negative sizes, or no heads");
+    if (a->heads % c.kv_heads || a->heads / c.kv_heads > 16)
+        return fail(FG_ERR_SHAPE, "cache attention: %d heads over %d key heads: the former have to be 1 to 16 times the latter", a->heads, c.kv_heads);
+    if (a->queries > (1 << 30)) return fail(FG_ERR_SHAPE, "cache attention: more than 2^30 queries");
+    const bool listed = a->topk != 0;
+    if (listed) {
+        if (a->topk < 0) return fail(FG_ERR_ARG, "cache attention: %d blocks a query", a->topk);
+        if (a->block != 32 && a->block != 64 && a->block != 128 && a->block != 256) return fail(FG_ERR_SHAPE, "cache attention: blocks of 32, 64, 128 or 256 keys, got %d", a->block);
+        if ((int64_t)a->topk * 128 > INT32_MAX / c.kv_heads) return fail(FG_ERR_SHAPE, "cache attention: too long a list");
+    }
+    *p = Problem{};
+    if ((rc = strides_of("q", a->q, a->q_strides, a->type == FG_TYPE_F32 ? 4 : 2, &p->qs, kWhat)) || (rc = aligned("out", a->out, 16, kWhat)) ||
+        (rc = aligned("blocks", a->blocks, 4, kWhat)) || (rc = aligned("lengths", a->lengths, 4, kWhat)) ||
+        (rc = aligned("q_lengths", a->q_lengths, 4, kWhat))) return rc;
+    p->batch = c.batch; p->queries = a->queries; p->keys = c.keys; p->heads = a->heads; p->kv_heads = c.kv_heads; p->group = a->heads / c.kv_heads;
+    p->causal = a->causal != 0; p->scale = a->scale; p->scale2 = a->scale * kLog2e;
+    p->q = a->q; p->lengths = a->lengths; p->q_lengths = a->q_lengths;
+    if (listed) {
+        p->block_shift = a->block == 32 ? 5 : a->block == 64 ? 6 : a->block == 128 ? 7 : 8;
+        p->blocks = (c.keys + a->block - 1) / a->block;
+        p->topk = a->topk;
+        p->list = sizes_only ? reinterpret_cast<const int32_t *>(16) : a->blocks;
+    }
+    return FG_OK;
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace fg
+
+extern "C" int64_t fg_cache_attention_workspace(const fg_cache_attention_args *args) {
+    fg::block::Problem p;
+    if (int rc = fg::cache::problem_of(args, &p, true)) return rc;
+    size_t need = 0;
+    const int rc = fg::cache::launch_t(p, args, nullptr, 0, &need, nullptr);
+    return rc ? rc : (int64_t)need;
+}
+
+extern "C" int fg_cache_attention(const fg_cache_attention_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+    fg::block::Problem p;
+    if (int rc = fg::cache::problem_of(args, &p, false)) return rc;
+    if ((int64_t)p.batch * p.queries == 0) return FG_OK;
+    if (!p.q || !args->out || (p.topk && !p.list)) return fg::fail(FG_ERR_ARG, "cache attention: null pointer");
+    if (int rc = fg::block::aligned("the workspace", workspace, 16, "cache attention")) return rc;
+    return fg::cache::launch_t(p, args, workspace, workspace_bytes, nullptr, static_cast<hipStream_t>(stream));
+}

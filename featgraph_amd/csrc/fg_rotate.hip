@@ -1,0 +1,405 @@
+// RMS norm of every head of queries and keys, and their rotation by position, in one pass; and its gradients.
+//   xh = x / sqrt(mean(x^2) + eps),  y = w xh (or x where there are no weights),  each pair (a, b) of the first rotary_len elements of y turned by
+//   t = 2 pi position[axis(pair)] turns[pair]:  (a cos t - b sin t, a sin t + b cos t);  pairs are (i, i + rotary_len / 2) or neighbours.
+//   Gradients: g = w (dout turned by -t),  dx = (g - xh mean(g xh)) / sqrt(mean(x^2) + eps),  dw = sum over all rows of xh (dout turned by -t).
+//
+// Angles are products in 64 bits, less their whole turns before they are rounded: a position of 10^6 has as good a sine as position 1.  A wavefront
+// makes a token's sines once, a pair a lane, and takes them from LDS for all its heads.
+// A lane holds one 16-byte piece of each half of a head's pairs, so that partners need no exchange; elements that are not turned
+// (rotary_len < head_len) are dealt to the halves the same way.
+// Sums in 32 bits; dw's sums over rows in 32 bits per wavefront and 64 after that.
+#include <algorithm>
+
+#include "fg_block.h"
+
+namespace fg {
+namespace rotate {
+
+namespace {
+
+using block::Strides;
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kPairs = 64;
+
+struct Problem {
+    int batch, tokens, heads, kv_heads, rotary_len, interleaved, axes, parts;
+    float eps;
+    const void *q, *k, *q_weight, *k_weight;
+    Strides qs, ks;
+    const int32_t *positions, *lengths, *q_lengths;
+    double turns[kPairs];              // of a pair and a position
+    uint8_t axis[kPairs];
+};
+
+template <typename T> struct Piece;                   // 16 bytes
+template <> struct Piece<float> { static constexpr int N = 4; typedef float V __attribute__((ext_vector_type(4))); };
+template <> struct Piece<_Float16> { static constexpr int N = 8; typedef _Float16 V __attribute__((ext_vector_type(8))); };
+template <> struct Piece<__bf16> { static constexpr int N = 8; typedef __bf16 V __attribute__((ext_vector_type(8))); };
+
+// What a lane holds of a head: E elements from `a` on and E from `b` on, and where their sines stand.
+template <typename T, int D> struct Lane {
+    static constexpr int E = Piece<T>::N, kLanes = D / 2 / E, kHeads = 64 / kLanes;      // lanes of a head; heads of a wavefront at a time
+    int slot, a, b, first[2];
+    bool turned;
+    __device__ __forceinline__ Lane(const Problem &p, int lane) {
+        const int half = p.rotary_len / 2, at = lane % kLanes * E;
+        slot = lane / kLanes;
+        turned = at < half;
+        a = turned ? at : p.rotary_len + at - half;
+        b = turned ? half + at : p.rotary_len + (D - p.rotary_len) / 2 + at - half;
+        first[0] = p.interleaved ? a / 2 : at;
+        first[1] = p.interleaved ? b / 2 : at + E / 2;
+    }
+};
+
+// A token's cosines and sines, for all lanes of a wavefront.
+__device__ __forceinline__ void make_angles(const Problem &p, int b, int i, int q_len, int lane, float2 *table) {
+    wave_lds_sync();                   // of the token before
+    if (lane < p.rotary_len / 2) {
+        int64_t position;
+        if (p.positions) position = p.positions[((int64_t)b * p.tokens + i) * p.axes + p.axis[lane]];
+        else position = (int64_t)(p.lengths ? p.lengths[b] : q_len) - q_len + i;
+        double t = (double)position * p.turns[lane];
+        t -= rint(t);
+        float2 cs;
+        sincospif((float)(2.0 * t), &cs.y, &cs.x);
+        table[lane] = cs;
+    }
+    wave_lds_sync();
+}
+
+// (a, b) of one lane turned; sign -1: back.
+template <typename T, int D>
+__device__ __forceinline__ void turn(const Problem &p, const Lane<T, D> &me, const float2 *cs, float sign, float (&a)[Piece<T>::N], float (&b)[Piece<T>::N]) {
+    constexpr int E = Piece<T>::N;
+    if (!me.turned) return;
+    if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            const float c0 = cs[i].x, s0 = sign * cs[i].y, c1 = cs[E / 2 + i].x, s1 = sign * cs[E / 2 + i].y;
+            const float x = a[2 * i], y = b[2 * i];
+            a[2 * i] = x * c0 - a[2 * i + 1] * s0;
+            a[2 * i + 1] = x * s0 + a[2 * i + 1] * c0;
+            b[2 * i] = y * c1 - b[2 * i + 1] * s1;
+            b[2 * i + 1] = y * s1 + b[2 * i + 1] * c1;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float x = a[i], s = sign * cs[i].y;
+            a[i] = x * cs[i].x - b[i] * s;
+            b[i] = x * s + b[i] * cs[i].x;
+        }
+    }
+}
+
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (L == 2) return v + dpp_move<0xB1>(v);
+    else return group_sum<L>(v);
+}
+
+// 1 / sqrt(mean(x^2) + eps) over a head's lanes.  Squares that leave the range of 32 bits are taken again of smaller numbers.
+template <typename T, int D>
+__device__ __forceinline__ float inverse_rms(const float (&a)[Piece<T>::N], const float (&b)[Piece<T>::N], float eps) {
+    constexpr int E = Piece<T>::N;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += a[i] * a[i] + b[i] * b[i];
+    s = lanes_sum<Lane<T, D>::kLanes>(s);
+    float r = 1.f / sqrtf(s * (1.f / D) + eps);
+    if (__any(!(s < __builtin_inff()))) {
+        constexpr float DOWN = 0x1p-70f;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) t += (a[i] * DOWN) * (a[i] * DOWN) + (b[i] * DOWN) * (b[i] * DOWN);
+        t = lanes_sum<Lane<T, D>::kLanes>(t);
+        if (!(s < __builtin_inff())) r = DOWN / sqrtf(t * (1.f / D));
+    }
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void fetch(const T *p, float (&f)[Piece<T>::N]) {
+    const typename Piece<T>::V v = *reinterpret_cast<const typename Piece<T>::V *>(p);
+#pragma unroll
+    for (int i = 0; i < Piece<T>::N; ++i) f[i] = (float)v[i];
+}
+template <typename T> __device__ __forceinline__ void put(T *p, const float (&f)[Piece<T>::N]) {
+    typename Piece<T>::V v;
+#pragma unroll
+    for (int i = 0; i < Piece<T>::N; ++i) v[i] = (T)f[i];
+    *reinterpret_cast<typename Piece<T>::V *>(p) = v;
+}
+
+// The sines of a lane's elements.
+template <typename T, int D> __device__ __forceinline__ void own_angles(const Lane<T, D> &me, const float2 *table, float2 (&cs)[Piece<T>::N]) {
+    constexpr int E = Piece<T>::N;
+#pragma unroll
+    for (int i = 0; i < E; ++i) cs[i] = me.turned ? table[me.first[i / (E / 2)] + i % (E / 2)] : make_float2(1.f, 0.f);
+}
+
+// A wavefront's share: one token, and every `parts`-th group of its heads.
+template <typename T, int D, bool NORM>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(const Problem p, T *q_out, T *k_out) {
+    constexpr int E = Piece<T>::N;
+    __shared__ float2 table[kWaves][kPairs];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * kWaves + wave, token = unit / p.parts;
+    if (token >= (int64_t)p.batch * p.tokens) return;
+    const int part = (int)(unit - token * p.parts), b = (int)(token / p.tokens), i = (int)(token - (int64_t)b * p.tokens);
+    const int q_len = p.q_lengths ? min(max(p.q_lengths[b], 0), p.tokens) : p.tokens;
+    const bool there = i < q_len;
+    const Lane<T, D> me(p, lane);
+    float2 cs[E];
+    if (there) {
+        make_angles(p, b, i, q_len, lane, table[wave]);
+        own_angles<T, D>(me, table[wave], cs);
+    }
+    auto side = [&](const void *data, const Strides &s, const void *weight, T *out, int heads, int skip) {
+        float wa[E], wb[E];
+        if (NORM) {
+            fetch(static_cast<const T *>(weight) + me.a, wa);
+            fetch(static_cast<const T *>(weight) + me.b, wb);
+        }
+        const T *src = static_cast<const T *>(data) + b * s.batch + (int64_t)i * s.row;
+        for (int h = ((part + p.parts - skip) % p.parts) * me.kHeads + me.slot; h < heads; h += p.parts * me.kHeads) {
+            float x[E] = {}, y[E] = {};
+            if (there) {
+                fetch(src + h * s.head + me.a, x);
+                fetch(src + h * s.head + me.b, y);
+                if (NORM) {
+                    const float r = inverse_rms<T, D>(x, y, p.eps);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) { x[e] = x[e] * r * wa[e]; y[e] = y[e] * r * wb[e]; }
+                }
+                turn<T, D>(p, me, cs, 1.f, x, y);
+            }
+            T *dst = out + (token * heads + h) * D;
+            put(dst + me.a, x);
+            put(dst + me.b, y);
+        }
+    };
+    side(p.q, p.qs, p.q_weight, q_out, p.heads, 0);
+    side(p.k, p.ks, p.k_weight, k_out, p.kv_heads, (p.heads + me.kHeads - 1) / me.kHeads % p.parts);
+}
+
+struct Grads { const void *dq_out, *dk_out; Strides dqs, dks; void *dq, *dk; float *sums; };
+
+// The same with the gradients; wavefronts take one token after the other and keep their share of dw: sums[workgroup][q, k][D].
+template <typename T, int D, bool NORM>
+__global__ __launch_bounds__(kThreads) void rotate_backward_kernel(const Problem p, const Grads grads) {
+    constexpr int E = Piece<T>::N;
+    __shared__ float2 table[kWaves][kPairs];
+    __shared__ float shares[kWaves][2][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lane<T, D> me(p, lane);
+    float sum[2][2][E] = {};
+    const int64_t units = (int64_t)p.batch * p.tokens * p.parts;
+    for (int64_t unit = (int64_t)blockIdx.x * kWaves + wave; unit < units; unit += (int64_t)gridDim.x * kWaves) {
+        const int64_t token = unit / p.parts;
+        const int part = (int)(unit - token * p.parts), b = (int)(token / p.tokens), i = (int)(token - (int64_t)b * p.tokens);
+        const int q_len = p.q_lengths ? min(max(p.q_lengths[b], 0), p.tokens) : p.tokens;
+        const bool there = i < q_len;
+        float2 cs[E];
+        if (there) {
+            make_angles(p, b, i, q_len, lane, table[wave]);
+            own_angles<T, D>(me, table[wave], cs);
+        }
+        auto side = [&](const void *data, const Strides &s, const void *weight, const void *dout, const Strides &ds, void *out, int heads, int skip, auto which) {
+            constexpr int K = decltype(which)::value;
+            float wa[E], wb[E];
+            if (NORM) {
+                fetch(static_cast<const T *>(weight) + me.a, wa);
+                fetch(static_cast<const T *>(weight) + me.b, wb);
+            }
+            const T *src = static_cast<const T *>(data) + b * s.batch + (int64_t)i * s.row;
+            const T *up = static_cast<const T *>(dout) + b * ds.batch + (int64_t)i * ds.row;
+            for (int h = ((part + p.parts - skip) % p.parts) * me.kHeads + me.slot; h < heads; h += p.parts * me.kHeads) {
+                float ga[E] = {}, gb[E] = {};
+                if (there) {
+                    fetch(up + h * ds.head + me.a, ga);
+                    fetch(up + h * ds.head + me.b, gb);
+                    turn<T, D>(p, me, cs, -1.f, ga, gb);
+                    if (NORM) {
+                        float x[E], y[E], dot = 0.f;
+                        fetch(src + h * s.head + me.a, x);
+                        fetch(src + h * s.head + me.b, y);
+                        const float r = inverse_rms<T, D>(x, y, p.eps);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            x[e] *= r; y[e] *= r;
+                            sum[K][0][e] += ga[e] * x[e];
+                            sum[K][1][e] += gb[e] * y[e];
+                            ga[e] *= wa[e]; gb[e] *= wb[e];
+                            dot += ga[e] * x[e] + gb[e] * y[e];
+                        }
+                        dot = lanes_sum<Lane<T, D>::kLanes>(dot) * (1.f / D);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) { ga[e] = (ga[e] - x[e] * dot) * r; gb[e] = (gb[e] - y[e] * dot) * r; }
+                    }
+                }
+                T *dst = static_cast<T *>(out) + (token * heads + h) * D;
+                put(dst + me.a, ga);
+                put(dst + me.b, gb);
+            }
+        };
+        side(p.q, p.qs, p.q_weight, grads.dq_out, grads.dqs, grads.dq, p.heads, 0, std::integral_constant<int, 0>{});
+        side(p.k, p.ks, p.k_weight, grads.dk_out, grads.dks, grads.dk, p.kv_heads, (p.heads + me.kHeads - 1) / me.kHeads % p.parts, std::integral_constant<int, 1>{});
+    }
+    if (!NORM) return;
+    // over the wavefront's heads, then its workgroup's wavefronts
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                float v = sum[k][h][e];
+                for (int d = Lane<T, D>::kLanes; d < 64; d <<= 1) v += __shfl_xor(v, d);
+                if (me.slot == 0) shares[wave][k][(h ? me.b : me.a) + e] = v;
+            }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * D; c += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v += shares[w][c / D][c % D];
+        grads.sums[(int64_t)blockIdx.x * 2 * D + c] = v;
+    }
+}
+
+// dw: 16 columns a workgroup, 16 threads a column, in 64 bits.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void weights_kernel(const float *sums, int rows, T *dq_weight, T *dk_weight) {
+    __shared__ double part[16][17];
+    const int col = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+    double v = 0.0;
+    for (int r = row; r < rows; r += 16) v += (double)sums[(int64_t)r * 2 * D + c];
+    part[row][col] = v;
+    __syncthreads();
+    if (row) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += part[r][col];
+    (c < D ? dq_weight : dk_weight)[c % D] = (T)(float)v;
+}
+
+constexpr const char *kWhat = "rotation";
+
+int problem_of(const fg_rotate_args *a, Problem *p) {
+    if (!a) return fail(FG_ERR_ARG, "rotation: arguments are a null pointer");
+    if (a->type != FG_TYPE_F32 && a->type != FG_TYPE_F16 && a->type != FG_TYPE_BF16) return fail(FG_ERR_ARG, "rotation: unknown type %d", a->type);
+    if (a->batch < 0 || a->tokens < 0 || a->heads < 1 || a->kv_heads < 1) return fail(FG_ERR_ARG, "rotation: negative sizes, or no heads");
+    if (a->head_len != 32 && a->head_len != 64 && a->head_len != 128) return fail(FG_ERR_SHAPE, "rotation: heads of 32, 64 or 128 elements, got %d", a->head_len);
+    if (a->rotary_len < 0 || a->rotary_len > a->head_len || a->rotary_len % 16)
+        return fail(FG_ERR_SHAPE, "rotation: a multiple of 16 elements of a head of %d can be turned, got %d", a->head_len, a->rotary_len);
+    if (a->tokens > (1 << 30) || a->heads > (1 << 20) || a->kv_heads > (1 << 20)) return fail(FG_ERR_SHAPE, "rotation: more than 2^30 tokens or 2^20 heads");
+    if (a->axes < 1 || a->axes > 8 || (a->axes > 1 && a->rotary_len && !a->positions))
+        return fail(FG_ERR_ARG, "rotation: 1 to 8 axes, and positions with more than one, got %d", a->axes);
+    *p = Problem{};
+    for (int i = 0; i < a->rotary_len / 2; ++i) {
+        if (a->axis[i] >= a->axes) return fail(FG_ERR_ARG, "rotation: pair %d turns by axis %d of %d", i, a->axis[i], a->axes);
+        p->turns[i] = a->turns[i];
+        p->axis[i] = a->axis[i];
+    }
+    if ((!a->q_weight) != (!a->k_weight)) return fail(FG_ERR_ARG, "rotation: weights for queries and keys come together");
+    const int size = a->type == FG_TYPE_F32 ? 4 : 2;
+    int rc;
+    if ((rc = block::strides_of("q", a->q, a->q_strides, size, &p->qs, kWhat)) || (rc = block::strides_of("k", a->k, a->k_strides, size, &p->ks, kWhat)) ||
+        (rc = block::aligned("the queries' weights", a->q_weight, 16, kWhat)) || (rc = block::aligned("the keys' weights", a->k_weight, 16, kWhat)) ||
+        (rc = block::aligned("positions", a->positions, 4, kWhat)) || (rc = block::aligned("lengths", a->lengths, 4, kWhat)) ||
+        (rc = block::aligned("q_lengths", a->q_lengths, 4, kWhat)) || (rc = block::aligned("the turned queries", a->q_out, 16, kWhat)) ||
+        (rc = block::aligned("the turned keys", a->k_out, 16, kWhat))) return rc;
+    p->batch = a->batch; p->tokens = a->tokens; p->heads = a->heads; p->kv_heads = a->kv_heads;
+    p->rotary_len = a->rotary_len; p->interleaved = a->interleaved != 0; p->axes = a->axes; p->eps = a->eps;
+    p->q = a->q; p->k = a->k; p->q_weight = a->q_weight; p->k_weight = a->k_weight;
+    p->positions = a->positions; p->lengths = a->lengths; p->q_lengths = a->q_lengths;
+    // groups of heads that a wavefront takes at a time; each gets a wavefront of its own where there are too few tokens to fill the card
+    const int lanes = a->head_len / 2 / (16 / size), each = 64 / lanes;
+    const int groups = (a->heads + each - 1) / each + (a->kv_heads + each - 1) / each;
+    p->parts = (int64_t)a->batch * a->tokens >= 4096 ? 1 : groups;
+    const int64_t grid = ((int64_t)a->batch * a->tokens * p->parts + kWaves - 1) / kWaves;
+    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "rotation: %lld workgroups do not fit a launch", (long long)grid);
+    return FG_OK;
+}
+
+// Workgroups of the gradients: eight wavefronts a SIMD at most, which go on from token to token.
+int backward_grid(const Problem &p) {
+    return (int)std::min<int64_t>(1024, ((int64_t)p.batch * p.tokens * p.parts + kWaves - 1) / kWaves);
+}
+
+template <typename F> int by_shape(const fg_rotate_args *a, F f) {
+    auto with_norm = [&](auto t, auto d) { return a->q_weight ? f(t, d, std::true_type{}) : f(t, d, std::false_type{}); };
+    auto with_length = [&](auto t) {
+        switch (a->head_len) {
+        case 32: return with_norm(t, std::integral_constant<int, 32>{});
+        case 64: return with_norm(t, std::integral_constant<int, 64>{});
+        default: return with_norm(t, std::integral_constant<int, 128>{});
+        }
+    };
+    switch (a->type) {
+    case FG_TYPE_F32: return with_length(float{});
+    case FG_TYPE_F16: return with_length(_Float16{});
+    default: return with_length(__bf16{});
+    }
+}
+
+}  // namespace
+}  // namespace rotate
+}  // namespace fg
+
+extern "C" int fg_rotate_heads(const fg_rotate_args *args, void *stream) {
+    using namespace fg;
+    using namespace fg::rotate;
+    Problem p;
+    if (int rc = problem_of(args, &p)) return rc;
+    if ((int64_t)p.batch * p.tokens == 0) return FG_OK;
+    if (!p.q || !p.k || !args->q_out || !args->k_out) return fail(FG_ERR_ARG, "rotation: null pointer");
+    const dim3 grid((unsigned)(((int64_t)p.batch * p.tokens * p.parts + kWaves - 1) / kWaves));
+    by_shape(args, [&](auto t, auto d, auto norm) {
+        typedef decltype(t) T;
+        rotate_kernel<T, decltype(d)::value, decltype(norm)::value><<<grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(
+            p, static_cast<T *>(args->q_out), static_cast<T *>(args->k_out));
+        return 0;
+    });
+    FG_HIP_TRY(hipGetLastError());
+    return FG_OK;
+}
+
+extern "C" int64_t fg_rotate_heads_backward_workspace(const fg_rotate_args *args) {
+    fg::rotate::Problem p;
+    if (int rc = fg::rotate::problem_of(args, &p)) return rc;
+    return args->q_weight ? (int64_t)fg::rotate::backward_grid(p) * 2 * args->head_len * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rotate_grads *grads, void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace fg;
+    using namespace fg::rotate;
+    Problem p;
+    int rc;
+    if ((rc = problem_of(args, &p))) return rc;
+    if (!grads) return fail(FG_ERR_ARG, "rotation: gradients are a null pointer");
+    const int size = args->type == FG_TYPE_F32 ? 4 : 2;
+    Grads g{grads->dq_out, grads->dk_out, {}, {}, grads->dq, grads->dk, static_cast<float *>(workspace)};
+    if ((rc = block::strides_of("dL/d(turned queries)", grads->dq_out, grads->dq_out_strides, size, &g.dqs, kWhat)) ||
+        (rc = block::strides_of("dL/d(turned keys)", grads->dk_out, grads->dk_out_strides, size, &g.dks, kWhat)) ||
+        (rc = block::aligned("dq", grads->dq, 16, kWhat)) || (rc = block::aligned("dk", grads->dk, 16, kWhat)) ||
+        (rc = block::aligned("the weights' gradients", grads->dq_weight, size, kWhat)) ||
+        (rc = block::aligned("the weights' gradients", grads->dk_weight, size, kWhat)) || (rc = block::aligned("the workspace", workspace, 16, kWhat))) return rc;
+    const bool norm = args->q_weight;
+    if (norm && (!grads->dq_weight || !grads->dk_weight)) return fail(FG_ERR_ARG, "rotation: null pointer");
+    const int rows = backward_grid(p);
+    const size_t need = norm ? (size_t)rows * 2 * args->head_len * sizeof(float) : 0;
+    if (workspace_bytes < need || (need && !workspace))
+        return fail(FG_ERR_ARG, "rotation: a workspace of %zu bytes, %zu needed (fg_rotate_heads_backward_workspace)", workspace_bytes, need);
+    if (rows && (!grads->dq_out || !grads->dk_out || !grads->dq || !grads->dk || (norm && (!p.q || !p.k)))) return fail(FG_ERR_ARG, "rotation: null pointer");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    rc = by_shape(args, [&](auto t, auto d, auto with_norm) -> int {
+        typedef decltype(t) T;
+        constexpr int D = decltype(d)::value;
+        constexpr bool NORM = decltype(with_norm)::value;
+        if (rows) rotate_backward_kernel<T, D, NORM><<<dim3((unsigned)rows), dim3(kThreads), 0, s>>>(p, g);
+        FG_HIP_TRY(hipGetLastError());
+        if (NORM) weights_kernel<T, D><<<dim3(2 * D / 16), dim3(kThreads), 0, s>>>(g.sums, rows, static_cast<T *>(grads->dq_weight), static_cast<T *>(grads->dk_weight));
+        FG_HIP_TRY(hipGetLastError());
+        return FG_OK;
+    });
+    return rc;
+}

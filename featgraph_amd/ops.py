@@ -12,7 +12,8 @@ operators between two operands on the same target, dot products that involve edg
 runs forward only and refuses inputs that require grad.
 
 pool_blocks / select_blocks / block_attention are attention over a graph that the data itself makes on the GPU: every query selects
-blocks of keys by a cheap score and attends to the keys in them.
+blocks of keys by a cheap score and attends to the keys in them.  rotate_heads makes their queries and keys (norms and positions); new_cache / write_cache /
+read_cache / cache_attention keep keys and values in 4 or 8 bits and attend to them as they are held.
 """
 import math
 
@@ -20,13 +21,19 @@ import torch
 
 from . import autograd
 from .module import block_attention as _block
+from .module import cache as _cache
+from .module import rotate as _rotate
+from .module.cache import KeyValueCache
 
 _BINARY = ("add", "sub", "mul", "div")
 
 
 def _no_grad_inputs(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
         raise NotImplementedError("%s has no gradient here; detach the inputs or run under torch.no_grad()" % what)
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 \
+            and any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no forward-mode gradient" % what)
 
 
 def gspmm(g, op, reduce_op, lhs_data, rhs_data):
@@ -159,3 +166,61 @@ def position_bounds(num_buckets, max_distance=128, causal=True):
     if causal:
         return tuple(ends(sides[0]))
     return tuple([1 - x for x in reversed(ends(sides[0]))] + [1] + [x + 1 for x in ends(sides[1])])
+
+
+def rotate_heads(q, k, q_weight=None, k_weight=None, positions=None, lengths=None, q_lengths=None, base=10000.0, frequencies=None, sections=None,
+                 rotary_len=None, interleaved=False, eps=1e-6):
+    """(q, k) with every head normed by its root mean square (where weights are given) and turned by its token's position, in one pass.
+
+    q (batch, tokens, heads, head_len), k (batch, tokens, kv_heads, head_len), float32, float16 or bfloat16, slices of a fused projection as they
+    are.  With q_weight and k_weight, (head_len,) each: x becomes weight x / sqrt(mean(x^2) + eps), per head.  Of the first rotary_len elements (default all,
+    a multiple of 16; 0: norms alone) each pair (a, b) -- elements i and i + rotary_len / 2, or 2 i and 2 i + 1 if `interleaved` --
+    becomes (a cos t - b sin t, a sin t + b cos t), t = position frequencies[i], frequencies base^(-2 i / rotary_len) unless given; angles are
+    made in 64 bits.
+
+    Token i of a sequence stands at position i, with lengths (int32 (batch,)) at lengths - q_lengths + i as in block_attention, or where
+    positions say: int32 (batch, tokens), or (batch, tokens, axes) with `sections`, the number of pairs, in order, that turn by each axis (time, height,
+    width).  Rows behind q_lengths are not read, and 0.
+
+    Differentiable in q, k and the weights; the same bits on every call.  head_len 32, 64 or 128."""
+    spec = _rotate.check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequencies, sections, rotary_len, interleaved, eps)
+    return autograd.rotate_heads(q, k, q_weight, k_weight, spec, positions, lengths, q_lengths)
+
+
+def new_cache(batch, keys, kv_heads, head_len, bits=4, device=None):
+    """An empty KeyValueCache for `batch` sequences with room for `keys` keys each, in 4 or 8 bits an element and a byte for 32 of them: 0.53 or 1.03
+    bytes an element where float16 takes 2.  head_len 32, 64 or 128."""
+    return _cache.new(batch, keys, kv_heads, head_len, bits, device)
+
+
+def write_cache(cache, k, v, lengths=None, q_lengths=None):
+    """New tokens' keys and values, (batch, tokens, kv_heads, head_len), float32, float16 or bfloat16, quantised into the cache.
+
+    Token i of a sequence becomes key lengths - q_lengths + i, so that with `lengths` (int32 (batch,), the keys of each sequence, the new ones among them) the last
+    new token is the last key; tokens behind q_lengths (default: all are there) are not read, keys before 0 are dropped and everything else in the cache
+    stays as it was.  32 neighbouring elements of a head share the least power of two with which the largest of them rounds to at most the largest
+    element (6 or 448); each is rounded to the nearest element, ties to the even code.  32 with an infinity or NaN among them become
+    NaN.  Not differentiable."""
+    _no_grad_inputs("write_cache", k, v)
+    _cache.write(cache, k, v, lengths, q_lengths)
+
+
+def read_cache(cache, dtype=torch.bfloat16, first=None, count=None, lengths=None):
+    """(k, v), each (batch, count, kv_heads, head_len) in `dtype`: keys first .. first + count - 1 of every sequence as the cache holds them.
+
+    first: int32 (batch,), default 0; count: default all that the cache has room for.  Keys before 0 and behind `lengths` (int32 (batch,), default: all) are not
+    read, and 0.  bfloat16 and float32 hold every value (bfloat16 but for fractions of 2^-126); float16 the nearest, up to 65504."""
+    return _cache.read(cache, dtype, first, count, lengths)
+
+
+def cache_attention(q, cache, blocks=None, block_size=None, scale=None, causal=True, lengths=None, q_lengths=None):
+    """out[b, i, h] = sum over the keys j that query i sees of softmax(scale <q[b, i, h], k[b, j, g]>) v[b, j, g], k and v as the cache holds them.
+
+    q (batch, queries, heads, head_len), float32, float16 or bfloat16; heads / kv_heads (1 to 16) query heads share key head g.  Without `blocks` a query sees
+    all keys, with them (int32 (batch, queries, kv_heads, topk) and block_size 32, 64, 128 or 256, as in block_attention) those of
+    its blocks; lengths, q_lengths, causal and scale as in block_attention.  A query that sees no key gives 0.
+
+    Made for single tokens and a few at a time: 16 / group tokens share one pass over the cache.  Powers and sums are kept in 32 bits; values that are not
+    finite reach the rows that see them and no others.  The same bits on every call.  Not differentiable."""
+    _no_grad_inputs("cache_attention", q)
+    return _cache.attention(q, cache, blocks, block_size, scale, bool(causal), lengths, q_lengths)

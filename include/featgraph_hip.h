@@ -673,6 +673,96 @@ int64_t fg_block_attention_backward_workspace(const fg_block_attention_args *arg
 int fg_block_attention_backward(const fg_block_attention_args *args, const fg_block_attention_grads *grads, void *workspace,
                                 size_t workspace_bytes, void *stream);
 
+/* ---- heads of queries and keys normed and rotated by position --------------------------- */
+
+/*
+ * Q (batch, tokens, heads, head_len) and K (batch, tokens, kv_heads, head_len), strided as above.  With weights every head x becomes
+ * w x / sqrt(mean(x^2) + eps) first; then the pairs (a, b) of its first rotary_len elements -- elements i and i + rotary_len / 2, or 2 i and 2 i + 1 with
+ * `interleaved` -- become (a cos t - b sin t, a sin t + b cos t), t = 2 pi turns[i] position[axis[i]], an angle made in 64 bits.  Rows behind
+ * q_lengths (int32 per sequence, or null: all) are not read, and 0 in the results.  (No counterpart in the reference.)
+ */
+typedef struct {
+    int32_t type;                      /* fg_type of Q, K, weights and results */
+    int32_t batch, tokens, heads, kv_heads;
+    int32_t head_len;                  /* 32, 64 or 128 */
+    int32_t rotary_len;                /* a multiple of 16, up to head_len; 0: norms alone */
+    int32_t interleaved;
+    int32_t axes;                      /* 1 to 8 */
+    float eps;
+    double turns[64];                  /* of pair i, for a step of one position: its frequency / (2 pi) */
+    uint8_t axis[64];                  /* of pair i, below `axes` */
+    const void *q, *k;
+    int64_t q_strides[3], k_strides[3];
+    const void *q_weight, *k_weight;   /* (head_len), at multiples of 16 bytes; both or neither (null) */
+    const int32_t *positions;          /* (batch, tokens, axes) dense, or null (one axis): token i of a sequence stands at  lengths - q_lengths + i */
+    const int32_t *lengths, *q_lengths;    /* int32 per sequence, or null; no lengths: token i stands at i */
+    void *q_out, *k_out;               /* dense, as Q and K, at multiples of 16 bytes */
+} fg_rotate_args;
+int fg_rotate_heads(const fg_rotate_args *args, void *stream);
+
+typedef struct {
+    const void *dq_out, *dk_out;       /* dL / d(q_out), dL / d(k_out) */
+    int64_t dq_out_strides[3], dk_out_strides[3];
+    void *dq, *dk;                     /* dense, as Q and K, at multiples of 16 bytes; rows behind q_lengths 0 */
+    void *dq_weight, *dk_weight;       /* (head_len); null without weights */
+} fg_rotate_grads;
+
+/* Gradients, from the same inputs (Q and K only where there are weights).  workspace: device memory of at least
+ * fg_rotate_heads_backward_workspace(args) bytes (which only looks at sizes; negative: an error), 16-byte aligned, of this call alone while
+ * it runs; null if that is 0.  The same sums in the same order on every call. */
+int64_t fg_rotate_heads_backward_workspace(const fg_rotate_args *args);
+int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rotate_grads *grads, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- a cache of keys and values in 4 or 8 bits ------------------------------------------ */
+
+/*
+ * K and V as (batch, kv_heads, keys, head_len) elements of 4 bits (e2m1: sign, two bits of exponent, one of mantissa; the lower half of a byte
+ * first) or 8 (e4m3), and for every 32 neighbouring ones of a head a scale 2^(byte - 127): (batch, kv_heads, keys, head_len / 32) bytes.  All dense;
+ * codes stand at multiples of 16 bytes, scales of 4.  Byte 255: all 32 are NaN.  (No counterpart in the reference.)
+ */
+typedef struct {
+    int32_t bits;                      /* 4 or 8 */
+    int32_t batch, keys, kv_heads;     /* keys: that each sequence has room for */
+    int32_t head_len;                  /* 32, 64 or 128 */
+    void *k, *k_scales, *v, *v_scales;
+} fg_kv_cache;
+
+/*
+ * New tokens' keys and values (batch, tokens, kv_heads, head_len), strided as above, of fg_type `type`, into the cache: token i of a sequence to key
+ * lengths - q_lengths + i (its last token to its last key; no lengths: keys, no q_lengths: tokens).  Nothing else of the cache is touched; tokens behind
+ * q_lengths are not read, keys before 0 dropped.  The scale of 32 values is the least power of two from 2^-127 on with which the largest of them rounds to
+ * the largest element at most (but 2^125 and 2^119 at most, where larger values become the largest element); each is the nearest element, ties to
+ * the even code.  32 values with an infinity or NaN among them become NaN.
+ */
+int fg_cache_write(const fg_kv_cache *cache, int type, const void *k_dev, const int64_t *k_strides, const void *v_dev, const int64_t *v_strides,
+                   int tokens, const int32_t *lengths_dev, const int32_t *q_lengths_dev, void *stream);
+
+/*
+ * Keys first .. first + count - 1 of every sequence (first_dev: int32 per sequence, or null: 0) as (batch, count, kv_heads, head_len) values of `type`, dense, at
+ * multiples of 16 bytes; 0 for keys before 0 and behind `lengths` (null: all).  float16 takes no value beyond 65504.
+ */
+int fg_cache_read(const fg_kv_cache *cache, int type, void *k_dev, void *v_dev, int count, const int32_t *first_dev, const int32_t *lengths_dev,
+                  void *stream);
+
+typedef struct {
+    int32_t type;                      /* fg_type of Q and results */
+    int32_t queries, heads;            /* per sequence; heads are 1 to 16 times the cache's */
+    int32_t causal;                    /* non-zero: a query sees no key behind its position */
+    int32_t block, topk;               /* keys of a block (32, 64, 128 or 256) and ids per query and key head; topk 0: all keys */
+    float scale;
+    fg_kv_cache cache;
+    const void *q;                     /* (batch, queries, heads, head_len) */
+    int64_t q_strides[3];
+    const int32_t *blocks;             /* (batch, queries, kv_heads, topk) dense, as for fg_block_attention; not read with topk 0 */
+    const int32_t *lengths, *q_lengths;
+    void *out;                         /* (batch, queries, heads, head_len) dense, at a multiple of 16 bytes; 0 where a query sees no key */
+} fg_cache_attention_args;
+
+/* Softmax attention over the cache as it is held, or over the selected blocks of it; made for few queries.  workspace: as for fg_block_attention.  The same
+ * sums in the same order on every call. */
+int64_t fg_cache_attention_workspace(const fg_cache_attention_args *args);
+int fg_cache_attention(const fg_cache_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,15 @@ namespace block {
 
 namespace {
 
+constexpr int kMergeStride = 36;       // floats between rows of the joining buffer (32 and 4 of padding)
+
 // ---- few queries ------------------------------------------------------------------------------------------
+
+// What gradients start from: a row's scores are relative to the first number, their powers' sum is 2 to the second.  In one number a reference
+// beyond 2^24, of a row that sees only masked keys, would take the sum away.
+__device__ __forceinline__ float2 log_sum(float reference, float sum) {
+    return sum == 0.f ? make_float2(__builtin_inff(), 0.f) : make_float2(reference, __builtin_amdgcn_logf(sum));
+}
 
 // How far below the largest score a row's reference stands, in base 2: float16 holds powers from 2^-14 on in full, and a long row's output may be
 // that of many small ones.  (They stay below 2^15: many_kernel's reference follows the maximum by up to 2^8.)
@@ -496,6 +504,27 @@ __global__ __launch_bounds__(kThreads) void redo_kernel(const Problem p, const R
     Buckets buckets;
     if (p.n_buckets) buckets = load_buckets<T>(p, h, dynamic + few_stage_bytes<T, D>());
     for (int i = 0; i < tiles; ++i) few_rows<T, D, true>(p, r, shared, dynamic, buckets, b, h, first + i, 0, 1);
+}
+
+// Joins the sums of several workgroups per row: four columns a thread.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void join_kernel(const float *part, const float2 *part_stats, T *out, T *remainder, float2 *lse, int64_t rows, int splits) {
+    const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = e / (D / 4);
+    const int col = (int)(e - row * (D / 4)) * 4;
+    if (row >= rows) return;
+    float top = -__builtin_inff(), total = 0.f;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_stats[s * rows + row].x);
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const float2 st = part_stats[s * rows + row];
+        const float share = __builtin_amdgcn_exp2f(st.x - ref);
+        total += st.y * share;
+        sum += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * D + col) * share;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    store_row<T>(out, remainder, row * D + col, sum * inv);
+    if (col == 0 && lse) lse[row] = log_sum(top, total);
 }
 
 // Which kernel takes a call, and how its work is cut.  many_kernel wants its workgroups' tiles at least half full and 256 workgroups (a CU each).

@@ -9,8 +9,9 @@
 // Rows of one token's heads and of neighbouring tokens make tiles of 16, RT of them a workgroup.  Its four wavefronts deal the keys out among themselves, 32 at a
 // time, and where there are too few workgroups for the card so do several workgroups, whose sums are joined after.  A
 // lane's keys come from memory as operands lie in registers (the sum over a head's elements takes them in any order), values go
-// through LDS as bfloat16 to be read by columns; the next two steps are under way while one is worked on.
-// A result that is not finite is computed again with infinities and NaN kept from the rows that do not see them (mma_masked).
+// through LDS as bfloat16 to be read by columns; the next step is under way while one is worked on.
+// Values that are no numbers are taken as 0 and marked; the marks of the keys that a row sees make its result NaN.  (Keys that are none, and queries that
+// are not finite, make scores of their own rows alone.)
 #include <algorithm>
 #include <type_traits>
 
@@ -56,7 +57,6 @@ template <int BYTES> __device__ __forceinline__ void load_words(const uint8_t *p
 template <int D, int BITS> struct Step {
     typedef Layout<D, BITS> Y;
     int key0;
-    unsigned who[2];                   // tokens of each tile that selected these keys
     uint32_t kw[2][Y::kKeyBytes / 4], vw[Y::kValueBytes / 4];
     unsigned ks[2][Y::kKeyChunks], vs[Y::kValueChunks];
 
@@ -79,6 +79,27 @@ template <int D, int BITS> struct Step {
             const int64_t row = min(first + at / Y::kPerRow, k_len - 1);
             load_words<Y::kValueChunk>(v.codes + row * Y::kRow + col * Y::kValueChunk, vw + j * Y::kValueChunk / 4);
             vs[j] = v.scales[row * (D / kGroup) + col * Y::kValueElements / kGroup];
+        }
+    }
+    // Whether any of the lane's values are no numbers; then, for all lanes: these become 0, and each key's mark has a bit for each 32 of them.
+    __device__ __forceinline__ bool odd() const {
+        unsigned most = 0;
+#pragma unroll
+        for (int j = 0; j < Y::kValueChunks; ++j) most = max(most, vs[j]);
+        return most == 255;
+    }
+    __device__ __forceinline__ void clear(uint8_t *marks, int lane) {
+#pragma unroll
+        for (int j = 0; j < Y::kValueChunks; ++j) {
+            unsigned mark = vs[j] == 255 ? 1u << ((j * 64 + lane) % Y::kPerRow * Y::kValueElements / kGroup) : 0u;
+            if (mark)
+#pragma unroll
+                for (int i = 0; i < Y::kValueChunk / 4; ++i) vw[j * Y::kValueChunk / 4 + i] = 0;
+            vs[j] = mark ? 0 : vs[j];
+            // a row's chunks lie in neighbouring lanes
+#pragma unroll
+            for (int d = 1; d < Y::kPerRow; d <<= 1) mark |= __shfl_xor(mark, d);
+            if (lane % Y::kPerRow == 0) marks[(j * 64 + lane) / Y::kPerRow] = (uint8_t)mark;
         }
     }
     __device__ __forceinline__ bf16x8 keys(int kt, int n) const {
@@ -120,17 +141,27 @@ template <typename T> __device__ __forceinline__ void parts_of(const T *src, bf1
 constexpr int kListed = 1024;          // blocks listed at a time
 struct NoList {};
 
+// Wavefronts of a SIMD that registers are left for: 128, 168 or 256 each.
+template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 : sizeof(T) == 4 ? 2 : (BITS == 4 ? 4 : 3) - LISTED;
+// Most tiles of 16 rows that a workgroup takes.
+template <typename T, int D> constexpr int kMostTiles = sizeof(T) == 4 && D == 128 ? 1 : 2;
+
+// Floats between rows, and between wavefronts, of the joining buffer: neighbours lie on other banks.
+template <int D> constexpr int kMergeRow = D + 4;
+template <int D> constexpr int kMergeWave = 16 * kMergeRow<D> + 4;
+
 template <int D> constexpr size_t stage_bytes() {
-    const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(__bf16), merge = (size_t)kWaves * 16 * kMergeStride * sizeof(float);
+    const size_t values = (size_t)kWaves * kUnit * (D + kPad) * sizeof(__bf16), merge = (size_t)kWaves * kMergeWave<D> * sizeof(float);
     return values > merge ? values : merge;
 }
 
 template <typename T, int D, int BITS, int RT, bool LISTED>
-__global__ __launch_bounds__(kThreads) void attention_kernel(const Problem p, const Held held, const Results r, int n_groups, int splits) {
+__global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void attention_kernel(const Problem p, const Held held, const Results r, int n_groups, int splits) {
     constexpr int DC = D / 32, DT = D / 16, NQ = kQueryParts<T>, NP = kPowerParts<T>;
     typedef List<RT, kListed> Listing;
     __shared__ typename std::conditional<LISTED, Listing, NoList>::type list;
     __shared__ float2 stats[kWaves][16], joined[16];
+    __shared__ uint8_t marks[kWaves][kUnit];
     __shared__ __align__(16) unsigned char dynamic[stage_bytes<D>()];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int unit = xcd_contiguous_block(), pair = unit / (n_groups * splits), rest = unit - pair * n_groups * splits;
@@ -143,22 +174,29 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(const Problem p, co
 
     __bf16 *stage = reinterpret_cast<__bf16 *>(dynamic) + wave * kUnit * (D + kPad);
     const Rows<D, BITS> keys(held.k, held.k_scales, pair, p.keys), vals(held.v, held.v_scales, pair, p.keys);
+    // scores are compared before they are scaled: a negative scale turns the queries' signs instead, and one of 0 takes the queries away
+    const float factor = p.scale2 == 0.f ? 1.f : fabsf(p.scale2);
     bf16x8 qf[RT][NQ][DC];
     int limit[RT];                     // last key that the lane's row may see; columns without a row see everything, nothing is written of them
+    unsigned lost[RT];                 // parts of 32 elements of the lane's row that are NaN
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int t = t0 + rt * tpt + tc;
         const bool there = used && t < q_len;
         limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
+        lost[rt] = 0;
         const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head;
 #pragma unroll
         for (int n = 0; n < DC; ++n) {
-            if (there) {
+            if (there && p.scale2 != 0.f) {
                 parts_of<T>(src + Layout<D, BITS>::element(n, g), &qf[rt][0][n], DC);
             } else {
 #pragma unroll
                 for (int j = 0; j < NQ; ++j) qf[rt][j][n] = zero8<__bf16>();
             }
+            if (p.scale2 < 0.f)
+#pragma unroll
+                for (int j = 0; j < NQ; ++j) qf[rt][j][n] = -qf[rt][j][n];
         }
     }
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + RT * tpt, q_len) - 1) : k_len - 1;
@@ -166,144 +204,129 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(const Problem p, co
 
     f32x4 o[RT][DT];
     float m[RT], l[RT];
-    auto sweep = [&](auto careful) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = -__builtin_inff(); l[rt] = 0.f;
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -__builtin_inff(); l[rt] = 0.f;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        auto window = [&](int first, int units) {
-            auto first_key = [&](int u) {
-                if constexpr (LISTED) return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
-                else return u << 5;
-            };
-            // the next unit, from u on, that holds a key anyone may see
-            auto find = [&](int u) {
-                if constexpr (LISTED)
-                    while (u < units && first_key(u) > last_key) u += stride;
-                return u;
-            };
-            auto fetch = [&](Step<D, BITS> &s, int u) {
-                s.fetch(keys, vals, first_key(u), k_len, lane);
-                if constexpr (LISTED)
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto window = [&](int first, int units) {
+        auto first_key = [&](int u) {
+            if constexpr (LISTED) return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
+            else return u << 5;
+        };
+        // the next unit, from u on, that holds a key anyone may see
+        auto find = [&](int u) {
+            if constexpr (LISTED)
+                while (u < units && first_key(u) > last_key) u += stride;
+            return u;
+        };
+        Step<D, BITS> step;
+        unsigned who[RT];              // tokens of each tile that selected these keys
+        auto fetch = [&](int u) {
+            step.fetch(keys, vals, first_key(u), k_len, lane);
+            if constexpr (LISTED)
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s.who[rt] = (unsigned)(list.bits[u >> sub_shift][0] >> (16 * rt)) & 0xffffu;
-            };
-            auto work = [&](const Step<D, BITS> &now) {
-                wave_lds_sync();
-                now.store_values(stage, lane);
-                f32x4 s[RT][2];
+                for (int rt = 0; rt < RT; ++rt) who[rt] = (unsigned)(list.bits[u >> sub_shift][0] >> (16 * rt)) & 0xffffu;
+        };
+        int u = find(wave + kWaves * split);
+        if (u < units) fetch(u);
+        while (u < units) {
+            const int key0 = step.key0;
+            int last[RT];              // keys that the lane's row sees: key0 + 16 kt + 4 g + i <= last
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
+            for (int rt = 0; rt < RT; ++rt) last[rt] = !LISTED || !used || (who[rt] >> tc) & 1 ? limit[rt] : -1;
+            wave_lds_sync();
+            const bool odd = step.odd();
+            if (__any(odd)) step.clear(marks[wave], lane);
+            step.store_values(stage, lane);
+            f32x4 s[RT][2];
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-                    for (int n = 0; n < DC; ++n) {
-                        const bf16x8 kf = now.keys(kt, n);
+                for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
+                for (int n = 0; n < DC; ++n) {
+                    const bf16x8 kf = step.keys(kt, n);
 #pragma unroll
-                            for (int j = NQ; j-- > 0;) s[rt][kt] = mma(kf, qf[rt][j][n], s[rt][kt]);
-                    }
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int j = NQ; j-- > 0;) s[rt][kt] = mma(kf, qf[rt][j][n], s[rt][kt]);
                 }
-                wave_lds_sync();
-                bf16x8 pf[RT][NP];
-                unsigned seen[RT];
+            }
+            u = find(u + stride);
+            if (u < units) fetch(u);
+            wave_lds_sync();
+            bf16x8 pf[RT][NP];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const int last = !LISTED || !used || (now.who[rt] >> tc) & 1 ? limit[rt] : -1;      // keys that the lane's row sees: key0 + 16 kt + 4 g + i <= last
-                    f32x4 z[2] = {s[rt][0] * p.scale2, s[rt][1] * p.scale2};
-                    seen[rt] = 0xff;
-                    if (!__all(now.key0 + kUnit - 1 <= last)) {
-                        seen[rt] = 0;
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const bool ok = now.key0 + 16 * kt + 4 * g + i <= last;
-                                z[kt][i] = ok ? z[kt][i] : -__builtin_inff();
-                                seen[rt] |= (unsigned)ok << (4 * kt + i);
-                            }
-                    }
-                    const float top = fmaxf(m[rt], largest_of_rows(largest(z[0], z[1])));
-                    const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
-                    if (__any(top != m[rt])) {
-                        const float shrink = __builtin_amdgcn_exp2f(m[rt] - ref);
-                        l[rt] *= shrink;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
-                        m[rt] = top;
-                    }
+            for (int rt = 0; rt < RT; ++rt) {
+                if (!__all(key0 + kUnit - 1 <= last[rt]))
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            z[kt][i] = z[kt][i] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][i], p.scale2, -ref));
-                    l[rt] += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
+                        for (int i = 0; i < 4; ++i) s[rt][kt][i] = key0 + 16 * kt + 4 * g + i <= last[rt] ? s[rt][kt][i] : -__builtin_inff();
+                if (__any(odd))
 #pragma unroll
-                    for (int j = 0; j < NP; ++j) {
-                        pf[rt][j] = pack<__bf16>(z[0], z[1]);
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = 16 * (i >> 2) + 4 * g + (i & 3);
+                        lost[rt] |= key0 + key <= last[rt] ? marks[wave][key] : 0u;
+                    }
+                const float top = fmaxf(m[rt], largest_of_rows(largest(s[rt][0], s[rt][1])) * factor);
+                const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
+                if (__any(top != m[rt])) {
+                    const float shrink = __builtin_amdgcn_exp2f(m[rt] - ref);
+                    l[rt] *= shrink;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
+                    m[rt] = top;
+                }
+                f32x4 z[2];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][i], factor, -ref));
+                l[rt] += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    pf[rt][j] = pack<__bf16>(z[0], z[1]);
+                    if (j + 1 < NP)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) { z[0][i] -= (float)pf[rt][j][i]; z[1][i] -= (float)pf[rt][j][4 + i]; }
-                    }
-                }
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const bf16x8 vf = transposed<__bf16, D>(stage, dt * 16, lane);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if constexpr (decltype(careful)::value) {
-                            o[rt][dt] = mma_masked<__bf16>(vf, pf[rt][0], pf[rt][1], seen[rt], o[rt][dt]);
-                            if (NP == 3) o[rt][dt] = mma_masked<__bf16>(vf, pf[rt][NP - 1], zero8<__bf16>(), seen[rt], o[rt][dt]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < NP; ++j) o[rt][dt] = mma(vf, pf[rt][j], o[rt][dt]);     // in the order of mma_masked: the same bits
-                        }
-                    }
-                }
-            };
-            Step<D, BITS> a, z;
-            int u = find(wave + kWaves * split);
-            if (u < units) {
-                fetch(a, u);
-                u = find(u + stride);
-                while (true) {
-                    const bool more = u < units;
-                    if (more) { fetch(z, u); u = find(u + stride); }
-                    work(a);
-                    if (!more) break;
-                    const bool again = u < units;
-                    if (again) { fetch(a, u); u = find(u + stride); }
-                    work(z);
-                    if (!again) break;
                 }
             }
-        };
-        if constexpr (LISTED) {
-            for (int first = 0; first < p.blocks; first += kListed)
-                window(first, build_list(list, p, b, h, t0, q_len, k_len, first, min(kListed, p.blocks - first)) << sub_shift);
-        } else {
-            window(0, (last_key + kUnit) / kUnit);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bf16x8 vf = transposed<__bf16, D>(stage, dt * 16, lane);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) o[rt][dt] = mma(vf, pf[rt][j], o[rt][dt]);
+            }
         }
     };
-    sweep(std::false_type{});
-    bool odd = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) odd |= not_finite(o[rt][dt]);
-    if (__syncthreads_or(odd)) sweep(std::true_type{});
+    if constexpr (LISTED) {
+        for (int first = 0; first < p.blocks; first += kListed)
+            window(first, build_list(list, p, b, h, t0, q_len, k_len, first, min(kListed, p.blocks - first)) << sub_shift);
+    } else {
+        window(0, (last_key + kUnit) / kUnit);
+    }
 
-    // the four wavefronts' sums, joined a strip of 32 columns at a time
+    // the wavefronts' sums, joined: the threads of a workgroup share the columns out, and where there are more of them the wavefronts too
+    constexpr int ITEMS = 16 * D / 4, SHARE = kThreads > ITEMS ? kThreads / ITEMS : 1, STEP = kThreads / SHARE;
     float *merge = reinterpret_cast<float *>(dynamic);
     const int64_t all_rows = (int64_t)p.batch * p.queries * p.heads;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float sum = rows_sum(l[rt]);
-        __syncthreads();               // the joining buffer of the tile before has been read
+        if (__any(lost[rt] != 0)) {
+            unsigned bad = lost[rt] | __shfl_xor(lost[rt], 16);
+            bad |= __shfl_xor(bad, 32);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                if (bad >> (dt / 2) & 1) o[rt][dt] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        }
         if (g == 0) stats[wave][c] = make_float2(m[rt], sum);
-        __syncthreads();
+        __syncthreads();               // the values' staging, or the joining buffer of the tile before, has been read
         float top = -__builtin_inff(), total = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][c].x);
@@ -312,41 +335,82 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(const Problem p, co
         for (int w = 0; w < kWaves; ++w) total += stats[w][c].y * __builtin_amdgcn_exp2f(stats[w][c].x - ref);
         const float share = __builtin_amdgcn_exp2f(m[rt] - ref);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= share;
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(merge + wave * kMergeWave<D> + c * kMergeRow<D> + 16 * dt + 4 * g) = o[rt][dt] * share;
         if (wave == 0 && g == 0) joined[c] = make_float2(top, total);
+        __syncthreads();
 #pragma unroll
-        for (int strip = 0; strip < DC; ++strip) {
-            __syncthreads();           // the values' staging, or the strip before, has been read
+        for (int item = tid / SHARE; item < ITEMS; item += STEP) {
+            const int row = item / (D / 4), col = item % (D / 4) * 4, at_token = row / p.group, t = t0 + rt * tpt + at_token;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4 *>(merge + (wave * 16 + c) * kMergeStride + 16 * j + 4 * g) = o[rt][2 * strip + j];
-            __syncthreads();
-            const int row = tid >> 3, col = (tid & 7) * 4, at_token = row / p.group, t = t0 + rt * tpt + at_token;
-            if (tid < 16 * 8 && at_token < tpt && t < p.queries) {
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int w = tid % SHARE; w < kWaves; w += SHARE) v += *reinterpret_cast<const f32x4 *>(merge + w * kMergeWave<D> + row * kMergeRow<D> + col);
+            if constexpr (SHARE > 1)
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(merge + (w * 16 + row) * kMergeStride + col);
-                const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (row - at_token * p.group);
-                const float2 st = joined[row];
-                if (splits == 1) {
-                    store_row<T>(static_cast<T *>(r.out), nullptr, at * D + strip * 32 + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
-                } else {
-                    *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + strip * 32 + col) = v;
-                    if (strip == 0 && col == 0) r.part_stats[split * all_rows + at] = st;
-                }
+                for (int i = 0; i < 4; ++i) v[i] += dpp_move<0xB1>(v[i]);        // two threads (heads of 32)
+            if (tid % SHARE || at_token >= tpt || t >= p.queries) continue;
+            const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (row - at_token * p.group);
+            const float2 st = joined[row];
+            if (splits == 1) {
+                store_row<T>(static_cast<T *>(r.out), nullptr, at * D + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
+            } else {
+                *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + col) = v;
+                if (col == 0) r.part_stats[split * all_rows + at] = st;
             }
         }
     }
 }
 
-// How a call's work is cut: workgroups that take all keys where they fill the card, else shares of at least four steps a wavefront.
-struct Shape { int n_groups, splits; };
-template <int RT> Shape shape_of(const Problem &p) {
-    const int tokens = RT * tile_tokens(p.group);
-    Shape s{(int)(((int64_t)p.queries + tokens - 1) / tokens), 1};
+// Joins the shares of one row: the threads of a workgroup take four columns of every so many of them.
+constexpr int kMostSplits = 256;
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part, const float2 *part_stats, T *out, int64_t rows, int splits) {
+    constexpr int C = D / 4, SUBS = kThreads / C;
+    __shared__ float weight[kMostSplits];
+    __shared__ f32x4 sums[SUBS][C];
+    const int tid = threadIdx.x, lane = tid & 63, col = tid % C, sub = tid / C;
+    const int64_t row = blockIdx.x;
+    float top = -__builtin_inff(), total = 0.f;
+    for (int s = lane; s < splits; s += 64) top = fmaxf(top, part_stats[s * rows + row].x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    for (int s = lane; s < splits; s += 64) {
+        const float2 st = part_stats[s * rows + row];
+        const float w = __builtin_amdgcn_exp2f(st.x - ref);
+        total += st.y * w;
+        if (tid < 64) weight[s] = w;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    __syncthreads();
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = sub; s < splits; s += SUBS) v += *reinterpret_cast<const f32x4 *>(part + (s * rows + row) * D + col * 4) * weight[s];
+    sums[sub][col] = v;
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int i = 1; i < SUBS; ++i) v += sums[i][col];
+    store_row<T>(out, nullptr, row * D + col * 4, v * (total == 0.f ? 0.f : 1.f / total));
+}
+
+// How a call's work is cut: where there are too few workgroups for the card, several share a row's keys out.  512 workgroups (two a CU) as long as each
+// has eight steps of 32 keys, 256 as long as each wavefront has one; rows of up to 512 keys stay whole, for joining takes a launch of 3.5 us.
+// Kernel and joining (us), shares as the rule has them / half / twice as many: 1 sequence of 8 key heads x 128, 4 bits, 32,768 keys (64 shares) 14.1 / 15.1 / 15.9, 8,192 keys (32) 8.6 / 10.6 /
+// 9.1; 8 sequences of 4,096 (8) 13.6 / 15.3 / 14.3; 32 of 32,768 (2) 199 / 260 / 206; 1 of 2,048 x 8 heads x 64, 8 bits (16) 7.2 / 7.8 / 7.3; 3 tokens
+// of 8 sequences, 16 blocks of 64 each (8) 10.9 / 12.4 / 11.9; 512 keys (1) 7.1, in four shares 7.1.
+// Workgroups take two tiles of rows where there are as many, which then share the work on the keys (64 tokens over 16,384 keys of 8 x 128, 8 bits: 55 -> 45 us); not with
+// lists, whose unions grow.
+struct Shape { int tiles, n_groups, splits; };
+Shape shape_of(const Problem &p, int most_tiles) {
+    const int tiles = !p.topk && p.queries > tile_tokens(p.group) ? most_tiles : 1, tokens = tiles * tile_tokens(p.group);
+    Shape s{tiles, (int)(((int64_t)p.queries + tokens - 1) / tokens), 1};
     const int64_t groups = std::max<int64_t>((int64_t)p.batch * p.kv_heads * s.n_groups, 1);
     int64_t units = ((int64_t)p.keys + kUnit - 1) / kUnit;
-    if (p.list) units = std::min<int64_t>(units, ((int64_t)p.topk * std::min(tokens, p.queries)) << (p.block_shift - 5));
-    if (units > 8 * kWaves) s.splits = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + groups - 1) / groups, units / (4 * kWaves)));
+    if (p.topk) units = std::min<int64_t>(units, ((int64_t)p.topk * std::min(tokens, p.queries)) << (p.block_shift - 5));
+    if (units > 4 * kWaves)
+        s.splits = (int)std::max<int64_t>(1, std::max(std::min({512 / groups, units / (2 * kWaves), (int64_t)kMostSplits}),
+                                                      std::min({256 / groups, units / kWaves, (int64_t)kMostSplits})));
     return s;
 }
 
@@ -354,8 +418,8 @@ size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <typename T, int D, int BITS>
 int launch(const Problem &p, const fg_cache_attention_args *a, void *workspace, size_t bytes, size_t *need, hipStream_t stream) {
-    constexpr int RT = 1;
-    const Shape s = shape_of<RT>(p);
+    constexpr int MOST = kMostTiles<T, D>;
+    const Shape s = shape_of(p, MOST);
     const size_t rows = (size_t)p.batch * p.queries * p.heads;
     const int64_t grid = (int64_t)p.batch * p.kv_heads * s.n_groups * s.splits;
     if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)grid);
@@ -367,13 +431,12 @@ int launch(const Problem &p, const fg_cache_attention_args *a, void *workspace, 
     const Results r{a->out, reinterpret_cast<float *>(w), reinterpret_cast<float2 *>(w + sums)};
     const Held held{a->cache.k, a->cache.k_scales, a->cache.v, a->cache.v_scales};
     const dim3 blocks((unsigned)grid), threads(kThreads);
-    if (p.list) attention_kernel<T, D, BITS, RT, true><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
-    else attention_kernel<T, D, BITS, RT, false><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
+    if (p.topk) attention_kernel<T, D, BITS, 1, true><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
+    else if (s.tiles == 1) attention_kernel<T, D, BITS, 1, false><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
+    else attention_kernel<T, D, BITS, MOST, false><<<blocks, threads, 0, stream>>>(p, held, r, s.n_groups, s.splits);
     FG_HIP_TRY(hipGetLastError());
     if (s.splits == 1) return FG_OK;
-    const int64_t each = (int64_t)rows * (D / 4), groups = (each + kThreads - 1) / kThreads;
-    if (groups >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)groups);
-    join_kernel<T, D><<<dim3((unsigned)groups), threads, 0, stream>>>(r.part, r.part_stats, static_cast<T *>(r.out), nullptr, nullptr, (int64_t)rows, s.splits);
+    join_shares_kernel<T, D><<<dim3((unsigned)rows), threads, 0, stream>>>(r.part, r.part_stats, static_cast<T *>(r.out), (int64_t)rows, s.splits);
     FG_HIP_TRY(hipGetLastError());
     return FG_OK;
 }
@@ -434,7 +497,7 @@ int problem_of(const fg_cache_attention_args *a, Problem *p, bool sizes_only) {
         p->block_shift = a->block == 32 ? 5 : a->block == 64 ? 6 : a->block == 128 ? 7 : 8;
         p->blocks = (c.keys + a->block - 1) / a->block;
         p->topk = a->topk;
-        p->list = sizes_only ? reinterpret_cast<const int32_t *>(16) : a->blocks;
+        p->list = a->blocks;
     }
     return FG_OK;
 }

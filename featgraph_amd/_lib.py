@@ -39,6 +39,7 @@ class FgBlockAttentionGrads(ctypes.Structure):
     _fields_ = [("dout", _vp), ("dout_strides", _i64 * 3), ("dq", _vp), ("dk", _vp), ("dv", _vp), ("dbias", _vp)]
 
 
+# likewise
 class FgRotateArgs(ctypes.Structure):
     _fields_ = [("type", ctypes.c_int32), ("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
                 ("head_len", ctypes.c_int32), ("rotary_len", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("axes", ctypes.c_int32),
@@ -131,7 +132,7 @@ SIGNATURES = {
     "fg_block_attention_backward": (_int, [_vp, ctypes.POINTER(FgBlockAttentionGrads), _vp, ctypes.c_size_t, _vp]),
     "fg_rotate_heads": (_int, [_vp, _vp]),
     "fg_rotate_heads_backward_workspace": (_i64, [_vp]),
-    "fg_rotate_heads_backward": (_int, [_vp, ctypes.POINTER(FgRotateGrads), _vp, ctypes.c_size_t, _vp]),
+    "fg_rotate_heads_backward": (_int, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "fg_cache_write": (_int, [_vp, _int, _vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64), _int, _vp, _vp, _vp]),
     "fg_cache_read": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp]),
     "fg_cache_attention_workspace": (_i64, [_vp]),

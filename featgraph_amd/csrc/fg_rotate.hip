@@ -118,11 +118,18 @@ __device__ __forceinline__ float inverse_rms(const float (&a)[Piece<T>::N], cons
     return r;
 }
 
-template <typename T> __device__ __forceinline__ void fetch(const T *p, float (&f)[Piece<T>::N]) {
-    const typename Piece<T>::V v = *reinterpret_cast<const typename Piece<T>::V *>(p);
+// What a lane holds of a head, as it is stored.
+template <typename T> struct Pair {
+    typename Piece<T>::V a, b;
+    __device__ __forceinline__ void load(const T *pa, const T *pb) {
+        a = *reinterpret_cast<const typename Piece<T>::V *>(pa);
+        b = *reinterpret_cast<const typename Piece<T>::V *>(pb);
+    }
+    __device__ __forceinline__ void widen(float (&x)[Piece<T>::N], float (&y)[Piece<T>::N]) const {
 #pragma unroll
-    for (int i = 0; i < Piece<T>::N; ++i) f[i] = (float)v[i];
-}
+        for (int i = 0; i < Piece<T>::N; ++i) { x[i] = (float)a[i]; y[i] = (float)b[i]; }
+    }
+};
 template <typename T> __device__ __forceinline__ void put(T *p, const float (&f)[Piece<T>::N]) {
     typename Piece<T>::V v;
 #pragma unroll
@@ -137,7 +144,8 @@ template <typename T, int D> __device__ __forceinline__ void own_angles(const La
     for (int i = 0; i < E; ++i) cs[i] = me.turned ? table[me.first[i / (E / 2)] + i % (E / 2)] : make_float2(1.f, 0.f);
 }
 
-// A wavefront's share: one token, and every `parts`-th group of its heads.
+// A wavefront's share: one token, and every `parts`-th group of its heads.  A head's elements are under way while the one before is worked on, the first
+// ones while angles are made.
 template <typename T, int D, bool NORM>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(const Problem p, T *q_out, T *k_out) {
     constexpr int E = Piece<T>::N;
@@ -149,44 +157,65 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const Problem p, T *q_
     const int q_len = p.q_lengths ? min(max(p.q_lengths[b], 0), p.tokens) : p.tokens;
     const bool there = i < q_len;
     const Lane<T, D> me(p, lane);
+    // heads of queries, then of keys: group g of kHeads heads is one wavefront's at a time
+    const int q_groups = (p.heads + me.kHeads - 1) / me.kHeads, groups = q_groups + (p.kv_heads + me.kHeads - 1) / me.kHeads;
+    const T *q = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)i * p.qs.row, *k = static_cast<const T *>(p.k) + b * p.ks.batch + (int64_t)i * p.ks.row;
+    Pair<T> next, weight;
+    int h;                             // of the group that is under way
+    auto fetch = [&](int group) {
+        const bool keys = group >= q_groups;
+        h = (keys ? group - q_groups : group) * me.kHeads + me.slot;
+        if (!there || h >= (keys ? p.kv_heads : p.heads)) return;
+        const T *src = keys ? k + h * p.ks.head : q + h * p.qs.head;
+        next.load(src + me.a, src + me.b);
+    };
+    auto weigh = [&](int group) {
+        const T *w = static_cast<const T *>(group >= q_groups ? p.k_weight : p.q_weight);
+        if (NORM) weight.load(w + me.a, w + me.b);
+    };
+    fetch(part);
+    weigh(part);
     float2 cs[E];
     if (there) {
         make_angles(p, b, i, q_len, lane, table[wave]);
         own_angles<T, D>(me, table[wave], cs);
     }
-    auto side = [&](const void *data, const Strides &s, const void *weight, T *out, int heads, int skip) {
-        float wa[E], wb[E];
-        if (NORM) {
-            fetch(static_cast<const T *>(weight) + me.a, wa);
-            fetch(static_cast<const T *>(weight) + me.b, wb);
-        }
-        const T *src = static_cast<const T *>(data) + b * s.batch + (int64_t)i * s.row;
-        for (int h = ((part + p.parts - skip) % p.parts) * me.kHeads + me.slot; h < heads; h += p.parts * me.kHeads) {
-            float x[E] = {}, y[E] = {};
-            if (there) {
-                fetch(src + h * s.head + me.a, x);
-                fetch(src + h * s.head + me.b, y);
-                if (NORM) {
-                    const float r = inverse_rms<T, D>(x, y, p.eps);
+    for (int group = part; group < groups; group += p.parts) {
+        const bool keys = group >= q_groups;
+        const int now = h, heads = keys ? p.kv_heads : p.heads;
+        float x[E], y[E];
+        next.widen(x, y);
+        if (group + p.parts < groups) fetch(group + p.parts);
+        if (there) {
+            if (NORM) {
+                float wa[E], wb[E];
+                weight.widen(wa, wb);
+                const float r = inverse_rms<T, D>(x, y, p.eps);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) { x[e] = x[e] * r * wa[e]; y[e] = y[e] * r * wb[e]; }
-                }
-                turn<T, D>(p, me, cs, 1.f, x, y);
+                for (int e = 0; e < E; ++e) { x[e] = x[e] * r * wa[e]; y[e] = y[e] * r * wb[e]; }
             }
-            T *dst = out + (token * heads + h) * D;
+            turn<T, D>(p, me, cs, 1.f, x, y);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = y[e] = 0.f;
+        }
+        if (now < heads) {
+            T *dst = (keys ? k_out : q_out) + (token * heads + now) * D;
             put(dst + me.a, x);
             put(dst + me.b, y);
         }
-    };
-    side(p.q, p.qs, p.q_weight, q_out, p.heads, 0);
-    side(p.k, p.ks, p.k_weight, k_out, p.kv_heads, (p.heads + me.kHeads - 1) / me.kHeads % p.parts);
+        if (!keys && group + p.parts >= q_groups) weigh(group + p.parts);
+    }
 }
 
 struct Grads { const void *dq_out, *dk_out; Strides dqs, dks; void *dq, *dk; float *sums; };
 
 // The same with the gradients; wavefronts take one token after the other and keep their share of dw: sums[workgroup][q, k][D].
+// Workgroups of a CU (wavefronts of a SIMD) that registers are left for.
+template <typename T, bool NORM> constexpr int kResident = NORM && sizeof(T) == 2 ? 3 : 4;
+
 template <typename T, int D, bool NORM>
-__global__ __launch_bounds__(kThreads) void rotate_backward_kernel(const Problem p, const Grads grads) {
+__global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backward_kernel(const Problem p, const Grads grads) {
     constexpr int E = Piece<T>::N;
     __shared__ float2 table[kWaves][kPairs];
     __shared__ float shares[kWaves][2][D];
@@ -194,36 +223,46 @@ __global__ __launch_bounds__(kThreads) void rotate_backward_kernel(const Problem
     const Lane<T, D> me(p, lane);
     float sum[2][2][E] = {};
     const int64_t units = (int64_t)p.batch * p.tokens * p.parts;
+    const int q_groups = (p.heads + me.kHeads - 1) / me.kHeads, k_groups = (p.kv_heads + me.kHeads - 1) / me.kHeads;
+    Pair<T> weights[2];
+    if (NORM) {
+        weights[0].load(static_cast<const T *>(p.q_weight) + me.a, static_cast<const T *>(p.q_weight) + me.b);
+        weights[1].load(static_cast<const T *>(p.k_weight) + me.a, static_cast<const T *>(p.k_weight) + me.b);
+    }
     for (int64_t unit = (int64_t)blockIdx.x * kWaves + wave; unit < units; unit += (int64_t)gridDim.x * kWaves) {
         const int64_t token = unit / p.parts;
         const int part = (int)(unit - token * p.parts), b = (int)(token / p.tokens), i = (int)(token - (int64_t)b * p.tokens);
         const int q_len = p.q_lengths ? min(max(p.q_lengths[b], 0), p.tokens) : p.tokens;
         const bool there = i < q_len;
-        float2 cs[E];
-        if (there) {
-            make_angles(p, b, i, q_len, lane, table[wave]);
-            own_angles<T, D>(me, table[wave], cs);
-        }
-        auto side = [&](const void *data, const Strides &s, const void *weight, const void *dout, const Strides &ds, void *out, int heads, int skip, auto which) {
+        bool angles = false;
+        auto side = [&](const void *data, const Strides &s, const void *dout, const Strides &ds, void *out, int heads, int from, int groups, auto which) {
             constexpr int K = decltype(which)::value;
-            float wa[E], wb[E];
-            if (NORM) {
-                fetch(static_cast<const T *>(weight) + me.a, wa);
-                fetch(static_cast<const T *>(weight) + me.b, wb);
-            }
             const T *src = static_cast<const T *>(data) + b * s.batch + (int64_t)i * s.row;
             const T *up = static_cast<const T *>(dout) + b * ds.batch + (int64_t)i * ds.row;
-            for (int h = ((part + p.parts - skip) % p.parts) * me.kHeads + me.slot; h < heads; h += p.parts * me.kHeads) {
-                float ga[E] = {}, gb[E] = {};
-                if (there) {
-                    fetch(up + h * ds.head + me.a, ga);
-                    fetch(up + h * ds.head + me.b, gb);
+            Pair<T> x_next, g_next;
+            auto fetch = [&](int group) {
+                const int h = group * me.kHeads + me.slot;
+                if (!there || h >= heads) return;
+                g_next.load(up + h * ds.head + me.a, up + h * ds.head + me.b);
+                if (NORM) x_next.load(src + h * s.head + me.a, src + h * s.head + me.b);
+            };
+            if (from < groups) fetch(from);
+            if (there && !angles) make_angles(p, b, i, q_len, lane, table[wave]);
+            angles = true;
+            for (int group = from; group < groups; group += p.parts) {
+                const int h = group * me.kHeads + me.slot;
+                float ga[E], gb[E], x[E], y[E];
+                g_next.widen(ga, gb);
+                if (NORM) x_next.widen(x, y);
+                if (group + p.parts < groups) fetch(group + p.parts);
+                if (there && h < heads) {
+                    float2 cs[E];
+                    own_angles<T, D>(me, table[wave], cs);
                     turn<T, D>(p, me, cs, -1.f, ga, gb);
                     if (NORM) {
-                        float x[E], y[E], dot = 0.f;
-                        fetch(src + h * s.head + me.a, x);
-                        fetch(src + h * s.head + me.b, y);
                         const float r = inverse_rms<T, D>(x, y, p.eps);
+                        float wa[E], wb[E], dot = 0.f;
+                        weights[K].widen(wa, wb);
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
                             x[e] *= r; y[e] *= r;
@@ -236,14 +275,19 @@ __global__ __launch_bounds__(kThreads) void rotate_backward_kernel(const Problem
 #pragma unroll
                         for (int e = 0; e < E; ++e) { ga[e] = (ga[e] - x[e] * dot) * r; gb[e] = (gb[e] - y[e] * dot) * r; }
                     }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) ga[e] = gb[e] = 0.f;
                 }
+                if (h >= heads) continue;
                 T *dst = static_cast<T *>(out) + (token * heads + h) * D;
                 put(dst + me.a, ga);
                 put(dst + me.b, gb);
             }
         };
-        side(p.q, p.qs, p.q_weight, grads.dq_out, grads.dqs, grads.dq, p.heads, 0, std::integral_constant<int, 0>{});
-        side(p.k, p.ks, p.k_weight, grads.dk_out, grads.dks, grads.dk, p.kv_heads, (p.heads + me.kHeads - 1) / me.kHeads % p.parts, std::integral_constant<int, 1>{});
+        // group g of queries and keys together is part g % parts'
+        side(p.q, p.qs, grads.dq_out, grads.dqs, grads.dq, p.heads, part, q_groups, std::integral_constant<int, 0>{});
+        side(p.k, p.ks, grads.dk_out, grads.dks, grads.dk, p.kv_heads, (part + p.parts - q_groups % p.parts) % p.parts, k_groups, std::integral_constant<int, 1>{});
     }
     if (!NORM) return;
     // over the wavefront's heads, then its workgroup's wavefronts
@@ -266,19 +310,30 @@ __global__ __launch_bounds__(kThreads) void rotate_backward_kernel(const Problem
     }
 }
 
-// dw: 16 columns a workgroup, 16 threads a column, in 64 bits.
+// dw in 64 bits: four columns a workgroup, a thread for every so many rows.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void weights_kernel(const float *sums, int rows, T *dq_weight, T *dk_weight) {
-    __shared__ double part[16][17];
-    const int col = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
-    double v = 0.0;
-    for (int r = row; r < rows; r += 16) v += (double)sums[(int64_t)r * 2 * D + c];
-    part[row][col] = v;
-    __syncthreads();
-    if (row) return;
+    __shared__ double part[kWaves][4];
+    const int lane = threadIdx.x & 63, c = blockIdx.x * 4;
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int r = threadIdx.x; r < rows; r += kThreads) {
+        const float4 x = *reinterpret_cast<const float4 *>(sums + (int64_t)r * 2 * D + c);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+    }
 #pragma unroll
-    for (int r = 1; r < 16; ++r) v += part[r][col];
-    (c < D ? dq_weight : dk_weight)[c % D] = (T)(float)v;
+    for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], d);
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[threadIdx.x >> 6][i] = v[i];
+    __syncthreads();
+    if (threadIdx.x >= 4) return;
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += part[w][threadIdx.x];
+    const int at = c + (int)threadIdx.x;
+    (at < D ? dq_weight : dk_weight)[at % D] = (T)(float)total;
 }
 
 constexpr const char *kWhat = "rotation";
@@ -320,9 +375,10 @@ int problem_of(const fg_rotate_args *a, Problem *p) {
     return FG_OK;
 }
 
-// Workgroups of the gradients: eight wavefronts a SIMD at most, which go on from token to token.
-int backward_grid(const Problem &p) {
-    return (int)std::min<int64_t>(1024, ((int64_t)p.batch * p.tokens * p.parts + kWaves - 1) / kWaves);
+// Workgroups of the gradients: as many as the card holds at a time, which go on from token to token.
+int backward_grid(const Problem &p, const fg_rotate_args *a) {
+    const int64_t most = 256 * (a->q_weight && a->type != FG_TYPE_F32 ? kResident<__bf16, true> : kResident<float, true>);
+    return (int)std::min(most, ((int64_t)p.batch * p.tokens * p.parts + kWaves - 1) / kWaves);
 }
 
 template <typename F> int by_shape(const fg_rotate_args *a, F f) {
@@ -366,7 +422,7 @@ extern "C" int fg_rotate_heads(const fg_rotate_args *args, void *stream) {
 extern "C" int64_t fg_rotate_heads_backward_workspace(const fg_rotate_args *args) {
     fg::rotate::Problem p;
     if (int rc = fg::rotate::problem_of(args, &p)) return rc;
-    return args->q_weight ? (int64_t)fg::rotate::backward_grid(p) * 2 * args->head_len * (int64_t)sizeof(float) : 0;
+    return args->q_weight ? (int64_t)fg::rotate::backward_grid(p, args) * 2 * args->head_len * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rotate_grads *grads, void *workspace, size_t workspace_bytes, void *stream) {
@@ -385,7 +441,7 @@ extern "C" int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rot
         (rc = block::aligned("the weights' gradients", grads->dk_weight, size, kWhat)) || (rc = block::aligned("the workspace", workspace, 16, kWhat))) return rc;
     const bool norm = args->q_weight;
     if (norm && (!grads->dq_weight || !grads->dk_weight)) return fail(FG_ERR_ARG, "rotation: null pointer");
-    const int rows = backward_grid(p);
+    const int rows = backward_grid(p, args);
     const size_t need = norm ? (size_t)rows * 2 * args->head_len * sizeof(float) : 0;
     if (workspace_bytes < need || (need && !workspace))
         return fail(FG_ERR_ARG, "rotation: a workspace of %zu bytes, %zu needed (fg_rotate_heads_backward_workspace)", workspace_bytes, need);
@@ -397,7 +453,7 @@ extern "C" int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rot
         constexpr bool NORM = decltype(with_norm)::value;
         if (rows) rotate_backward_kernel<T, D, NORM><<<dim3((unsigned)rows), dim3(kThreads), 0, s>>>(p, g);
         FG_HIP_TRY(hipGetLastError());
-        if (NORM) weights_kernel<T, D><<<dim3(2 * D / 16), dim3(kThreads), 0, s>>>(g.sums, rows, static_cast<T *>(grads->dq_weight), static_cast<T *>(grads->dk_weight));
+        if (NORM) weights_kernel<T, D><<<dim3(2 * D / 4), dim3(kThreads), 0, s>>>(g.sums, rows, static_cast<T *>(grads->dq_weight), static_cast<T *>(grads->dk_weight));
         FG_HIP_TRY(hipGetLastError());
         return FG_OK;
     });

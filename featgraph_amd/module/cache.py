@@ -120,9 +120,22 @@ assert ctypes.sizeof(_lib.FgCacheAttentionArgs) == _HEAD.size + _CACHE.size + _R
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace(head, cache_sizes):
-    """Device memory that a call of these sizes needs."""
-    return _lib.check(_lib.lib().fg_cache_attention_workspace(head + _CACHE.pack(*cache_sizes, 0, 0, 0, 0) + bytes(_REST.size)))
+def _plan(dtype, queries, heads, causal, block, topk, scale, *cache_sizes):
+    """(the part of a call's arguments that goes by its sizes, the device memory that it needs)."""
+    head = _HEAD.pack(_TYPES[dtype], queries, heads, causal, block, topk, scale)
+    return head, _lib.check(_lib.lib().fg_cache_attention_workspace(head + _CACHE.pack(*cache_sizes, 0, 0, 0, 0) + bytes(_REST.size)))
+
+
+def _check_blocks(blocks, block_size, batch, queries, cache):
+    if blocks is None or block_size is None:
+        raise ValueError("blocks and block_size come together")
+    _check_sizes(cache.head_len, block_size)
+    if not isinstance(blocks, torch.Tensor):
+        raise TypeError("blocks must be a torch tensor, got %s" % type(blocks))
+    if blocks.dtype != torch.int32 or blocks.device != cache.device or blocks.dim() != 4 or tuple(blocks.shape[:3]) != (batch, queries, cache.kv_heads) \
+            or blocks.shape[3] < 1:
+        raise ValueError("blocks must be int32 (%d, %d, %d, topk) on %s, got %s of %s on %s"
+                         % (batch, queries, cache.kv_heads, cache.device, tuple(blocks.shape), blocks.dtype, blocks.device))
 
 
 def attention(q, cache, blocks, block_size, scale, causal, lengths, q_lengths):
@@ -130,30 +143,21 @@ def attention(q, cache, blocks, block_size, scale, causal, lengths, q_lengths):
     _check("q", q, 4)
     batch, queries, heads, head_len = q.shape
     device = q.device
-    if (batch, head_len) != (cache.batch, cache.head_len) or device != cache.device:
+    if batch != cache.batch or head_len != cache.head_len or device != cache.device:
         raise ValueError("q must be (%d, queries, heads, %d) on %s as the cache is, got %s on %s"
                          % (cache.batch, cache.head_len, cache.device, tuple(q.shape), device))
     if heads % cache.kv_heads or not 1 <= heads // cache.kv_heads <= MAX_GROUP:
         raise ValueError("%d query heads over %d key heads: 1 to %d of the former to each of the latter" % (heads, cache.kv_heads, MAX_GROUP))
-    if (blocks is None) != (block_size is None):
-        raise ValueError("blocks and block_size come together")
     topk = 0
-    if blocks is not None:
-        _check_sizes(head_len, block_size)
-        if not isinstance(blocks, torch.Tensor):
-            raise TypeError("blocks must be a torch tensor, got %s" % type(blocks))
-        if blocks.dtype != torch.int32 or blocks.device != device or blocks.dim() != 4 or tuple(blocks.shape[:3]) != (batch, queries, cache.kv_heads) \
-                or blocks.shape[3] < 1:
-            raise ValueError("blocks must be int32 (%d, %d, %d, topk) on %s, got %s of %s on %s"
-                             % (batch, queries, cache.kv_heads, device, tuple(blocks.shape), blocks.dtype, blocks.device))
+    if blocks is not None or block_size is not None:
+        _check_blocks(blocks, block_size, batch, queries, cache)
         blocks, topk = blocks.contiguous(), blocks.shape[3]
     _check_counts("lengths", lengths, batch, device)
     _check_counts("q_lengths", q_lengths, batch, device)
-    scale = head_len ** -0.5 if scale is None else float(scale)
     q = _rows(q)
+    head, need = _plan(q.dtype, queries, heads, causal, block_size or 0, topk, head_len ** -0.5 if scale is None else float(scale), cache.bits, batch,
+                       cache.keys, cache.kv_heads, head_len)
     out = torch.empty((batch, queries, heads, head_len), dtype=q.dtype, device=device)
-    head = _HEAD.pack(_TYPES[q.dtype], queries, heads, causal, block_size or 0, topk, scale)
-    need = _workspace(head, (cache.bits, batch, cache.keys, cache.kv_heads, head_len))
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     raw = head + cache.raw() + _REST.pack(q.data_ptr(), *q.stride()[:3], _ptr(blocks), _ptr(lengths), _ptr(q_lengths), out.data_ptr())
     _lib.check(_call(device, lambda L, stream: L.fg_cache_attention(raw, _ptr(work), need, stream)))

@@ -133,7 +133,7 @@ SIGNATURES = {
     "fg_rotate_heads": (_int, [_vp, _vp]),
     "fg_rotate_heads_backward_workspace": (_i64, [_vp]),
     "fg_rotate_heads_backward": (_int, [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
-    "fg_cache_write": (_int, [_vp, _int, _vp, ctypes.POINTER(_i64), _vp, ctypes.POINTER(_i64), _int, _vp, _vp, _vp]),
+    "fg_cache_write": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp]),
     "fg_cache_read": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp]),
     "fg_cache_attention_workspace": (_i64, [_vp]),
     "fg_cache_attention": (_int, [_vp, _vp, ctypes.c_size_t, _vp]),

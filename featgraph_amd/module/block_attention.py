@@ -66,6 +66,17 @@ def _call(device, f):
         return f(_lib.lib(), common.stream_ptr())
 
 
+def _launch(device, function, *args):
+    """function(*args, current stream) of the library with `device` current, its status checked."""
+    if torch.cuda.current_device() == device.index:
+        status = function(*args, common.stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            status = function(*args, common.stream_ptr())
+    if status < 0:
+        _lib.check(status)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 

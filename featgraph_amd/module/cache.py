@@ -12,7 +12,7 @@ import struct
 import torch
 
 from .. import _lib
-from .block_attention import _TYPES, HEAD_LENGTHS, MAX_GROUP, _call, _check, _check_counts, _check_sizes, _ptr, _rows, _strides
+from .block_attention import _TYPES, HEAD_LENGTHS, MAX_GROUP, _check, _check_counts, _check_sizes, _launch, _ptr, _rows
 
 GROUP = 32                                 # elements of one scale
 
@@ -78,39 +78,54 @@ def _check_cache(cache):
         raise TypeError("cache must be a KeyValueCache, got %s" % type(cache))
 
 
-def write(cache, k, v, lengths, q_lengths):
+def _check_write(cache, k, v):
     _check_cache(cache)
     _check("k", k, 4)
     _check("v", v, 4, k)
-    batch, tokens, kv_heads, head_len = k.shape
-    if k.shape != v.shape or (batch, kv_heads, head_len) != (cache.batch, cache.kv_heads, cache.head_len):
+    if k.shape != v.shape or (k.shape[0], k.shape[2], k.shape[3]) != (cache.batch, cache.kv_heads, cache.head_len):
         raise ValueError("k and v must be (%d, tokens, %d, %d) as the cache is, got %s and %s"
                          % (cache.batch, cache.kv_heads, cache.head_len, tuple(k.shape), tuple(v.shape)))
     if k.device != cache.device:
         raise ValueError("k is on %s, the cache on %s" % (k.device, cache.device))
-    _check_counts("lengths", lengths, batch, k.device)
-    _check_counts("q_lengths", q_lengths, batch, k.device)
+
+
+_STRIDES = struct.Struct("=3q")
+
+
+def write(cache, k, v, lengths, q_lengths):
+    try:                                    # whether the arguments are fine as they are, at a glance; what is not is looked at one by one for the message
+        batch, tokens, kv_heads, head_len = k.shape
+        plain = (v.shape == k.shape and k.dtype in _TYPES and v.dtype == k.dtype and k.device == cache.device and v.device == cache.device
+                 and batch == cache.batch and kv_heads == cache.kv_heads and head_len == cache.head_len)
+    except (AttributeError, ValueError, TypeError):
+        plain = False
+    if not plain:
+        _check_write(cache, k, v)
+    device = cache.device
+    if lengths is not None:
+        _check_counts("lengths", lengths, batch, device)
+    if q_lengths is not None:
+        _check_counts("q_lengths", q_lengths, batch, device)
     if tokens > cache.keys and (lengths is None or q_lengths is None):
         raise ValueError("%d new tokens for a cache of %d keys" % (tokens, cache.keys))
     k, v = _rows(k), _rows(v)
-    raw = cache.raw()
-    _lib.check(_call(k.device, lambda L, stream: L.fg_cache_write(
-        raw, _TYPES[k.dtype], k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), tokens, _ptr(lengths), _ptr(q_lengths), stream)))
+    _launch(device, _lib.lib().fg_cache_write, cache.raw(), _TYPES[k.dtype], k.data_ptr(), _STRIDES.pack(*k.stride()[:3]), v.data_ptr(),
+            _STRIDES.pack(*v.stride()[:3]), tokens, _ptr(lengths), _ptr(q_lengths))
 
 
 def read(cache, dtype, first, count, lengths):
     _check_cache(cache)
     if dtype not in _TYPES:
         raise ValueError("values are read as float32, float16 or bfloat16, got %s" % (dtype,))
-    _check_counts("first", first, cache.batch, cache.device)
-    _check_counts("lengths", lengths, cache.batch, cache.device)
+    device = cache.device
+    _check_counts("first", first, cache.batch, device)
+    _check_counts("lengths", lengths, cache.batch, device)
     count = cache.keys if count is None else count
     if count < 0:
         raise ValueError("%d keys to read" % count)
-    k, v = (torch.empty((cache.batch, count, cache.kv_heads, cache.head_len), dtype=dtype, device=cache.device) for _ in "kv")
-    raw = cache.raw()
-    _lib.check(_call(cache.device, lambda L, stream: L.fg_cache_read(
-        raw, _TYPES[dtype], k.data_ptr(), v.data_ptr(), count, _ptr(first), _ptr(lengths), stream)))
+    shape = (cache.batch, count, cache.kv_heads, cache.head_len)
+    k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    _launch(device, _lib.lib().fg_cache_read, cache.raw(), _TYPES[dtype], k.data_ptr(), v.data_ptr(), count, _ptr(first), _ptr(lengths))
     return k, v
 
 
@@ -138,27 +153,40 @@ def _check_blocks(blocks, block_size, batch, queries, cache):
                          % (batch, queries, cache.kv_heads, cache.device, tuple(blocks.shape), blocks.dtype, blocks.device))
 
 
-def attention(q, cache, blocks, block_size, scale, causal, lengths, q_lengths):
+def _check_attention(q, cache):
     _check_cache(cache)
     _check("q", q, 4)
     batch, queries, heads, head_len = q.shape
-    device = q.device
-    if batch != cache.batch or head_len != cache.head_len or device != cache.device:
+    if batch != cache.batch or head_len != cache.head_len or q.device != cache.device:
         raise ValueError("q must be (%d, queries, heads, %d) on %s as the cache is, got %s on %s"
-                         % (cache.batch, cache.head_len, cache.device, tuple(q.shape), device))
+                         % (cache.batch, cache.head_len, cache.device, tuple(q.shape), q.device))
     if heads % cache.kv_heads or not 1 <= heads // cache.kv_heads <= MAX_GROUP:
         raise ValueError("%d query heads over %d key heads: 1 to %d of the former to each of the latter" % (heads, cache.kv_heads, MAX_GROUP))
+
+
+def attention(q, cache, blocks, block_size, scale, causal, lengths, q_lengths):
+    try:
+        batch, queries, heads, head_len = q.shape
+        dtype, device = q.dtype, q.device
+        plain = (batch == cache.batch and head_len == cache.head_len and device == cache.device and dtype in _TYPES and not heads % cache.kv_heads
+                 and 1 <= heads // cache.kv_heads <= MAX_GROUP)
+    except (AttributeError, ValueError, TypeError):
+        plain = False
+    if not plain:
+        _check_attention(q, cache)
     topk = 0
     if blocks is not None or block_size is not None:
         _check_blocks(blocks, block_size, batch, queries, cache)
         blocks, topk = blocks.contiguous(), blocks.shape[3]
-    _check_counts("lengths", lengths, batch, device)
-    _check_counts("q_lengths", q_lengths, batch, device)
+    if lengths is not None:
+        _check_counts("lengths", lengths, batch, device)
+    if q_lengths is not None:
+        _check_counts("q_lengths", q_lengths, batch, device)
     q = _rows(q)
-    head, need = _plan(q.dtype, queries, heads, causal, block_size or 0, topk, head_len ** -0.5 if scale is None else float(scale), cache.bits, batch,
+    head, need = _plan(dtype, queries, heads, causal, block_size or 0, topk, head_len ** -0.5 if scale is None else float(scale), cache.bits, batch,
                        cache.keys, cache.kv_heads, head_len)
-    out = torch.empty((batch, queries, heads, head_len), dtype=q.dtype, device=device)
+    out = q.new_empty(q.shape)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     raw = head + cache.raw() + _REST.pack(q.data_ptr(), *q.stride()[:3], _ptr(blocks), _ptr(lengths), _ptr(q_lengths), out.data_ptr())
-    _lib.check(_call(device, lambda L, stream: L.fg_cache_attention(raw, _ptr(work), need, stream)))
+    _launch(device, _lib.lib().fg_cache_attention, raw, _ptr(work), need)
     return out

@@ -11,7 +11,7 @@ import struct
 import torch
 
 from .. import _lib
-from .block_attention import _TYPES, HEAD_LENGTHS, _call, _check, _check_counts, _ptr, _rows
+from .block_attention import _TYPES, HEAD_LENGTHS, _check, _check_counts, _launch, _ptr, _rows
 
 MAX_AXES = 8
 
@@ -67,8 +67,22 @@ def _plan(dtype, q_shape, k_shape, normed, base, frequencies, sections, rotary_l
     return _Plan(len(sections), sizes + _ANGLES.pack(*[f / (2 * math.pi) for f in frequencies], *none, *axis, *none))
 
 
-def check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequencies, sections, rotary_len, interleaved, eps):
-    """The call's plan, after everything that can be seen of its arguments without looking at their values on the GPU."""
+def _plain(q, k, q_weight, k_weight):
+    """Whether types and devices are fine as they are, at a glance; what is not is looked at one by one for the message."""
+    try:
+        dtype, device = q.dtype, q.device
+        if dtype not in _TYPES or k.dtype != dtype or device.type != "cuda" or k.device != device:
+            return False
+        if q_weight is None or k_weight is None:
+            return q_weight is k_weight
+        shape = q.shape[3:]
+        return (q_weight.shape == shape and k_weight.shape == shape and q_weight.dtype == dtype and k_weight.dtype == dtype
+                and q_weight.device == device and k_weight.device == device)
+    except AttributeError:
+        return False
+
+
+def _check_tensors(q, k, q_weight, k_weight):
     _check("q", q, 4)
     _check("k", k, 4, q)
     if (q_weight is None) != (k_weight is None):
@@ -78,6 +92,12 @@ def check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequen
             _check(name, w, 1, q)
             if w.shape[0] != q.shape[3]:
                 raise ValueError("%s must be (%d,), got %s" % (name, q.shape[3], tuple(w.shape)))
+
+
+def check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequencies, sections, rotary_len, interleaved, eps):
+    """The call's plan, after everything that can be seen of its arguments without looking at their values on the GPU."""
+    if not _plain(q, k, q_weight, k_weight):
+        _check_tensors(q, k, q_weight, k_weight)
     # a tuple can be looked up
     if frequencies is not None and type(frequencies) is not tuple:
         frequencies = tuple(float(x) for x in frequencies)
@@ -111,7 +131,7 @@ def _vector(w):
 
 
 def _new(t):
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return t.new_empty(t.shape)
 
 
 _NOTHING = (0, 0, 0)
@@ -129,7 +149,7 @@ def forward(q, k, q_weight, k_weight, plan, positions, lengths, q_lengths):
     positions = None if positions is None else positions.contiguous()
     q_out, k_out = _new(q), _new(k)
     raw = _arguments(plan, q, k, q_weight, k_weight, positions, lengths, q_lengths, q_out, k_out)
-    _lib.check(_call(q.device, lambda L, stream: L.fg_rotate_heads(raw, stream)))
+    _launch(q.device, _lib.lib().fg_rotate_heads, raw)
     return q_out, k_out
 
 
@@ -146,5 +166,5 @@ def backward(q, k, q_weight, k_weight, plan, positions, lengths, q_lengths, dq_o
                         _ptr(dq_weight), _ptr(dk_weight))
     need = plan.workspace(raw)
     work = torch.empty(need, dtype=torch.uint8, device=dq.device) if need else None
-    _lib.check(_call(dq.device, lambda L, stream: L.fg_rotate_heads_backward(raw, grads, _ptr(work), need, stream)))
+    _launch(dq.device, _lib.lib().fg_rotate_heads_backward, raw, grads, _ptr(work), need)
     return dq, dk, dq_weight, dk_weight

@@ -138,11 +138,95 @@ template <typename T> __device__ __forceinline__ void parts_of(const T *src, bf1
     }
 }
 
+// The queries of a lane's column as operands: D / 32 times eight elements, the first of the n-th from element_of(n) on.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void load_queries(const Problem &p, int b, int t, int head, bool there, bf16x8 (&q)[kQueryParts<T>][D / 32], F element_of) {
+    const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+        if (there && p.scale2 != 0.f) {
+            parts_of<T>(src + element_of(n), &q[0][n], D / 32);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kQueryParts<T>; ++j) q[j][n] = zero8<__bf16>();
+        }
+        if (p.scale2 < 0.f)
+#pragma unroll
+            for (int j = 0; j < kQueryParts<T>; ++j) q[j][n] = -q[j][n];
+    }
+}
+// Scores are compared before they are scaled: a negative scale turns the queries' signs instead, and one of 0 takes the queries away.
+__device__ __forceinline__ float factor_of(const Problem &p) { return p.scale2 == 0.f ? 1.f : fabsf(p.scale2); }
+
+// Last key that a lane's row may see; columns that no row of the result belongs to see everything, so that they do not keep a tile from skipping its masks.
+__device__ __forceinline__ int limit_of(const Problem &p, bool used, int t, int q_len, int k_len) {
+    if (!used || t >= p.queries) return k_len - 1;
+    return t >= q_len ? -1 : p.causal ? min(k_len - q_len + t, k_len - 1) : k_len - 1;
+}
+
+// One row's softmax: scores are relative to `m`, its sum is `l`, `lost` the parts of 32 elements that are NaN.
+template <int D> struct Row {
+    float m, l;
+    unsigned lost;
+    f32x4 o[D / 16];
+    __device__ __forceinline__ void clear() {
+        m = -__builtin_inff(); l = 0.f; lost = 0;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // 32 keys: scores s of keys key0 + 16 kt + 4 g + i, of which the row sees those up to `last`, become the parts of their powers.
+    template <int NP> __device__ __forceinline__ void weigh(f32x4 (&s)[2], int key0, int g, int last, float factor, bf16x8 (&part)[NP]) {
+        if (!__all(key0 + kUnit - 1 <= last))
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[kt][i] = key0 + 16 * kt + 4 * g + i <= last ? s[kt][i] : -__builtin_inff();
+        const float top = fmaxf(m, largest_of_rows(largest(s[0], s[1])) * factor);
+        const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
+        if (__any(top != m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - ref);
+            l *= shrink;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) o[dt] *= shrink;
+            m = top;
+        }
+        f32x4 z[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], factor, -ref));
+        l += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            part[j] = pack<__bf16>(z[0], z[1]);
+            if (j + 1 < NP)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { z[0][i] -= (float)part[j][i]; z[1][i] -= (float)part[j][4 + i]; }
+        }
+    }
+    // Marks of 32 keys, a byte each.
+    __device__ __forceinline__ void mark(const uint8_t *marks, int key0, int g, int last) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = 16 * (i >> 2) + 4 * g + (i & 3);
+            lost |= key0 + key <= last ? marks[key] : 0u;
+        }
+    }
+    __device__ __forceinline__ void lose() {
+        if (!__any(lost != 0)) return;
+        unsigned bad = lost | __shfl_xor(lost, 16);
+        bad |= __shfl_xor(bad, 32);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+            if (bad >> (dt / 2) & 1) o[dt] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+    }
+};
+
 constexpr int kListed = 1024;          // blocks listed at a time
 struct NoList {};
 
 // Wavefronts of a SIMD that registers are left for: 128, 168 or 256 each.
-template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 : sizeof(T) == 4 ? 2 : (BITS == 4 ? 4 : 3) - LISTED;
+template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 : sizeof(T) == 4 ? 2 : (BITS == 4 && std::is_same<T, __bf16>::value ? 4 : 3) - LISTED;
 // Most tiles of 16 rows that a workgroup takes.
 template <typename T, int D> constexpr int kMostTiles = sizeof(T) == 4 && D == 128 ? 1 : 2;
 
@@ -174,42 +258,20 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
 
     __bf16 *stage = reinterpret_cast<__bf16 *>(dynamic) + wave * kUnit * (D + kPad);
     const Rows<D, BITS> keys(held.k, held.k_scales, pair, p.keys), vals(held.v, held.v_scales, pair, p.keys);
-    // scores are compared before they are scaled: a negative scale turns the queries' signs instead, and one of 0 takes the queries away
-    const float factor = p.scale2 == 0.f ? 1.f : fabsf(p.scale2);
+    const float factor = factor_of(p);
     bf16x8 qf[RT][NQ][DC];
-    int limit[RT];                     // last key that the lane's row may see; columns without a row see everything, nothing is written of them
-    unsigned lost[RT];                 // parts of 32 elements of the lane's row that are NaN
+    int limit[RT];
+    Row<D> row[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int t = t0 + rt * tpt + tc;
-        const bool there = used && t < q_len;
-        limit[rt] = there ? (p.causal ? min(offset + t, k_len - 1) : k_len - 1) : used ? -1 : k_len - 1;
-        lost[rt] = 0;
-        const T *src = static_cast<const T *>(p.q) + b * p.qs.batch + (int64_t)t * p.qs.row + head * p.qs.head;
-#pragma unroll
-        for (int n = 0; n < DC; ++n) {
-            if (there && p.scale2 != 0.f) {
-                parts_of<T>(src + Layout<D, BITS>::element(n, g), &qf[rt][0][n], DC);
-            } else {
-#pragma unroll
-                for (int j = 0; j < NQ; ++j) qf[rt][j][n] = zero8<__bf16>();
-            }
-            if (p.scale2 < 0.f)
-#pragma unroll
-                for (int j = 0; j < NQ; ++j) qf[rt][j][n] = -qf[rt][j][n];
-        }
+        limit[rt] = limit_of(p, used, t, q_len, k_len);
+        row[rt].clear();
+        load_queries<T, D>(p, b, t, head, used && t < q_len, qf[rt], [&](int n) { return Layout<D, BITS>::element(n, g); });
     }
     const int last_key = p.causal ? min(k_len - 1, offset + min(t0 + RT * tpt, q_len) - 1) : k_len - 1;
     const int sub_shift = LISTED ? p.block_shift - 5 : 0, stride = kWaves * splits;
 
-    f32x4 o[RT][DT];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__builtin_inff(); l[rt] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
     auto window = [&](int first, int units) {
         auto first_key = [&](int u) {
             if constexpr (LISTED) return __builtin_amdgcn_readfirstlane(((first + list.id[u >> sub_shift]) << p.block_shift) + ((u & ((1 << sub_shift) - 1)) << 5));
@@ -235,7 +297,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
             const int key0 = step.key0;
             int last[RT];              // keys that the lane's row sees: key0 + 16 kt + 4 g + i <= last
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) last[rt] = !LISTED || !used || (who[rt] >> tc) & 1 ? limit[rt] : -1;
+            for (int rt = 0; rt < RT; ++rt) last[rt] = !LISTED || !used || t0 + rt * tpt + tc >= p.queries || (who[rt] >> tc) & 1 ? limit[rt] : -1;
             wave_lds_sync();
             const bool odd = step.odd();
             if (__any(odd)) step.clear(marks[wave], lane);
@@ -260,39 +322,8 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
             bf16x8 pf[RT][NP];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                if (!__all(key0 + kUnit - 1 <= last[rt]))
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[rt][kt][i] = key0 + 16 * kt + 4 * g + i <= last[rt] ? s[rt][kt][i] : -__builtin_inff();
-                if (__any(odd))
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int key = 16 * (i >> 2) + 4 * g + (i & 3);
-                        lost[rt] |= key0 + key <= last[rt] ? marks[wave][key] : 0u;
-                    }
-                const float top = fmaxf(m[rt], largest_of_rows(largest(s[rt][0], s[rt][1])) * factor);
-                const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
-                if (__any(top != m[rt])) {
-                    const float shrink = __builtin_amdgcn_exp2f(m[rt] - ref);
-                    l[rt] *= shrink;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= shrink;
-                    m[rt] = top;
-                }
-                f32x4 z[2];
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) z[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][kt][i], factor, -ref));
-                l[rt] += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
-#pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    pf[rt][j] = pack<__bf16>(z[0], z[1]);
-                    if (j + 1 < NP)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) { z[0][i] -= (float)pf[rt][j][i]; z[1][i] -= (float)pf[rt][j][4 + i]; }
-                }
+                row[rt].weigh(s[rt], key0, g, last[rt], factor, pf[rt]);
+                if (__any(odd)) row[rt].mark(marks[wave], key0, g, last[rt]);
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
@@ -300,7 +331,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int j = 0; j < NP; ++j) o[rt][dt] = mma(vf, pf[rt][j], o[rt][dt]);
+                    for (int j = 0; j < NP; ++j) row[rt].o[dt] = mma(vf, pf[rt][j], row[rt].o[dt]);
             }
         }
     };
@@ -317,15 +348,9 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
     const int64_t all_rows = (int64_t)p.batch * p.queries * p.heads;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = rows_sum(l[rt]);
-        if (__any(lost[rt] != 0)) {
-            unsigned bad = lost[rt] | __shfl_xor(lost[rt], 16);
-            bad |= __shfl_xor(bad, 32);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                if (bad >> (dt / 2) & 1) o[rt][dt] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        }
-        if (g == 0) stats[wave][c] = make_float2(m[rt], sum);
+        const float sum = rows_sum(row[rt].l);
+        row[rt].lose();
+        if (g == 0) stats[wave][c] = make_float2(row[rt].m, sum);
         __syncthreads();               // the values' staging, or the joining buffer of the tile before, has been read
         float top = -__builtin_inff(), total = 0.f;
 #pragma unroll
@@ -333,23 +358,23 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
         const float ref = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) total += stats[w][c].y * __builtin_amdgcn_exp2f(stats[w][c].x - ref);
-        const float share = __builtin_amdgcn_exp2f(m[rt] - ref);
+        const float share = __builtin_amdgcn_exp2f(row[rt].m - ref);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(merge + wave * kMergeWave<D> + c * kMergeRow<D> + 16 * dt + 4 * g) = o[rt][dt] * share;
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(merge + wave * kMergeWave<D> + c * kMergeRow<D> + 16 * dt + 4 * g) = row[rt].o[dt] * share;
         if (wave == 0 && g == 0) joined[c] = make_float2(top, total);
         __syncthreads();
 #pragma unroll
         for (int item = tid / SHARE; item < ITEMS; item += STEP) {
-            const int row = item / (D / 4), col = item % (D / 4) * 4, at_token = row / p.group, t = t0 + rt * tpt + at_token;
+            const int r16 = item / (D / 4), col = item % (D / 4) * 4, at_token = r16 / p.group, t = t0 + rt * tpt + at_token;
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = tid % SHARE; w < kWaves; w += SHARE) v += *reinterpret_cast<const f32x4 *>(merge + w * kMergeWave<D> + row * kMergeRow<D> + col);
+            for (int w = tid % SHARE; w < kWaves; w += SHARE) v += *reinterpret_cast<const f32x4 *>(merge + w * kMergeWave<D> + r16 * kMergeRow<D> + col);
             if constexpr (SHARE > 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += dpp_move<0xB1>(v[i]);        // two threads (heads of 32)
             if (tid % SHARE || at_token >= tpt || t >= p.queries) continue;
-            const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (row - at_token * p.group);
-            const float2 st = joined[row];
+            const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (r16 - at_token * p.group);
+            const float2 st = joined[r16];
             if (splits == 1) {
                 store_row<T>(static_cast<T *>(r.out), nullptr, at * D + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
             } else {
@@ -395,7 +420,7 @@ __global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part
 }
 
 // How a call's work is cut: where there are too few workgroups for the card, several share a row's keys out.  512 workgroups (two a CU) as long as each
-// has eight steps of 32 keys, 256 as long as each wavefront has one; rows of up to 512 keys stay whole, for joining takes a launch of 3.5 us.
+// has eight steps of 32 keys for every tile, 256 as long as each wavefront has one; rows of up to 512 keys stay whole, for joining takes a launch of 3.5 us.
 // Kernel and joining (us), shares as the rule has them / half / twice as many: 1 sequence of 8 key heads x 128, 4 bits, 32,768 keys (64 shares) 14.1 / 15.1 / 15.9, 8,192 keys (32) 8.6 / 10.6 /
 // 9.1; 8 sequences of 4,096 (8) 13.6 / 15.3 / 14.3; 32 of 32,768 (2) 199 / 260 / 206; 1 of 2,048 x 8 heads x 64, 8 bits (16) 7.2 / 7.8 / 7.3; 3 tokens
 // of 8 sequences, 16 blocks of 64 each (8) 10.9 / 12.4 / 11.9; 512 keys (1) 7.1, in four shares 7.1.
@@ -403,13 +428,14 @@ __global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part
 // lists, whose unions grow.
 struct Shape { int tiles, n_groups, splits; };
 Shape shape_of(const Problem &p, int most_tiles) {
-    const int tiles = !p.topk && p.queries > tile_tokens(p.group) ? most_tiles : 1, tokens = tiles * tile_tokens(p.group);
+    const int tpt = tile_tokens(p.group);
+    const int tiles = !p.topk && p.queries > tpt ? most_tiles : 1, tokens = tiles * tpt;
     Shape s{tiles, (int)(((int64_t)p.queries + tokens - 1) / tokens), 1};
     const int64_t groups = std::max<int64_t>((int64_t)p.batch * p.kv_heads * s.n_groups, 1);
     int64_t units = ((int64_t)p.keys + kUnit - 1) / kUnit;
     if (p.topk) units = std::min<int64_t>(units, ((int64_t)p.topk * std::min(tokens, p.queries)) << (p.block_shift - 5));
     if (units > 4 * kWaves)
-        s.splits = (int)std::max<int64_t>(1, std::max(std::min({512 / groups, units / (2 * kWaves), (int64_t)kMostSplits}),
+        s.splits = (int)std::max<int64_t>(1, std::max(std::min({512 / groups, units / (2 * kWaves * s.tiles), (int64_t)kMostSplits}),
                                                       std::min({256 / groups, units / kWaves, (int64_t)kMostSplits})));
     return s;
 }

@@ -98,29 +98,34 @@ template <int L> __device__ __forceinline__ float lanes_sum(float v) {
     else return group_sum<L>(v);
 }
 
-// 1 / sqrt(mean(x^2) + eps) over a head's lanes.  Squares that leave the range of 32 bits are taken again of smaller numbers.
+// 1 / sqrt(mean(x^2) + eps) over a head's lanes.  Where squares leave the range of 32 bits the elements are scaled by a power of two, `by`, first, in
+// place: the result is that of the scaled ones, and `by` times it that of the elements.
 template <typename T, int D>
-__device__ __forceinline__ float inverse_rms(const float (&a)[Piece<T>::N], const float (&b)[Piece<T>::N], float eps) {
+__device__ __forceinline__ float inverse_rms(float (&a)[Piece<T>::N], float (&b)[Piece<T>::N], float eps, float *by) {
     constexpr int E = Piece<T>::N;
-    float s = 0.f;
+    auto sum = [&]() {
+        float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += a[i] * a[i] + b[i] * b[i];
-    s = lanes_sum<Lane<T, D>::kLanes>(s);
-    float r = 1.f / sqrtf(s * (1.f / D) + eps);
-    if (__any(!(s < __builtin_inff()))) {
-        constexpr float DOWN = 0x1p-70f;
-        float t = 0.f;
+        for (int i = 0; i < E; ++i) s += a[i] * a[i] + b[i] * b[i];
+        return lanes_sum<Lane<T, D>::kLanes>(s);
+    };
+    *by = 1.f;
+    float s = sum();
+    // small squares are lost beside any eps that is not small itself
+    const bool large = !(s < __builtin_inff()), small = s < 0x1p-100f && eps < 0x1p-60f;
+    if (__any(large || small)) {
+        *by = large ? 0x1p-70f : small ? 0x1p60f : 1.f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) t += (a[i] * DOWN) * (a[i] * DOWN) + (b[i] * DOWN) * (b[i] * DOWN);
-        t = lanes_sum<Lane<T, D>::kLanes>(t);
-        if (!(s < __builtin_inff())) r = DOWN / sqrtf(t * (1.f / D));
+        for (int i = 0; i < E; ++i) { a[i] *= *by; b[i] *= *by; }
+        const float t = sum();
+        s = large || small ? t : s;    // the others keep their sum to the bit, whoever stands beside them
     }
-    return r;
+    return 1.f / sqrtf(s * (1.f / D) + eps * *by * *by);
 }
 
 // What a lane holds of a head, as it is stored.
 template <typename T> struct Pair {
-    typename Piece<T>::V a, b;
+    typename Piece<T>::V a = {}, b = {};
     __device__ __forceinline__ void load(const T *pa, const T *pb) {
         a = *reinterpret_cast<const typename Piece<T>::V *>(pa);
         b = *reinterpret_cast<const typename Piece<T>::V *>(pb);
@@ -190,7 +195,8 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const Problem p, T *q_
             if (NORM) {
                 float wa[E], wb[E];
                 weight.widen(wa, wb);
-                const float r = inverse_rms<T, D>(x, y, p.eps);
+                float by;
+                const float r = inverse_rms<T, D>(x, y, p.eps, &by);
 #pragma unroll
                 for (int e = 0; e < E; ++e) { x[e] = x[e] * r * wa[e]; y[e] = y[e] * r * wb[e]; }
             }
@@ -260,8 +266,8 @@ __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backwar
                     own_angles<T, D>(me, table[wave], cs);
                     turn<T, D>(p, me, cs, -1.f, ga, gb);
                     if (NORM) {
-                        const float r = inverse_rms<T, D>(x, y, p.eps);
-                        float wa[E], wb[E], dot = 0.f;
+                        float by, wa[E], wb[E], dot = 0.f;
+                        const float r = inverse_rms<T, D>(x, y, p.eps, &by);
                         weights[K].widen(wa, wb);
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
@@ -273,7 +279,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backwar
                         }
                         dot = lanes_sum<Lane<T, D>::kLanes>(dot) * (1.f / D);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) { ga[e] = (ga[e] - x[e] * dot) * r; gb[e] = (gb[e] - y[e] * dot) * r; }
+                        for (int e = 0; e < E; ++e) { ga[e] = (ga[e] - x[e] * dot) * r * by; gb[e] = (gb[e] - y[e] * dot) * r * by; }
                     }
                 } else {
 #pragma unroll

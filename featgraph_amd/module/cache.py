@@ -27,7 +27,8 @@ class KeyValueCache(object):
     k and v: uint8 (batch, kv_heads, keys, head_len * bits / 8), a head's elements in order, 4-bit ones the lower half of a byte first; k_scales and
     v_scales: uint8 (batch, kv_heads, keys, head_len / 32), the exponent plus 127 of the power of two that 32 neighbouring elements
     share (255: none of the 32 is a number).  Elements have a sign and two bits of exponent and one of mantissa (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6) or four and
-    three (e4m3, up to 448).  The tensors are the caller's: dense, on one GPU, at multiples of 16 bytes (scales of 4); zeros hold zeros."""
+    three (e4m3, up to 448; not its codes 127 and 255, which are no numbers).  Scales reach 2^125 and 2^119.  The tensors are the caller's: dense, on one GPU, at
+    multiples of 16 bytes (scales of 4); zeros hold zeros.  A cache's tensors are not replaced once it is made."""
     __slots__ = ("k", "k_scales", "v", "v_scales", "bits", "batch", "keys", "kv_heads", "head_len", "device")
 
     def __init__(self, k, k_scales, v, v_scales, bits):
@@ -52,8 +53,14 @@ class KeyValueCache(object):
                              % (tuple(k.shape), scales, tuple(v.shape), tuple(k_scales.shape), tuple(v_scales.shape)))
         if kv_heads < 1:
             raise ValueError("the cache has no heads: shape %s" % (tuple(k.shape),))
-        self.k, self.k_scales, self.v, self.v_scales, self.bits = k, k_scales, v, v_scales, bits
-        self.batch, self.keys, self.kv_heads, self.head_len, self.device = batch, keys, kv_heads, head_len, k.device
+        for name, value in zip(self.__slots__, (k, k_scales, v, v_scales, bits, batch, keys, kv_heads, head_len, k.device)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("a cache's %s is as it was made: make another KeyValueCache" % name)      # checked once, addressed by every call
+
+    def __reduce__(self):
+        return KeyValueCache, (self.k, self.k_scales, self.v, self.v_scales, self.bits)
 
     def raw(self):
         """fg_kv_cache as bytes."""
@@ -106,7 +113,7 @@ def write(cache, k, v, lengths, q_lengths):
         _check_counts("lengths", lengths, batch, device)
     if q_lengths is not None:
         _check_counts("q_lengths", q_lengths, batch, device)
-    if tokens > cache.keys and (lengths is None or q_lengths is None):
+    if tokens > cache.keys and lengths is None and q_lengths is None:
         raise ValueError("%d new tokens for a cache of %d keys" % (tokens, cache.keys))
     k, v = _rows(k), _rows(v)
     _launch(device, _lib.lib().fg_cache_write, cache.raw(), _TYPES[k.dtype], k.data_ptr(), _STRIDES.pack(*k.stride()[:3]), v.data_ptr(),

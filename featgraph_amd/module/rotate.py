@@ -100,9 +100,9 @@ def check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequen
         _check_tensors(q, k, q_weight, k_weight)
     # a tuple can be looked up
     if frequencies is not None and type(frequencies) is not tuple:
-        frequencies = tuple(float(x) for x in frequencies)
+        frequencies = tuple(frequencies)
     if sections is not None and type(sections) is not tuple:
-        sections = tuple(int(x) for x in sections)
+        sections = tuple(sections)
     plan = _plan(q.dtype, q.shape, k.shape, q_weight is not None, base, frequencies, sections, rotary_len, interleaved, eps)
     if positions is None and lengths is None and q_lengths is None and plan.axes == 1:
         return plan

@@ -717,8 +717,8 @@ int fg_rotate_heads_backward(const fg_rotate_args *args, const fg_rotate_grads *
 
 /*
  * K and V as (batch, kv_heads, keys, head_len) elements of 4 bits (e2m1: sign, two bits of exponent, one of mantissa; the lower half of a byte
- * first) or 8 (e4m3), and for every 32 neighbouring ones of a head a scale 2^(byte - 127): (batch, kv_heads, keys, head_len / 32) bytes.  All dense;
- * codes stand at multiples of 16 bytes, scales of 4.  Byte 255: all 32 are NaN.  (No counterpart in the reference.)
+ * first) or 8 (e4m3, but not its codes 127 and 255), and for every 32 neighbouring ones of a head a scale 2^(byte - 127): (batch, kv_heads, keys, head_len / 32) bytes.  All dense;
+ * codes stand at multiples of 16 bytes, scales of 4.  Scales are 2^125 and 2^119 at most.  Byte 255: all 32 are NaN.  (No counterpart in the reference.)
  */
 typedef struct {
     int32_t bits;                      /* 4 or 8 */

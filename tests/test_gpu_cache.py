@@ -139,6 +139,31 @@ def test_more_tokens_than_room_keep_the_last_ones():
     gen = torch.Generator().manual_seed(5)
     k, v = (torch.randn((2, 12, 1, 32), generator=gen).cuda() for _ in "kv")
     check_write(rubbish(2, 8, 1, 32, 8), k, v, ints(8, 4), ints(12, 7))
+    check_write(rubbish(2, 8, 1, 32, 4), k, v, ints(8, 4))
+    check_write(rubbish(2, 8, 1, 32, 4), k, v, None, ints(3, 0))
+
+
+def test_a_cache_stays_as_it_was_made():
+    import copy
+    from featgraph_amd import ops
+    cache = rubbish(1, 8, 1, 32, 4)
+    with pytest.raises(AttributeError, match="as it was made"):
+        cache.k = torch.zeros(1)
+    other = copy.deepcopy(cache)
+    x = torch.randn((1, 1, 1, 32), device="cuda")
+    before = parts(cache)
+    ops.write_cache(other, x, x)
+    assert all(np.array_equal(a, b) for a, b in zip(before, parts(cache))) and not np.array_equal(before[0], parts(other)[0])
+    for bad in (lambda: ops.KeyValueCache(cache.k[:, :, ::2], cache.k_scales, cache.v, cache.v_scales, 4), lambda: ops.KeyValueCache(cache.k, cache.k_scales, cache.v, cache.v_scales, 8),
+                lambda: ops.KeyValueCache(cache.k, cache.v, cache.v, cache.v_scales, 4), lambda: ops.KeyValueCache(cache.k.int(), cache.k_scales, cache.v, cache.v_scales, 4),
+                lambda: ops.write_cache(cache, x.expand(1, 9, 1, 32), x.expand(1, 9, 1, 32)), lambda: ops.write_cache(cache, x[..., :16], x[..., :16]),
+                lambda: ops.write_cache(cache, x, x.half()), lambda: ops.write_cache(cache, x, x, lengths=torch.ones(1, device="cuda")),
+                lambda: ops.write_cache(cache, x.expand(2, 1, 1, 32), x.expand(2, 1, 1, 32)), lambda: ops.read_cache(cache, torch.float64),
+                lambda: ops.read_cache(cache, count=-1), lambda: ops.read_cache(cache, first=ints(1, 2)), lambda: ops.write_cache(cache, x.cpu(), x.cpu())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        ops.write_cache(cache, x.clone().requires_grad_(), x)
 
 
 @pytest.mark.parametrize("bits", [4, 8])

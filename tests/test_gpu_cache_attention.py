@@ -215,6 +215,31 @@ def test_strides():
     assert torch.equal(ops.cache_attention(one, cache), ops.cache_attention(one.contiguous(), cache))
 
 
+def test_refusals():
+    from featgraph_amd import ops
+    q, cache, options = make(topk=2)
+    blocks = options["blocks"]
+    for bad in (lambda: ops.cache_attention(q[:, :, :3], cache), lambda: ops.cache_attention(q[..., :32], cache), lambda: ops.cache_attention(q[:1], cache),
+                lambda: ops.cache_attention(q[:, :, :0], cache), lambda: ops.cache_attention(q.cpu(), cache), lambda: ops.cache_attention(q.double(), cache),
+                lambda: ops.cache_attention(q[0], cache), lambda: ops.cache_attention(q, cache, blocks=blocks), lambda: ops.cache_attention(q, cache, block_size=32),
+                lambda: ops.cache_attention(q, cache, blocks=blocks, block_size=48), lambda: ops.cache_attention(q, cache, blocks=blocks.long(), block_size=32),
+                lambda: ops.cache_attention(q, cache, blocks=blocks[..., :0], block_size=32), lambda: ops.cache_attention(q, cache, blocks=blocks[:, :, :1], block_size=32),
+                lambda: ops.cache_attention(q, cache, lengths=ints(1)), lambda: ops.cache_attention(q, cache, q_lengths=ints(1, 1).long())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        ops.cache_attention(q, cache, blocks=[0, 1], block_size=32)
+    leaf = q.clone().requires_grad_()
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        ops.cache_attention(leaf, cache)
+    with torch.no_grad():
+        assert torch.equal(ops.cache_attention(leaf, cache), ops.cache_attention(q, cache))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.cache_attention(dual, cache)
+
+
 def test_offsets_beyond_32_bits():
     from featgraph_amd import ops
     keys = (1 << 26) + 77                   # 4.3 GB of codes in a head

@@ -140,10 +140,15 @@ def test_squares_beyond_32_bits(dtype):
     # x^2 overflows, the mean square of the scaled values does not; with eps = 0 a head's size does not matter
     s = make(dtype, seed=8)
     plain = step(s, eps=0.0)
-    for power in (2.0 ** 90, 2.0 ** -40):
+    for power in (2.0 ** 90, 2.0 ** -40, 2.0 ** -80, 2.0 ** -110):
         got = step(dict(s, q=s["q"] * power, k=s["k"] * power), eps=0.0)
         ref.check(got["q.y"], want(s, eps=0.0)["q.y"])
-        ref.check(got["k.dx"] * power, want(s, eps=0.0)["k.dx"])
+        ref.check(got["q.dw"], want(s, eps=0.0)["q.dw"])
+        ref.check(got["k.dx"].double() * power, want(s, eps=0.0)["k.dx"])
+    mixed = dict(s, q=s["q"] * torch.exp2(torch.tensor([-110.0, 0.0, 90.0, 3.0], device="cuda")).to(dtype)[:, None])      # side by side in a wavefront
+    ref.check(step(mixed, eps=0.0)["q.y"], want(s, eps=0.0)["q.y"])
+    tiny = step(dict(s, q=s["q"] * 2.0 ** -80))["q.y"]             # beside an eps of ordinary size: x w / sqrt(eps)
+    ref.check(tiny.double() * 2.0 ** 80, (want(dict(s, q=s["q"] * 2.0 ** -80))["q.y"][0] * 2.0 ** 80, want(dict(s, q=s["q"] * 2.0 ** -80))["q.y"][1] * 2.0 ** 80))
     assert not torch.isnan(plain["q.y"]).any()
 
 
@@ -214,6 +219,8 @@ def test_one_sided_gradients_and_second_ones():
     (grad,) = torch.autograd.grad(ops.rotate_heads(q, s["k"], *s["weights"])[0].square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+    with pytest.raises(TypeError):
+        ops.rotate_heads(s["q"], s["k"], sections=[16.5, 15.5], positions=torch.zeros((2, 9, 2), dtype=torch.int32, device="cuda"))
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(s["q"].contiguous(), torch.ones_like(s["q"].contiguous()))
         with pytest.raises(Exception):

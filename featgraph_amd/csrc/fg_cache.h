@@ -25,6 +25,7 @@ template <int D, int BITS> struct Rows {
     const uint8_t *codes, *scales;
     __device__ __forceinline__ Rows(const void *c, const void *s, int64_t head, int64_t keys)
         : codes(static_cast<const uint8_t *>(c) + head * keys * kBytes), scales(static_cast<const uint8_t *>(s) + head * keys * kScales) {}
+    __device__ __forceinline__ Rows(const Rows &r, int64_t key) : codes(r.codes + key * kBytes), scales(r.scales + key * kScales) {}     // from a key on
 };
 
 __device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }     // as the conversions read it: its exponent alone

@@ -2,7 +2,10 @@
 //   write:  for 32 neighbouring elements x of a head  e = the least power with which max |x| 2^-e rounds to at most the largest element (6 of e2m1,
 //           448 of e4m3), -127 <= e; codes = x 2^-e to the nearest element, ties to the even code.  A power of two divides without rounding, so that
 //           codes are the same on every machine that follows the rule.
-//   read:   code 2^e, rounded to the type (and no further than its largest number: an element may be up to 1 / 16 above the value it came from).
+//   read:   code 2^e, rounded to the type (float16: and no further than its largest number, for an element may be larger than the value it came from).
+//
+// What bounds them.  16,384 tokens of 8 heads of 128, K and V, bfloat16 and 4 bits (86 MB): written in 17.5 us, 4.9 TB/s, the rate of a large copy; read in
+// 14.2 us (6.0 TB/s, part of it from the Infinity Cache). One token each of 32 sequences 3.3 us, a launch.
 #include <algorithm>
 #include <limits>
 
@@ -27,7 +30,7 @@ struct Window {                        // tokens of a call and where they stand 
 
 // A thread takes kEach times eight elements of one head of K or V.  The D / 8 of a token follow one another, then the tokens of the head: codes are
 // written, and read, as whole lines.  2^lanes_shift threads share one of `parts` parts of a head, the others of a workgroup take other heads, so that an
-// index is divided once a thread (one division for every eight elements: 16,384 tokens of 8 x 128 written 21.8 us, read 20.5).
+// index is divided once a thread (with divisions for every eight elements, and these alone a thread's, 16,384 tokens of 8 x 128 are written in 21.8 us and read in 20.5).
 constexpr int kEach = 4;
 template <int D> struct Places {
     static constexpr int C = D / 8;

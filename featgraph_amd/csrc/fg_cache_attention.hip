@@ -5,13 +5,20 @@
 //
 // Every value of the cache is a bfloat16, so that products with it are bfloat16 products of the matrix cores, exact up to the sums in 32
 // bits, whatever type the queries have: a float16 is the sum of two bfloat16, a number of 32 bits of three.  Powers are taken apart the
-// same way, into two parts for 16-bit results (2^-17 of a power is lost) and three for 32-bit ones.
+// same way, each rounded to nearest: into two parts for 16-bit results (2^-18 of a power is lost) and three for 32-bit ones (2^-27).
 // Rows of one token's heads and of neighbouring tokens make tiles of 16, RT of them a workgroup.  Its four wavefronts deal the keys out among themselves, 32 at a
 // time, and where there are too few workgroups for the card so do several workgroups, whose sums are joined after.  A
 // lane's keys come from memory as operands lie in registers (the sum over a head's elements takes them in any order), values go
 // through LDS as bfloat16 to be read by columns; the next step is under way while one is worked on.
 // Values that are no numbers are taken as 0 and marked; the marks of the keys that a row sees make its result NaN.  (Keys that are none, and queries that
 // are not finite, make scores of their own rows alone.)
+//
+// What bounds it.  32 requests of 32,768 keys of 8 heads x 128 in 4 bits, one token of 32 heads each (1.14 GB): 198 us, 5.8 TB/s, above the rate of a large copy (5.1),
+// for it only reads; 128 registers leave room for four wavefronts a SIMD, which keep 17 KB each on their way. With a sweep of its own for values that are not finite in
+// the same kernel it took 276 registers and 353 us.  One request of 2,048 keys x 8 heads x 64: 7.1 us, of which 3.5 are the joining launch and the rest the chain
+// length, keys, softmax, joining. Many rows, 64 tokens over 16,384 keys of 8 x 128 in 8 bits: 44 us, 390 TFLOP/s counted once; with two tiles of rows two
+// wavefronts fit a SIMD, and each waits for its own chain scores, softmax, product.  (Four wavefronts that share the widened keys through LDS and take two tiles
+// each have the same chain, and barriers: 46 us, and 134 where this takes 116, 512 tokens over 8,192 keys.)
 #include <algorithm>
 #include <type_traits>
 
@@ -60,24 +67,28 @@ template <int D, int BITS> struct Step {
     uint32_t kw[2][Y::kKeyBytes / 4], vw[Y::kValueBytes / 4];
     unsigned ks[2][Y::kKeyChunks], vs[Y::kValueChunks];
 
-    // rows behind the last key read it again: what a padded cache holds there is never touched
+    // Rows behind the last key read it again: what a padded cache holds there is never touched.  Whole steps are addressed from one place for all lanes.
     __device__ __forceinline__ void fetch(const Rows<D, BITS> &k, const Rows<D, BITS> &v, int first, int k_len, int lane) {
-        const int g = lane >> 4, c = lane & 15;
         key0 = first;
+        const int64_t at = first;
+        if (first + kUnit <= k_len) fetch_rows(Rows<D, BITS>{k, at}, Rows<D, BITS>{v, at}, lane, [](int r) { return r; });
+        else fetch_rows(Rows<D, BITS>{k, at}, Rows<D, BITS>{v, at}, lane, [&](int r) { return min(r, k_len - 1 - first); });
+    }
+    template <typename F> __device__ __forceinline__ void fetch_rows(const Rows<D, BITS> k, const Rows<D, BITS> v, int lane, F row_of) {
+        const int g = lane >> 4, c = lane & 15;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const int64_t row = min(first + 16 * kt + c, k_len - 1);
+            const int row = row_of(16 * kt + c);
 #pragma unroll
             for (int j = 0; j < Y::kKeyChunks; ++j) {
-                load_words<Y::kKeyChunk>(k.codes + row * Y::kRow + (4 * j + g) * Y::kKeyChunk, kw[kt] + j * Y::kKeyChunk / 4);
+                load_words<Y::kKeyChunk>(k.codes + (row * Y::kRow + (4 * j + g) * Y::kKeyChunk), kw[kt] + j * Y::kKeyChunk / 4);
                 ks[kt][j] = k.scales[row * (D / kGroup) + (4 * j + g) * Y::kKeyElements / kGroup];
             }
         }
 #pragma unroll
         for (int j = 0; j < Y::kValueChunks; ++j) {
-            const int at = j * 64 + lane, col = at % Y::kPerRow;
-            const int64_t row = min(first + at / Y::kPerRow, k_len - 1);
-            load_words<Y::kValueChunk>(v.codes + row * Y::kRow + col * Y::kValueChunk, vw + j * Y::kValueChunk / 4);
+            const int at = j * 64 + lane, col = at % Y::kPerRow, row = row_of(at / Y::kPerRow);
+            load_words<Y::kValueChunk>(v.codes + (row * Y::kRow + col * Y::kValueChunk), vw + j * Y::kValueChunk / 4);
             vs[j] = v.scales[row * (D / kGroup) + col * Y::kValueElements / kGroup];
         }
     }
@@ -164,13 +175,15 @@ __device__ __forceinline__ int limit_of(const Problem &p, bool used, int t, int 
     return t >= q_len ? -1 : p.causal ? min(k_len - q_len + t, k_len - 1) : k_len - 1;
 }
 
-// One row's softmax: scores are relative to `m`, its sum is `l`, `lost` the parts of 32 elements that are NaN.
+// One row's softmax: powers are relative to `m`, which follows the largest score when that has moved by more than 2^8; their sum is any of `sum` (a product with ones
+// makes it, of the parts that weigh the values); `lost` are the parts of 32 elements that are NaN.
 template <int D> struct Row {
-    float m, l;
+    float m;
     unsigned lost;
-    f32x4 o[D / 16];
+    f32x4 sum, o[D / 16];
     __device__ __forceinline__ void clear() {
-        m = -__builtin_inff(); l = 0.f; lost = 0;
+        m = -__builtin_inff(); lost = 0;
+        sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -181,24 +194,28 @@ template <int D> struct Row {
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[kt][i] = key0 + 16 * kt + 4 * g + i <= last ? s[kt][i] : -__builtin_inff();
-        const float top = fmaxf(m, largest_of_rows(largest(s[0], s[1])) * factor);
-        const float ref = top == -__builtin_inff() ? 0.f : top;       // nothing above -inf so far: every power below is 0
-        if (__any(top != m)) {
-            const float shrink = __builtin_amdgcn_exp2f(m - ref);
-            l *= shrink;
+        const float top = largest_of_rows(largest(s[0], s[1])) * factor;
+        const bool moved = top > m + 8.f;
+        if (__any(moved)) {            // rows whose own largest score has not moved are multiplied by 1
+            const float to = moved ? top : m, shrink = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+            sum *= shrink;
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt) o[dt] *= shrink;
-            m = top;
+            m = to;
         }
+        const float ref = m == -__builtin_inff() ? 0.f : m;           // nothing above -inf so far: every power below is 0
         f32x4 z[2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], factor, -ref));
-        l += ((z[0][0] + z[0][1]) + (z[0][2] + z[0][3])) + ((z[1][0] + z[1][1]) + (z[1][2] + z[1][3]));
+        bf16x8 ones;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             part[j] = pack<__bf16>(z[0], z[1]);
+            sum = mma(ones, part[j], sum);
             if (j + 1 < NP)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { z[0][i] -= (float)part[j][i]; z[1][i] -= (float)part[j][4 + i]; }
@@ -348,9 +365,8 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
     const int64_t all_rows = (int64_t)p.batch * p.queries * p.heads;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = rows_sum(row[rt].l);
         row[rt].lose();
-        if (g == 0) stats[wave][c] = make_float2(row[rt].m, sum);
+        if (g == 0) stats[wave][c] = make_float2(row[rt].m, row[rt].sum[0]);
         __syncthreads();               // the values' staging, or the joining buffer of the tile before, has been read
         float top = -__builtin_inff(), total = 0.f;
 #pragma unroll
@@ -421,10 +437,10 @@ __global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part
 
 // How a call's work is cut: where there are too few workgroups for the card, several share a row's keys out.  512 workgroups (two a CU) as long as each
 // has eight steps of 32 keys for every tile, 256 as long as each wavefront has one; rows of up to 512 keys stay whole, for joining takes a launch of 3.5 us.
-// Kernel and joining (us), shares as the rule has them / half / twice as many: 1 sequence of 8 key heads x 128, 4 bits, 32,768 keys (64 shares) 14.1 / 15.1 / 15.9, 8,192 keys (32) 8.6 / 10.6 /
-// 9.1; 8 sequences of 4,096 (8) 13.6 / 15.3 / 14.3; 32 of 32,768 (2) 199 / 260 / 206; 1 of 2,048 x 8 heads x 64, 8 bits (16) 7.2 / 7.8 / 7.3; 3 tokens
-// of 8 sequences, 16 blocks of 64 each (8) 10.9 / 12.4 / 11.9; 512 keys (1) 7.1, in four shares 7.1.
-// Workgroups take two tiles of rows where there are as many, which then share the work on the keys (64 tokens over 16,384 keys of 8 x 128, 8 bits: 55 -> 45 us); not with
+// Kernel and joining (us), shares as the rule has them / half / twice as many: 1 sequence of 8 key heads x 128, 4 bits, 32,768 keys (64 shares) 13.6 / 15.0 / 15.5, 8,192 keys (32) 8.5 / 10.4 /
+// 9.1; 8 sequences of 4,096 (8) 13.1 / 14.6 / 13.8; 32 of 32,768 (2) 198 / 270 / 207; 1 of 2,048 x 8 heads x 64, 8 bits (16) 7.1 / 7.9 / 7.3; 3 tokens
+// of 8 sequences, 16 blocks of 64 each (8) 11.0 / 12.7 / 12.0; 512 keys (1) 6.9, in four shares 7.1; 8 tokens over 16,384 keys (32) 15.4 / 18.9 / 18.6, 64 (8) 44 / 50 / 50.
+// Workgroups take two tiles of rows where there are as many, which then share the work on the keys (64 tokens over 16,384 keys of 8 x 128, 8 bits: 44 us, with one tile 55); not with
 // lists, whose unions grow.
 struct Shape { int tiles, n_groups, splits; };
 Shape shape_of(const Problem &p, int most_tiles) {

@@ -8,6 +8,10 @@
 // A lane holds one 16-byte piece of each half of a head's pairs, so that partners need no exchange; elements that are not turned
 // (rotary_len < head_len) are dealt to the halves the same way.
 // Sums in 32 bits; dw's sums over rows in 32 bits per wavefront and 64 after that.
+//
+// What bounds them.  16,384 tokens of 32 / 8 heads of 128 in bfloat16: 67 us, 5.0 TB/s, the rate of a large copy; gradients of 2 x 4,096 tokens of 16 / 4
+// heads 29.6 us, 4.3 TB/s (three wavefronts a SIMD: 32 sums, two heads' elements and the next ones' take 168 registers), their weights' sums 4. One token
+// each of 32 sequences 3.4 us: the chain lengths, angles, LDS, store.
 #include <algorithm>
 
 #include "fg_block.h"
@@ -372,10 +376,13 @@ int problem_of(const fg_rotate_args *a, Problem *p) {
     p->rotary_len = a->rotary_len; p->interleaved = a->interleaved != 0; p->axes = a->axes; p->eps = a->eps;
     p->q = a->q; p->k = a->k; p->q_weight = a->q_weight; p->k_weight = a->k_weight;
     p->positions = a->positions; p->lengths = a->lengths; p->q_lengths = a->q_lengths;
-    // groups of heads that a wavefront takes at a time; each gets a wavefront of its own where there are too few tokens to fill the card
+    // A wavefront takes all groups of a token's heads, for which it makes the angles once, or one of them where tokens alone would not fill the card.
+    // One wavefront a token / one a group, forward and gradients (us): 32 / 8 heads of 128 in bfloat16 256 tokens 6.9 and 13.8 / 3.9 and 11.1, 1,024 8.0 and 15.6 /
+    // 6.3 and 15.9, 2,048 10.4 and 19.9 / 10.4 and 21.3, 4,096 15.3 and 25.8 / 17.0 and 29.6; 6 / 2 of 64 in 32 bits 1,024 4.1 and 9.0 / 3.6 and 9.2, 2,048
+    // 4.7 and 10.2 / 4.7 and 11.7, 8,192 9.1 and 18.3 / 10.7 and 20.8.
     const int lanes = a->head_len / 2 / (16 / size), each = 64 / lanes;
     const int groups = (a->heads + each - 1) / each + (a->kv_heads + each - 1) / each;
-    p->parts = (int64_t)a->batch * a->tokens >= 4096 ? 1 : groups;
+    p->parts = (int64_t)a->batch * a->tokens >= 2048 ? 1 : groups;
     const int64_t grid = ((int64_t)a->batch * a->tokens * p->parts + kWaves - 1) / kWaves;
     if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "rotation: %lld workgroups do not fit a launch", (long long)grid);
     return FG_OK;

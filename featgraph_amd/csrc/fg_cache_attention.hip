@@ -243,7 +243,7 @@ constexpr int kListed = 1024;          // blocks listed at a time
 struct NoList {};
 
 // Wavefronts of a SIMD that registers are left for: 128, 168 or 256 each.
-template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 : sizeof(T) == 4 ? 2 : (BITS == 4 && std::is_same<T, __bf16>::value ? 4 : 3) - LISTED;
+template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 - (sizeof(T) == 4 && BITS == 8 && LISTED) : sizeof(T) == 4 ? 2 : (BITS == 4 && std::is_same<T, __bf16>::value ? 4 : 3) - LISTED;
 // Most tiles of 16 rows that a workgroup takes.
 template <typename T, int D> constexpr int kMostTiles = sizeof(T) == 4 && D == 128 ? 1 : 2;
 

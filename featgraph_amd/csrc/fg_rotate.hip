@@ -220,10 +220,10 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const Problem p, T *q_
 
 struct Grads { const void *dq_out, *dk_out; Strides dqs, dks; void *dq, *dk; float *sums; };
 
-// The same with the gradients; wavefronts take one token after the other and keep their share of dw: sums[workgroup][q, k][D].
 // Workgroups of a CU (wavefronts of a SIMD) that registers are left for.
 template <typename T, bool NORM> constexpr int kResident = NORM && sizeof(T) == 2 ? 3 : 4;
 
+// The same with the gradients; wavefronts take one token after the other and keep their share of dw: sums[workgroup][q, k][D].
 template <typename T, int D, bool NORM>
 __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backward_kernel(const Problem p, const Grads grads) {
     constexpr int E = Piece<T>::N;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backwar
                 put(dst + me.b, gb);
             }
         };
-        // group g of queries and keys together is part g % parts'
+        // group n of queries and keys together is part n modulo the parts'
         side(p.q, p.qs, grads.dq_out, grads.dqs, grads.dq, p.heads, part, q_groups, std::integral_constant<int, 0>{});
         side(p.k, p.ks, grads.dk_out, grads.dks, grads.dk, p.kv_heads, (part + p.parts - q_groups % p.parts) % p.parts, k_groups, std::integral_constant<int, 1>{});
     }

@@ -29,10 +29,15 @@ _BINARY = ("add", "sub", "mul", "div")
 
 
 def _no_grad_inputs(what, *tensors):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError("%s has no gradient here; detach the inputs or run under torch.no_grad()" % what)
-    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 \
-            and any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+
+
+def _no_gradients(what, *tensors):
+    """The same, and no tangents, which would be dropped without a word."""
+    tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
+    _no_grad_inputs(what, *tensors)
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("%s has no forward-mode gradient" % what)
 
 
@@ -201,7 +206,7 @@ def write_cache(cache, k, v, lengths=None, q_lengths=None):
     stays as it was.  32 neighbouring elements of a head share the least power of two with which the largest of them rounds to at most the largest
     element (6 or 448); each is rounded to the nearest element, ties to the even code.  32 with an infinity or NaN among them become
     NaN.  Not differentiable."""
-    _no_grad_inputs("write_cache", k, v)
+    _no_gradients("write_cache", k, v)
     _cache.write(cache, k, v, lengths, q_lengths)
 
 
@@ -222,5 +227,5 @@ def cache_attention(q, cache, blocks=None, block_size=None, scale=None, causal=T
 
     Made for single tokens and a few at a time: 16 / group tokens share one pass over the cache.  Powers and sums are kept in 32 bits; values that are not
     finite reach the rows that see them and no others.  The same bits on every call.  Not differentiable."""
-    _no_grad_inputs("cache_attention", q)
+    _no_gradients("cache_attention", q)
     return _cache.attention(q, cache, blocks, block_size, scale, bool(causal), lengths, q_lengths)

@@ -239,6 +239,21 @@ def test_offsets_beyond_32_bits():
             assert not x[:, 0].any() and np.array_equal(x[:, 1:].cpu().double().numpy(), want)
 
 
+def test_sources_and_results_beyond_32_bits():
+    from featgraph_amd import ops
+    tokens = (1 << 21) + 3                  # 2^31 elements of keys and more, 4.3 GB
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.empty((1, tokens, 8, 128), dtype=F16, device="cuda")
+    for i in range(0, tokens, 1 << 17):
+        x[:, i:i + (1 << 17)].normal_(generator=gen)
+    cache, few = ops.new_cache(1, tokens, 8, 128, 4), ops.new_cache(1, 5, 8, 128, 4)
+    ops.write_cache(cache, x, x)
+    ops.write_cache(few, x[:, -5:], x[:, -5:])
+    assert torch.equal(cache.k[:, :, -5:], few.k) and torch.equal(cache.v_scales[:, :, -5:], few.v_scales)
+    back = ops.read_cache(cache, F16)
+    assert all(torch.equal(a[:, -5:], b) for a, b in zip(back, ops.read_cache(few, F16)))
+
+
 def test_captured_and_another_stream():
     from featgraph_amd import ops
     gen = torch.Generator().manual_seed(10)

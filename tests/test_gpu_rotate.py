@@ -241,6 +241,35 @@ def test_the_same_bits_on_every_call_and_another_stream():
     assert all(torch.equal(first[x], other[x]) for x in first)
 
 
+def test_a_row_is_the_same_whoever_stands_beside_it():
+    from featgraph_amd import ops
+    s = make(BF16, 2, 1300, 20, 3, 64, seed=24)     # 2,600 tokens: a wavefront each; alone a wavefront for every group of heads
+    s["q"][0, 7, 3] *= 2.0 ** 100                   # squares out of range, in the same wavefront as others
+    positions = torch.arange(1300, dtype=torch.int32, device="cuda").expand(2, 1300)
+    q, k = ops.rotate_heads(s["q"], s["k"], *s["weights"], positions=positions)
+    for i in (0, 7, 1299):
+        one = ops.rotate_heads(s["q"][:, i:i + 1], s["k"][:, i:i + 1], *s["weights"], positions=positions[:, i:i + 1])
+        assert torch.equal(one[0], q[:, i:i + 1]) and torch.equal(one[1], k[:, i:i + 1])
+
+
+def test_offsets_beyond_32_bits():
+    from featgraph_amd import ops
+    tokens = (1 << 18) + 5                          # 2^31 elements of queries and more, 4.3 GB
+    gen = torch.Generator(device="cuda").manual_seed(25)
+    q = torch.empty((1, tokens, 64, 128), dtype=BF16, device="cuda")
+    for i in range(0, tokens, 1 << 14):
+        q[:, i:i + (1 << 14)].normal_(generator=gen)
+    k, w = q[:, :, :1], torch.ones(128, dtype=BF16, device="cuda")
+    out, _ = ops.rotate_heads(q, k, w, w)
+    few = ops.rotate_heads(q[:, -3:], k[:, -3:], w, w, lengths=ints(tokens))[0]
+    assert torch.equal(out[:, -3:], few)
+    from featgraph_amd.module import rotate
+    plan = rotate.check(q, k, w, w, None, None, None, 10000.0, None, None, None, False, 1e-6)
+    dq = rotate.backward(q, k, w, w, plan, None, None, None, q, k)[0]
+    plan = rotate.check(q[:, -3:], k[:, -3:], w, w, None, ints(tokens), None, 10000.0, None, None, None, False, 1e-6)
+    assert torch.equal(dq[:, -3:], rotate.backward(q[:, -3:], k[:, -3:], w, w, plan, None, ints(tokens), None, q[:, -3:], k[:, -3:])[0])
+
+
 def test_captured():
     from featgraph_amd import ops
     s = make(BF16, 2, 50, 8, 2, 128, seed=16)

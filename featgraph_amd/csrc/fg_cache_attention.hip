@@ -13,12 +13,12 @@
 // Values that are no numbers are taken as 0 and marked; the marks of the keys that a row sees make its result NaN.  (Keys that are none, and queries that
 // are not finite, make scores of their own rows alone.)
 //
-// What bounds it.  32 requests of 32,768 keys of 8 heads x 128 in 4 bits, one token of 32 heads each (1.14 GB): 198 us, 5.8 TB/s, above the rate of a large copy (5.1),
+// What bounds it.  32 requests of 32,768 keys of 8 heads x 128 in 4 bits, one token of 32 heads each (1.14 GB): 196 us, 5.8 TB/s, above the rate of a large copy (5.1),
 // for it only reads; 128 registers leave room for four wavefronts a SIMD, which keep 17 KB each on their way. With a sweep of its own for values that are not finite in
 // the same kernel it took 276 registers and 353 us.  One request of 2,048 keys x 8 heads x 64: 7.1 us, of which 3.5 are the joining launch and the rest the chain
-// length, keys, softmax, joining. Many rows, 64 tokens over 16,384 keys of 8 x 128 in 8 bits: 44 us, 390 TFLOP/s counted once; with two tiles of rows two
-// wavefronts fit a SIMD, and each waits for its own chain scores, softmax, product.  (Four wavefronts that share the widened keys through LDS and take two tiles
-// each have the same chain, and barriers: 46 us, and 134 where this takes 116, 512 tokens over 8,192 keys.)
+// length, keys, softmax, joining. Many rows, 64 tokens over 16,384 keys of 8 x 128 in 8 bits: 43 us, 400 TFLOP/s counted once; with two tiles of rows two
+// wavefronts fit a SIMD, whose vector instructions (430 a step) and products together fill 85 % of the time.  (Four wavefronts that share the widened keys through LDS and take two tiles
+// each wait for one another: 46 us, and 134 where this takes 111, 512 tokens over 8,192 keys.)
 #include <algorithm>
 #include <type_traits>
 
@@ -187,23 +187,25 @@ template <int D> struct Row {
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // 32 keys: scores s of keys key0 + 16 kt + 4 g + i, of which the row sees those up to `last`, become the parts of their powers.
-    template <int NP> __device__ __forceinline__ void weigh(f32x4 (&s)[2], int key0, int g, int last, float factor, bf16x8 (&part)[NP]) {
-        if (!__all(key0 + kUnit - 1 <= last))
+    // Scores s of keys key0 + 16 kt + 4 g + i, of which the row sees those up to `last`: the others become -inf.
+    static __device__ __forceinline__ void mask(f32x4 (&s)[2], int key0, int g, int last) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[kt][i] = key0 + 16 * kt + 4 * g + i <= last ? s[kt][i] : -__builtin_inff();
-        const float top = largest_of_rows(largest(s[0], s[1])) * factor;
+            for (int i = 0; i < 4; ++i) s[kt][i] = key0 + 16 * kt + 4 * g + i <= last ? s[kt][i] : -__builtin_inff();
+    }
+    // A row whose own largest score has not moved is multiplied by 1, whoever stands beside it.
+    __device__ __forceinline__ void follow(float top) {
         const bool moved = top > m + 8.f;
-        if (__any(moved)) {            // rows whose own largest score has not moved are multiplied by 1
-            const float to = moved ? top : m, shrink = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
-            sum *= shrink;
+        const float to = moved ? top : m, shrink = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+        sum *= shrink;
 #pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) o[dt] *= shrink;
-            m = to;
-        }
-        const float ref = m == -__builtin_inff() ? 0.f : m;           // nothing above -inf so far: every power below is 0
+        for (int dt = 0; dt < D / 16; ++dt) o[dt] *= shrink;
+        m = to;
+    }
+    // The scores' powers, in parts.
+    template <int NP> __device__ __forceinline__ void powers(const f32x4 (&s)[2], float factor, bf16x8 (&part)[NP]) {
+        const float ref = m == -__builtin_inff() ? 0.f : m;           // nothing above -inf so far: every power is 0
         f32x4 z[2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -336,12 +338,25 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
             u = find(u + stride);
             if (u < units) fetch(u);
             wave_lds_sync();
-            bf16x8 pf[RT][NP];
+            // each part of the softmax for all tiles, so that their chains run side by side
+            bool edge = false, moved = false;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) edge |= key0 + kUnit - 1 > last[rt];
+            if (__any(edge))
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) Row<D>::mask(s[rt], key0, g, last[rt]);
+            float top[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                row[rt].weigh(s[rt], key0, g, last[rt], factor, pf[rt]);
-                if (__any(odd)) row[rt].mark(marks[wave], key0, g, last[rt]);
+                top[rt] = largest_of_rows(largest(s[rt][0], s[rt][1])) * factor;
+                moved |= top[rt] > row[rt].m + 8.f;
             }
+            if (__any(moved))
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) row[rt].follow(top[rt]);
+            bf16x8 pf[RT][NP];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) row[rt].powers(s[rt], factor, pf[rt]);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const bf16x8 vf = transposed<__bf16, D>(stage, dt * 16, lane);
@@ -350,6 +365,9 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
 #pragma unroll
                     for (int j = 0; j < NP; ++j) row[rt].o[dt] = mma(vf, pf[rt][j], row[rt].o[dt]);
             }
+            if (__any(odd))
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) row[rt].mark(marks[wave], key0, g, last[rt]);
         }
     };
     if constexpr (LISTED) {
@@ -439,8 +457,8 @@ __global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part
 // has eight steps of 32 keys for every tile, 256 as long as each wavefront has one; rows of up to 512 keys stay whole, for joining takes a launch of 3.5 us.
 // Kernel and joining (us), shares as the rule has them / half / twice as many: 1 sequence of 8 key heads x 128, 4 bits, 32,768 keys (64 shares) 13.6 / 15.0 / 15.5, 8,192 keys (32) 8.5 / 10.4 /
 // 9.1; 8 sequences of 4,096 (8) 13.1 / 14.6 / 13.8; 32 of 32,768 (2) 198 / 270 / 207; 1 of 2,048 x 8 heads x 64, 8 bits (16) 7.1 / 7.9 / 7.3; 3 tokens
-// of 8 sequences, 16 blocks of 64 each (8) 11.0 / 12.7 / 12.0; 512 keys (1) 6.9, in four shares 7.1; 8 tokens over 16,384 keys (32) 15.4 / 18.9 / 18.6, 64 (8) 44 / 50 / 50.
-// Workgroups take two tiles of rows where there are as many, which then share the work on the keys (64 tokens over 16,384 keys of 8 x 128, 8 bits: 44 us, with one tile 55); not with
+// of 8 sequences, 16 blocks of 64 each (8) 11.0 / 12.7 / 12.0; 512 keys (1) 6.9, in four shares 7.1; 8 tokens over 16,384 keys (32) 15.4 / 18.9 / 18.6, 64 (8) 43 / 48 / 48.
+// Workgroups take two tiles of rows where there are as many, which then share the work on the keys (64 tokens over 16,384 keys of 8 x 128, 8 bits: 43 us, with one tile 55); not with
 // lists, whose unions grow.
 struct Shape { int tiles, n_groups, splits; };
 Shape shape_of(const Problem &p, int most_tiles) {

@@ -355,6 +355,7 @@ int problem_of(const fg_rotate_args *a, Problem *p) {
     if (a->head_len != 32 && a->head_len != 64 && a->head_len != 128) return fail(FG_ERR_SHAPE, "rotation: heads of 32, 64 or 128 elements, got %d", a->head_len);
     if (a->rotary_len < 0 || a->rotary_len > a->head_len || a->rotary_len % 16)
         return fail(FG_ERR_SHAPE, "rotation: a multiple of 16 elements of a head of %d can be turned, got %d", a->head_len, a->rotary_len);
+    if (!(a->eps >= 0.f)) return fail(FG_ERR_ARG, "rotation: eps has to be 0 or more");
     if (a->tokens > (1 << 30) || a->heads > (1 << 20) || a->kv_heads > (1 << 20)) return fail(FG_ERR_SHAPE, "rotation: more than 2^30 tokens or 2^20 heads");
     if (a->axes < 1 || a->axes > 8 || (a->axes > 1 && a->rotary_len && !a->positions))
         return fail(FG_ERR_ARG, "rotation: 1 to 8 axes, and positions with more than one, got %d", a->axes);

@@ -116,7 +116,7 @@ def test_attention_refuses_null_pointers_and_small_workspaces():
 @pytest.mark.parametrize("change,status,words", [
     (dict(type=3), -1, "type"), (dict(batch=-1), -1, "negative"), (dict(heads=0), -1, "no heads"), (dict(kv_heads=0), -1, "no heads"), (dict(head_len=96), -2, "96"),
     (dict(rotary_len=8), -2, "multiple of 16"), (dict(rotary_len=80), -2, "multiple of 16"), (dict(rotary_len=-16), -2, "multiple of 16"),
-    (dict(axes=0), -1, "axes"), (dict(axes=9), -1, "axes"), (dict(axes=2), -1, "positions"), (dict(axis=1), -1, "axis 1 of 1"),
+    (dict(axes=0), -1, "axes"), (dict(axes=9), -1, "axes"), (dict(axes=2), -1, "positions"), (dict(eps=-1.0), -1, "eps"), (dict(eps=float("nan")), -1, "eps"), (dict(axis=1), -1, "axis 1 of 1"),
     (dict(q_weight=None), -1, "come together"), (dict(q=72), -1, "16 bytes"), (dict(k_strides=(64, 1, 64)), -1, "16 bytes"), (dict(k_weight=72), -1, "16 bytes"),
     (dict(positions=66), -1, "4 bytes"), (dict(lengths=66), -1, "4 bytes"), (dict(q_out=72), -1, "16 bytes"), (dict(tokens=(1 << 30) + 1), -2, "2\\^30"),
     (dict(tokens=1 << 30, batch=1 << 10, heads=1 << 10), -2, "workgroups")])

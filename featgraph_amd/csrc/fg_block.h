@@ -137,14 +137,21 @@ template <typename T> __device__ __forceinline__ void store_row(T *out, T *rest,
     if (rest) *reinterpret_cast<T4 *>(rest + at) = y;
 }
 
-// The largest of eight numbers (NaN only if all are).  Written out: of products of the matrix cores the compiler takes every operand's
-// maximum with itself first, which doubles the instructions.
+// The largest of three numbers (NaN only if all are), and of the eight of two results of the matrix cores.  Written out: of products of the matrix cores the compiler
+// takes every operand's maximum with itself first, which doubles the instructions.
+// The compiler counts the waits between a product and its first reader for its own instructions only, so that text which reads products has to wait itself, for all of them
+// and before its first instruction: 16x16x32 products take 8 wait states, 16x16x4 ones of 32 bits 10.  max3 is for numbers that have been through another instruction.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm volatile("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));        // volatile: not moved behind a branch
     return d;
 }
-__device__ __forceinline__ float largest(f32x4 a, f32x4 b) { return max3(max3(max3(a[0], a[1], a[2]), a[3], b[0]), max3(b[1], b[2], b[3]), b[3]); }
+__device__ __forceinline__ float largest(f32x4 a, f32x4 b) {
+    float d, e;
+    asm volatile("s_nop 9\n\tv_max3_f32 %0, %2, %3, %4\n\tv_max3_f32 %1, %7, %8, %9\n\tv_max3_f32 %0, %0, %5, %6\n\tv_max3_f32 %0, %0, %1, %9"
+                 : "=&v"(d), "=&v"(e) : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]));
+    return d;
+}
 // The largest of lanes l, l ^ 16, l ^ 32, l ^ 48; every lane gets it.
 __device__ __forceinline__ float largest_of_rows(float v) {
     float w = v;

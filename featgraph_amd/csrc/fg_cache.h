@@ -58,6 +58,12 @@ template <int BITS, typename T = __bf16> __device__ __forceinline__ block::V8<T>
     return block::V8<T>{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// A number as it is rounded to T: an element may be larger than the value it came from (65504 is held as 65536), and float16 takes no such number.
+template <typename T> __device__ __forceinline__ float within(float f) {
+    if constexpr (std::is_same<T, _Float16>::value) return f != f ? f : fminf(fmaxf(f, -65504.f), 65504.f);
+    else return f;
+}
+
 // FG_OK, or why the arrays cannot be such a cache.
 int check(const fg_kv_cache *c);
 

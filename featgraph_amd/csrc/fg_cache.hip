@@ -165,11 +165,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const Window w, const Ta
         if (key >= 0 && key < k_len) {
             const auto y = values<BITS, typename std::conditional<sizeof(T) == 4, float, __bf16>::type>(word[u], scale_of(byte[u]));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float f = (float)y[e];
-                if constexpr (std::is_same<T, _Float16>::value) x[e] = (T)(f != f ? f : fminf(fmaxf(f, -65504.f), 65504.f));
-                else x[e] = (T)f;
-            }
+            for (int e = 0; e < 8; ++e) x[e] = (T)within<T>((float)y[e]);
         }
         *reinterpret_cast<V8<T> *>(static_cast<T *>(t.out) + (((int64_t)p.b * w.tokens + i) * w.kv_heads + p.g) * D + p.col) = x;
     }

@@ -241,6 +241,13 @@ template <int D> struct Row {
     }
 };
 
+// Four consecutive elements of a result.
+template <typename T> __device__ __forceinline__ void store_result(T *out, int64_t at, f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = within<T>(v[i]);
+    store_row<T>(out, nullptr, at, v);
+}
+
 constexpr int kListed = 1024;          // blocks listed at a time
 struct NoList {};
 
@@ -411,7 +418,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
             const int64_t at = ((int64_t)b * p.queries + t) * p.heads + h * p.group + (r16 - at_token * p.group);
             const float2 st = joined[r16];
             if (splits == 1) {
-                store_row<T>(static_cast<T *>(r.out), nullptr, at * D + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
+                store_result<T>(static_cast<T *>(r.out), at * D + col, v * (st.y == 0.f ? 0.f : 1.f / st.y));
             } else {
                 *reinterpret_cast<f32x4 *>(r.part + (split * all_rows + at) * D + col) = v;
                 if (col == 0) r.part_stats[split * all_rows + at] = st;
@@ -451,7 +458,7 @@ __global__ __launch_bounds__(kThreads) void join_shares_kernel(const float *part
     if (sub) return;
 #pragma unroll
     for (int i = 1; i < SUBS; ++i) v += sums[i][col];
-    store_row<T>(out, nullptr, row * D + col * 4, v * (total == 0.f ? 0.f : 1.f / total));
+    store_result<T>(out, row * D + col * 4, v * (total == 0.f ? 0.f : 1.f / total));
 }
 
 // How a call's work is cut: where there are too few workgroups for the card, several share a row's keys out.  512 workgroups (two a CU) as long as each

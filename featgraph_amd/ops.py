@@ -223,7 +223,8 @@ def cache_attention(q, cache, blocks=None, block_size=None, scale=None, causal=T
 
     q (batch, queries, heads, head_len), float32, float16 or bfloat16; heads / kv_heads (1 to 16) query heads share key head g.  Without `blocks` a query sees
     all keys, with them (int32 (batch, queries, kv_heads, topk) and block_size 32, 64, 128 or 256, as in block_attention) those of
-    its blocks; lengths, q_lengths, causal and scale as in block_attention.  A query that sees no key gives 0.
+    its blocks; lengths, q_lengths, causal and scale as in block_attention.  A query that sees no key gives 0.  float16 results end at 65504, as
+    read_cache's do: a value near that is held as 65536.
 
     Made for single tokens and a few at a time: 16 / group tokens share one pass over the cache.  Powers and sums are kept in 32 bits; values that are not
     finite reach the rows that see them and no others.  The same bits on every call.  Not differentiable."""

@@ -755,7 +755,7 @@ typedef struct {
     int64_t q_strides[3];
     const int32_t *blocks;             /* (batch, queries, kv_heads, topk) dense, as for fg_block_attention; not read with topk 0 */
     const int32_t *lengths, *q_lengths;
-    void *out;                         /* (batch, queries, heads, head_len) dense, at a multiple of 16 bytes; 0 where a query sees no key */
+    void *out;                         /* (batch, queries, heads, head_len) dense, at a multiple of 16 bytes; 0 where a query sees no key; float16 up to 65504, as for fg_cache_read */
 } fg_cache_attention_args;
 
 /* Softmax attention over the cache as it is held, or over the selected blocks of it; made for few queries.  workspace: as for fg_block_attention.  The same

@@ -51,3 +51,27 @@ def test_rows_behind_the_queries_walk_no_keys(causal):
     assert not got[:, 1:].any()
     # shares of the keys differ between the two calls, and so does the order of their sums
     torch.testing.assert_close(got[:, :1].float(), alone.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("head_len", [32, 64, 128])
+@pytest.mark.parametrize("keys,queries", [(1, 1), (5, 3), (9001, 1), (700, 40)])
+def test_float16_results_end_where_read_values_do(bits, head_len, keys, queries):
+    # 65504 is held as 65536, every result is that value, and float16 ends between the two; 57344 is 65536 in 4 bits
+    from featgraph_amd import ops
+    cache = ops.new_cache(1, keys, 2, head_len, bits)
+    x = torch.full((1, keys, 2, head_len), 65504.0, dtype=F16, device="cuda")
+    x[..., 1::3] *= -1
+    x[..., 2::3] = 57344.0
+    ops.write_cache(cache, torch.randn(x.shape, device="cuda").to(F16), x)
+    q = torch.randn((1, queries, 4, head_len), device="cuda").to(F16)
+    held = ops.read_cache(cache, F16, count=1)[1][:, :, [0, 0, 1, 1]].expand_as(q)
+    assert held.abs().max() == 65504
+    lists = torch.arange(-(-keys // 32), dtype=torch.int32, device="cuda").expand(1, queries, 2, -1)
+    for options in ({}, dict(causal=False), dict(blocks=lists, block_size=32)):
+        got = ops.cache_attention(q, cache, **options)
+        # an average of equal numbers is that number, within float16's step once sums are rounded
+        assert torch.isfinite(got).all() and ((got - held).float().abs() <= 32).all() and torch.equal(got.abs() == 65504, held.abs() == 65504)
+    cache.v_scales[0, 1, 0] = 255           # no numbers stay none
+    got = ops.cache_attention(q, cache, causal=False)
+    assert torch.isnan(got[:, :, 2:]).all() and torch.isfinite(got[:, :, :2]).all()

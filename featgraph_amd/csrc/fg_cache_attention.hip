@@ -92,13 +92,14 @@ template <int D, int BITS> struct Step {
             vs[j] = v.scales[row * (D / kGroup) + col * Y::kValueElements / kGroup];
         }
     }
-    // Whether any of the lane's values are no numbers; then, for all lanes: these become 0, and each key's mark has a bit for each 32 of them.
-    __device__ __forceinline__ bool odd() const {
+    // The largest scale of the lane's values: 255 where some are no numbers.
+    __device__ __forceinline__ unsigned most() const {
         unsigned most = 0;
 #pragma unroll
         for (int j = 0; j < Y::kValueChunks; ++j) most = max(most, vs[j]);
-        return most == 255;
+        return most;
     }
+    // For all lanes, where any has such values: these become 0, and each key's mark has a bit for each 32 of them.
     __device__ __forceinline__ void clear(uint8_t *marks, int lane) {
 #pragma unroll
         for (int j = 0; j < Y::kValueChunks; ++j) {
@@ -177,6 +178,11 @@ __device__ __forceinline__ int limit_of(const Problem &p, bool used, int t, int 
 
 // One row's softmax: powers are relative to `m`, which follows the largest score when that has moved by more than 2^8; their sum is any of `sum` (a product with ones
 // makes it, of the parts that weigh the values); `lost` are the parts of 32 elements that are NaN.
+// Sums are divided at the end.  Of 2^30 keys, the most there are, with powers of up to 2^8 and elements of up to 448 x 2^80 they stay below 2^127; caches hold elements of
+// up to 2^128.  Where a step has a larger scale than 2^80 the reference goes to kLift above its largest score, which keeps its powers below 2^-kLift.  Powers are
+// then rounded to 2^-19 of themselves by their exponents, and lost below 2^-86, which is why this is not done for all.
+constexpr unsigned kLargeScale = 127 + 80;
+constexpr float kLift = 40.f;
 template <int D> struct Row {
     float m;
     unsigned lost;
@@ -195,9 +201,10 @@ template <int D> struct Row {
             for (int i = 0; i < 4; ++i) s[kt][i] = key0 + 16 * kt + 4 * g + i <= last ? s[kt][i] : -__builtin_inff();
     }
     // A row whose own largest score has not moved is multiplied by 1, whoever stands beside it.
-    __device__ __forceinline__ void follow(float top) {
-        const bool moved = top > m + 8.f;
-        const float to = moved ? top : m, shrink = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+    __device__ __forceinline__ void follow(float top, bool large) {
+        const float at = large ? top + kLift : top;
+        const bool moved = large ? at > m : top > m + 8.f;
+        const float to = moved ? at : m, shrink = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
         sum *= shrink;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[dt] *= shrink;
@@ -326,8 +333,12 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) last[rt] = !LISTED || !used || t0 + rt * tpt + tc >= p.queries || (who[rt] >> tc) & 1 ? limit[rt] : -1;
             wave_lds_sync();
-            const bool odd = step.odd();
-            if (__any(odd)) step.clear(marks[wave], lane);
+            bool odd = false, large = false;       // of all lanes
+            if (__any(step.most() > kLargeScale)) {
+                odd = __any(step.most() == 255);
+                if (odd) step.clear(marks[wave], lane);
+                large = __any(step.most() > kLargeScale);
+            }
             step.store_values(stage, lane);
             f32x4 s[RT][2];
 #pragma unroll
@@ -359,9 +370,9 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
                 top[rt] = largest_of_rows(largest(s[rt][0], s[rt][1])) * factor;
                 moved |= top[rt] > row[rt].m + 8.f;
             }
-            if (__any(moved))
+            if (large || __any(moved))
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) row[rt].follow(top[rt]);
+                for (int rt = 0; rt < RT; ++rt) row[rt].follow(top[rt], large);
             bf16x8 pf[RT][NP];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) row[rt].powers(s[rt], factor, pf[rt]);
@@ -373,7 +384,7 @@ __global__ __launch_bounds__(kThreads, (kResident<T, D, BITS, RT, LISTED>)) void
 #pragma unroll
                     for (int j = 0; j < NP; ++j) row[rt].o[dt] = mma(vf, pf[rt][j], row[rt].o[dt]);
             }
-            if (__any(odd))
+            if (odd)
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) row[rt].mark(marks[wave], key0, g, last[rt]);
         }

@@ -1,5 +1,8 @@
 """Attention over a cache of 4 or 8 bits (ops.cache_attention): what rows that are padding cost, and values at the ends of their ranges."""
+import numpy as np
 import pytest
+
+import cache_reference as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +78,71 @@ def test_float16_results_end_where_read_values_do(bits, head_len, keys, queries)
     cache.v_scales[0, 1, 0] = 255           # no numbers stay none
     got = ops.cache_attention(q, cache, causal=False)
     assert torch.isnan(got[:, :, 2:]).all() and torch.isfinite(got[:, :, :2]).all()
+
+
+def check_large(q, cache, blocks=None, block_size=None, **options):
+    """Powers of steps with large scales are 2^40 below their reference: the difference of score and reference is off by half a step of 32 bits at 2^6, 2^-18 at most
+    (2^-19, and as much for what is added to a reference), powers below 2^-86 of the largest are lost, and what is lost of either reaches the sum of powers too."""
+    from featgraph_amd import ops
+    got = ops.cache_attention(q, cache, blocks, block_size, **options)
+    k, v = ref.held(cache)
+    out, bound = ref.attention(q, k, v, blocks, block_size, **options)
+    assert np.isfinite(v).all()
+    mean = ref.attention(q, k, np.abs(v), blocks, block_size, **options)[0]        # sum of p |v|
+    ref.check(got, out, bound + 2 * np.log(2) * 2.0 ** -18 * mean + 2.0 ** -84 * cache.keys * np.abs(v).max())
+    return got
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("keys,queries", [(1, 1), (2, 1), (300, 3), (9001, 1), (700, 40)])
+def test_the_largest_values_of_a_cache_have_a_mean(bits, dtype, keys, queries):
+    # sums of powers times values are beyond 32 bits, the result is not: 6 2^125 and 448 2^119, each with its sign
+    from featgraph_amd import ops
+    cache = ops.new_cache(2, keys, 2, 64, bits)
+    largest = 6 * 2.0 ** 125 if bits == 4 else 448 * 2.0 ** 119
+    x = torch.full((2, keys, 2, 64), largest, device="cuda")
+    x[..., 1::2] *= -1
+    ops.write_cache(cache, torch.randn(x.shape, device="cuda"), x)
+    q = 3 * torch.randn((2, queries, 4, 64), device="cuda").to(dtype)
+    lists = torch.arange(-(-keys // 32), dtype=torch.int32, device="cuda").expand(2, queries, 2, -1)
+    for options in ({}, dict(causal=False), dict(blocks=lists, block_size=32)):
+        got = check_large(q, cache, **options)
+        assert (got[..., 0::2] > 0).all() and (got[..., 1::2] < 0).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,head_len", [(F32, 32), (BF16, 128), (F32, 128), (BF16, 64)])
+@pytest.mark.parametrize("order", ["up", "down", "mixed"])
+def test_values_of_very_different_sizes(bits, dtype, head_len, order):
+    # sizes from 2^-20 to the largest, among them steps of 32 keys without a large one; scores that rise, fall or do neither along the keys
+    from featgraph_amd import ops
+    gen = torch.Generator().manual_seed(3)
+    keys = 2000
+    power = torch.where(torch.arange(keys) // 32 % 3 > 0, torch.randint(-20, 20, (keys,), generator=gen), torch.randint(70, 125, (keys,), generator=gen)).double()
+    v = torch.randn((2, keys, 2, head_len), generator=gen).clamp(-3, 3).double() * torch.exp2(power)[:, None, None]
+    k = torch.randn((2, keys, 2, head_len), generator=gen)
+    if order != "mixed":
+        k[..., :32] = torch.linspace(-1, 1, keys)[:, None, None] * (1 if order == "up" else -1)
+    cache = ops.new_cache(2, keys, 2, head_len, bits)
+    ops.write_cache(cache, k.cuda(), v.float().cuda())
+    q = torch.randn((2, 3, 4, head_len), generator=gen)
+    if order != "mixed":
+        q = q.abs()
+        q[..., :32] = 20 * head_len ** 0.5 / 32
+    check_large((q * 2).to(dtype).cuda(), cache)
+    few = torch.randint(0, 63, (2, 3, 2, 12), generator=gen, dtype=torch.int32).cuda()
+    check_large((q * 2).to(dtype).cuda(), cache, few, 32)
+
+
+def test_large_values_behind_what_a_row_sees_change_nothing():
+    from featgraph_amd import ops
+    cache = arbitrary(1, 500, 2, 64, 4)
+    q = torch.randn((1, 3, 4, 64), device="cuda").to(BF16)
+    clean = ops.cache_attention(q, cache, lengths=ints(400))
+    cache.v_scales[:, :, 400:] = 250
+    assert torch.equal(ops.cache_attention(q, cache, lengths=ints(400)), clean)
+    cache.v_scales[:, :, 384:] = 250        # token 0 of three that end at 385 sees keys up to 383, and the step of 32 from 384 on only in passing
+    got = ops.cache_attention(q, cache, lengths=ints(384 + 2), q_lengths=ints(3))
+    clean = ops.cache_attention(q, cache, lengths=ints(384), q_lengths=ints(1))
+    assert torch.equal(got[:, :1], clean[:, :1]) and torch.isfinite(got).all()

@@ -5,7 +5,7 @@
 //
 // Every value of the cache is a bfloat16, so that products with it are bfloat16 products of the matrix cores, exact up to the sums in 32
 // bits, whatever type the queries have: a float16 is the sum of two bfloat16, a number of 32 bits of three.  Powers are taken apart the
-// same way, each rounded to nearest: into two parts for 16-bit results (2^-18 of a power is lost) and three for 32-bit ones (2^-27).
+// same way, each rounded to nearest: into two parts for 16-bit results (up to 2^-17 of a power is lost) and three for 32-bit ones (nothing is).
 // Rows of one token's heads and of neighbouring tokens make tiles of 16, RT of them a workgroup.  Its four wavefronts deal the keys out among themselves, 32 at a
 // time, and where there are too few workgroups for the card so do several workgroups, whose sums are joined after.  A
 // lane's keys come from memory as operands lie in registers (the sum over a head's elements takes them in any order), values go

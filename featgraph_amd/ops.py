@@ -226,7 +226,9 @@ def cache_attention(q, cache, blocks=None, block_size=None, scale=None, causal=T
     its blocks; lengths, q_lengths, causal and scale as in block_attention.  A query that sees no key gives 0.  float16 results end at 65504, as
     read_cache's do: a value near that is held as 65536.
 
-    Made for single tokens and a few at a time: 16 / group tokens share one pass over the cache.  Powers and sums are kept in 32 bits; values that are not
-    finite reach the rows that see them and no others.  The same bits on every call.  Not differentiable."""
+    Made for single tokens and a few at a time: 16 / group tokens share one pass over the cache.  Scores, maxima and sums are kept in 32 bits (a score beyond
+    them is infinite).  The powers that are summed and weigh the values are made of bfloat16 parts: two for 16-bit results, which loses up to 2^-17 of
+    a power (a result is rounded by up to 2^-8 or 2^-11 of itself), three for float32, which are all of it; beside values beyond 2^80 powers are rounded to 2^-19.  Values that
+    are not finite reach the rows that see them and no others.  The same bits on every call.  Not differentiable."""
     _no_gradients("cache_attention", q)
     return _cache.attention(q, cache, blocks, block_size, scale, bool(causal), lengths, q_lengths)

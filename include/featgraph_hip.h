@@ -758,8 +758,9 @@ typedef struct {
     void *out;                         /* (batch, queries, heads, head_len) dense, at a multiple of 16 bytes; 0 where a query sees no key; float16 up to 65504, as for fg_cache_read */
 } fg_cache_attention_args;
 
-/* Softmax attention over the cache as it is held, or over the selected blocks of it; made for few queries.  workspace: as for fg_block_attention.  The same
- * sums in the same order on every call. */
+/* Softmax attention over the cache as it is held, or over the selected blocks of it; made for few queries.  Scores and sums in 32 bits; the powers that are
+ * summed and weigh the values lose up to 2^-17 of themselves for 16-bit results (nothing for 32-bit ones), and are rounded to 2^-19 beside values beyond 2^80.
+ * workspace: as for fg_block_attention.  The same sums in the same order on every call. */
 int64_t fg_cache_attention_workspace(const fg_cache_attention_args *args);
 int fg_cache_attention(const fg_cache_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
 

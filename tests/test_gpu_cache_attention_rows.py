@@ -146,3 +146,19 @@ def test_large_values_behind_what_a_row_sees_change_nothing():
     got = ops.cache_attention(q, cache, lengths=ints(384 + 2), q_lengths=ints(3))
     clean = ops.cache_attention(q, cache, lengths=ints(384), q_lengths=ints(1))
     assert torch.equal(got[:, :1], clean[:, :1]) and torch.isfinite(got).all()
+
+
+def test_many_equal_keys_far_apart():
+    """Offsets beyond 32 bits again, bounded by the steps that are added up: 2^26 keys are cut into 256 shares of four wavefronts, so that one adds 2,048 steps of 32
+    keys, in two parts each.  Every score is 0 and every power 1: their sums, of whole numbers up to 2^16, are exact, and values' sums are off by half a step of 32 bits for each addition."""
+    from featgraph_amd import ops
+    keys = 1 << 26
+    cache = ops.new_cache(1, keys, 1, 32, 4)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    cache.v.copy_(torch.randint(0, 256, (16,), generator=gen, device="cuda", dtype=torch.uint8))        # the same key everywhere
+    cache.v_scales.fill_(127)
+    q = torch.randn((1, 1, 4, 32), device="cuda")
+    got = ops.cache_attention(q, cache)
+    want = ops.read_cache(cache, F32, count=1)[1].expand_as(q)
+    assert ((got - want).abs() <= (2048 * 32 + 256 * 4) * 2.0 ** -24 * want.abs()).all()
+    del cache

@@ -24,6 +24,32 @@ _GRADS = struct.Struct("=2Q6q4Q")
 assert ctypes.sizeof(_lib.FgRotateGrads) == _GRADS.size
 
 
+def _host(name, x):
+    """What a tensor holds as Python numbers (one on the GPU is waited for), everything else as it is."""
+    if not isinstance(x, torch.Tensor):
+        return x
+    if x.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("%s have no gradient; detach them or run under torch.no_grad()" % name)
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise ValueError("%s are numbers on the host: a tensor on the GPU cannot be read during capture" % name)
+    return x.tolist()
+
+
+def _options(base, frequencies, sections, rotary_len, interleaved, eps):
+    """A call's options as numbers and tuples of numbers, by whose values its plan is kept."""
+    if type(base) is not float:
+        base = float(_host("base", base))
+    if type(eps) is not float:
+        eps = float(_host("eps", eps))
+    if frequencies is not None and (type(frequencies) is not tuple or any(type(x) is not float for x in frequencies)):
+        frequencies = tuple([float(_host("frequencies", x)) for x in _host("frequencies", frequencies)])
+    if sections is not None and (type(sections) is not tuple or any(type(x) is not int for x in sections)):
+        sections = tuple([operator.index(_host("sections", x)) for x in _host("sections", sections)])
+    if rotary_len is not None and type(rotary_len) is not int:
+        rotary_len = operator.index(_host("rotary_len", rotary_len))
+    return base, frequencies, sections, rotary_len, bool(interleaved), eps
+
+
 class _Plan(object):
     """What a call's sizes and options come to: the part of its arguments that goes by them, and the gradients' device memory."""
 
@@ -44,15 +70,14 @@ def _plan(dtype, q_shape, k_shape, normed, base, frequencies, sections, rotary_l
     batch, tokens, heads, head_len = q_shape
     if head_len not in HEAD_LENGTHS:
         raise ValueError("heads of 32, 64 or 128 elements, got %d" % head_len)
-    rotary_len = head_len if rotary_len is None else operator.index(rotary_len)
+    rotary_len = head_len if rotary_len is None else rotary_len
     if rotary_len < 0 or rotary_len > head_len or rotary_len % 16:
         raise ValueError("a multiple of 16 elements of a head of %d can be turned, got %s" % (head_len, rotary_len))
     pairs = rotary_len // 2
-    sections = (pairs,) if sections is None else tuple(operator.index(x) for x in sections)
+    sections = (pairs,) if sections is None else sections
     if not 1 <= len(sections) <= MAX_AXES or min(sections) < 0 or sum(sections) != pairs:
         raise ValueError("sections must share the %d pairs out to 1 to %d axes, got %s" % (pairs, MAX_AXES, sections))
     if frequencies is not None:
-        frequencies = [float(x) for x in frequencies]
         if len(frequencies) != pairs or not all(math.isfinite(x) for x in frequencies):
             raise ValueError("frequencies must be %d finite numbers, got %s" % (pairs, frequencies))
     elif not (base > 0 and math.isfinite(base)):
@@ -63,7 +88,7 @@ def _plan(dtype, q_shape, k_shape, normed, base, frequencies, sections, rotary_l
         raise ValueError("eps must be 0 or more, got %s" % (eps,))
     axis = [a for a, many in enumerate(sections) for _ in range(many)]
     none = [0] * (64 - pairs)
-    sizes = _SIZES.pack(_TYPES[dtype], batch, tokens, heads, k_shape[2], head_len, rotary_len, bool(interleaved), len(sections), float(eps))
+    sizes = _SIZES.pack(_TYPES[dtype], batch, tokens, heads, k_shape[2], head_len, rotary_len, interleaved, len(sections), eps)
     return _Plan(len(sections), sizes + _ANGLES.pack(*[f / (2 * math.pi) for f in frequencies], *none, *axis, *none))
 
 
@@ -98,12 +123,7 @@ def check(q, k, q_weight, k_weight, positions, lengths, q_lengths, base, frequen
     """The call's plan, after everything that can be seen of its arguments without looking at their values on the GPU."""
     if not _plain(q, k, q_weight, k_weight):
         _check_tensors(q, k, q_weight, k_weight)
-    # a tuple can be looked up
-    if frequencies is not None and type(frequencies) is not tuple:
-        frequencies = tuple(frequencies)
-    if sections is not None and type(sections) is not tuple:
-        sections = tuple(sections)
-    plan = _plan(q.dtype, q.shape, k.shape, q_weight is not None, base, frequencies, sections, rotary_len, interleaved, eps)
+    plan = _plan(q.dtype, q.shape, k.shape, q_weight is not None, *_options(base, frequencies, sections, rotary_len, interleaved, eps))
     if positions is None and lengths is None and q_lengths is None and plan.axes == 1:
         return plan
     batch, tokens = q.shape[:2]

@@ -181,7 +181,8 @@ def rotate_heads(q, k, q_weight=None, k_weight=None, positions=None, lengths=Non
     are.  With q_weight and k_weight, (head_len,) each: x becomes weight x / sqrt(mean(x^2) + eps), per head.  Of the first rotary_len elements (default all,
     a multiple of 16; 0: norms alone) each pair (a, b) -- elements i and i + rotary_len / 2, or 2 i and 2 i + 1 if `interleaved` --
     becomes (a cos t - b sin t, a sin t + b cos t), t = position frequencies[i], frequencies base^(-2 i / rotary_len) unless given; angles are
-    made in 64 bits.
+    made in 64 bits.  frequencies, base, sections and eps are numbers on the host, without gradients: a tensor of them is read in every call, one on the GPU after waiting
+    for it (not while a graph is captured), so that a tuple of floats is made of it once.
 
     Token i of a sequence stands at position i, with lengths (int32 (batch,)) at lengths - q_lengths + i as in block_attention, or where
     positions say: int32 (batch, tokens), or (batch, tokens, axes) with `sections`, the number of pairs, in order, that turn by each axis (time, height,

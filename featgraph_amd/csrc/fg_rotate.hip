@@ -115,10 +115,10 @@ __device__ __forceinline__ float inverse_rms(float (&a)[Piece<T>::N], float (&b)
     };
     *by = 1.f;
     float s = sum();
-    // small squares are lost beside any eps that is not small itself
+    // small squares are lost beside any eps that is not small itself.  2^90 brings the smallest number there is to 2^-59 and leaves those that are small here, and eps, below 2^60
     const bool large = !(s < __builtin_inff()), small = s < 0x1p-100f && eps < 0x1p-60f;
     if (__any(large || small)) {
-        *by = large ? 0x1p-70f : small ? 0x1p60f : 1.f;
+        *by = large ? 0x1p-70f : small ? 0x1p90f : 1.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) { a[i] *= *by; b[i] *= *by; }
         const float t = sum();

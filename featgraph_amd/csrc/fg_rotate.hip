@@ -3,11 +3,11 @@
 //   t = 2 pi position[axis(pair)] turns[pair]:  (a cos t - b sin t, a sin t + b cos t);  pairs are (i, i + rotary_len / 2) or neighbours.
 //   Gradients: g = w (dout turned by -t),  dx = (g - xh mean(g xh)) / sqrt(mean(x^2) + eps),  dw = sum over all rows of xh (dout turned by -t).
 //
-// Angles are products in 64 bits, less their whole turns before they are rounded: a position of 10^6 has as good a sine as position 1.  A wavefront
-// makes a token's sines once, a pair a lane, and takes them from LDS for all its heads.
+// Angles are products in 64 bits, less their whole turns before they are rounded: a position of 10^6 has as good a sine as position 1.  What that rounding takes, l, follows
+// in cos - l sin and sin + l cos.  A wavefront makes a token's sines once, a pair a lane, and takes them from LDS for all its heads.
 // A lane holds one 16-byte piece of each half of a head's pairs, so that partners need no exchange; elements that are not turned
 // (rotary_len < head_len) are dealt to the halves the same way.
-// Sums in 32 bits; dw's sums over rows in 32 bits per wavefront and 64 after that.
+// Sums in 32 bits; dw's sums over rows in 32 bits per wavefront and 64 after that, for 32-bit results in 32 bits for 16 rows of a lane and 64 after that.
 //
 // What bounds them.  16,384 tokens of 32 / 8 heads of 128 in bfloat16: 67 us, 5.0 TB/s, the rate of a large copy; gradients of 2 x 4,096 tokens of 16 / 4
 // heads 29.6 us, 4.3 TB/s (three wavefronts a SIMD: 32 sums, two heads' elements and the next ones' take 168 registers), their weights' sums 4. One token
@@ -64,10 +64,11 @@ __device__ __forceinline__ void make_angles(const Problem &p, int b, int i, int 
         if (p.positions) position = p.positions[((int64_t)b * p.tokens + i) * p.axes + p.axis[lane]];
         else position = (int64_t)(p.lengths ? p.lengths[b] : q_len) - q_len + i;
         double t = (double)position * p.turns[lane];
-        t -= rint(t);
+        t = 2.0 * (t - rint(t));
+        const float near = (float)t, rest = (float)((t - (double)near) * 3.14159265358979323846);      // what rounding takes from an angle
         float2 cs;
-        sincospif((float)(2.0 * t), &cs.y, &cs.x);
-        table[lane] = cs;
+        sincospif(near, &cs.y, &cs.x);
+        table[lane] = make_float2(cs.x - rest * cs.y, cs.y + rest * cs.x);
     }
     wave_lds_sync();
 }
@@ -222,16 +223,47 @@ struct Grads { const void *dq_out, *dk_out; Strides dqs, dks; void *dq, *dk; flo
 
 // Workgroups of a CU (wavefronts of a SIMD) that registers are left for.
 template <typename T, bool NORM> constexpr int kResident = NORM && sizeof(T) == 2 ? 3 : 4;
+// dw's sums: a wavefront's in 64 bits for results of 32, to which a lane's go every sixteen rows, through LDS.  Gradients of 3 x 1,237 tokens of 6 / 2 heads of 64 12.6 us with the
+// weights' sums (with shuffles of 32-bit sums, one a wavefront, 13.7; of 64-bit ones 14.9), 64 x 8,192 of 4 / 4 heads of 32 567 (562); lanes with 64-bit sums take
+// three wavefronts a SIMD and 14.6 and 671.  16-bit results are rounded by more than all of it.
+template <typename T> using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;
+template <typename T> constexpr int kRows = sizeof(T) == 4 ? 16 : 0;
 
 // The same with the gradients; wavefronts take one token after the other and keep their share of dw: sums[workgroup][q, k][D].
 template <typename T, int D, bool NORM>
 __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backward_kernel(const Problem p, const Grads grads) {
     constexpr int E = Piece<T>::N;
     __shared__ float2 table[kWaves][kPairs];
-    __shared__ float shares[kWaves][2][D];
+    __shared__ Sum<T> shares[kWaves][2][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lane<T, D> me(p, lane);
     float sum[2][2][E] = {};
+    // 32-bit results: the lanes' sums into the wavefront's, by way of LDS
+    __shared__ __align__(16) float parts[kRows<T> ? kWaves : 1][Lane<T, D>::kHeads][2][D];
+    auto collect = [&]() {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                parts[wave][me.slot][k][me.a + e] = sum[k][0][e];
+                parts[wave][me.slot][k][me.b + e] = sum[k][1][e];
+                sum[k][0][e] = sum[k][1][e] = 0.f;
+            }
+        }
+        wave_lds_sync();
+#pragma unroll
+        for (int c = lane; c < 2 * D; c += 64) {
+            Sum<T> v = shares[wave][c / D][c % D];
+#pragma unroll
+            for (int h = 0; h < Lane<T, D>::kHeads; ++h) v += parts[wave][h][c / D][c % D];
+            shares[wave][c / D][c % D] = v;
+        }
+        wave_lds_sync();
+    };
+    int rows = 0;                      // in a lane's sums
+    if (NORM && kRows<T>)
+#pragma unroll
+        for (int c = lane; c < 2 * D; c += 64) shares[wave][c / D][c % D] = 0;
     const int64_t units = (int64_t)p.batch * p.tokens * p.parts;
     const int q_groups = (p.heads + me.kHeads - 1) / me.kHeads, k_groups = (p.kv_heads + me.kHeads - 1) / me.kHeads;
     Pair<T> weights[2];
@@ -298,25 +330,34 @@ __global__ __launch_bounds__(kThreads, (kResident<T, NORM>)) void rotate_backwar
         // group n of queries and keys together is part n modulo the parts'
         side(p.q, p.qs, grads.dq_out, grads.dqs, grads.dq, p.heads, part, q_groups, std::integral_constant<int, 0>{});
         side(p.k, p.ks, grads.dk_out, grads.dks, grads.dk, p.kv_heads, (part + p.parts - q_groups % p.parts) % p.parts, k_groups, std::integral_constant<int, 1>{});
+        if constexpr (NORM && kRows<T>)
+            if ((rows += (q_groups + k_groups + p.parts - 1) / p.parts) >= kRows<T>) {
+                collect();
+                rows = 0;
+            }
     }
     if (!NORM) return;
     // over the wavefront's heads, then its workgroup's wavefronts
+    if constexpr (kRows<T> != 0) {
+        collect();
+    } else {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float v = sum[k][h][e];
-                for (int d = Lane<T, D>::kLanes; d < 64; d <<= 1) v += __shfl_xor(v, d);
-                if (me.slot == 0) shares[wave][k][(h ? me.b : me.a) + e] = v;
-            }
+                for (int e = 0; e < E; ++e) {
+                    float v = sum[k][h][e];
+                    for (int d = Lane<T, D>::kLanes; d < 64; d <<= 1) v += __shfl_xor(v, d);
+                    if (me.slot == 0) shares[wave][k][(h ? me.b : me.a) + e] = v;
+                }
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * D; c += kThreads) {
-        float v = 0.f;
+        Sum<T> v = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) v += shares[w][c / D][c % D];
-        grads.sums[(int64_t)blockIdx.x * 2 * D + c] = v;
+        grads.sums[(int64_t)blockIdx.x * 2 * D + c] = (float)v;
     }
 }
 

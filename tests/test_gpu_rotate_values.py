@@ -42,3 +42,38 @@ def test_the_smallest_numbers_are_normed(dtype, head_len, eps):
     (grad,) = torch.autograd.grad(y, big, dout.cuda())
     cos, sin, there = ref.angles(big.shape, head_len)
     ref.check(grad, ref.rotate(x[:, -20:], w, cos, sin, there, head_len, eps=eps, dout=dout)["dx"])
+
+
+@pytest.mark.parametrize("head_len", [32, 128])
+def test_angles_are_those_of_64_bits(head_len):
+    """What float32 takes from an angle is made up for: of (1, 0) turned by t the error in the angle's direction is no multiple of that remainder.  The sine's own rounding, up to 2^-24 and
+    independent of it, leaves a slope of 2^-24 / (pi 2^-26 sqrt(n)), 0.02 for n = 10^4; without the remainder it is -1."""
+    from featgraph_amd import ops
+    tokens, pairs = 4000, head_len // 2
+    q = torch.zeros((1, tokens, 1, head_len), device="cuda")
+    q[..., :pairs] = 1
+    got = ops.rotate_heads(q, q, lengths=ints(131072 + 17))[0].cpu().double().numpy()[0, :, 0]
+    position = np.arange(tokens) + 131072 + 17 - tokens
+    turns = np.array([10000.0 ** (-i / pairs) / (2 * np.pi) for i in range(pairs)])
+    t = position[:, None] * turns
+    t = 2 * (t - np.rint(t))
+    rest = np.pi * (t - t.astype(np.float32).astype(np.float64))
+    cos, sin = np.cos(np.pi * t), np.sin(np.pi * t)
+    off = got[:, pairs:] * cos - got[:, :pairs] * sin                          # of the angle
+    assert np.abs(off).max() <= 3 * 2.0 ** -24
+    assert abs((off * rest).sum() / (rest * rest).sum()) < 0.1
+
+
+def test_weights_gradients_of_many_rows():
+    """Rows of ones and minus ones are their own norm, so that the weights' gradient is a plain sum of the outputs' gradients with signs: 2^20 rows in 4,096 wavefronts.  A lane adds 16 in
+    32 bits (additions 2 to 16 of numbers whose sum grows like sqrt(i), each off by 2^-24 / sqrt(3) of it at most: 2.8 of 2^-48 together), then sums are 64 bits up to a workgroup's, rounded, and the result, rounded.
+    All of 256 rows in 32 bits would give 43 in place of 2.8."""
+    from featgraph_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = [torch.randint(0, 2, (1, 1 << 20, 1, 32), generator=gen, device="cuda").float() * 2 - 1 for _ in "qk"]
+    w = [torch.ones(32, device="cuda").requires_grad_() for _ in "qk"]
+    dout = [torch.randn(t.shape, generator=gen, device="cuda") for t in x]
+    grads = torch.autograd.grad(ops.rotate_heads(*x, *w, rotary_len=0, eps=0.0), w, dout)
+    want = [(t.double() * d.double()).sum((0, 1, 2)) for t, d in zip(x, dout)]
+    off = torch.cat([g.double() - v for g, v in zip(grads, want)])
+    assert float(off.norm() / torch.cat(want).norm()) <= (2.8 + 1 / 3 + 1 / 3) ** 0.5 * 2.0 ** -24

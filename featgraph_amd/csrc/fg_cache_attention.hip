@@ -258,8 +258,13 @@ template <typename T> __device__ __forceinline__ void store_result(T *out, int64
 constexpr int kListed = 1024;          // blocks listed at a time
 struct NoList {};
 
-// Wavefronts of a SIMD that registers are left for: 128, 168 or 256 each.
-template <typename T, int D, int BITS, int RT, bool LISTED> constexpr int kResident = RT > 1 ? 2 : D < 128 ? 4 - (sizeof(T) == 4 && BITS == 8 && LISTED) : sizeof(T) == 4 ? 2 : (BITS == 4 && std::is_same<T, __bf16>::value ? 4 : 3) - LISTED;
+// Wavefronts of a SIMD that registers are left for: 128, 168 or 256 each; as many as spill nothing.  One token over 32 x 32,768 keys of 8 x 128 (us): bfloat16 / 4 bits (four) 199, float16 / 4 (three) 201,
+// bfloat16 / 8 (three) 381, float16 / 8 with two 385, with three and 24 bytes in scratch 380, over 32,768 keys alone 19.5 and 20.0, 4 tokens over 8 x 4,096 20.1 and 20.9; float32 (two) 227 and 386.
+template <typename T, int D, int BITS, int RT, bool LISTED>
+constexpr int kResident = RT > 1 ? 2
+    : D < 128 ? 4 - (sizeof(T) == 4 && BITS == 8 && LISTED)
+    : sizeof(T) == 4 || (std::is_same<T, _Float16>::value && BITS == 8) ? 2
+    : (BITS == 4 && std::is_same<T, __bf16>::value ? 4 : 3) - LISTED;
 // Most tiles of 16 rows that a workgroup takes.
 template <typename T, int D> constexpr int kMostTiles = sizeof(T) == 4 && D == 128 ? 1 : 2;
 

@@ -37,6 +37,7 @@ template <typename T> using V8 = typename Vec<T>::type;
 constexpr int kUnit = 32;              // keys (or query rows) of one step
 constexpr int kWaves = 4;              // wavefronts of a workgroup
 constexpr int kThreads = 64 * kWaves;
+constexpr int64_t kMostGroups = (1ll << 32) / kThreads - 1;    // workgroups of a launch: it takes fewer than 2^32 threads
 constexpr int kPad = 16;               // elements between staged rows: 16 rows' 32-byte pieces, and 128-bit writes, spread over the banks
 constexpr float kLog2e = 1.4426950408889634f;
 

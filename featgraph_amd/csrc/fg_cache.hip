@@ -196,7 +196,7 @@ int cut(Window *w, int head_len, unsigned *grid) {
     while ((1 << w->lanes_shift) < kThreads && (1 << w->lanes_shift) < pieces) ++w->lanes_shift;
     const int64_t lanes = 1 << w->lanes_shift, heads = kThreads >> w->lanes_shift, parts = (pieces + lanes * kEach - 1) / (lanes * kEach);
     const int64_t n = 2 * ((rows + heads - 1) / heads) * parts;
-    if (pieces > INT32_MAX - kThreads * kEach || rows > INT32_MAX || n >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache: %lld workgroups do not fit a launch", (long long)n);
+    if (pieces > INT32_MAX - kThreads * kEach || rows > INT32_MAX || n > block::kMostGroups) return fail(FG_ERR_SHAPE, "cache: %lld workgroups do not fit a launch", (long long)n);
     w->parts = (int)parts;
     *grid = (unsigned)n;
     return FG_OK;

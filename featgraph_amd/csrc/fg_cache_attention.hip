@@ -506,7 +506,7 @@ int launch(const Problem &p, const fg_cache_attention_args *a, void *workspace, 
     const Shape s = shape_of(p, MOST);
     const size_t rows = (size_t)p.batch * p.queries * p.heads;
     const int64_t grid = (int64_t)p.batch * p.kv_heads * s.n_groups * s.splits;
-    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)grid);
+    if (grid > kMostGroups) return fail(FG_ERR_SHAPE, "cache attention: %lld workgroups do not fit a launch", (long long)grid);
     const size_t sums = s.splits > 1 ? round_up(rows * s.splits * D * sizeof(float)) : 0, stats = s.splits > 1 ? round_up(rows * s.splits * sizeof(float2)) : 0;
     if (need) { *need = sums + stats; return FG_OK; }
     if (bytes < sums + stats || (sums && !workspace))

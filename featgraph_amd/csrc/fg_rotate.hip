@@ -426,7 +426,7 @@ int problem_of(const fg_rotate_args *a, Problem *p) {
     const int groups = (a->heads + each - 1) / each + (a->kv_heads + each - 1) / each;
     p->parts = (int64_t)a->batch * a->tokens >= 2048 ? 1 : groups;
     const int64_t grid = ((int64_t)a->batch * a->tokens * p->parts + kWaves - 1) / kWaves;
-    if (grid >= (1ll << 31)) return fail(FG_ERR_SHAPE, "rotation: %lld workgroups do not fit a launch", (long long)grid);
+    if (grid > block::kMostGroups) return fail(FG_ERR_SHAPE, "rotation: %lld workgroups do not fit a launch", (long long)grid);
     return FG_OK;
 }
 

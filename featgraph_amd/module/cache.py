@@ -7,6 +7,7 @@ The reference has no such operator.
 """
 import ctypes
 import functools
+import operator
 import struct
 
 import torch
@@ -43,6 +44,7 @@ class KeyValueCache(object):
                 raise ValueError("%s must be uint8 with 4 axes on %s, got %s of %s on %s" % (name, k.device, tuple(t.shape), t.dtype, t.device))
             if not t.is_contiguous() or t.data_ptr() % (4 if "scales" in name else 16):
                 raise ValueError("%s must be dense and stand at a multiple of %d bytes" % (name, 4 if "scales" in name else 16))
+        bits = int(bits)
         batch, kv_heads, keys, row = k.shape
         head_len = row * 8 // bits
         if head_len not in HEAD_LENGTHS or row * 8 != head_len * bits:
@@ -127,7 +129,7 @@ def read(cache, dtype, first, count, lengths):
     device = cache.device
     _check_counts("first", first, cache.batch, device)
     _check_counts("lengths", lengths, cache.batch, device)
-    count = cache.keys if count is None else count
+    count = cache.keys if count is None else operator.index(count)
     if count < 0:
         raise ValueError("%d keys to read" % count)
     shape = (cache.batch, count, cache.kv_heads, cache.head_len)
@@ -184,7 +186,7 @@ def attention(q, cache, blocks, block_size, scale, causal, lengths, q_lengths):
     topk = 0
     if blocks is not None or block_size is not None:
         _check_blocks(blocks, block_size, batch, queries, cache)
-        blocks, topk = blocks.contiguous(), blocks.shape[3]
+        blocks, block_size, topk = blocks.contiguous(), int(block_size), blocks.shape[3]
     if lengths is not None:
         _check_counts("lengths", lengths, batch, device)
     if q_lengths is not None:

@@ -162,3 +162,16 @@ def test_many_equal_keys_far_apart():
     want = ops.read_cache(cache, F32, count=1)[1].expand_as(q)
     assert ((got - want).abs() <= (2048 * 32 + 256 * 4) * 2.0 ** -24 * want.abs()).all()
     del cache
+
+
+def test_sizes_are_whole_numbers_whatever_holds_them():
+    from featgraph_amd import ops
+    cache = arbitrary(2, 70, 2, 64, 4)
+    other = ops.KeyValueCache(cache.k, cache.k_scales, cache.v, cache.v_scales, 4.0)
+    q = torch.randn((2, 1, 4, 64), device="cuda")
+    blocks = torch.zeros((2, 1, 2, 1), dtype=torch.int32, device="cuda")
+    right = ops.cache_attention(q, cache, blocks, 32)
+    assert torch.equal(ops.cache_attention(q, other, blocks, 32.0), right) and torch.equal(ops.cache_attention(q, cache, blocks, np.int64(32)), right)
+    assert torch.equal(ops.read_cache(other, F32, count=np.int64(3))[0], ops.read_cache(cache, F32, count=3)[0])
+    with pytest.raises(TypeError):
+        ops.read_cache(cache, count=3.0)

@@ -223,7 +223,7 @@ struct Grads { const void *dq_out, *dk_out; Strides dqs, dks; void *dq, *dk; flo
 
 // Workgroups of a CU (wavefronts of a SIMD) that registers are left for.
 template <typename T, bool NORM> constexpr int kResident = NORM && sizeof(T) == 2 ? 3 : 4;
-// dw's sums: a wavefront's in 64 bits for results of 32, to which a lane's go every sixteen rows, through LDS.  Gradients of 3 x 1,237 tokens of 6 / 2 heads of 64 12.6 us with the
+// dw's sums: a wavefront's in 64 bits for results of 32, to which a lane's go after every token that ends sixteen rows or more, through LDS.  Gradients of 3 x 1,237 tokens of 6 / 2 heads of 64 12.6 us with the
 // weights' sums (with shuffles of 32-bit sums, one a wavefront, 13.7; of 64-bit ones 14.9), 64 x 8,192 of 4 / 4 heads of 32 567 (562); lanes with 64-bit sums take
 // three wavefronts a SIMD and 14.6 and 671.  16-bit results are rounded by more than all of it.
 template <typename T> using Sum = typename std::conditional<sizeof(T) == 4, double, float>::type;

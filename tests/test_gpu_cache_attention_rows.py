@@ -175,3 +175,39 @@ def test_sizes_are_whole_numbers_whatever_holds_them():
     assert torch.equal(ops.read_cache(other, F32, count=np.int64(3))[0], ops.read_cache(cache, F32, count=3)[0])
     with pytest.raises(TypeError):
         ops.read_cache(cache, count=3.0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype,queries", [(F32, 1), (F16, 3), (BF16, 40)])
+def test_large_values_beside_ones_that_are_no_numbers(bits, dtype, queries):
+    # both in one step of 32 keys; float16 results end at 65504
+    from featgraph_amd import ops
+    cache = arbitrary(1, 200, 2, 64, bits)
+    cache.v_scales[:, :, 128:160, 0] = 200 if bits == 8 else 240
+    cache.v_scales[:, :, 140, 1] = 255
+    q = torch.randn((1, queries, 4, 64), device="cuda").to(dtype)
+    got = ops.cache_attention(q, cache)
+    assert torch.isnan(got[..., 32:]).all() and torch.isfinite(got[..., :32]).all()
+    if dtype == F16:
+        assert got[..., :32].abs().max() == 65504
+    else:
+        cache.v_scales[:, :, 140, 1] = 127  # numbers again: the others keep their bits
+        assert torch.equal(ops.cache_attention(q, cache)[..., :32], got[..., :32])
+        if bits == 4:
+            check_large(q, cache)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_values_captured(dtype):
+    from featgraph_amd import ops
+    cache = arbitrary(2, 3000, 2, 64, 4)
+    q = torch.randn((2, 1, 4, 64), device="cuda").to(dtype)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.cache_attention(q, cache)
+    for scale in (127, 250, 130, 251):
+        cache.v_scales[:, :, 1000:1100] = scale
+        q.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.cache_attention(q, cache)) and torch.isfinite(out).all()

@@ -77,3 +77,39 @@ def test_weights_gradients_of_many_rows():
     want = [(t.double() * d.double()).sum((0, 1, 2)) for t, d in zip(x, dout)]
     off = torch.cat([g.double() - v for g, v in zip(grads, want)])
     assert float(off.norm() / torch.cat(want).norm()) <= (2.8 + 1 / 3 + 1 / 3) ** 0.5 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,head_len", [(700, 40, 1, 64), (3000, 5, 17, 32), (9000, 9, 4, 128)])
+def test_weights_gradients_across_sums_of_rows(tokens, heads, kv_heads, head_len):
+    # rows that do not come in sixteens, wavefronts of one group of heads and of all of a token's, captured and replayed
+    from featgraph_amd import ops
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda *shape: torch.randn(shape, generator=gen, device="cuda")
+    q, k, w = new(1, tokens, heads, head_len), new(1, tokens, kv_heads, head_len), [1 + 0.3 * new(head_len) for _ in "qk"]
+    douts = new(*q.shape), new(*k.shape)
+    leaves = [t.requires_grad_() for t in [q, k] + w]
+    there_are = ints(tokens - 3)
+    step = lambda: torch.autograd.grad(ops.rotate_heads(*leaves, q_lengths=there_are), leaves, douts)
+    got = step()
+    cos, sin, there = ref.angles(q.shape, head_len, q_lengths=[tokens - 3])
+    for i, (x, weight, dout) in enumerate(zip((q, k), w, douts)):
+        want = ref.rotate(x, weight, cos, sin, there, head_len, dout=dout)
+        ref.check(got[i], want["dx"])
+        # the terms' own rounding, and sixteen rows, a workgroup's sum and the result in 32 bits, in place of all rows
+        e = (head_len + 12) * ref.W
+        value, bound = want["dw"]
+        rows = x.numel() // head_len
+        ref.check(got[2 + i], (value, bound * (2 * e + 20 * ref.W) / (2 * e + rows * ref.W) + ref.U[F32] * np.abs(value)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, got))
+        step()

@@ -14,11 +14,11 @@
 // are not finite, make scores of their own rows alone.)
 //
 // What bounds it.  32 requests of 32,768 keys of 8 heads x 128 in 4 bits, one token of 32 heads each (1.14 GB): 196 us, 5.8 TB/s, above the rate of a large copy (5.1),
-// for it only reads; 128 registers leave room for four wavefronts a SIMD, which keep 17 KB each on their way. With a sweep of its own for values that are not finite in
-// the same kernel it took 276 registers and 353 us.  One request of 2,048 keys x 8 heads x 64: 7.1 us, of which 3.5 are the joining launch and the rest the chain
-// length, keys, softmax, joining. Many rows, 64 tokens over 16,384 keys of 8 x 128 in 8 bits: 43 us, 400 TFLOP/s counted once; with two tiles of rows two
-// wavefronts fit a SIMD, whose vector instructions (430 a step) and products together fill 85 % of the time.  (Four wavefronts that share the widened keys through LDS and take two tiles
-// each wait for one another: 46 us, and 134 where this takes 111, 512 tokens over 8,192 keys.)
+// for it only reads; two wavefronts a SIMD, which is what the rule for shares launches there, keep 8.7 KB each SIMD on their way. With a sweep of its own for values that are not finite in
+// the same kernel it took 276 registers and 353 us.  One request of 2,048 keys x 8 heads x 64: 7.6 us captured, of which some 3.5 are the joining launch and the rest the chain
+// length, keys, softmax, joining. Many rows, 64 tokens over 16,384 keys of 8 x 128 in 8 bits: 42 us, 410 TFLOP/s counted once; with two tiles of rows two
+// wavefronts fit a SIMD, each of which issues a vector instruction or a product in 31 % of its cycles and waits in 26 % (348 vector instructions a step, 52 of them products).  (Four
+// wavefronts that share the widened keys through LDS and take two tiles each wait for one another: 46 us, and 134 where this takes 111, 512 tokens over 8,192 keys.)
 #include <algorithm>
 #include <type_traits>
 
